@@ -35,6 +35,36 @@ class ArrayResultByte(ctypes.Structure):
     _fields_ = [("Data", ctypes.POINTER(ctypes.c_char)), ("Length", ctypes.c_ulong)]
 
 
+class LayerNormArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("ldx", ctypes.c_long), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+                ("y", ctypes.c_void_p), ("ldy", ctypes.c_long), ("mean", ctypes.c_void_p), ("rstd", ctypes.c_void_p),
+                ("dy", ctypes.c_void_p), ("lddy", ctypes.c_long), ("dx", ctypes.c_void_p), ("lddx", ctypes.c_long),
+                ("dweight", ctypes.c_void_p), ("dbias", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspaceBytes", ctypes.c_size_t),
+                ("rows", ctypes.c_long), ("width", ctypes.c_int), ("type", ctypes.c_int), ("paramType", ctypes.c_int),
+                ("eps", ctypes.c_float)]
+
+
+class GatedMLPArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("ldx", ctypes.c_long), ("gate", ctypes.c_void_p), ("ldgate", ctypes.c_long),
+                ("up", ctypes.c_void_p), ("ldup", ctypes.c_long), ("down", ctypes.c_void_p), ("lddown", ctypes.c_long),
+                ("y", ctypes.c_void_p), ("ldy", ctypes.c_long), ("g", ctypes.c_void_p), ("u", ctypes.c_void_p),
+                ("dy", ctypes.c_void_p), ("lddy", ctypes.c_long), ("dx", ctypes.c_void_p), ("lddx", ctypes.c_long),
+                ("dgate", ctypes.c_void_p), ("dup", ctypes.c_void_p), ("ddown", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspaceBytes", ctypes.c_size_t),
+                ("rows", ctypes.c_long), ("width", ctypes.c_int), ("hidden", ctypes.c_int), ("type", ctypes.c_int),
+                ("act", ctypes.c_int), ("coef", ctypes.c_float * 4)]
+
+
+class CrossEntropyArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("ldx", ctypes.c_long), ("table", ctypes.c_void_p), ("ldtable", ctypes.c_long),
+                ("target", ctypes.c_void_p), ("loss", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("dloss", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("lddx", ctypes.c_long), ("dtable", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspaceBytes", ctypes.c_size_t),
+                ("rows", ctypes.c_long), ("width", ctypes.c_int), ("vocab", ctypes.c_int), ("ignore", ctypes.c_longlong),
+                ("type", ctypes.c_int)]
+
+
 _ARRAY_TYPES = (ArrayResultInt, ArrayResultFloat, ArrayResultUInt64)
 
 
@@ -281,6 +311,18 @@ _SIGNATURES = {
     "KernelTimingEnable": ([_I], _I),
     "KernelTimingGet": ([_c.c_char_p, _c.POINTER(_c.c_long), _c.POINTER(_c.c_double)], _I),
     "GetMemoryStats": ([_PU64, _PU64, _PU64], _I),
+    # training and scoring in the clear (called with torch tensors by helrm_amd.cleartext)
+    "LayerNorm": ([_c.c_void_p, _c.c_void_p], _I),
+    "LayerNormGradWorkspace": ([_c.c_void_p], _c.c_long),
+    "LayerNormGrad": ([_c.c_void_p, _c.c_void_p], _I),
+    "GatedMLPWorkspace": ([_c.c_void_p], _c.c_long),
+    "GatedMLP": ([_c.c_void_p, _c.c_void_p], _I),
+    "GatedMLPGradWorkspace": ([_c.c_void_p], _c.c_long),
+    "GatedMLPGrad": ([_c.c_void_p, _c.c_void_p], _I),
+    "CrossEntropyWorkspace": ([_c.c_void_p], _c.c_long),
+    "CrossEntropy": ([_c.c_void_p, _c.c_void_p], _I),
+    "CrossEntropyGradWorkspace": ([_c.c_void_p], _c.c_long),
+    "CrossEntropyGrad": ([_c.c_void_p, _c.c_void_p], _I),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

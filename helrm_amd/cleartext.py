@@ -1,0 +1,345 @@
+"""Operators that train and score a model in the clear, on torch tensors.
+
+The encrypted path (`orion_host`) evaluates a model that was trained: its
+table, its Linears, its degree-3 activations.  These are the operators of
+that training and of scoring beside it, on the same card:
+
+    layer_norm      y = (x - mean) / sqrt(var + eps) * weight + bias
+    gated_mlp       y = (act(x gate^T) * (x up^T)) down^T
+    cross_entropy   log sum_v exp <x, table[v]> - <x, table[target]>
+
+Each has a `_forward` and a `_backward` call, which a training loop of one's
+own makes, and a form for torch's autograd.  The matrices' last dimension is
+the vector; leading dimensions are rows.  Types: float32, bfloat16, float16,
+one for all of an operator's tensors (a norm's weight and bias may be float32
+beside any); sums and softmax statistics are float32.
+
+Work goes to torch's current stream of the tensors' device and nothing waits
+for it.  Outputs and workspaces come from torch's allocator; a tensor that
+another stream made or still writes has to be waited for by the caller, as
+with torch's own operators.  A layout that the kernels do not take (a last
+dimension that is not contiguous, rows that overlap) is copied first.
+Shapes and types that do not fit raise ValueError; HipError holds what the
+library refuses.
+"""
+import ctypes
+
+import torch
+
+from .backend import CrossEntropyArgs, GatedMLPArgs, HipError, LayerNormArgs, load_library
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ACTS = {"silu": 0, "gelu": 1}
+
+_lib = None
+
+
+def _library():
+    global _lib
+    if _lib is None:
+        lib = load_library()
+        # a stream or pointer of one HIP runtime means nothing to another one: torch brings its own, and the
+        # library takes that one if it is there when the library is loaded
+        with open("/proc/self/maps") as f:
+            runtimes = {line.split()[-1] for line in f if "libamdhip64.so" in line}
+        if len(runtimes) > 1:
+            raise HipError("two HIP runtimes in one process (" + ", ".join(sorted(runtimes))
+                           + "): import torch before the library is loaded")
+        for name in ("LayerNorm", "LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad"):
+            call = getattr(lib, name)
+            call.argtypes, call.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
+        for name in ("LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad"):
+            size = getattr(lib, name + "Workspace")
+            size.argtypes, size.restype = [ctypes.c_void_p], ctypes.c_long
+        _lib = lib
+    return _lib
+
+
+def _refused(lib):
+    raise HipError(lib.GetLastError().decode())
+
+
+def _call(name, args, device, sized=True):
+    """Queue one entry point on the current stream, with a workspace of the size it asks for."""
+    lib = _lib or _library()
+    ref = ctypes.byref(args)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return _call(name, args, device, sized)
+    space = None
+    if sized:
+        need = getattr(lib, name + "Workspace")(ref)
+        if need < 0:
+            _refused(lib)
+        space = torch.empty(need, dtype=torch.uint8, device=device)
+        args.workspace, args.workspaceBytes = space.data_ptr(), need
+    if getattr(lib, name)(ref, torch.cuda.current_stream(device).cuda_stream):
+        _refused(lib)
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _rows(t, width, name, like=None):
+    """[rows, width] of a tensor whose last dimension is the vector, in a layout that the kernels take."""
+    _need(t.dim() >= 1 and t.shape[-1] == width, f"{name}: the last dimension is {list(t.shape)[-1:]}, not {width}")
+    _need(t.dtype in _TYPES, f"{name}: {t.dtype} is not float32, bfloat16 or float16")
+    _need(t.is_cuda, f"{name}: not on the GPU")
+    if like is not None:
+        _need(t.dtype == like.dtype and t.device == like.device, f"{name}: {t.dtype} on {t.device}, not {like.dtype} on {like.device}")
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    if (width > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < width):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _vector(t, n, name, dtype, device):
+    _need(tuple(t.shape) == (n,), f"{name}: {list(t.shape)}, not [{n}]")
+    _need(t.dtype == dtype and t.device == device, f"{name}: {t.dtype} on {t.device}, not {dtype} on {device}")
+    return t.contiguous()
+
+
+# ---- layer norm --------------------------------------------------------------------
+
+
+def _norm_args(x, weight, bias, eps):
+    _need(x.dim() >= 1 and x.shape[-1] >= 1, "x: no last dimension")
+    width = x.shape[-1]
+    x2 = _rows(x, width, "x")
+    _need(weight.dtype == x.dtype or weight.dtype == torch.float32, f"weight: {weight.dtype}, neither {x.dtype} nor float32")
+    weight = _vector(weight, width, "weight", weight.dtype, x.device)
+    if bias is not None:
+        bias = _vector(bias, width, "bias", weight.dtype, x.device)
+    a = LayerNormArgs()
+    a.x, a.ldx = x2.data_ptr(), _ld(x2)
+    a.weight, a.bias = weight.data_ptr(), bias.data_ptr() if bias is not None else None
+    a.rows, a.width = x2.shape[0], width
+    a.type, a.paramType = _TYPES[x.dtype], _TYPES[weight.dtype]
+    a.eps = eps
+    return a, x2, weight, bias
+
+
+def _norm_forward(x, weight, bias, eps, keep):
+    a, x2, weight, bias = _norm_args(x, weight, bias, eps)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    a.y, a.ldy = y.data_ptr(), a.width
+    mean = rstd = None
+    if keep:
+        mean, rstd = torch.empty((2, a.rows), dtype=torch.float32, device=x.device)
+        a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
+    _call("LayerNorm", a, x.device, sized=False)
+    return y, mean, rstd
+
+
+def layer_norm_forward(x, weight, bias=None, eps=1e-5):
+    """(y, mean, rstd): the norm over the last dimension, and what its gradient needs of each row."""
+    return _norm_forward(x, weight, bias, eps, True)
+
+
+def layer_norm_backward(grad, x, weight, mean, rstd, has_bias=True):
+    """(dx, dweight, dbias) of the norm; dbias is None without a bias."""
+    a, x2, weight, _ = _norm_args(x, weight, None, 0.0)
+    g2 = _rows(grad, a.width, "grad", x)
+    _need(g2.shape[0] == a.rows, f"grad: {g2.shape[0]} rows, not {a.rows}")
+    mean = _vector(mean, a.rows, "mean", torch.float32, x.device)
+    rstd = _vector(rstd, a.rows, "rstd", torch.float32, x.device)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dweight = torch.empty_like(weight)
+    dbias = torch.empty_like(weight) if has_bias else None
+    a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
+    a.dy, a.lddy = g2.data_ptr(), _ld(g2)
+    a.dx, a.lddx = dx.data_ptr(), a.width
+    a.dweight, a.dbias = dweight.data_ptr(), dbias.data_ptr() if has_bias else None
+    _call("LayerNormGrad", a, x.device)
+    return dx, dweight, dbias
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = layer_norm_forward(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.has_bias = bias is not None
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return layer_norm_backward(grad, *ctx.saved_tensors, has_bias=ctx.has_bias) + (None,)
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def layer_norm(x, weight, bias=None, eps=1e-5):
+    """The norm of x over its last dimension."""
+    if _wants_grad(x, weight, bias):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return _norm_forward(x, weight, bias, eps, False)[0]
+
+
+# ---- gated feed-forward block ----------------------------------------------------------
+
+
+def _mlp_args(x, gate, up, down, activation):
+    _need(gate.dim() == 2 and up.dim() == 2 and down.dim() == 2, "gate, up and down are matrices")
+    hidden, width = gate.shape
+    _need(hidden >= 1 and width >= 1, "gate: no elements")
+    x2 = _rows(x, width, "x")
+    gate, up, down = _rows(gate, width, "gate", x), _rows(up, width, "up", x), _rows(down, hidden, "down", x)
+    _need(up.shape[0] == hidden, f"up: {up.shape[0]} rows, not {hidden}")
+    _need(down.shape[0] == width, f"down: {down.shape[0]} rows, not {width}")
+    a = GatedMLPArgs()
+    a.x, a.ldx = x2.data_ptr(), _ld(x2)
+    a.gate, a.ldgate = gate.data_ptr(), _ld(gate)
+    a.up, a.ldup = up.data_ptr(), _ld(up)
+    a.down, a.lddown = down.data_ptr(), _ld(down)
+    a.rows, a.width, a.hidden, a.type = x2.shape[0], width, hidden, _TYPES[x.dtype]
+    if isinstance(activation, str):
+        _need(activation in _ACTS, f"activation {activation!r}: neither silu, gelu nor four coefficients")
+        a.act = _ACTS[activation]
+    else:
+        coef = tuple(float(c) for c in activation)
+        _need(len(coef) == 4, "activation: a cubic has four coefficients, lowest degree first")
+        a.act, a.coef = 2, coef
+    return a, (x2, gate, up, down)
+
+
+def _mlp_forward(x, gate, up, down, activation, keep):
+    a, held = _mlp_args(x, gate, up, down, activation)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    a.y, a.ldy = y.data_ptr(), a.width
+    saved = None
+    if keep:
+        saved = torch.empty((2, a.rows, a.hidden), dtype=torch.float32, device=x.device)
+        if saved.numel():
+            a.g = saved.data_ptr()
+            a.u = a.g + 4 * a.rows * a.hidden
+    _call("GatedMLP", a, x.device)
+    return y, saved
+
+
+def gated_mlp_forward(x, gate, up, down, activation="silu"):
+    """(y, saved): the block's output and, for its gradient, both projections in float32 ([2, rows, hidden]: rounded
+    to 16 bits they would cost the gradients more than their own rounding does)."""
+    return _mlp_forward(x, gate, up, down, activation, True)
+
+
+def gated_mlp_backward(grad, x, gate, up, down, saved, activation="silu"):
+    """(dx, dgate, dup, ddown)."""
+    a, held = _mlp_args(x, gate, up, down, activation)
+    g2 = _rows(grad, a.width, "grad", x)
+    _need(g2.shape[0] == a.rows, f"grad: {g2.shape[0]} rows, not {a.rows}")
+    _need(tuple(saved.shape) == (2, a.rows, a.hidden) and saved.dtype == torch.float32 and saved.device == x.device
+          and saved.is_contiguous(), "saved: not what the forward call returned")
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dgate, dup, ddown = (torch.empty(w.shape, dtype=x.dtype, device=x.device) for w in (gate, up, down))
+    a.dy, a.lddy = g2.data_ptr(), _ld(g2)
+    a.dx, a.lddx = dx.data_ptr(), a.width
+    if saved.numel():
+        a.g = saved.data_ptr()
+        a.u = a.g + 4 * a.rows * a.hidden
+    a.dgate, a.dup, a.ddown = dgate.data_ptr(), dup.data_ptr(), ddown.data_ptr()
+    _call("GatedMLPGrad", a, x.device)
+    return dx, dgate, dup, ddown
+
+
+class _GatedMLP(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, up, down, activation):
+        y, saved = gated_mlp_forward(x, gate, up, down, activation)
+        ctx.save_for_backward(x, gate, up, down, saved)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return gated_mlp_backward(grad, *ctx.saved_tensors, ctx.activation) + (None,)
+
+
+def gated_mlp(x, gate, up, down, activation="silu"):
+    """The gated feed-forward block (act(x gate^T) * (x up^T)) down^T: gate, up [hidden, width], down [width, hidden].
+    activation: "silu", "gelu" or a cubic's four coefficients, lowest degree first, which the block can also be
+    evaluated with under encryption."""
+    if _wants_grad(x, gate, up, down):
+        return _GatedMLP.apply(x, gate, up, down, activation)
+    return _mlp_forward(x, gate, up, down, activation, False)[0]
+
+
+# ---- softmax cross entropy against a table ------------------------------------------------
+
+
+def _loss_args(x, table, target, ignore_index):
+    _need(table.dim() == 2 and table.shape[0] >= 1 and table.shape[1] >= 1, "table: not a matrix with elements")
+    vocab, width = table.shape
+    x2 = _rows(x, width, "x")
+    table = _rows(table, width, "table", x)
+    target = _vector(target.reshape(-1), x2.shape[0], "target", torch.int64, x.device)
+    a = CrossEntropyArgs()
+    a.x, a.ldx = x2.data_ptr(), _ld(x2)
+    a.table, a.ldtable = table.data_ptr(), _ld(table)
+    a.target = target.data_ptr()
+    a.rows, a.width, a.vocab, a.ignore, a.type = x2.shape[0], width, vocab, ignore_index, _TYPES[x.dtype]
+    return a, (x2, table, target)
+
+
+def cross_entropy_forward(x, table, target, ignore_index=-100):
+    """(losses, lse), float32 for each row: the softmax cross entropy of x's products with the table's rows, and the
+    logarithm of the softmax's sum.  Rows whose target is `ignore_index` have 0 for both; a target outside the table
+    gives NaN.  The logits are never in memory."""
+    a, held = _loss_args(x, table, target, ignore_index)
+    losses, lse = torch.empty((2, a.rows), dtype=torch.float32, device=x.device)
+    a.loss, a.lse = losses.data_ptr(), lse.data_ptr()
+    _call("CrossEntropy", a, x.device)
+    return losses.view(x.shape[:-1]), lse.view(x.shape[:-1])
+
+
+def cross_entropy_backward(grad, x, table, target, lse, ignore_index=-100):
+    """(dx, dtable) for the gradient `grad` of the losses (float32); lse as the forward call gave it.  The logits are
+    computed again, a piece of the table at a time."""
+    a, held = _loss_args(x, table, target, ignore_index)
+    grad = _vector(grad.reshape(-1), a.rows, "grad", torch.float32, x.device)
+    lse = _vector(lse.reshape(-1), a.rows, "lse", torch.float32, x.device)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dtable = torch.empty(table.shape, dtype=x.dtype, device=x.device)
+    a.dloss, a.lse = grad.data_ptr(), lse.data_ptr()
+    a.dx, a.lddx, a.dtable = dx.data_ptr(), a.width, dtable.data_ptr()
+    _call("CrossEntropyGrad", a, x.device)
+    return dx, dtable
+
+
+class _CrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, table, target, ignore_index):
+        losses, lse = cross_entropy_forward(x, table, target, ignore_index)
+        ctx.save_for_backward(x, table, target, lse)
+        ctx.ignore_index = ignore_index
+        return losses
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return cross_entropy_backward(grad, *ctx.saved_tensors, ctx.ignore_index) + (None, None)
+
+
+def cross_entropy(x, table, target, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of x [..., width] against table [vocab, width]: the mean over the rows that have a target
+    (0 where none has one), their "sum", or "none" for a loss a row."""
+    _need(reduction in ("mean", "sum", "none"), f"reduction {reduction!r}: neither mean, sum nor none")
+    if _wants_grad(x, table):
+        losses = _CrossEntropy.apply(x, table, target, ignore_index)
+    else:
+        losses = cross_entropy_forward(x, table, target, ignore_index)[0]
+    if reduction == "none":
+        return losses
+    total = losses.sum()
+    return total if reduction == "sum" else total / (target != ignore_index).sum().clamp(min=1)

@@ -1,0 +1,40 @@
+// cleartext.h -- internal declarations of the operators that train and score
+// the model in the clear (layer norm, gated feed-forward block, softmax cross
+// entropy against a table).  Not part of the C ABI.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+#include <stdexcept>
+#include <string>
+
+// The element types of an operator's tensors, as the C ABI numbers them.
+enum DType { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
+inline int dtype_size(int t) { return t == DT_F32 ? 4 : 2; }
+
+// Records the message GetLastError() returns; the value is -1 (runtime.hip).
+int report_error(const char* what);
+
+namespace clr {
+
+struct Error : std::runtime_error { using std::runtime_error::runtime_error; };
+inline void require(bool ok, const char* what) { if (!ok) throw Error(what); }
+inline void check_hip(hipError_t e, const char* what) {
+  if (e != hipSuccess) throw Error(std::string("HIP error: ") + hipGetErrorString(e) + " at " + what);
+}
+template <class F> int guarded(F&& f) {
+  try { f(); check_hip(hipGetLastError(), "a kernel launch"); return 0; }
+  catch (const std::exception& e) { return report_error(e.what()); }
+  catch (...) { return report_error("unknown error"); }
+}
+inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
+inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// f(T{}) with T the C++ type of a DType
+template <class F> void with_type(int t, F&& f) {
+  if (t == DT_F32) f(float{});
+  else if (t == DT_BF16) f(__bf16{});
+  else f(_Float16{});
+}
+
+}  // namespace clr

@@ -26,6 +26,7 @@
 #include <unordered_set>
 #include <vector>
 
+#include "cleartext.h"
 #include "fpntt.h"
 #include "hipckks.h"
 #include "kernels.h"
@@ -2043,6 +2044,11 @@ std::vector<uint8_t> serialize_galois_key(u64 galel, const DU64& key) {
 }
 
 }  // namespace
+
+int report_error(const char* what) {
+  try { g_err = what; } catch (...) { g_err.clear(); }
+  return -1;
+}
 
 // ============================================================================
 // C ABI

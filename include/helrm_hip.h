@@ -271,6 +271,85 @@ unsigned long long LiveHeapBytes(void);
 int StartLiveHeapSampler(int intervalMs);
 unsigned long long StopLiveHeapSampler(void);
 
+/* ---- [ext] training and scoring in the clear -------------------------------------
+ * The model whose table, Linears and activations the entry points above take
+ * under encryption is trained in the clear on the same card.  These need no
+ * scheme: tensors are device pointers, work is queued on `stream` (a
+ * hipStream_t; NULL: the default stream) of the current device, nothing waits
+ * and nothing is allocated, so calls may be captured into a graph.  Each
+ * ...Workspace call says how many bytes of device memory at `workspace`
+ * (256-byte aligned) the same arguments need: -1 on failure, workspace and
+ * outputs may be NULL there.  A workspace is free again once the work queued
+ * by its call is done.  Element types: 0 float32, 1 bfloat16, 2 float16; sums,
+ * means and softmax statistics are float32 for each.  A matrix's rows are
+ * contiguous and `ld...` elements apart.  Outputs do not overlap inputs
+ * except where said. */
+#define HELRM_F32 0
+#define HELRM_BF16 1
+#define HELRM_F16 2
+typedef struct {
+  const void* x; long ldx;               /* [rows][width] */
+  const void* weight; const void* bias;  /* [width], of paramType; bias may be NULL */
+  void* y; long ldy;                     /* may be x */
+  float* mean; float* rstd;              /* [rows]: the row's mean and (variance + eps)^-1/2; written by LayerNorm unless NULL */
+  const void* dy; long lddy;             /* LayerNormGrad: gradient of y; dx may be dy */
+  void* dx; long lddx;
+  void* dweight; void* dbias;            /* [width], of paramType; dbias may be NULL */
+  void* workspace; size_t workspaceBytes; /* LayerNormGrad only */
+  long rows; int width;
+  int type; int paramType;
+  float eps;
+} LayerNormArgs;
+int LayerNorm(const LayerNormArgs* args, void* stream);
+long LayerNormGradWorkspace(const LayerNormArgs* args);
+int LayerNormGrad(const LayerNormArgs* args, void* stream);
+
+/* y = (act(x gate^T) * (x up^T)) down^T: the gated feed-forward block.
+ * act 0: silu, 1: gelu (erf), 2: cubic, coef lowest degree first, the form
+ * that EvaluatePolynomial takes. */
+typedef struct {
+  const void* x; long ldx;               /* [rows][width] */
+  const void* gate; long ldgate;         /* [hidden][width] */
+  const void* up; long ldup;             /* [hidden][width] */
+  const void* down; long lddown;         /* [width][hidden] */
+  void* y; long ldy;                     /* [rows][width] */
+  float* g; float* u;                    /* [rows][hidden] each: x gate^T and x up^T, kept for the gradient (both or neither) */
+  const void* dy; long lddy;             /* GatedMLPGrad */
+  void* dx; long lddx;
+  void* dgate; void* dup; void* ddown;   /* as the weights, contiguous */
+  void* workspace; size_t workspaceBytes;
+  long rows; int width; int hidden;
+  int type; int act;
+  float coef[4];
+} GatedMLPArgs;
+long GatedMLPWorkspace(const GatedMLPArgs* args);
+int GatedMLP(const GatedMLPArgs* args, void* stream);
+long GatedMLPGradWorkspace(const GatedMLPArgs* args);
+int GatedMLPGrad(const GatedMLPArgs* args, void* stream);
+
+/* loss[t] = lse[t] - <x[t], table[target[t]]>, lse[t] = log sum_v exp <x[t], table[v]>:
+ * softmax cross entropy against a table of `vocab` rows, without keeping the
+ * logits.  A row whose target is `ignore` has loss, lse and gradients 0, and
+ * nothing it holds reaches another row's; a target outside [0, vocab) that is
+ * not `ignore` gives a loss and gradients of NaN.  dtable is contiguous. */
+typedef struct {
+  const void* x; long ldx;               /* [rows][width] */
+  const void* table; long ldtable;       /* [vocab][width] */
+  const long long* target;               /* [rows] */
+  float* loss; float* lse;               /* [rows]; CrossEntropyGrad reads lse */
+  const float* dloss;                    /* [rows] */
+  void* dx; long lddx;                   /* [rows][width] */
+  void* dtable;                          /* [vocab][width] */
+  void* workspace; size_t workspaceBytes;
+  long rows; int width; int vocab;
+  long long ignore;
+  int type;
+} CrossEntropyArgs;
+long CrossEntropyWorkspace(const CrossEntropyArgs* args);
+int CrossEntropy(const CrossEntropyArgs* args, void* stream);
+long CrossEntropyGradWorkspace(const CrossEntropyArgs* args);
+int CrossEntropyGrad(const CrossEntropyArgs* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
