@@ -213,22 +213,26 @@ def _mlp_args(x, gate, up, down, activation):
     return a, (x2, gate, up, down)
 
 
+def _saved_width(a):
+    return (a.hidden + 7) // 8 * 8
+
+
 def _mlp_forward(x, gate, up, down, activation, keep):
     a, held = _mlp_args(x, gate, up, down, activation)
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     a.y, a.ldy = y.data_ptr(), a.width
     saved = None
     if keep:
-        saved = torch.empty((2, a.rows, a.hidden), dtype=torch.float32, device=x.device)
-        if saved.numel():
+        saved = torch.empty((2, a.rows, _saved_width(a)), dtype=torch.float32, device=x.device)
+        if a.rows:
             a.g = saved.data_ptr()
-            a.u = a.g + 4 * a.rows * a.hidden
+            a.u = a.g + 2 * saved.numel()
     _call("GatedMLP", a, x.device)
     return y, saved
 
 
 def gated_mlp_forward(x, gate, up, down, activation="silu"):
-    """(y, saved): the block's output and, for its gradient, both projections in float32 ([2, rows, hidden]: rounded
+    """(y, saved): the block's output and, for its gradient, both projections in float32 (rounded
     to 16 bits they would cost the gradients more than their own rounding does)."""
     return _mlp_forward(x, gate, up, down, activation, True)
 
@@ -238,15 +242,15 @@ def gated_mlp_backward(grad, x, gate, up, down, saved, activation="silu"):
     a, held = _mlp_args(x, gate, up, down, activation)
     g2 = _rows(grad, a.width, "grad", x)
     _need(g2.shape[0] == a.rows, f"grad: {g2.shape[0]} rows, not {a.rows}")
-    _need(tuple(saved.shape) == (2, a.rows, a.hidden) and saved.dtype == torch.float32 and saved.device == x.device
+    _need(tuple(saved.shape) == (2, a.rows, _saved_width(a)) and saved.dtype == torch.float32 and saved.device == x.device
           and saved.is_contiguous(), "saved: not what the forward call returned")
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dgate, dup, ddown = (torch.empty(w.shape, dtype=x.dtype, device=x.device) for w in (gate, up, down))
     a.dy, a.lddy = g2.data_ptr(), _ld(g2)
     a.dx, a.lddx = dx.data_ptr(), a.width
-    if saved.numel():
+    if a.rows:
         a.g = saved.data_ptr()
-        a.u = a.g + 4 * a.rows * a.hidden
+        a.u = a.g + 2 * saved.numel()
     a.dgate, a.dup, a.ddown = dgate.data_ptr(), dup.data_ptr(), ddown.data_ptr()
     _call("GatedMLPGrad", a, x.device)
     return dx, dgate, dup, ddown

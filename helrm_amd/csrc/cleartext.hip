@@ -28,12 +28,13 @@ void check_space(const void* ws, size_t have, size_t need) {
   require(have >= need && (ws || !need), "workspace too small");
   require((uintptr_t)ws % 256 == 0, "workspace not aligned to 256 bytes");
 }
-// Rows of a matrix: the tiles' row count fits a launch, and a row's stride covers it.
+// A matrix is there, and a row's stride covers it.
 void check_matrix(const void* p, long ld, long rows, long width, const char* what) {
   require(p || !rows, what);
   require(rows <= 1 || ld >= width, what);
 }
-constexpr long MAX_ROWS = 4L << 20;  // 65,535 tiles of 64
+constexpr long MAX_ROWS = 1L << 30;
+constexpr long MAX_LD = 1L << 21;  // 256 rows are within a buffer descriptor's 31-bit offsets
 
 // ---- layer norm ----
 void check_norm(const LayerNormArgs* a) {
@@ -59,7 +60,7 @@ void check_mlp(const GatedMLPArgs* a) {
   require(a, "no arguments");
   check_type(a->type);
   require(a->rows >= 0 && a->rows < MAX_ROWS, "GatedMLP: bad number of rows");
-  require(a->width >= 1 && a->hidden >= 1 && a->width < MAX_ROWS && a->hidden < MAX_ROWS, "GatedMLP: bad width");
+  require(a->width >= 1 && a->hidden >= 1 && a->width < MAX_LD && a->hidden < MAX_LD, "GatedMLP: bad width");
   require(a->act >= ACT_SILU && a->act <= ACT_CUBIC, "GatedMLP: unknown activation");
 }
 void check_mlp_tensors(const GatedMLPArgs* a) {
@@ -73,66 +74,110 @@ void set_act(ProductArgs& p, const GatedMLPArgs* a) {
   for (int i = 0; i < 4; i++) p.coef[i] = a->coef[i];
 }
 
-size_t mlp_forward(const GatedMLPArgs* a, void* ws, hipStream_t st) {
-  Arena m{(char*)ws};
-  const long F = a->hidden;
-  void* h = m.bytes((size_t)a->rows * F * dtype_size(a->type));
-  if (!ws) return m.used;
+// A matrix as the products take it: where it is, or a copy in the workspace.
+struct Held {
+  const uint16_t* p;
+  long ld, part;             // part: elements from one part of a float32 matrix to the next
+  const uint16_t* at(int k) const { return p + k * part; }
+};
+long up8(long n) { return (n + 7) & ~7L; }
+bool fits(const void* p, long ld, long rows, long width, int type) {
+  return type != DT_F32 && (uintptr_t)p % 16 == 0 && width % 8 == 0 && (rows <= 1 || ld % 8 == 0) && ld < MAX_LD;
+}
+// An intermediate of the operator's own.
+Held hold(Arena& m, long rows, long width, int type) {
+  const long ld = up8(width), part = rows * ld;
+  return {m.take<uint16_t>((size_t)part * (type == DT_F32 ? 3 : 1)), ld, part};
+}
+// Where alignment, an odd width or float32 does not let the tiles be loaded
+// from the matrix itself it is copied first: a pass over it, which a product
+// of more than a few rows reads many times.
+Held held(Arena& m, const void* p, long ld, long rows, long width, int type, hipStream_t st, bool same_ld_as_next = true) {
+  if (fits(p, ld, rows, width, type) && same_ld_as_next) return {(const uint16_t*)p, rows > 1 ? ld : width, 0};
+  Held h = hold(m, rows, width, type);
+  if (m.base) lay_out(p, ld, type, (void*)h.p, h.ld, h.part, nullptr, nullptr, rows, (int)width, st);
+  return h;
+}
+// The pairs of parts whose products make one product: of three parts of 8 bits
+// each those above 2^-24, smallest first.
+int add_pairs(ProductArgs& p, const Held& a, const Held& b, const Held* b2 = nullptr) {
+  static const int part_a[6] = {0, 1, 2, 0, 1, 0}, part_b[6] = {2, 1, 0, 1, 0, 0};
+  const int n = p.dtype == DT_F32 ? 6 : 1;
+  for (int k = 0; k < n; k++) {
+    const int ia = n == 1 ? 0 : part_a[k], ib = n == 1 ? 0 : part_b[k];
+    p.a[p.pairs] = a.at(ia);
+    p.b[p.pairs] = b.at(ib);
+    if (b2) p.b2[p.pairs] = b2->at(ib);
+    p.pairs++;
+  }
+  p.lda = a.ld; p.ldb = b.ld;
+  return p.pairs;
+}
+
+size_t mlp_forward(const GatedMLPArgs* a, bool count, hipStream_t st) {
+  Arena m{count ? nullptr : (char*)a->workspace};
+  const int type = a->type;
+  const bool same = a->ldgate == a->ldup;
+  const Held h = hold(m, a->rows, a->hidden, type);
+  const Held x = held(m, a->x, a->ldx, a->rows, a->width, type, st);
+  const Held gate = held(m, a->gate, a->ldgate, a->hidden, a->width, type, st, same && fits(a->up, a->ldup, a->hidden, a->width, type));
+  const Held up = held(m, a->up, a->ldup, a->hidden, a->width, type, st, same && fits(a->gate, a->ldgate, a->hidden, a->width, type));
+  const Held down = held(m, a->down, a->lddown, a->width, a->hidden, type, st);
+  if (count) return m.used;
   ProductArgs p{};
-  p.dtype = a->type;
-  p.M = (int)a->rows; p.N = a->hidden; p.K = a->width; p.pairs = 1;
-  p.a[0] = {a->x, a->ldx, 1};
-  p.b[0] = {a->gate, a->ldgate, 1};
-  p.b[1] = {a->up, a->ldup, 1};
-  p.g = a->g; p.u = a->u; p.h = h;
+  p.dtype = type;
+  p.M = (int)a->rows; p.N = a->hidden; p.K = a->width;
+  add_pairs(p, x, gate, &up);
+  p.g = a->g; p.u = a->u; p.h = (void*)h.p; p.ldh = h.ld; p.hpart = h.part;
   set_act(p, a);
   product_gate(p, st);
   ProductArgs q{};
-  q.dtype = q.ctype = a->type;
-  q.M = (int)a->rows; q.N = a->width; q.K = a->hidden; q.pairs = 1;
-  q.a[0] = {h, F, 1};
-  q.b[0] = {a->down, a->lddown, 1};
+  q.dtype = q.ctype = type;
+  q.M = (int)a->rows; q.N = a->width; q.K = a->hidden;
+  add_pairs(q, h, down);
   q.c = a->y; q.ldc = a->ldy;
-  product_store(q, st);
+  product_nt(q, st);
   return m.used;
 }
 
-size_t mlp_backward(const GatedMLPArgs* a, void* ws, hipStream_t st) {
-  Arena m{(char*)ws};
-  const long F = a->hidden, D = a->width;
-  const size_t n = (size_t)a->rows * F * dtype_size(a->type);
-  void* dg = m.bytes(n); void* du = m.bytes(n); void* h = m.bytes(n);
-  if (!ws) return m.used;
-  ProductArgs p{};
-  p.dtype = p.ctype = a->type;
+size_t mlp_backward(const GatedMLPArgs* a, bool count, hipStream_t st) {
+  Arena m{count ? nullptr : (char*)a->workspace};
+  const int type = a->type;
+  const bool same = a->ldgate == a->ldup;
+  const Held dg = hold(m, a->rows, a->hidden, type), du = hold(m, a->rows, a->hidden, type), h = hold(m, a->rows, a->hidden, type);
+  const Held x = held(m, a->x, a->ldx, a->rows, a->width, type, st), dy = held(m, a->dy, a->lddy, a->rows, a->width, type, st);
+  const Held gate = held(m, a->gate, a->ldgate, a->hidden, a->width, type, st, same && fits(a->up, a->ldup, a->hidden, a->width, type));
+  const Held up = held(m, a->up, a->ldup, a->hidden, a->width, type, st, same && fits(a->gate, a->ldgate, a->hidden, a->width, type));
+  const Held down = held(m, a->down, a->lddown, a->width, a->hidden, type, st);
+  if (count) return m.used;
   // dh = dy down, and through the product and the activation
-  p.M = (int)a->rows; p.N = a->hidden; p.K = a->width; p.pairs = 1;
-  p.a[0] = {a->dy, a->lddy, 1};
-  p.b[0] = {a->down, 1, a->lddown};
-  p.g = a->g; p.u = a->u; p.h = h; p.dg = dg; p.du = du;
+  ProductArgs p{};
+  p.dtype = type;
+  p.M = (int)a->rows; p.N = a->hidden; p.K = a->width;
+  add_pairs(p, dy, down);
+  p.g = a->g; p.u = a->u; p.h = (void*)h.p; p.dg = (void*)dg.p; p.du = (void*)du.p; p.ldh = h.ld; p.hpart = h.part;
   set_act(p, a);
   product_gate_grad(p, st);
   // dx = dg gate + du up
   ProductArgs q{};
-  q.dtype = q.ctype = a->type;
-  q.M = (int)a->rows; q.N = a->width; q.K = a->hidden; q.pairs = 2;
-  q.a[0] = {dg, F, 1}; q.b[0] = {a->gate, 1, a->ldgate};
-  q.a[1] = {du, F, 1}; q.b[1] = {a->up, 1, a->ldup};
+  q.dtype = q.ctype = type;
+  q.M = (int)a->rows; q.N = a->width; q.K = a->hidden;
+  add_pairs(q, dg, gate);
+  add_pairs(q, du, up);
   q.c = a->dx; q.ldc = a->lddx;
-  product_store(q, st);
+  product_nn(q, st);
   // the weights' gradients: sums over the rows
-  ProductArgs w{};
-  w.dtype = w.ctype = a->type;
-  w.K = (int)a->rows; w.pairs = 1;
-  w.M = a->hidden; w.N = a->width; w.ldc = D;
-  w.b[0] = {a->x, 1, a->ldx};
-  w.a[0] = {dg, 1, F}; w.c = a->dgate;
-  product_store(w, st);
-  w.a[0] = {du, 1, F}; w.c = a->dup;
-  product_store(w, st);
-  w.M = a->width; w.N = a->hidden; w.ldc = F;
-  w.a[0] = {a->dy, 1, a->lddy}; w.b[0] = {h, 1, F}; w.c = a->ddown;
-  product_store(w, st);
+  auto weight = [&](const Held& l, const Held& r, long rows, long cols, void* out) {
+    ProductArgs w{};
+    w.dtype = w.ctype = type;
+    w.M = (int)rows; w.N = (int)cols; w.K = (int)a->rows;
+    add_pairs(w, l, r);
+    w.c = out; w.ldc = cols;
+    product_tn(w, st);
+  };
+  weight(dg, x, a->hidden, a->width, a->dgate);
+  weight(du, x, a->hidden, a->width, a->dup);
+  weight(dy, h, a->width, a->hidden, a->ddown);
   return m.used;
 }
 
@@ -141,7 +186,7 @@ void check_ce(const CrossEntropyArgs* a) {
   require(a, "no arguments");
   check_type(a->type);
   require(a->rows >= 0 && a->rows < MAX_ROWS, "CrossEntropy: bad number of rows");
-  require(a->width >= 1 && a->width < MAX_ROWS, "CrossEntropy: bad width");
+  require(a->width >= 1 && a->width < MAX_LD, "CrossEntropy: bad width");
   require(a->vocab >= 1, "CrossEntropy: bad number of table rows");
 }
 void check_ce_tensors(const CrossEntropyArgs* a) {
@@ -151,23 +196,23 @@ void check_ce_tensors(const CrossEntropyArgs* a) {
   require(a->lse || !a->rows, "CrossEntropy: lse");
 }
 
-size_t ce_forward(const CrossEntropyArgs* a, void* ws, hipStream_t st) {
-  Arena m{(char*)ws};
+size_t ce_forward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
+  Arena m{count ? nullptr : (char*)a->workspace};
   const long n = a->rows;
   const int parts = softmax_parts(a->vocab);
   RowsArgs r{a->target, nullptr, n, a->ignore, a->vocab};
   r.rows = m.take<int>(n); r.tgt = m.take<int>(n); r.count = m.take<int>(1);
   r.picked = m.take<float>(n); r.loss = a->loss; r.lse = a->lse;
-  void* xc = m.bytes((size_t)n * a->width * dtype_size(a->type));
+  const Held x = hold(m, n, a->width, a->type);
   float2* part = m.take<float2>((size_t)n * parts);
-  if (!ws) return m.used;
+  const Held table = held(m, a->table, a->ldtable, a->vocab, a->width, a->type, st);
+  if (count) return m.used;
   kept_rows(r, st);
-  gather_rows(a->x, a->ldx, xc, a->width, r.rows, r.count, n, a->width, a->type, st);
+  lay_out(a->x, a->ldx, a->type, (void*)x.p, x.ld, x.part, r.rows, r.count, n, a->width, st);
   ProductArgs p{};
   p.dtype = a->type;
-  p.M = (int)n; p.N = a->vocab; p.K = a->width; p.pairs = 1;
-  p.a[0] = {xc, a->width, 1};
-  p.b[0] = {a->table, a->ldtable, 1};
+  p.M = (int)n; p.N = a->vocab; p.K = a->width;
+  add_pairs(p, x, table);
   p.count = r.count; p.target = r.tgt; p.picked = r.picked; p.part = part; p.parts = parts;
   product_softmax(p, st);
   softmax_finish(part, parts, r.picked, r.rows, r.count, n, a->loss, a->lse, st);
@@ -177,53 +222,47 @@ size_t ce_forward(const CrossEntropyArgs* a, void* ws, hipStream_t st) {
 // Rows of the table whose gradients of the logits are held at a time: those
 // of all rows of x take at most 256 MiB, what the last-level cache holds.
 int piece_rows(const CrossEntropyArgs* a) {
-  const long most = (256L << 20) / (std::max<long>(a->rows, 1) * dtype_size(a->type));
-  return (int)std::min<long>(a->vocab, std::max<long>(1024, most / 1024 * 1024));
+  const long most = (256L << 20) / (std::max<long>(a->rows, 1) * (a->type == DT_F32 ? 6 : 2));
+  return (int)std::min<long>(up8(a->vocab), std::max<long>(1024, most / 1024 * 1024));
 }
 
-size_t ce_backward(const CrossEntropyArgs* a, void* ws, hipStream_t st) {
-  Arena m{(char*)ws};
+size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
+  Arena m{count ? nullptr : (char*)a->workspace};
   const long n = a->rows, D = a->width;
   const int piece = piece_rows(a);
   RowsArgs r{a->target, a->dloss, n, a->ignore, a->vocab};
   r.rows = m.take<int>(n); r.tgt = m.take<int>(n); r.count = m.take<int>(1);
-  if (a->type == DT_F16) r.scale = m.take<float>(1);
-  else m.take<float>(1);
-  void* xc = m.bytes((size_t)n * D * dtype_size(a->type));
+  float* scale = m.take<float>(1);
+  if (a->type == DT_F16) r.scale = scale;
+  const Held x = hold(m, n, a->width, a->type), dl = hold(m, n, piece, a->type);
   float* acc = m.take<float>((size_t)n * D);
-  void* dl = m.bytes((size_t)n * piece * dtype_size(a->type));
-  if (!ws) return m.used;
+  const Held table = held(m, a->table, a->ldtable, a->vocab, a->width, a->type, st);
+  if (count) return m.used;
   kept_rows(r, st);
-  gather_rows(a->x, a->ldx, xc, D, r.rows, r.count, n, a->width, a->type, st);
+  lay_out(a->x, a->ldx, a->type, (void*)x.p, x.ld, x.part, r.rows, r.count, n, a->width, st);
   for (long v0 = 0; v0 < a->vocab; v0 += piece) {
     const int len = (int)std::min<long>(piece, a->vocab - v0);
-    const char* rows = (const char*)a->table + v0 * a->ldtable * dtype_size(a->type);
+    const Held rows{table.p + v0 * table.ld, table.ld, table.part};
     ProductArgs p{};
-    p.dtype = p.ctype = a->type;
-    p.pairs = 1; p.count = r.count;
+    p.dtype = a->type; p.count = r.count;
     p.M = (int)n; p.N = len; p.K = a->width;
-    p.a[0] = {xc, D, 1};
-    p.b[0] = {rows, a->ldtable, 1};
-    p.c = dl; p.ldc = piece;
+    add_pairs(p, x, rows);
+    p.c = (void*)dl.p; p.ldc = dl.ld; p.hpart = dl.part;
     p.n0 = (int)v0; p.target = r.tgt; p.rows = r.rows; p.lse = a->lse; p.grad = a->dloss; p.scale = r.scale;
     product_softmax_grad(p, st);
     ProductArgs q{};
-    q.dtype = a->type; q.ctype = DT_F32;
-    q.pairs = 1; q.count = r.count;
+    q.dtype = a->type; q.ctype = DT_F32; q.count = r.count;
     q.M = (int)n; q.N = a->width; q.K = len;
-    q.a[0] = {dl, piece, 1};
-    q.b[0] = {rows, 1, a->ldtable};
+    add_pairs(q, dl, rows);
     q.c = acc; q.ldc = D; q.add = v0 > 0;
-    product_store(q, st);
+    product_nn(q, st);
     ProductArgs w{};
-    w.dtype = w.ctype = a->type;
-    w.pairs = 1; w.count = r.count; w.count_k = true;
+    w.dtype = w.ctype = a->type; w.count = r.count; w.count_k = true;
     w.M = len; w.N = a->width; w.K = (int)n;
-    w.a[0] = {dl, 1, piece};
-    w.b[0] = {xc, 1, D};
+    add_pairs(w, dl, x);
     w.c = (char*)a->dtable + v0 * D * dtype_size(a->type); w.ldc = D;
     w.unscale = r.scale;
-    product_store(w, st);
+    product_tn(w, st);
   }
   scatter_rows(acc, D, r.rows, r.count, r.scale, a->dx, a->lddx, n, a->width, a->type, st);
   return m.used;
@@ -270,7 +309,7 @@ int LayerNormGrad(const LayerNormArgs* a, void* stream) {
 }
 
 long GatedMLPWorkspace(const GatedMLPArgs* a) {
-  return sized([&] { check_mlp(a); return mlp_forward(a, nullptr, nullptr); });
+  return sized([&] { check_mlp(a); return mlp_forward(a, true, nullptr); });
 }
 int GatedMLP(const GatedMLPArgs* a, void* stream) {
   return clr::guarded([&] {
@@ -278,13 +317,14 @@ int GatedMLP(const GatedMLPArgs* a, void* stream) {
     check_mlp_tensors(a);
     check_matrix(a->y, a->ldy, a->rows, a->width, "GatedMLP: y");
     require(!a->g == !a->u, "GatedMLP: g and u are kept together");
+    require(((uintptr_t)a->g | (uintptr_t)a->u) % 16 == 0, "GatedMLP: g and u are not aligned to 16 bytes");
     if (!a->rows) return;
-    check_space(a->workspace, a->workspaceBytes, mlp_forward(a, nullptr, nullptr));
-    mlp_forward(a, a->workspace, (hipStream_t)stream);
+    check_space(a->workspace, a->workspaceBytes, mlp_forward(a, true, nullptr));
+    mlp_forward(a, false, (hipStream_t)stream);
   });
 }
 long GatedMLPGradWorkspace(const GatedMLPArgs* a) {
-  return sized([&] { check_mlp(a); return mlp_backward(a, nullptr, nullptr); });
+  return sized([&] { check_mlp(a); return mlp_backward(a, true, nullptr); });
 }
 int GatedMLPGrad(const GatedMLPArgs* a, void* stream) {
   return clr::guarded([&] {
@@ -293,19 +333,20 @@ int GatedMLPGrad(const GatedMLPArgs* a, void* stream) {
     check_matrix(a->dy, a->lddy, a->rows, a->width, "GatedMLPGrad: dy");
     check_matrix(a->dx, a->lddx, a->rows, a->width, "GatedMLPGrad: dx");
     require((a->g && a->u) || !a->rows, "GatedMLPGrad: g and u");
+    require(((uintptr_t)a->g | (uintptr_t)a->u) % 16 == 0, "GatedMLPGrad: g and u are not aligned to 16 bytes");
     require(a->dgate && a->dup && a->ddown, "GatedMLPGrad: the weights' gradients");
     const size_t n = (size_t)a->width * a->hidden * dtype_size(a->type);
     if (!a->rows) {
       for (void* p : {a->dgate, a->dup, a->ddown}) fill_zero(p, n, (hipStream_t)stream);
       return;
     }
-    check_space(a->workspace, a->workspaceBytes, mlp_backward(a, nullptr, nullptr));
-    mlp_backward(a, a->workspace, (hipStream_t)stream);
+    check_space(a->workspace, a->workspaceBytes, mlp_backward(a, true, nullptr));
+    mlp_backward(a, false, (hipStream_t)stream);
   });
 }
 
 long CrossEntropyWorkspace(const CrossEntropyArgs* a) {
-  return sized([&] { check_ce(a); return ce_forward(a, nullptr, nullptr); });
+  return sized([&] { check_ce(a); return ce_forward(a, true, nullptr); });
 }
 int CrossEntropy(const CrossEntropyArgs* a, void* stream) {
   return clr::guarded([&] {
@@ -313,12 +354,12 @@ int CrossEntropy(const CrossEntropyArgs* a, void* stream) {
     check_ce_tensors(a);
     require(a->loss || !a->rows, "CrossEntropy: loss");
     if (!a->rows) return;
-    check_space(a->workspace, a->workspaceBytes, ce_forward(a, nullptr, nullptr));
-    ce_forward(a, a->workspace, (hipStream_t)stream);
+    check_space(a->workspace, a->workspaceBytes, ce_forward(a, true, nullptr));
+    ce_forward(a, false, (hipStream_t)stream);
   });
 }
 long CrossEntropyGradWorkspace(const CrossEntropyArgs* a) {
-  return sized([&] { check_ce(a); return ce_backward(a, nullptr, nullptr); });
+  return sized([&] { check_ce(a); return ce_backward(a, true, nullptr); });
 }
 int CrossEntropyGrad(const CrossEntropyArgs* a, void* stream) {
   return clr::guarded([&] {
@@ -331,8 +372,8 @@ int CrossEntropyGrad(const CrossEntropyArgs* a, void* stream) {
       fill_zero(a->dtable, (size_t)a->vocab * a->width * dtype_size(a->type), (hipStream_t)stream);
       return;
     }
-    check_space(a->workspace, a->workspaceBytes, ce_backward(a, nullptr, nullptr));
-    ce_backward(a, a->workspace, (hipStream_t)stream);
+    check_space(a->workspace, a->workspaceBytes, ce_backward(a, true, nullptr));
+    ce_backward(a, false, (hipStream_t)stream);
   });
 }
 

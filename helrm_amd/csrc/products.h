@@ -6,27 +6,31 @@
 // act(g): silu g/(1 + e^-g), gelu g Phi(g), cubic ((c3 g + c2) g + c1) g + c0
 enum Act { ACT_SILU = 0, ACT_GELU = 1, ACT_CUBIC = 2 };
 
-// C[m][n] = sum over k of A(m, k) B(n, k), for one or two pairs of factors
-// that are added.  A factor's element (row, k) is at row * s + k * t.
-struct Factor { const void* p; long s, t; };
-
+// C[m][n] = sum over k of A(m, k) B(n, k), for up to 12 pairs of factors that
+// are added.  Factors are 16-bit, 16-byte aligned, their rows `ld` elements
+// (a multiple of 8) apart and filled up with zeros to a multiple of 8
+// elements.  Whether a factor's rows run along k or along m (n) goes by the
+// product.
 struct ProductArgs {
-  Factor a[2], b[2];
+  const uint16_t* a[12]; const uint16_t* b[12];
+  const uint16_t* b2[6];     // gate: the up projection's
   int pairs;
+  long lda, ldb;
   int M, N, K;
-  int dtype;                 // of the factors
+  int dtype;                 // of the operator; the factors of a float32 one are its bfloat16 parts
   const int* count;          // on the device, may be null: the rows present, in the place of M
   bool count_k;              // in the place of K
   // store
   void* c; long ldc; int ctype; bool add;  // add: c (float32) += the product
   const float* unscale;      // the product is divided by this, where there is one
   // gate
-  float* g; float* u;        // [M][N] float32, kept for the backward pass; may be null
-  void* h; void* dg; void* du;  // [M][N] in the type of the factors
+  float* g; float* u;        // [M][ldh] float32, kept for the backward pass; may be null
+  void* h; void* dg; void* du;  // [M][ldh], `hpart` elements from one part to the next
+  long ldh, hpart;           // (hpart also of the c of softmax_grad)
   int act; float coef[4];
   // softmax: table rows n0 .. n0 + N
   int n0;
-  const int* target;         // of tile row i; -1: none (its loss is NaN)
+  const int* target;         // of row i of the tiles; -1: none (its loss is NaN)
   float2* part; int parts;   // [M][parts] running maximum and sum of a piece of a row
   float* picked;             // the target's logit
   const int* rows;           // row i of the tiles is row rows[i] of lse and grad
@@ -34,17 +38,23 @@ struct ProductArgs {
   const float* scale;        // the gradient's factor in a 16-bit type
 };
 
-// h = act(A B0^T) * (A B1^T)
+// h = act(A B^T) * (A B2^T); rows of all three run along k
 void product_gate(const ProductArgs& p, hipStream_t st);
-// dh = A B; dg = dh u act'(g), du = dh act(g), h = act(g) u
+// v = A B, A's rows along k, B's along n: dg = v u act'(g), du = v act(g), h = act(g) u
 void product_gate_grad(const ProductArgs& p, hipStream_t st);
-void product_store(const ProductArgs& p, hipStream_t st);
+void product_nt(const ProductArgs& p, hipStream_t st);  // A B^T
+void product_nn(const ProductArgs& p, hipStream_t st);  // A B
+void product_tn(const ProductArgs& p, hipStream_t st);  // A^T B
 // the products of rows of A with rows of the table go into part and picked
 void product_softmax(const ProductArgs& p, hipStream_t st);
-// (exp(A B^T - lse) - onehot(target)) grad into c
+// (exp(A B^T - lse) - onehot(target)) grad into c, in the layout of a factor
 void product_softmax_grad(const ProductArgs& p, hipStream_t st);
 // pieces of a row that product_softmax leaves for a table of N rows
 int softmax_parts(int N);
+
+// A factor in the layout above: row rows[i] (or i) of `from` to row i of `to`, for i < *count (or n); a float32 one
+// as three parts `part` elements apart.
+void lay_out(const void* from, long ld, int dtype, void* to, long ldto, long part, const int* rows, const int* count, long n, int width, hipStream_t st);
 
 // Rows whose target is not `ignore`, in order: rows[], target[] (-1: outside
 // [0, vocab)), *count, and picked[] = NaN; loss and lse (may be null) of the
@@ -57,8 +67,6 @@ struct RowsArgs {
   float* picked; float* loss; float* lse; float* scale;
 };
 void kept_rows(const RowsArgs& a, hipStream_t st);
-// to[i] = from[rows[i]], i < *count
-void gather_rows(const void* from, long ld, void* to, long ldto, const int* rows, const int* count, long n, int width, int dtype, hipStream_t st);
 // loss[row] = lse - picked, lse = the logarithm of the parts' sum
 void softmax_finish(const float2* part, int parts, const float* picked, const int* rows, const int* count, long n, float* loss, float* lse, hipStream_t st);
 // out[row] = acc[i] / *scale, 0 for rows that are not kept

@@ -313,7 +313,8 @@ typedef struct {
   const void* up; long ldup;             /* [hidden][width] */
   const void* down; long lddown;         /* [width][hidden] */
   void* y; long ldy;                     /* [rows][width] */
-  float* g; float* u;                    /* [rows][hidden] each: x gate^T and x up^T, kept for the gradient (both or neither) */
+  float* g; float* u;                    /* x gate^T and x up^T, kept for the gradient (both or neither), 16-byte aligned:
+                                            [rows][hidden rounded up to a multiple of 8] each, the rest of a row 0 */
   const void* dy; long lddy;             /* GatedMLPGrad */
   void* dx; long lddx;
   void* dgate; void* dup; void* ddown;   /* as the weights, contiguous */
