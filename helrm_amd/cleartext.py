@@ -32,6 +32,8 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {"silu": 0, "gelu": 1}
 
 _lib = None
+# the handle of the current stream, without making a Stream object of it (a microsecond of a small call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _library():
@@ -62,10 +64,11 @@ def _refused(lib):
 def _call(name, args, device, sized=True):
     """Queue one entry point on the current stream, with a workspace of the size it asks for."""
     lib = _lib or _library()
-    ref = ctypes.byref(args)
-    if device.index != torch.cuda.current_device():
+    index = device.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return _call(name, args, device, sized)
+    ref = ctypes.byref(args)
     space = None
     if sized:
         need = getattr(lib, name + "Workspace")(ref)
@@ -73,7 +76,7 @@ def _call(name, args, device, sized=True):
             _refused(lib)
         space = torch.empty(need, dtype=torch.uint8, device=device)
         args.workspace, args.workspaceBytes = space.data_ptr(), need
-    if getattr(lib, name)(ref, torch.cuda.current_stream(device).cuda_stream):
+    if getattr(lib, name)(ref, _raw_stream(index)):
         _refused(lib)
 
 
@@ -84,12 +87,19 @@ def _need(ok, what):
 
 def _rows(t, width, name, like=None):
     """[rows, width] of a tensor whose last dimension is the vector, in a layout that the kernels take."""
-    _need(t.dim() >= 1 and t.shape[-1] == width, f"{name}: the last dimension is {list(t.shape)[-1:]}, not {width}")
-    _need(t.dtype in _TYPES, f"{name}: {t.dtype} is not float32, bfloat16 or float16")
-    _need(t.is_cuda, f"{name}: not on the GPU")
-    if like is not None:
-        _need(t.dtype == like.dtype and t.device == like.device, f"{name}: {t.dtype} on {t.device}, not {like.dtype} on {like.device}")
-    if t.dim() != 2:
+    shape = t.shape
+    if not shape or shape[-1] != width:
+        raise ValueError(f"{name}: the last dimension is {list(shape)[-1:]}, not {width}")
+    if like is None:
+        if t.dtype not in _TYPES:
+            raise ValueError(f"{name}: {t.dtype} is not float32, bfloat16 or float16")
+        if not t.is_cuda:
+            raise ValueError(f"{name}: not on the GPU")
+    elif t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name}: {t.dtype} on {t.device}, not {like.dtype} on {like.device}")
+    if len(shape) == 2 and t.is_contiguous():
+        return t
+    if len(shape) != 2:
         t = t.reshape(-1, width)
     if (width > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < width):
         t = t.contiguous()
@@ -101,40 +111,40 @@ def _ld(t):
 
 
 def _vector(t, n, name, dtype, device):
-    _need(tuple(t.shape) == (n,), f"{name}: {list(t.shape)}, not [{n}]")
-    _need(t.dtype == dtype and t.device == device, f"{name}: {t.dtype} on {t.device}, not {dtype} on {device}")
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name}: {list(t.shape)}, not [{n}]")
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name}: {t.dtype} on {t.device}, not {dtype} on {device}")
     return t.contiguous()
 
 
 # ---- layer norm --------------------------------------------------------------------
 
 
-def _norm_args(x, weight, bias, eps):
+def _norm_tensors(x, weight, bias):
     _need(x.dim() >= 1 and x.shape[-1] >= 1, "x: no last dimension")
     width = x.shape[-1]
     x2 = _rows(x, width, "x")
-    _need(weight.dtype == x.dtype or weight.dtype == torch.float32, f"weight: {weight.dtype}, neither {x.dtype} nor float32")
+    if weight.dtype != x.dtype and weight.dtype != torch.float32:
+        raise ValueError(f"weight: {weight.dtype}, neither {x.dtype} nor float32")
     weight = _vector(weight, width, "weight", weight.dtype, x.device)
     if bias is not None:
         bias = _vector(bias, width, "bias", weight.dtype, x.device)
-    a = LayerNormArgs()
-    a.x, a.ldx = x2.data_ptr(), _ld(x2)
-    a.weight, a.bias = weight.data_ptr(), bias.data_ptr() if bias is not None else None
-    a.rows, a.width = x2.shape[0], width
-    a.type, a.paramType = _TYPES[x.dtype], _TYPES[weight.dtype]
-    a.eps = eps
-    return a, x2, weight, bias
+    return x2, weight, bias
 
 
 def _norm_forward(x, weight, bias, eps, keep):
-    a, x2, weight, bias = _norm_args(x, weight, bias, eps)
+    x2, weight, bias = _norm_tensors(x, weight, bias)
+    rows, width = x2.shape
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a.y, a.ldy = y.data_ptr(), a.width
     mean = rstd = None
     if keep:
-        mean, rstd = torch.empty((2, a.rows), dtype=torch.float32, device=x.device)
-        a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
-    _call("LayerNorm", a, x.device, sized=False)
+        mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+        rstd = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _call("LayerNorm", LayerNormArgs(
+        x=x2.data_ptr(), ldx=_ld(x2), weight=weight.data_ptr(), bias=None if bias is None else bias.data_ptr(),
+        y=y.data_ptr(), ldy=width, mean=mean.data_ptr() if keep else None, rstd=rstd.data_ptr() if keep else None,
+        rows=rows, width=width, type=_TYPES[x.dtype], paramType=_TYPES[weight.dtype], eps=eps), x.device, sized=False)
     return y, mean, rstd
 
 
@@ -145,19 +155,21 @@ def layer_norm_forward(x, weight, bias=None, eps=1e-5):
 
 def layer_norm_backward(grad, x, weight, mean, rstd, has_bias=True):
     """(dx, dweight, dbias) of the norm; dbias is None without a bias."""
-    a, x2, weight, _ = _norm_args(x, weight, None, 0.0)
-    g2 = _rows(grad, a.width, "grad", x)
-    _need(g2.shape[0] == a.rows, f"grad: {g2.shape[0]} rows, not {a.rows}")
-    mean = _vector(mean, a.rows, "mean", torch.float32, x.device)
-    rstd = _vector(rstd, a.rows, "rstd", torch.float32, x.device)
+    x2, weight, _ = _norm_tensors(x, weight, None)
+    rows, width = x2.shape
+    g2 = _rows(grad, width, "grad", x)
+    if g2.shape[0] != rows:
+        raise ValueError(f"grad: {g2.shape[0]} rows, not {rows}")
+    mean = _vector(mean, rows, "mean", torch.float32, x.device)
+    rstd = _vector(rstd, rows, "rstd", torch.float32, x.device)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dweight = torch.empty_like(weight)
     dbias = torch.empty_like(weight) if has_bias else None
-    a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
-    a.dy, a.lddy = g2.data_ptr(), _ld(g2)
-    a.dx, a.lddx = dx.data_ptr(), a.width
-    a.dweight, a.dbias = dweight.data_ptr(), dbias.data_ptr() if has_bias else None
-    _call("LayerNormGrad", a, x.device)
+    _call("LayerNormGrad", LayerNormArgs(
+        x=x2.data_ptr(), ldx=_ld(x2), weight=weight.data_ptr(), mean=mean.data_ptr(), rstd=rstd.data_ptr(),
+        dy=g2.data_ptr(), lddy=_ld(g2), dx=dx.data_ptr(), lddx=width,
+        dweight=dweight.data_ptr(), dbias=dbias.data_ptr() if has_bias else None,
+        rows=rows, width=width, type=_TYPES[x.dtype], paramType=_TYPES[weight.dtype]), x.device)
     return dx, dweight, dbias
 
 

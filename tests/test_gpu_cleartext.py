@@ -546,10 +546,10 @@ def test_workspace_refusals(ct):
     from helrm_amd.backend import LayerNormArgs
     gen = seeded(1)
     x, w = normal(gen, 4, 8), normal(gen, 8)
-    a, x2, _, _ = ct._norm_args(x, w, None, 1e-5)
     mean, rstd = torch.zeros(2, 4, device=DEV)
     dx, dw = torch.empty_like(x), torch.empty_like(w)
-    a.mean, a.rstd, a.dy, a.lddy, a.dx, a.lddx, a.dweight = mean.data_ptr(), rstd.data_ptr(), x.data_ptr(), 8, dx.data_ptr(), 8, dw.data_ptr()
+    a = LayerNormArgs(x=x.data_ptr(), ldx=8, weight=w.data_ptr(), mean=mean.data_ptr(), rstd=rstd.data_ptr(), dy=x.data_ptr(), lddy=8,
+                      dx=dx.data_ptr(), lddx=8, dweight=dw.data_ptr(), rows=4, width=8)
     with pytest.raises(HipError, match="workspace too small"):
         ct._call("LayerNormGrad", a, x.device, sized=False)
     space = torch.empty(1 << 20, dtype=torch.uint8, device=DEV)
