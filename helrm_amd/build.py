@@ -26,6 +26,8 @@ FLAGS = [
     # float64 encoder/decoder arithmetic must not be contracted into FMAs
     "-ffp-contract=off",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+    # matrix instructions on ordinary registers: with accumulation registers the compiler moves the sums to and fro
+    "-mllvm", "-amdgpu-mfma-vgpr-form",
 ]
 
 

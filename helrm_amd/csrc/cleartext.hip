@@ -114,6 +114,9 @@ int add_pairs(ProductArgs& p, const Held& a, const Held& b, const Held* b2 = nul
   return p.pairs;
 }
 
+// The scratch of the largest of an operator's products, which use it in turn.
+float* scratch(Arena& m, std::initializer_list<size_t> sizes) { return m.take<float>(std::max(sizes) / sizeof(float)); }
+
 size_t mlp_forward(const GatedMLPArgs* a, bool count, hipStream_t st) {
   Arena m{count ? nullptr : (char*)a->workspace};
   const int type = a->type;
@@ -123,6 +126,8 @@ size_t mlp_forward(const GatedMLPArgs* a, bool count, hipStream_t st) {
   const Held gate = held(m, a->gate, a->ldgate, a->hidden, a->width, type, st, same && fits(a->up, a->ldup, a->hidden, a->width, type));
   const Held up = held(m, a->up, a->ldup, a->hidden, a->width, type, st, same && fits(a->gate, a->ldgate, a->hidden, a->width, type));
   const Held down = held(m, a->down, a->lddown, a->width, a->hidden, type, st);
+  const int parts = type == DT_F32 ? 6 : 1;
+  float* partial = scratch(m, {product_scratch(a->rows, a->width, a->hidden, parts)});
   if (count) return m.used;
   ProductArgs p{};
   p.dtype = type;
@@ -135,6 +140,7 @@ size_t mlp_forward(const GatedMLPArgs* a, bool count, hipStream_t st) {
   q.dtype = q.ctype = type;
   q.M = (int)a->rows; q.N = a->width; q.K = a->hidden;
   add_pairs(q, h, down);
+  q.partial = partial;
   q.c = a->y; q.ldc = a->ldy;
   product_nt(q, st);
   return m.used;
@@ -149,6 +155,9 @@ size_t mlp_backward(const GatedMLPArgs* a, bool count, hipStream_t st) {
   const Held gate = held(m, a->gate, a->ldgate, a->hidden, a->width, type, st, same && fits(a->up, a->ldup, a->hidden, a->width, type));
   const Held up = held(m, a->up, a->ldup, a->hidden, a->width, type, st, same && fits(a->gate, a->ldgate, a->hidden, a->width, type));
   const Held down = held(m, a->down, a->lddown, a->width, a->hidden, type, st);
+  const int parts = type == DT_F32 ? 6 : 1;
+  float* partial = scratch(m, {product_scratch(a->rows, a->width, a->hidden, 2 * parts), product_scratch(a->hidden, a->width, a->rows, parts),
+                               product_scratch(a->width, a->hidden, a->rows, parts)});
   if (count) return m.used;
   // dh = dy down, and through the product and the activation
   ProductArgs p{};
@@ -164,6 +173,7 @@ size_t mlp_backward(const GatedMLPArgs* a, bool count, hipStream_t st) {
   q.M = (int)a->rows; q.N = a->width; q.K = a->hidden;
   add_pairs(q, dg, gate);
   add_pairs(q, du, up);
+  q.partial = partial;
   q.c = a->dx; q.ldc = a->lddx;
   product_nn(q, st);
   // the weights' gradients: sums over the rows
@@ -172,6 +182,7 @@ size_t mlp_backward(const GatedMLPArgs* a, bool count, hipStream_t st) {
     w.dtype = w.ctype = type;
     w.M = (int)rows; w.N = (int)cols; w.K = (int)a->rows;
     add_pairs(w, l, r);
+    w.partial = partial;
     w.c = out; w.ldc = cols;
     product_tn(w, st);
   };
@@ -234,8 +245,12 @@ size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
   r.rows = m.take<int>(n); r.tgt = m.take<int>(n); r.count = m.take<int>(1);
   float* scale = m.take<float>(1);
   if (a->type == DT_F16) r.scale = scale;
+  r.lse = a->lse; r.lse_kept = m.take<float>(n); r.grad_kept = m.take<float>(n);
   const Held x = hold(m, n, a->width, a->type), dl = hold(m, n, piece, a->type);
   float* acc = m.take<float>((size_t)n * D);
+  const int parts = a->type == DT_F32 ? 6 : 1, last = a->vocab % piece ? a->vocab % piece : piece;
+  float* partial = scratch(m, {product_scratch(n, D, piece, parts), product_scratch(n, D, last, parts), product_scratch(piece, D, n, parts),
+                               product_scratch(last, D, n, parts)});
   const Held table = held(m, a->table, a->ldtable, a->vocab, a->width, a->type, st);
   if (count) return m.used;
   kept_rows(r, st);
@@ -248,18 +263,20 @@ size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
     p.M = (int)n; p.N = len; p.K = a->width;
     add_pairs(p, x, rows);
     p.c = (void*)dl.p; p.ldc = dl.ld; p.hpart = dl.part;
-    p.n0 = (int)v0; p.target = r.tgt; p.rows = r.rows; p.lse = a->lse; p.grad = a->dloss; p.scale = r.scale;
+    p.n0 = (int)v0; p.target = r.tgt; p.lse = r.lse_kept; p.grad = r.grad_kept; p.scale = r.scale;
     product_softmax_grad(p, st);
     ProductArgs q{};
     q.dtype = a->type; q.ctype = DT_F32; q.count = r.count;
     q.M = (int)n; q.N = a->width; q.K = len;
     add_pairs(q, dl, rows);
+    q.partial = partial;
     q.c = acc; q.ldc = D; q.add = v0 > 0;
     product_nn(q, st);
     ProductArgs w{};
     w.dtype = w.ctype = a->type; w.count = r.count; w.count_k = true;
     w.M = len; w.N = a->width; w.K = (int)n;
     add_pairs(w, dl, x);
+    w.partial = partial;
     w.c = (char*)a->dtable + v0 * D * dtype_size(a->type); w.ldc = D;
     w.unscale = r.scale;
     product_tn(w, st);

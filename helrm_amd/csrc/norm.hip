@@ -210,6 +210,7 @@ __global__ __launch_bounds__(SUM_COLS* SUM_ROWS) void norm_param_sum(const float
   if (!out) return;
   float s = 0;
   if (i < width)
+#pragma unroll 8
     for (int k = r; k < parts; k += SUM_ROWS) s += part[((long)k * 2 + blockIdx.y) * width + i];
   lds[r][c] = s;
   __syncthreads();

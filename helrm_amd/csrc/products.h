@@ -21,6 +21,8 @@ struct ProductArgs {
   const int* count;          // on the device, may be null: the rows present, in the place of M
   bool count_k;              // in the place of K
   // store
+  float* partial;            // product_scratch bytes
+  int splits;                // (of the launch)
   void* c; long ldc; int ctype; bool add;  // add: c (float32) += the product
   const float* unscale;      // the product is divided by this, where there is one
   // gate
@@ -33,8 +35,7 @@ struct ProductArgs {
   const int* target;         // of row i of the tiles; -1: none (its loss is NaN)
   float2* part; int parts;   // [M][parts] running maximum and sum of a piece of a row
   float* picked;             // the target's logit
-  const int* rows;           // row i of the tiles is row rows[i] of lse and grad
-  const float* lse; const float* grad;
+  const float* lse; const float* grad;  // of row i of the tiles
   const float* scale;        // the gradient's factor in a 16-bit type
 };
 
@@ -42,6 +43,8 @@ struct ProductArgs {
 void product_gate(const ProductArgs& p, hipStream_t st);
 // v = A B, A's rows along k, B's along n: dg = v u act'(g), du = v act(g), h = act(g) u
 void product_gate_grad(const ProductArgs& p, hipStream_t st);
+// Bytes that the next three need of a product's shape at `partial`.
+size_t product_scratch(long M, long N, long K, int pairs);
 void product_nt(const ProductArgs& p, hipStream_t st);  // A B^T
 void product_nn(const ProductArgs& p, hipStream_t st);  // A B
 void product_tn(const ProductArgs& p, hipStream_t st);  // A^T B
@@ -56,15 +59,15 @@ int softmax_parts(int N);
 // as three parts `part` elements apart.
 void lay_out(const void* from, long ld, int dtype, void* to, long ldto, long part, const int* rows, const int* count, long n, int width, hipStream_t st);
 
-// Rows whose target is not `ignore`, in order: rows[], target[] (-1: outside
-// [0, vocab)), *count, and picked[] = NaN; loss and lse (may be null) of the
-// others are 0.  scale (may be null): the power of two that brings the
-// largest |grad| of these rows near 2^14.
+// Rows whose target is not `ignore`, in order: rows[], tgt[] (-1: outside [0,
+// vocab)), *count.  Forward (loss): picked[] = NaN, and loss and lse of the
+// others are 0.  Backward (lse_kept): their lse and grad, and in scale (may be
+// null) the power of two that brings the largest |grad| near 2^14.
 struct RowsArgs {
   const long long* target; const float* grad;
   long n; long long ignore; int vocab;
   int* rows; int* tgt; int* count;
-  float* picked; float* loss; float* lse; float* scale;
+  float* picked; float* loss; float* lse; float* lse_kept; float* grad_kept; float* scale;
 };
 void kept_rows(const RowsArgs& a, hipStream_t st);
 // loss[row] = lse - picked, lse = the logarithm of the parts' sum

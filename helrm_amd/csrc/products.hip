@@ -8,9 +8,11 @@
 //
 // A workgroup has a BM x BN tile of C, k advances by 64.  Both factors' tiles
 // go from memory to LDS directly (16 bytes a lane, no registers), into one of
-// two buffers while the other is multiplied; one barrier a step.  Elements
-// outside a factor are read as 0 through the bounds of its buffer
-// descriptor, so no tile has a special case.
+// two or four buffers while others are multiplied; one barrier a step.
+// Elements outside a factor are read as 0 through the bounds of its buffer
+// descriptor, so no tile has a special case.  Products whose tiles would
+// leave CUs idle are split along k into float32 sums that a second kernel adds
+// in order.
 //
 // LDS layout.  A factor whose rows run along k is held as [row][64 k], its
 // 16-byte chunk c of row r at chunk c ^ (r & 7): the 16 rows that a wave reads
@@ -122,6 +124,22 @@ __device__ __forceinline__ void get4(const float* c, float v[4]) {
   v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
 }
 
+// Four neighbouring columns of a product.
+template <class T> __device__ __forceinline__ void store4(const ProductArgs& p, long m, long n, float v[4]) {
+  const int left = (int)(p.N - n);
+  if (p.add) {
+    const float* c = (const float*)p.c + m * p.ldc + n;
+#pragma unroll
+    for (int e = 0; e < 4; e++) if (e < left) v[e] += c[e];
+  }
+  if (p.unscale) {
+    const float factor = 1.0f / *p.unscale;   // a power of two
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] *= factor;
+  }
+  put_out<T>(p.c, p.ctype, m * p.ldc + n, v, left);
+}
+
 // One factor's loads of a step.  ALONG_K: its rows run along k.  R rows of the
 // tile, W waves; every wave issues R / 8 / W loads of 1 KiB.
 template <bool ALONG_K, int R, int W> struct Loader {
@@ -150,10 +168,10 @@ template <bool ALONG_K, int R, int W> struct Loader {
     }
   }
   // `left`: k that the factor still has from here on
-  template <int J> __device__ __forceinline__ void one(const u16* p, int left, u16* lds, int wave) const {
+  __device__ __forceinline__ void one(int j, const u16* p, int left, u16* lds, int wave) const {
     __amdgpu_buffer_rsrc_t d = __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0x7fffffff, 0x00027000);
-    const unsigned o = kk + (ALONG_K ? 0 : J * PER) < left ? off[J] : OUTSIDE;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (__attribute__((address_space(3))) void*)(lds + (wave * N + J) * 512), 16, o, 0, 0, 0);
+    const unsigned o = kk + (ALONG_K ? 0 : j * PER) < left ? off[j] : OUTSIDE;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (__attribute__((address_space(3))) void*)(lds + (wave * N + j) * 512), 16, o, 0, 0, 0);
   }
 };
 
@@ -196,141 +214,169 @@ __device__ __forceinline__ void tile_of(int id, int total, int nm, int nn, int& 
   n = in / rows;
 }
 
-// The wave's accumulators, and what becomes of them.  acc[i][j][e] is
-// (m, n) = (mw + 16 i + lane % 16, nw + 16 j + 4 (lane / 16) + e).
-template <class T, int EPI, int FM, int FN, int WAVES_N>
-__device__ __forceinline__ void finish(const ProductArgs& p, f32x4 (&acc)[FM][FN], long M, long mw, long nw, int lane, int wave_n, int wave_m, int tile_n,
-                                       float2* lds) {
-  const int quad = lane >> 4;
-  if (EPI == EPI_SOFTMAX) {
-    // a row's maximum and sum over the tile's columns: over the lane's, over the four lanes that share the row, over
-    // the waves beside one another
-#pragma unroll
-    for (int i = 0; i < FM; i++) {
-      const long m = mw + 16 * i + (lane & 15);
-      const int t = m < M ? p.target[m] : -1;
-      float top = -INFINITY;
-      bool nan = false;
-#pragma unroll
-      for (int j = 0; j < FN; j++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const long n = nw + 16 * j + 4 * quad + e;
-          const float v = acc[i][j][e];
-          if (n < p.N) { top = fmaxf(top, v); nan |= v != v; }
-          if (n < p.N && n == t) p.picked[m] = v;
-        }
-      if (nan) top = NAN;
-      float sum = 0;
-#pragma unroll
-      for (int j = 0; j < FN; j++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (nw + 16 * j + 4 * quad + e < p.N) sum += top == -INFINITY ? 1.0f : __expf(acc[i][j][e] - top);
-      float2 run = make_float2(top, sum);
-#pragma unroll
-      for (int o = 16; o < 64; o <<= 1) run = join(run, make_float2(__shfl_xor(run.x, o), __shfl_xor(run.y, o)));
-      if (lane < 16) lds[((wave_m * FM + i) * 16 + lane) * WAVES_N + wave_n] = run;
-    }
-    __syncthreads();
-    const int rows = blockDim.x / 64 / WAVES_N * FM * 16;
-    for (int r = threadIdx.x; r < rows; r += blockDim.x) {
-      const long m = mw - wave_m * FM * 16 + r;
-      if (m >= M) break;
-      float2 run = lds[r * WAVES_N];
-#pragma unroll
-      for (int k = 1; k < WAVES_N; k++) run = join(run, lds[r * WAVES_N + k]);
-      p.part[m * p.parts + tile_n] = run;
-    }
-    return;
-  }
+// A row's maximum and sum over the tile's columns: over the lane's, over the
+// four lanes that share the row, over the waves beside one another.  acc[i][j][e]
+// is (m, n) = (mw + 16 i + lane % 16, nw + 16 j + 4 (lane / 16) + e).
+template <int FM, int FN, int WAVES_M, int WAVES_N>
+__device__ __forceinline__ void softmax_piece(const ProductArgs& p, const f32x4 (&acc)[FM][FN], int M, long m0, long n0, int wave_m, int wave_n, int tile_n,
+                                              float2* lds) {
+  const int lane = threadIdx.x & 63, quad = lane >> 4;
+  const int left = (int)min((long)p.N - n0 - wave_n * FN * 16, 1L << 20) - 4 * quad;   // columns from the lane's first one on
 #pragma unroll
   for (int i = 0; i < FM; i++) {
-    const long m = mw + 16 * i + (lane & 15);
-    if (m >= M) continue;
-    if (EPI == EPI_GATE) {
+    const int r = (wave_m * FM + i) * 16 + (lane & 15);
+    const long m = m0 + r;
+    const int t = m < M ? p.target[m] - (int)(n0 + wave_n * FN * 16 + 4 * quad) : -1;   // the target's place from there
+    float top = -INFINITY, picked = 0;
+    bool nan = false, hit = false;
 #pragma unroll
-      for (int j = 0; j < FN; j += 2) {
-        const long n = nw + 8 * j + 4 * quad;
-        if (n >= p.ldh) continue;
-        float g[4], u[4], h[4], d[4];
+    for (int j = 0; j < FN; j++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {   // the columns that fill a row up are 0
-          const bool in = n + e < p.N;
-          g[e] = in ? acc[i][j][e] : 0.0f;
-          u[e] = in ? acc[i][j + 1][e] : 0.0f;
-        }
-        act4(p.act, p.coef, g, h, d);
-#pragma unroll
-        for (int e = 0; e < 4; e++) h[e] *= u[e];
-        const long at = m * p.ldh + n;
-        if (p.g) { *(float4*)(p.g + at) = make_float4(g[0], g[1], g[2], g[3]); *(float4*)(p.u + at) = make_float4(u[0], u[1], u[2], u[3]); }
-        put_held<T>(p.h, p.dtype, p.hpart, at, h);
+      for (int e = 0; e < 4; e++) {
+        const float v = acc[i][j][e];
+        const int c = 16 * j + e;
+        if (c < left) { top = fmaxf(top, v); nan |= v != v; }
+        if (c == t) { picked = v; hit = true; }
       }
-      continue;
+    if (nan) top = NAN;
+    float sum = 0;
+#pragma unroll
+    for (int j = 0; j < FN; j++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (16 * j + e < left) sum += top == -INFINITY ? 1.0f : __expf(acc[i][j][e] - top);
+    float2 run = make_float2(top, sum);
+#pragma unroll
+    for (int o = 16; o < 64; o <<= 1) run = join(run, make_float2(__shfl_xor(run.x, o), __shfl_xor(run.y, o)));
+    if (hit && m < M) p.picked[m] = picked;
+    if (lane < 16) lds[r * WAVES_N + wave_n] = run;
+  }
+  __syncthreads();
+  for (int r = threadIdx.x; r < WAVES_M * FM * 16 && m0 + r < M; r += WAVES_M * WAVES_N * 64) {
+    float2 run = lds[r * WAVES_N];
+#pragma unroll
+    for (int k = 1; k < WAVES_N; k++) run = join(run, lds[r * WAVES_N + k]);
+    p.part[(m0 + r) * p.parts + tile_n] = run;
+  }
+}
+
+// What becomes of four neighbouring columns of a row (gate: v of the gate, u of the up projection).
+template <class T, int EPI> __device__ __forceinline__ void emit4(const ProductArgs& p, int split, float scale, long m, long n, float v[4], float u[4]) {
+  if (EPI == EPI_STORE) {
+    if (n >= p.N) return;
+    if (p.splits > 1) *(float4*)(p.partial + ((long)split * p.M + m) * ((p.N + 3) & ~3) + n) = make_float4(v[0], v[1], v[2], v[3]);
+    else store4<T>(p, m, n, v);
+    return;
+  }
+  const int left = (int)min((long)p.N - n, 4L);   // the columns that fill a row up are 0
+  if (EPI == EPI_GATE) {
+    if (n >= p.ldh) return;
+    float h[4], d[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) if (e >= left) v[e] = u[e] = 0.0f;
+    act4(p.act, p.coef, v, h, d);
+#pragma unroll
+    for (int e = 0; e < 4; e++) h[e] *= u[e];
+    const long at = m * p.ldh + n;
+    if (p.g) { *(float4*)(p.g + at) = make_float4(v[0], v[1], v[2], v[3]); *(float4*)(p.u + at) = make_float4(u[0], u[1], u[2], u[3]); }
+    put_held<T>(p.h, p.dtype, p.hpart, at, h);
+  } else if (EPI == EPI_GATE_GRAD) {
+    if (n >= p.ldh) return;
+    const long at = m * p.ldh + n;
+    float g[4], a[4], d[4];
+    get4(p.g + at, g);
+    get4(p.u + at, u);
+    act4(p.act, p.coef, g, a, d);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (e >= left) v[e] = 0.0f;   // (g and u are 0 there)
+      d[e] *= v[e] * u[e];
+      v[e] *= a[e];
+      a[e] *= u[e];
     }
-    const int row = EPI == EPI_SOFTMAX_GRAD ? p.rows[m] : 0, t = EPI == EPI_SOFTMAX_GRAD ? p.target[m] : 0;
-    const float lse = EPI == EPI_SOFTMAX_GRAD ? p.lse[row] : 0.0f;
-    const float grad = EPI == EPI_SOFTMAX_GRAD ? p.grad[row] * (p.scale ? *p.scale : 1.0f) : 0.0f;
-    const float factor = EPI == EPI_STORE && p.unscale ? 1.0f / *p.unscale : 1.0f;
+    put_held<T>(p.dg, p.dtype, p.hpart, at, d);
+    put_held<T>(p.du, p.dtype, p.hpart, at, v);
+    put_held<T>(p.h, p.dtype, p.hpart, at, a);
+  } else {
+    if (n >= ((p.N + 7) & ~7)) return;   // the row is filled up to a multiple of 8
+    const int target = p.target[m], t = target - (int)(p.n0 + n);
+    const float lse = p.lse[m], grad = target < 0 ? NAN : p.grad[m] * scale;
 #pragma unroll
-    for (int j = 0; j < FN; j++) {
-      const long n = nw + 16 * j + 4 * quad;
-      const int left = (int)(p.N - n);
-      float v[4];
+    for (int e = 0; e < 4; e++) v[e] = e < left ? (__expf(v[e] - lse) - (t == e ? 1.0f : 0.0f)) * grad : 0.0f;
+    put_held<T>(p.c, p.dtype, p.hpart, m * p.ldc + n, v);
+  }
+}
+
+// A wave's accumulators go through its own part of LDS, 64 rows of 64 float32
+// columns at a time (16 bytes c of row r at c ^ (r & 15)), so that what is
+// stored are whole lines of a row and the code of it is there once.
+template <class T, int EPI, int FM, int FN>
+__device__ __forceinline__ void emit(const ProductArgs& p, const f32x4 (&acc)[FM][FN], int M, long mw, long nw, int split, float* lds) {
+  static_assert(FN == 4 && FM % 4 == 0, "64 x 64 a time");
+  constexpr int LANES = EPI == EPI_GATE ? 8 : 16, ROWS = 64 / LANES;   // of a row; rows a time
+  const int lane = threadIdx.x & 63, col = lane % LANES;
+  const float scale = EPI == EPI_SOFTMAX_GRAD && p.scale ? *p.scale : 1.0f;
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = acc[i][j][e];
-      if (EPI == EPI_STORE) {
-        if (left <= 0) continue;
-        if (p.add) {
-          const float* c = (const float*)p.c + m * p.ldc + n;
+  for (int part = 0; part < FM / 4; part++) {
 #pragma unroll
-          for (int e = 0; e < 4; e++) if (e < left) v[e] += c[e];
-        }
+    for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] *= factor;
-        put_out<T>(p.c, p.ctype, m * p.ldc + n, v, left);
-      } else if (EPI == EPI_GATE_GRAD) {
-        if (n >= p.ldh) continue;
-        const long at = m * p.ldh + n;
-        float g[4], u[4], a[4], d[4];
-        get4(p.g + at, g);
-        get4(p.u + at, u);
-        act4(p.act, p.coef, g, a, d);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          if (e >= left) v[e] = 0.0f;   // with g and u of 0, the columns that fill a row up are 0
-          d[e] *= v[e] * u[e];
-          v[e] *= a[e];
-          a[e] *= u[e];
-        }
-        put_held<T>(p.dg, p.dtype, p.hpart, at, d);
-        put_held<T>(p.du, p.dtype, p.hpart, at, v);
-        put_held<T>(p.h, p.dtype, p.hpart, at, a);
-      } else if (EPI == EPI_SOFTMAX_GRAD) {
-        if (n >= ((p.N + 7) & ~7)) continue;   // the row is filled up with zeros to a multiple of 8
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          float d = __expf(v[e] - lse);
-          if (t == p.n0 + n + e) d -= 1.0f;
-          if (t < 0) d = NAN;
-          v[e] = e < left ? d * grad : 0.0f;
-        }
-        put_held<T>(p.c, p.dtype, p.hpart, m * p.ldc + n, v);
+      for (int j = 0; j < 4; j++) {
+        const int r = i * 16 + (lane & 15), c = j * 4 + (lane >> 4);
+        *(f32x4*)(lds + r * 64 + ((c ^ (r & 15)) * 4)) = acc[part * 4 + i][j];
       }
+#pragma unroll 4
+    for (int r0 = 0; r0 < 64; r0 += ROWS) {
+      const int r = r0 + lane / LANES;
+      const long m = mw + part * 64 + r;
+      // gate: the columns are 16 of the gate, the same 16 of the up projection, 16 of the gate, ...
+      const int c = EPI == EPI_GATE ? (col >> 2) * 8 + (col & 3) : col;
+      float v[4], u[4] = {0, 0, 0, 0};
+      get4(lds + r * 64 + ((c ^ (r & 15)) * 4), v);
+      if (EPI == EPI_GATE) get4(lds + r * 64 + (((c + 4) ^ (r & 15)) * 4), u);
+      if (m < M) emit4<T, EPI>(p, split, scale, m, nw + col * 4, v, u);
     }
   }
 }
 
-template <class T, int BM, int BN, int WM, int WN, bool A_K, bool B_K, int EPI>
+// Waits until the wave's LDS reads are done, and all but its newest `LEFT`
+// loads have arrived, then for the other waves.
+__device__ __forceinline__ void everybody() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void arrive() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
+
+// Tells the compiler to issue LDS reads one by one between matrix
+// instructions, over the first three quarters of them, and to keep both here:
+// left to itself it bunches the reads before the barrier that waits for them.
+template <int READS, int MULS> __device__ __forceinline__ void spread() {
+  constexpr int OVER = MULS * 3 / 4;
+  if constexpr (READS > 0) {
+#pragma unroll
+    for (int i = 0; i < READS; i++) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+#pragma unroll
+      for (int m = i * OVER / READS; m < (i + 1) * OVER / READS; m++) __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, MULS - OVER, 0);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+template <class T, int BM, int BN, int WM, int WN, int STAGES, bool A_K, bool B_K, int EPI>
 __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const ProductArgs p) {
   constexpr int W = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr int COLS = EPI == EPI_GATE ? BN / 2 : BN;   // columns of C in a tile
+  // Arrays of their own, not one: only so does the compiler see that a load into one does not concern reads of another.
+  constexpr int MORE = STAGES > 2 ? STEP : 0;
   __shared__ __align__(1024) u16 a0[BM * STEP], b0[BN * STEP], a1[BM * STEP], b1[BN * STEP];
+  __shared__ __align__(1024) u16 a2[BM * MORE + 8], b2[BN * MORE + 8], a3[BM * MORE + 8], b3[BN * MORE + 8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave_m = wave / WN, wave_n = wave % WN;
+  const int nm = (p.M + BM - 1) / BM, nn = (p.N + COLS - 1) / COLS;
+  const int split = blockIdx.x / (nm * nn);
   int tile_m, tile_n;
-  tile_of(blockIdx.x, gridDim.x, (int)((p.M + BM - 1) / BM), (int)((p.N + COLS - 1) / COLS), tile_m, tile_n);
+  tile_of(blockIdx.x - split * nm * nn, nm * nn, nm, nn, tile_m, tile_n);
   const long m0 = (long)tile_m * BM, n0 = (long)tile_n * COLS;
   int M = p.M, K = p.K;
   if (p.count) { if (p.count_k) K = *p.count; else M = *p.count; }
@@ -338,6 +384,8 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const ProductArgs 
   // a row along k is filled up with zeros to a multiple of 8
   const int KA = A_K ? (K + 7) & ~7 : K, KB = B_K ? (K + 7) & ~7 : K;
 
+  constexpr int LA = Loader<A_K, BM, W>::N, LB = Loader<B_K, BN, W>::N;
+  static_assert(LA == 4 && LB == 4 && (STAGES == 2 || STAGES == 4), "the steps below");
   Loader<A_K, BM, W> la;
   Loader<B_K, BN, W> lb;
   Reader<T, A_K, BM> ra;
@@ -351,77 +399,198 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const ProductArgs 
   ra.init(wave_m * FM * 16, lane);
   rb.init(wave_n * FN * 16, lane);
 
-  const int steps_of = (K + STEP - 1) / STEP, steps = steps_of * p.pairs;
-  int pair = 0, k = 0;   // of the next load
+  const int steps_of = (K + STEP - 1) / STEP;
+  const int from = (int)((long)steps_of * p.pairs * split / p.splits), to = (int)((long)steps_of * p.pairs * (split + 1) / p.splits);
+  // The place of the loads.  Without a step left every address is outside: nothing is read, the load only counts.
   const long arow = A_K ? m0 * p.lda : m0, brow = B_K ? n0 * p.ldb : n0;
-  auto load = [&](u16* a, u16* b) {
-    const u16* pa = p.a[pair] + arow + (A_K ? k : k * p.lda);
-    const u16* pb = p.b[pair] + brow + (B_K ? k : k * p.ldb);
-    const int left_a = KA - k, left_b = KB - k;
-    la.template one<0>(pa, left_a, a, wave);
-    la.template one<1>(pa, left_a, a, wave);
-    la.template one<2>(pa, left_a, a, wave);
-    la.template one<3>(pa, left_a, a, wave);
-    const u16* pu = EPI == EPI_GATE ? p.b2[pair] + brow + k : pb;
-    lb.template one<0>(pb, left_b, b, wave);
-    lb.template one<1>(pb, left_b, b, wave);
-    lb.template one<2>(pu, left_b, b, wave);
-    lb.template one<3>(pu, left_b, b, wave);
+  int pair = steps_of ? from / steps_of : 0, k = (from - pair * steps_of) * STEP, left = to - from;
+  const u16 *pa = p.a[0], *pb = p.b[0], *pu = pb;
+  auto seek = [&] {
+    pa = p.a[pair] + arow + (A_K ? k : k * p.lda);
+    pb = p.b[pair] + brow + (B_K ? k : k * p.ldb);
+    if (EPI == EPI_GATE) pu = p.b2[pair] + brow + k;
+  };
+  if (left > 0) seek();
+  auto load_a = [&](u16* a, int j) { la.one(j, pa, left > 0 ? KA - k : 0, a, wave); };
+  // (the tile's rows by 16: gate, up, gate, ...)
+  auto load_b = [&](u16* b, int j) { lb.one(j, EPI == EPI_GATE && (j >> 1 & 1) ? pu : pb, left > 0 ? KB - k : 0, b, wave); };
+  auto next = [&] {
+    left--;
     k += STEP;
-    if (k >= K) { k = 0; pair++; }
+    pa += A_K ? STEP : STEP * p.lda;
+    pb += B_K ? STEP : STEP * p.ldb;
+    pu += STEP;
+    if (k >= K && left > 0) { k = 0; pair++; seek(); }
   };
-  static_assert(Loader<A_K, BM, W>::N == 4 && Loader<B_K, BN, W>::N == 4, "four loads a wave and factor");
 
+  // Quarter q of a step multiplies the fragments of A rows' half q / 2 and of k's half q & 1, while those of the next
+  // quarter are read; B's fragments of both halves of k stay.
+  constexpr int HALF = FM / 2;
   f32x4 acc[FM][FN] = {};
-  auto multiply = [&](const u16* a, const u16* b) {
-    // the addresses of the fragments are computed anew in every step: kept, they would not fit in the registers
-    asm volatile("" : "+v"(ra.flip), "+v"(rb.flip));
+  typename Vec8<T>::type fa[2][HALF], fb[2][FN];
+  auto read_b = [&](const u16* b, int q) {
+    // the addresses of the fragments are computed anew: kept, they would not fit in the registers
+    asm volatile("" : "+v"(rb.flip));
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
-      typename Vec8<T>::type fa[FM], fb[FN];
-#pragma unroll
-      for (int j = 0; j < FN; j++) fb[j] = rb.get(b, j, s);
-#pragma unroll
-      for (int i = 0; i < FM; i++) fa[i] = ra.get(a, i, s);
-#pragma unroll
-      for (int i = 0; i < FM; i++)
-#pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = mfma(fb[j], fa[i], acc[i][j]);
-    }
+    for (int j = 0; j < FN; j++) fb[q & 1][j] = rb.get(b, j, q & 1);
   };
-  // One step is multiplied while the next one arrives.  The barrier says both that a buffer has arrived and that
-  // nobody reads the other one any more.  An odd step comes first, then the two buffers take turns.
-  if (steps & 1) {
-    load(a1, b1);
-    __syncthreads();
-    if (steps > 1) load(a0, b0);
-    multiply(a1, b1);
-  } else if (steps) {
-    load(a0, b0);
+  auto read_a = [&](const u16* a, int q) {
+    asm volatile("" : "+v"(ra.flip));
+#pragma unroll
+    for (int i = 0; i < HALF; i++) fa[q & 1][i] = ra.get(a, (q >> 1) * HALF + i, q & 1);
+  };
+  auto multiply = [&](int q, int part) {   // of two parts
+#pragma unroll
+    for (int i = part * HALF / 2; i < (part + 1) * HALF / 2; i++)
+#pragma unroll
+      for (int j = 0; j < FN; j++) {
+        f32x4& c = acc[(q >> 1) * HALF + i][j];
+        c = mfma(fb[q & 1][j], fa[q & 1][i], c);
+      }
+  };
+  constexpr int MULS = HALF / 2 * FN, READ_A = HALF * (A_K ? 1 : 2), READ_B = FN * (B_K ? 1 : 2);
+  // Step t is in buffer t % STAGES.  Its eight loads a wave go out one by one among the matrix instructions: sent
+  // together they would hold the wave up until the last one is taken.  Four buffers: step t + 3 is loaded during step t,
+  // into the buffer that step t - 1 has left.  Two buffers: B of step t + 2 is loaded once everybody has step t's
+  // fragments of B (the first barrier), half of A once everybody has step t's of A (the second one) and the other half
+  // at the beginning of step t + 1.  Steps that fill the last round up are zeros.
+  const int total = (to - from + STAGES - 1) / STAGES * STAGES;
+  auto step = [&](u16* a, u16* b, u16* na, u16* nb, u16* la, u16* lb) {
+    // la, lb: two buffers: those of the step before; four: those of step t + 3
+    load_a(la, STAGES == 2 ? 2 : 0);
+    read_b(b, 1);
+    multiply(0, 0);
+    spread<READ_B, MULS>();
+    load_a(la, STAGES == 2 ? 3 : 1);
+    read_a(a, 1);
+    multiply(0, 1);
+    spread<READ_A, MULS>();
+    if (STAGES == 2) {
+      everybody();
+      next();
+      lb = b;
+      la = a;
+    }
+    load_b(lb, 0);
+    read_a(a, 2);
+    multiply(1, 0);
+    spread<READ_A, MULS>();
+    load_b(lb, 1);
+    multiply(1, 1);
+    spread<0, MULS>();
+    load_b(lb, 2);
+    read_a(a, 3);
+    multiply(2, 0);
+    spread<READ_A, MULS>();
+    load_b(lb, 3);
+    multiply(2, 1);
+    spread<0, MULS>();
+    arrive<STAGES == 2 ? 4 : 14>();   // the next step's loads are there, and everybody has this one's fragments
+    load_a(la, STAGES == 2 ? 0 : 2);
+    read_a(na, 0);
+    multiply(3, 0);
+    spread<READ_A, MULS>();
+    load_a(la, STAGES == 2 ? 1 : 3);
+    read_b(nb, 0);
+    multiply(3, 1);
+    spread<READ_B, MULS>();
+    if (STAGES == 4) next();
+  };
+  auto load_all = [&](u16* a, u16* b) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) load_b(b, j);
+#pragma unroll
+    for (int j = 0; j < 4; j++) load_a(a, j);
+  };
+  if (total) {
+    load_all(a0, b0);
+    next();
+    if (STAGES == 2) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) load_b(b1, j);
+      load_a(a1, 0);
+      load_a(a1, 1);
+      arrive<6>();
+    } else {
+      load_all(a1, b1);
+      next();
+      load_all(a2, b2);
+      next();
+      arrive<16>();
+    }
+    read_a(a0, 0);
+    read_b(b0, 0);
   }
-  for (int t = steps >> 1; t > 0; t--) {
-    __syncthreads();
-    load(a1, b1);
-    multiply(a0, b0);
-    __syncthreads();
-    if (t > 1) load(a0, b0);
-    multiply(a1, b1);
+  for (int t = 0; t < total; t += STAGES) {
+    if (STAGES == 2) {
+      step(a0, b0, a1, b1, a1, b1);
+      step(a1, b1, a0, b0, a0, b0);
+    } else {
+      step(a0, b0, a1, b1, a3, b3);
+      step(a1, b1, a2, b2, a0, b0);
+      step(a2, b2, a3, b3, a1, b1);
+      step(a3, b3, a0, b0, a2, b2);
+    }
   }
-  if (EPI == EPI_SOFTMAX) __syncthreads();
-  finish<T, EPI, FM, FN, WN>(p, acc, M, m0 + wave_m * FM * 16, n0 + wave_n * FN * (EPI == EPI_GATE ? 8 : 16), lane, wave_n, wave_m, tile_n, (float2*)a0);
+  arrive<0>();   // no load may still write LDS when it is used again, or given away
+  if constexpr (EPI == EPI_SOFTMAX) {
+    softmax_piece<FM, FN, WM, WN>(p, acc, M, m0, n0, wave_m, wave_n, tile_n, (float2*)a0);
+  } else {
+    const int q = STAGES == 2 ? wave >> 1 : wave;   // 16 KiB a wave
+    u16* mine = (q == 0 ? a0 : q == 1 ? b0 : q == 2 ? a1 : b1) + (STAGES == 2 ? (wave & 1) * 8192 : 0);
+    emit<T, EPI, FM, FN>(p, acc, M, m0 + wave_m * FM * 16, n0 + wave_n * FN * (EPI == EPI_GATE ? 8 : 16), split, (float*)mine);
+  }
 }
 
-template <class T, bool A_K, bool B_K, int EPI> void launch_type(const ProductArgs& p, hipStream_t st) {
+// The sums of a split product, four columns a thread.
+template <class T>
+__global__ __launch_bounds__(256) void join_kernel(const ProductArgs p) {
+  const long cols = (p.N + 3) / 4, i = blockIdx.x * 256L + threadIdx.x;
+  const long m = i / cols, n = (i - m * cols) * 4;
+  if (m >= (p.count && !p.count_k ? *p.count : p.M)) return;
+  float v[4] = {0, 0, 0, 0};
+  for (int s = 0; s < p.splits; s++) {
+    float t[4];
+    get4(p.partial + ((long)s * p.M + m) * (cols * 4) + n, t);
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] += t[e];
+  }
+  store4<T>(p, m, n, v);
+}
+
+// The tile and the splits of a product: the fewest rounds of steps over the
+// 256 CUs.  Microseconds of a step, measured: 256 x 256 tiles 1.75, of 128 x
+// 128 ones, one a CU, 0.70.  Two tile sizes serve all: the large one has half the traffic
+// for each product, the small one fills the GPU with a quarter of the rows.
+struct Plan { bool big; int splits; };
+Plan plan_of(long M, long N, long steps, bool gate, bool may_split) {
+  Plan best{};
+  double least = 1e30;
+  for (int big = 0; big < 2; big++) {
+    const long size = big ? 256 : 128, tiles = clr::ceil_div(M, size) * clr::ceil_div(N, gate ? size / 2 : size);
+    for (int s = 1; s <= (may_split ? 16 : 1); s++) {
+      if (s > 1 && steps / s < 4) break;
+      const double sums = s > 1 ? 4.0 + (s + 1) * (double)M * N * 4 / 3e6 : 0.0;   // of a kernel more, and its traffic
+      const double t = (double)clr::ceil_div(tiles * s, 256) * (clr::ceil_div(steps, s) + 2) * (big ? 1.75 : 0.70) + sums;
+      if (t < least) { least = t; best = {big != 0, s}; }
+    }
+  }
+  return best;
+}
+Plan plan_of(const ProductArgs& p, bool gate, bool may_split) {
+  return plan_of(p.M, p.N, clr::ceil_div(p.K, STEP) * p.pairs, gate, may_split);
+}
+
+template <class T, bool A_K, bool B_K, int EPI> void launch_type(ProductArgs p, hipStream_t st) {
   if (p.M <= 0 || p.N <= 0) return;
   constexpr int half = EPI == EPI_GATE ? 2 : 1;
-  // 256 x 256 has half the memory traffic; a launch that would leave most of the 256 CUs without a tile takes 128 x 128
-  const long big = clr::ceil_div(p.M, 256) * clr::ceil_div(p.N, 256 / half);
-  if (big >= 192 || EPI == EPI_SOFTMAX) {
-    product_kernel<T, 256, 256, 2, 4, A_K, B_K, EPI><<<(unsigned)big, 512, 0, st>>>(p);
-  } else {
-    const long n = clr::ceil_div(p.M, 128) * clr::ceil_div(p.N, 128 / half);
-    product_kernel<T, 128, 128, 2, 2, A_K, B_K, EPI><<<(unsigned)n, 256, 0, st>>>(p);
-  }
+  Plan plan = plan_of(p, EPI == EPI_GATE, EPI == EPI_STORE);
+  if (EPI == EPI_SOFTMAX) plan.big = true;
+  p.splits = plan.splits;
+  const long size = plan.big ? 256 : 128, n = clr::ceil_div(p.M, size) * clr::ceil_div(p.N, size / half) * p.splits;
+  if (plan.big) product_kernel<T, 256, 256, 2, 4, 2, A_K, B_K, EPI><<<(unsigned)n, 512, 0, st>>>(p);
+  else product_kernel<T, 128, 128, 2, 2, 4, A_K, B_K, EPI><<<(unsigned)n, 256, 0, st>>>(p);
+  if (p.splits > 1) join_kernel<T><<<(unsigned)clr::ceil_div((long)p.M * clr::ceil_div(p.N, 4), 256), 256, 0, st>>>(p);
 }
 template <bool A_K, bool B_K, int EPI> void launch(const ProductArgs& p, hipStream_t st) {
   if (p.dtype == DT_F16) launch_type<_Float16, A_K, B_K, EPI>(p, st);
@@ -469,11 +638,11 @@ __global__ __launch_bounds__(ROWS_BLOCK) void kept_rows_kernel(RowsArgs a) {
       const int i = before + __popcll(mask & ((1ull << lane) - 1));
       a.rows[i] = (int)r;
       a.tgt[i] = t >= 0 && t < a.vocab ? (int)t : -1;
+      if (a.lse_kept) { a.lse_kept[i] = a.lse[r]; a.grad_kept[i] = a.grad[r]; }
       if (a.picked) a.picked[i] = NAN;
       if (a.scale) top = fmaxf(top, fabsf(a.grad[r]));
     } else if (r < a.n) {
-      if (a.loss) a.loss[r] = 0.0f;
-      if (a.lse) a.lse[r] = 0.0f;
+      if (a.loss) { a.loss[r] = 0.0f; a.lse[r] = 0.0f; }
     }
     base += all;
     __syncthreads();
@@ -527,6 +696,10 @@ __global__ void zero_kernel(uint16_t* p, size_t n) {
 
 }  // namespace
 
+size_t product_scratch(long M, long N, long K, int pairs) {
+  const Plan plan = plan_of(M, N, clr::ceil_div(K, STEP) * pairs, false, true);
+  return plan.splits > 1 ? (size_t)plan.splits * M * ((N + 3) & ~3L) * sizeof(float) : 0;
+}
 int softmax_parts(int N) { return (int)clr::ceil_div(N, 256); }
 void product_gate(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_GATE>(p, st); }
 void product_gate_grad(const ProductArgs& p, hipStream_t st) { launch<true, false, EPI_GATE_GRAD>(p, st); }
