@@ -210,7 +210,7 @@ void check_ce_tensors(const CrossEntropyArgs* a) {
 size_t ce_forward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
   Arena m{count ? nullptr : (char*)a->workspace};
   const long n = a->rows;
-  const int parts = softmax_parts(a->vocab);
+  const int parts = softmax_parts(n, a->vocab, a->width, a->type == DT_F32 ? 6 : 1);
   RowsArgs r{a->target, nullptr, n, a->ignore, a->vocab};
   r.rows = m.take<int>(n); r.tgt = m.take<int>(n); r.count = m.take<int>(1);
   r.picked = m.take<float>(n); r.loss = a->loss; r.lse = a->lse;

@@ -52,8 +52,8 @@ void product_tn(const ProductArgs& p, hipStream_t st);  // A^T B
 void product_softmax(const ProductArgs& p, hipStream_t st);
 // (exp(A B^T - lse) - onehot(target)) grad into c, in the layout of a factor
 void product_softmax_grad(const ProductArgs& p, hipStream_t st);
-// pieces of a row that product_softmax leaves for a table of N rows
-int softmax_parts(int N);
+// pieces of a row that product_softmax leaves
+int softmax_parts(long M, long N, long K, int pairs);
 
 // A factor in the layout above: row rows[i] (or i) of `from` to row i of `to`, for i < *count (or n); a float32 one
 // as three parts `part` elements apart.

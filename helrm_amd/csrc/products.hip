@@ -8,7 +8,7 @@
 //
 // A workgroup has a BM x BN tile of C, k advances by 64.  Both factors' tiles
 // go from memory to LDS directly (16 bytes a lane, no registers), into one of
-// two or four buffers while others are multiplied; one barrier a step.
+// two buffers while the other one is multiplied.
 // Elements outside a factor are read as 0 through the bounds of its buffer
 // descriptor, so no tile has a special case.  Products whose tiles would
 // leave CUs idle are split along k into float32 sums that a second kernel adds
@@ -47,7 +47,7 @@ __device__ __forceinline__ void act4(int act, const float* c, const float g[4], 
   if (act == ACT_SILU) {
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const float s = 1.0f / (1.0f + __expf(-g[e]));
+      const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g[e]));   // (within 1 ulp)
       a[e] = g[e] * s;
       d[e] = s * (1.0f + g[e] * (1.0f - s));
     }
@@ -67,10 +67,10 @@ __device__ __forceinline__ void act4(int act, const float* c, const float g[4], 
   }
 }
 
-// (maximum, sum of exponentials about it) of two pieces of a row.  Where both
-// hold nothing above -inf there is nothing to rescale; a NaN stays one.
+// (maximum, sum of exponentials about it) of two pieces of a row, (-inf, 0) for
+// one that holds nothing above -inf.  A NaN is in the sum and stays there.
 __device__ __forceinline__ float2 join(float2 a, float2 b) {
-  const float m = a.x > b.x || a.x != a.x ? a.x : b.x;
+  const float m = fmaxf(a.x, b.x);
   if (m == -INFINITY) return make_float2(m, a.y + b.y);
   return make_float2(m, a.y * __expf(a.x - m) + b.y * __expf(b.x - m));
 }
@@ -83,22 +83,28 @@ __device__ __forceinline__ void split3(float v, __bf16 out[3]) {
   out[2] = (__bf16)(r - (float)out[1]);
 }
 
-// Four neighbouring elements into an intermediate in the layout of a factor
-// (8-byte aligned; a float32 operator's: three parts, `part` elements apart).
 __device__ __forceinline__ u16 bits(__bf16 v) { return __builtin_bit_cast(u16, v); }
 __device__ __forceinline__ u16 bits(_Float16 v) { return __builtin_bit_cast(u16, v); }
-__device__ __forceinline__ void put8(u16* c, u16 a, u16 b, u16 d, u16 e) {
-  *(uint2*)c = make_uint2((unsigned)a | (unsigned)b << 16, (unsigned)d | (unsigned)e << 16);
+template <class T> __device__ __forceinline__ uint2 pack4(const float v[4]) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  const f32x4 f = {v[0], v[1], v[2], v[3]};
+  return __builtin_bit_cast(uint2, __builtin_convertvector(f, T4));
 }
-template <class T> __device__ __forceinline__ void put_held(void* c, int type, long part, long at, const float v[4]) {
-  u16* o = (u16*)c + at;
-  put8(o, bits((T)v[0]), bits((T)v[1]), bits((T)v[2]), bits((T)v[3]));
-  if (sizeof(T) == 2 && type == DT_F32) {
-    __bf16 s[4][3];
+// Four neighbouring elements into an intermediate in the layout of a factor
+// (8-byte aligned; a float32 operator's: three parts, `part` elements apart).
+template <class T> __device__ __forceinline__ void put_held(u16* o, int type, long part, const float v[4]) {
+  *(uint2*)o = pack4<T>(v);
+  if (type == DT_F32) {
+    float r[2][4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) split3(v[e], s[e]);
+    for (int e = 0; e < 4; e++) {
+      __bf16 s[3];
+      split3(v[e], s);
+      r[0][e] = (float)s[1];
+      r[1][e] = (float)s[2];
+    }
 #pragma unroll
-    for (int k = 1; k < 3; k++) put8(o + k * part, bits(s[0][k]), bits(s[1][k]), bits(s[2][k]), bits(s[3][k]));
+    for (int k = 0; k < 2; k++) *(uint2*)(o + (k + 1) * part) = pack4<__bf16>(r[k]);
   }
 }
 // The first n of four neighbouring elements of a tensor of the caller's.
@@ -112,7 +118,7 @@ template <class T> __device__ __forceinline__ void put_out(void* c, int type, lo
     }
   } else {
     u16* o = (u16*)c + at;
-    if (n >= 4 && ((uintptr_t)o & 7) == 0) put8(o, bits((T)v[0]), bits((T)v[1]), bits((T)v[2]), bits((T)v[3]));
+    if (n >= 4 && ((uintptr_t)o & 7) == 0) *(uint2*)o = pack4<T>(v);
     else {
 #pragma unroll
       for (int e = 0; e < 4; e++) if (e < n) o[e] = bits((T)v[e]);
@@ -124,11 +130,10 @@ __device__ __forceinline__ void get4(const float* c, float v[4]) {
   v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
 }
 
-// Four neighbouring columns of a product.
-template <class T> __device__ __forceinline__ void store4(const ProductArgs& p, long m, long n, float v[4]) {
-  const int left = (int)(p.N - n);
+// The first `left` of four neighbouring columns of a product, at element `at` of c.
+template <class T> __device__ __forceinline__ void store4(const ProductArgs& p, long at, int left, float v[4]) {
   if (p.add) {
-    const float* c = (const float*)p.c + m * p.ldc + n;
+    const float* c = (const float*)p.c + at;
 #pragma unroll
     for (int e = 0; e < 4; e++) if (e < left) v[e] += c[e];
   }
@@ -137,7 +142,7 @@ template <class T> __device__ __forceinline__ void store4(const ProductArgs& p, 
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] *= factor;
   }
-  put_out<T>(p.c, p.ctype, m * p.ldc + n, v, left);
+  put_out<T>(p.c, p.ctype, at, v, left);
 }
 
 // One factor's loads of a step.  ALONG_K: its rows run along k.  R rows of the
@@ -222,33 +227,29 @@ __device__ __forceinline__ void softmax_piece(const ProductArgs& p, const f32x4 
                                               float2* lds) {
   const int lane = threadIdx.x & 63, quad = lane >> 4;
   const int left = (int)min((long)p.N - n0 - wave_n * FN * 16, 1L << 20) - 4 * quad;   // columns from the lane's first one on
+  const bool whole = left >= FN * 16;
 #pragma unroll
   for (int i = 0; i < FM; i++) {
     const int r = (wave_m * FM + i) * 16 + (lane & 15);
     const long m = m0 + r;
     const int t = m < M ? p.target[m] - (int)(n0 + wave_n * FN * 16 + 4 * quad) : -1;   // the target's place from there
-    float top = -INFINITY, picked = 0;
-    bool nan = false, hit = false;
+    float v[FN * 4], top = -INFINITY, sum = 0;
 #pragma unroll
-    for (int j = 0; j < FN; j++)
+    for (int c = 0; c < FN * 4; c++) {
+      v[c] = whole || 16 * (c >> 2) + (c & 3) < left ? acc[i][c >> 2][c & 3] : -INFINITY;
+      top = fmaxf(top, v[c]);
+    }
+    if (t >= 0 && t < FN * 16) {   // (seldom: one tile has it)
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float v = acc[i][j][e];
-        const int c = 16 * j + e;
-        if (c < left) { top = fmaxf(top, v); nan |= v != v; }
-        if (c == t) { picked = v; hit = true; }
-      }
-    if (nan) top = NAN;
-    float sum = 0;
+      for (int c = 0; c < FN * 4; c++) if (16 * (c >> 2) + (c & 3) == t) p.picked[m] = v[c];
+    }
+    // fmaxf passes over a NaN; its exponential is one again
+    const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-    for (int j = 0; j < FN; j++)
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (16 * j + e < left) sum += top == -INFINITY ? 1.0f : __expf(acc[i][j][e] - top);
+    for (int c = 0; c < FN * 4; c++) sum += __expf(v[c] - base);
     float2 run = make_float2(top, sum);
 #pragma unroll
     for (int o = 16; o < 64; o <<= 1) run = join(run, make_float2(__shfl_xor(run.x, o), __shfl_xor(run.y, o)));
-    if (hit && m < M) p.picked[m] = picked;
     if (lane < 16) lds[r * WAVES_N + wave_n] = run;
   }
   __syncthreads();
@@ -260,81 +261,89 @@ __device__ __forceinline__ void softmax_piece(const ProductArgs& p, const f32x4 
   }
 }
 
-// What becomes of four neighbouring columns of a row (gate: v of the gate, u of the up projection).
-template <class T, int EPI> __device__ __forceinline__ void emit4(const ProductArgs& p, int split, float scale, long m, long n, float v[4], float u[4]) {
-  if (EPI == EPI_STORE) {
-    if (n >= p.N) return;
-    if (p.splits > 1) *(float4*)(p.partial + ((long)split * p.M + m) * ((p.N + 3) & ~3) + n) = make_float4(v[0], v[1], v[2], v[3]);
-    else store4<T>(p, m, n, v);
-    return;
-  }
-  const int left = (int)min((long)p.N - n, 4L);   // the columns that fill a row up are 0
-  if (EPI == EPI_GATE) {
-    if (n >= p.ldh) return;
-    float h[4], d[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) if (e >= left) v[e] = u[e] = 0.0f;
-    act4(p.act, p.coef, v, h, d);
-#pragma unroll
-    for (int e = 0; e < 4; e++) h[e] *= u[e];
-    const long at = m * p.ldh + n;
-    if (p.g) { *(float4*)(p.g + at) = make_float4(v[0], v[1], v[2], v[3]); *(float4*)(p.u + at) = make_float4(u[0], u[1], u[2], u[3]); }
-    put_held<T>(p.h, p.dtype, p.hpart, at, h);
-  } else if (EPI == EPI_GATE_GRAD) {
-    if (n >= p.ldh) return;
-    const long at = m * p.ldh + n;
-    float g[4], a[4], d[4];
-    get4(p.g + at, g);
-    get4(p.u + at, u);
-    act4(p.act, p.coef, g, a, d);
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      if (e >= left) v[e] = 0.0f;   // (g and u are 0 there)
-      d[e] *= v[e] * u[e];
-      v[e] *= a[e];
-      a[e] *= u[e];
-    }
-    put_held<T>(p.dg, p.dtype, p.hpart, at, d);
-    put_held<T>(p.du, p.dtype, p.hpart, at, v);
-    put_held<T>(p.h, p.dtype, p.hpart, at, a);
-  } else {
-    if (n >= ((p.N + 7) & ~7)) return;   // the row is filled up to a multiple of 8
-    const int target = p.target[m], t = target - (int)(p.n0 + n);
-    const float lse = p.lse[m], grad = target < 0 ? NAN : p.grad[m] * scale;
-#pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = e < left ? (__expf(v[e] - lse) - (t == e ? 1.0f : 0.0f)) * grad : 0.0f;
-    put_held<T>(p.c, p.dtype, p.hpart, m * p.ldc + n, v);
-  }
-}
-
 // A wave's accumulators go through its own part of LDS, 64 rows of 64 float32
 // columns at a time (16 bytes c of row r at c ^ (r & 15)), so that what is
-// stored are whole lines of a row and the code of it is there once.
+// stored are whole lines of a row and the code of it is there once.  A place is
+// a 32-bit offset from the wave's first element (rows are under 2^21 elements).
 template <class T, int EPI, int FM, int FN>
 __device__ __forceinline__ void emit(const ProductArgs& p, const f32x4 (&acc)[FM][FN], int M, long mw, long nw, int split, float* lds) {
   static_assert(FN == 4 && FM % 4 == 0, "64 x 64 a time");
   constexpr int LANES = EPI == EPI_GATE ? 8 : 16, ROWS = 64 / LANES;   // of a row; rows a time
   const int lane = threadIdx.x & 63, col = lane % LANES;
-  const float scale = EPI == EPI_SOFTMAX_GRAD && p.scale ? *p.scale : 1.0f;
+  // gate: the columns are 16 of the gate, the same 16 of the up projection, 16 of the gate, ...
+  const int c = EPI == EPI_GATE ? (col >> 2) * 8 + (col & 3) : col;
+  const bool sums = EPI == EPI_STORE && p.splits > 1;
+  const unsigned ld = sums ? (p.N + 3) & ~3 : EPI == EPI_STORE || EPI == EPI_SOFTMAX_GRAD ? (unsigned)p.ldc : (unsigned)p.ldh;
+  const long first = mw * ld + nw;
+  // columns that there are from the lane's first one on, and columns with the zeros that fill an intermediate's row up
+  const int left = (int)min((long)p.N - nw, 64L) - col * 4;
+  const int room = EPI == EPI_STORE ? left : (int)min(((p.N + 7L) & ~7L) - nw, 64L) - col * 4;
+  float* const sum_at = sums ? p.partial + (long)split * p.M * ld + first : nullptr;
+  u16* const h = (u16*)(EPI == EPI_SOFTMAX_GRAD ? p.c : p.h) + first;
 #pragma unroll
   for (int part = 0; part < FM / 4; part++) {
+    float lse = 0, grad = 0;   // of row `lane` of the 64
+    int target = 0;
+    if (EPI == EPI_SOFTMAX_GRAD && mw + part * 64 + lane < M) {
+      const long m = mw + part * 64 + lane;
+      target = p.target[m];
+      lse = p.lse[m];
+      grad = target < 0 ? NAN : p.grad[m] * (p.scale ? *p.scale : 1.0f);
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int r = i * 16 + (lane & 15), c = j * 4 + (lane >> 4);
-        *(f32x4*)(lds + r * 64 + ((c ^ (r & 15)) * 4)) = acc[part * 4 + i][j];
+        const int r = i * 16 + (lane & 15), at = j * 4 + (lane >> 4);
+        *(f32x4*)(lds + r * 64 + ((at ^ (r & 15)) * 4)) = acc[part * 4 + i][j];
       }
+    const int rows = (int)min(M - mw - part * 64, 64L);
 #pragma unroll 4
     for (int r0 = 0; r0 < 64; r0 += ROWS) {
       const int r = r0 + lane / LANES;
-      const long m = mw + part * 64 + r;
-      // gate: the columns are 16 of the gate, the same 16 of the up projection, 16 of the gate, ...
-      const int c = EPI == EPI_GATE ? (col >> 2) * 8 + (col & 3) : col;
       float v[4], u[4] = {0, 0, 0, 0};
       get4(lds + r * 64 + ((c ^ (r & 15)) * 4), v);
       if (EPI == EPI_GATE) get4(lds + r * 64 + (((c + 4) ^ (r & 15)) * 4), u);
-      if (m < M) emit4<T, EPI>(p, split, scale, m, nw + col * 4, v, u);
+      const float row_lse = EPI == EPI_SOFTMAX_GRAD ? __shfl(lse, r) : 0.0f, row_grad = EPI == EPI_SOFTMAX_GRAD ? __shfl(grad, r) : 0.0f;
+      const int t = EPI == EPI_SOFTMAX_GRAD ? __shfl(target, r) - (int)(p.n0 + nw) - col * 4 : 0;
+      if (r >= rows || room <= 0) continue;
+      const unsigned at = (part * 64 + r) * ld + col * 4;
+      if (left < 4) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) if (e >= left) v[e] = u[e] = 0.0f;
+      }
+      if (EPI == EPI_STORE) {
+        if (sums) *(float4*)(sum_at + at) = make_float4(v[0], v[1], v[2], v[3]);
+        else store4<T>(p, first + at, left, v);
+      } else if (EPI == EPI_GATE) {
+        float a[4], d[4];
+        act4(p.act, p.coef, v, a, d);
+#pragma unroll
+        for (int e = 0; e < 4; e++) a[e] *= u[e];
+        if (p.g) {
+          __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, (f32x4*)(p.g + first + at));
+          __builtin_nontemporal_store(f32x4{u[0], u[1], u[2], u[3]}, (f32x4*)(p.u + first + at));
+        }
+        put_held<T>(h + at, p.dtype, p.hpart, a);
+      } else if (EPI == EPI_GATE_GRAD) {
+        float g[4], a[4], d[4];
+        get4(p.g + first + at, g);
+        get4(p.u + first + at, u);
+        act4(p.act, p.coef, g, a, d);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {   // (g, u and v are 0 in the columns that fill a row up)
+          d[e] *= v[e] * u[e];
+          v[e] *= a[e];
+          a[e] *= u[e];
+        }
+        put_held<T>((u16*)p.dg + first + at, p.dtype, p.hpart, d);
+        put_held<T>((u16*)p.du + first + at, p.dtype, p.hpart, v);
+        put_held<T>(h + at, p.dtype, p.hpart, a);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = e < left ? (__expf(v[e] - row_lse) - (t == e ? 1.0f : 0.0f)) * row_grad : 0.0f;
+        put_held<T>(h + at, p.dtype, p.hpart, v);
+      }
     }
   }
 }
@@ -363,14 +372,12 @@ template <int READS, int MULS> __device__ __forceinline__ void spread() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-template <class T, int BM, int BN, int WM, int WN, int STAGES, bool A_K, bool B_K, int EPI>
+template <class T, int BM, int BN, int WM, int WN, bool A_K, bool B_K, int EPI>
 __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const ProductArgs p) {
   constexpr int W = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr int COLS = EPI == EPI_GATE ? BN / 2 : BN;   // columns of C in a tile
   // Arrays of their own, not one: only so does the compiler see that a load into one does not concern reads of another.
-  constexpr int MORE = STAGES > 2 ? STEP : 0;
   __shared__ __align__(1024) u16 a0[BM * STEP], b0[BN * STEP], a1[BM * STEP], b1[BN * STEP];
-  __shared__ __align__(1024) u16 a2[BM * MORE + 8], b2[BN * MORE + 8], a3[BM * MORE + 8], b3[BN * MORE + 8];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave_m = wave / WN, wave_n = wave % WN;
   const int nm = (p.M + BM - 1) / BM, nn = (p.N + COLS - 1) / COLS;
@@ -385,7 +392,7 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const ProductArgs 
   const int KA = A_K ? (K + 7) & ~7 : K, KB = B_K ? (K + 7) & ~7 : K;
 
   constexpr int LA = Loader<A_K, BM, W>::N, LB = Loader<B_K, BN, W>::N;
-  static_assert(LA == 4 && LB == 4 && (STAGES == 2 || STAGES == 4), "the steps below");
+  static_assert(LA == 4 && LB == 4, "the steps below");
   Loader<A_K, BM, W> la;
   Loader<B_K, BN, W> lb;
   Reader<T, A_K, BM> ra;
@@ -449,95 +456,68 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const ProductArgs 
       }
   };
   constexpr int MULS = HALF / 2 * FN, READ_A = HALF * (A_K ? 1 : 2), READ_B = FN * (B_K ? 1 : 2);
-  // Step t is in buffer t % STAGES.  Its eight loads a wave go out one by one among the matrix instructions: sent
-  // together they would hold the wave up until the last one is taken.  Four buffers: step t + 3 is loaded during step t,
-  // into the buffer that step t - 1 has left.  Two buffers: B of step t + 2 is loaded once everybody has step t's
-  // fragments of B (the first barrier), half of A once everybody has step t's of A (the second one) and the other half
-  // at the beginning of step t + 1.  Steps that fill the last round up are zeros.
-  const int total = (to - from + STAGES - 1) / STAGES * STAGES;
-  auto step = [&](u16* a, u16* b, u16* na, u16* nb, u16* la, u16* lb) {
-    // la, lb: two buffers: those of the step before; four: those of step t + 3
-    load_a(la, STAGES == 2 ? 2 : 0);
+  // Step t is in buffer t % 2.  Its eight loads a wave go out one by one among the matrix instructions: sent together
+  // they would hold the wave up until the last one is taken.  B of step t + 2 is loaded into step t's place once
+  // everybody has step t's fragments of B (the first barrier), half of A once everybody has those of A (the second) and
+  // the other half at the beginning of step t + 1.  An odd number of steps is filled up with one of zeros.
+  auto step = [&](u16* a, u16* b, u16* na, u16* nb) {
+    load_a(na, 2);
     read_b(b, 1);
     multiply(0, 0);
     spread<READ_B, MULS>();
-    load_a(la, STAGES == 2 ? 3 : 1);
+    load_a(na, 3);
     read_a(a, 1);
     multiply(0, 1);
     spread<READ_A, MULS>();
-    if (STAGES == 2) {
-      everybody();
-      next();
-      lb = b;
-      la = a;
-    }
-    load_b(lb, 0);
+    everybody();
+    next();
+    load_b(b, 0);
     read_a(a, 2);
     multiply(1, 0);
     spread<READ_A, MULS>();
-    load_b(lb, 1);
+    load_b(b, 1);
     multiply(1, 1);
     spread<0, MULS>();
-    load_b(lb, 2);
+    load_b(b, 2);
     read_a(a, 3);
     multiply(2, 0);
     spread<READ_A, MULS>();
-    load_b(lb, 3);
+    load_b(b, 3);
     multiply(2, 1);
     spread<0, MULS>();
-    arrive<STAGES == 2 ? 4 : 14>();   // the next step's loads are there, and everybody has this one's fragments
-    load_a(la, STAGES == 2 ? 0 : 2);
+    arrive<4>();   // the next step's loads are there (those of B since are not its), and everybody has this one's fragments
+    load_a(a, 0);
     read_a(na, 0);
     multiply(3, 0);
     spread<READ_A, MULS>();
-    load_a(la, STAGES == 2 ? 1 : 3);
+    load_a(a, 1);
     read_b(nb, 0);
     multiply(3, 1);
     spread<READ_B, MULS>();
-    if (STAGES == 4) next();
   };
-  auto load_all = [&](u16* a, u16* b) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) load_b(b, j);
-#pragma unroll
-    for (int j = 0; j < 4; j++) load_a(a, j);
-  };
+  const int total = (to - from + 1) / 2;
   if (total) {
-    load_all(a0, b0);
-    next();
-    if (STAGES == 2) {
 #pragma unroll
-      for (int j = 0; j < 4; j++) load_b(b1, j);
-      load_a(a1, 0);
-      load_a(a1, 1);
-      arrive<6>();
-    } else {
-      load_all(a1, b1);
-      next();
-      load_all(a2, b2);
-      next();
-      arrive<16>();
-    }
+    for (int j = 0; j < 4; j++) { load_b(b0, j); load_a(a0, j); }
+    next();
+#pragma unroll
+    for (int j = 0; j < 4; j++) load_b(b1, j);
+    load_a(a1, 0);
+    load_a(a1, 1);
+    arrive<6>();
     read_a(a0, 0);
     read_b(b0, 0);
   }
-  for (int t = 0; t < total; t += STAGES) {
-    if (STAGES == 2) {
-      step(a0, b0, a1, b1, a1, b1);
-      step(a1, b1, a0, b0, a0, b0);
-    } else {
-      step(a0, b0, a1, b1, a3, b3);
-      step(a1, b1, a2, b2, a0, b0);
-      step(a2, b2, a3, b3, a1, b1);
-      step(a3, b3, a0, b0, a2, b2);
-    }
+  for (int t = 0; t < total; t++) {
+    step(a0, b0, a1, b1);
+    step(a1, b1, a0, b0);
   }
   arrive<0>();   // no load may still write LDS when it is used again, or given away
   if constexpr (EPI == EPI_SOFTMAX) {
     softmax_piece<FM, FN, WM, WN>(p, acc, M, m0, n0, wave_m, wave_n, tile_n, (float2*)a0);
   } else {
-    const int q = STAGES == 2 ? wave >> 1 : wave;   // 16 KiB a wave
-    u16* mine = (q == 0 ? a0 : q == 1 ? b0 : q == 2 ? a1 : b1) + (STAGES == 2 ? (wave & 1) * 8192 : 0);
+    const int q = BM == 256 ? wave >> 1 : wave;   // 16 KiB a wave
+    u16* mine = (q == 0 ? a0 : q == 1 ? b0 : q == 2 ? a1 : b1) + (BM == 256 ? (wave & 1) * 8192 : 0);
     emit<T, EPI, FM, FN>(p, acc, M, m0 + wave_m * FM * 16, n0 + wave_n * FN * (EPI == EPI_GATE ? 8 : 16), split, (float*)mine);
   }
 }
@@ -555,13 +535,14 @@ __global__ __launch_bounds__(256) void join_kernel(const ProductArgs p) {
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] += t[e];
   }
-  store4<T>(p, m, n, v);
+  store4<T>(p, m * p.ldc + n, (int)min(p.N - n, 4L), v);
 }
 
-// The tile and the splits of a product: the fewest rounds of steps over the
-// 256 CUs.  Microseconds of a step, measured: 256 x 256 tiles 1.75, of 128 x
-// 128 ones, one a CU, 0.70.  Two tile sizes serve all: the large one has half the traffic
-// for each product, the small one fills the GPU with a quarter of the rows.
+// The tile and the splits of a product: the least time of its rounds over the
+// 256 CUs, which hold one 256 x 256 tile or two 128 x 128 ones (whose steps
+// and ends overlap).  Microseconds, measured: a step 1.6 and 1.0, the end of a
+// tile 10 and 6. The large tile has half the traffic for each product, the
+// small one fills the GPU with a quarter of the rows.
 struct Plan { bool big; int splits; };
 Plan plan_of(long M, long N, long steps, bool gate, bool may_split) {
   Plan best{};
@@ -571,7 +552,8 @@ Plan plan_of(long M, long N, long steps, bool gate, bool may_split) {
     for (int s = 1; s <= (may_split ? 16 : 1); s++) {
       if (s > 1 && steps / s < 4) break;
       const double sums = s > 1 ? 4.0 + (s + 1) * (double)M * N * 4 / 3e6 : 0.0;   // of a kernel more, and its traffic
-      const double t = (double)clr::ceil_div(tiles * s, 256) * (clr::ceil_div(steps, s) + 2) * (big ? 1.75 : 0.70) + sums;
+      const long rounds = clr::ceil_div(tiles * s, 256), each = clr::ceil_div(steps, s);
+      const double t = (big ? rounds * (each * 1.6 + 10) : (rounds + 1) / 2 * (each * 1.0 + 6) * (rounds == 1 ? 0.6 : 1.0)) + sums;
       if (t < least) { least = t; best = {big != 0, s}; }
     }
   }
@@ -584,12 +566,11 @@ Plan plan_of(const ProductArgs& p, bool gate, bool may_split) {
 template <class T, bool A_K, bool B_K, int EPI> void launch_type(ProductArgs p, hipStream_t st) {
   if (p.M <= 0 || p.N <= 0) return;
   constexpr int half = EPI == EPI_GATE ? 2 : 1;
-  Plan plan = plan_of(p, EPI == EPI_GATE, EPI == EPI_STORE);
-  if (EPI == EPI_SOFTMAX) plan.big = true;
+  const Plan plan = plan_of(p, EPI == EPI_GATE, EPI == EPI_STORE);
   p.splits = plan.splits;
   const long size = plan.big ? 256 : 128, n = clr::ceil_div(p.M, size) * clr::ceil_div(p.N, size / half) * p.splits;
-  if (plan.big) product_kernel<T, 256, 256, 2, 4, 2, A_K, B_K, EPI><<<(unsigned)n, 512, 0, st>>>(p);
-  else product_kernel<T, 128, 128, 2, 2, 4, A_K, B_K, EPI><<<(unsigned)n, 256, 0, st>>>(p);
+  if (plan.big) product_kernel<T, 256, 256, 2, 4, A_K, B_K, EPI><<<(unsigned)n, 512, 0, st>>>(p);
+  else product_kernel<T, 128, 128, 2, 2, A_K, B_K, EPI><<<(unsigned)n, 256, 0, st>>>(p);
   if (p.splits > 1) join_kernel<T><<<(unsigned)clr::ceil_div((long)p.M * clr::ceil_div(p.N, 4), 256), 256, 0, st>>>(p);
 }
 template <bool A_K, bool B_K, int EPI> void launch(const ProductArgs& p, hipStream_t st) {
@@ -700,7 +681,9 @@ size_t product_scratch(long M, long N, long K, int pairs) {
   const Plan plan = plan_of(M, N, clr::ceil_div(K, STEP) * pairs, false, true);
   return plan.splits > 1 ? (size_t)plan.splits * M * ((N + 3) & ~3L) * sizeof(float) : 0;
 }
-int softmax_parts(int N) { return (int)clr::ceil_div(N, 256); }
+int softmax_parts(long M, long N, long K, int pairs) {
+  return (int)clr::ceil_div(N, plan_of(M, N, clr::ceil_div(K, STEP) * pairs, false, false).big ? 256 : 128);
+}
 void product_gate(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_GATE>(p, st); }
 void product_gate_grad(const ProductArgs& p, hipStream_t st) { launch<true, false, EPI_GATE_GRAD>(p, st); }
 void product_nt(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_STORE>(p, st); }
