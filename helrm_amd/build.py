@@ -15,7 +15,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "libhelrm_hip.so")
-SOURCES = ["kernels.hip", "ntt.hip", "encoder.hip", "runtime.hip", "norm.hip", "products.hip", "cleartext.hip"]
+SOURCES = ["kernels.hip", "ntt.hip", "encoder.hip", "runtime.hip", "norm.hip", "products.hip", "skinny.hip",
+           "cleartext.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 FLAGS = [

@@ -201,45 +201,47 @@ def layer_norm(x, weight, bias=None, eps=1e-5):
 # ---- gated feed-forward block ----------------------------------------------------------
 
 
-def _mlp_args(x, gate, up, down, activation):
+_NO_COEF = (0.0, 0.0, 0.0, 0.0)
+
+
+def _mlp_tensors(x, gate, up, down):
     _need(gate.dim() == 2 and up.dim() == 2 and down.dim() == 2, "gate, up and down are matrices")
     hidden, width = gate.shape
     _need(hidden >= 1 and width >= 1, "gate: no elements")
     x2 = _rows(x, width, "x")
     gate, up, down = _rows(gate, width, "gate", x), _rows(up, width, "up", x), _rows(down, hidden, "down", x)
-    _need(up.shape[0] == hidden, f"up: {up.shape[0]} rows, not {hidden}")
-    _need(down.shape[0] == width, f"down: {down.shape[0]} rows, not {width}")
-    a = GatedMLPArgs()
-    a.x, a.ldx = x2.data_ptr(), _ld(x2)
-    a.gate, a.ldgate = gate.data_ptr(), _ld(gate)
-    a.up, a.ldup = up.data_ptr(), _ld(up)
-    a.down, a.lddown = down.data_ptr(), _ld(down)
-    a.rows, a.width, a.hidden, a.type = x2.shape[0], width, hidden, _TYPES[x.dtype]
+    if up.shape[0] != hidden:
+        raise ValueError(f"up: {up.shape[0]} rows, not {hidden}")
+    if down.shape[0] != width:
+        raise ValueError(f"down: {down.shape[0]} rows, not {width}")
+    return x2, gate, up, down
+
+
+def _act(activation):
+    """The number of an activation, and a cubic's coefficients."""
     if isinstance(activation, str):
         _need(activation in _ACTS, f"activation {activation!r}: neither silu, gelu nor four coefficients")
-        a.act = _ACTS[activation]
-    else:
-        coef = tuple(float(c) for c in activation)
-        _need(len(coef) == 4, "activation: a cubic has four coefficients, lowest degree first")
-        a.act, a.coef = 2, coef
-    return a, (x2, gate, up, down)
-
-
-def _saved_width(a):
-    return (a.hidden + 7) // 8 * 8
+        return _ACTS[activation], _NO_COEF
+    coef = tuple(float(c) for c in activation)
+    _need(len(coef) == 4, "activation: a cubic has four coefficients, lowest degree first")
+    return 2, coef
 
 
 def _mlp_forward(x, gate, up, down, activation, keep):
-    a, held = _mlp_args(x, gate, up, down, activation)
+    x2, gate, up, down = _mlp_tensors(x, gate, up, down)
+    act, coef = _act(activation)
+    rows, hidden, width = x2.shape[0], gate.shape[0], gate.shape[1]
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    a.y, a.ldy = y.data_ptr(), a.width
-    saved = None
+    saved = g = u = None
     if keep:
-        saved = torch.empty((2, a.rows, _saved_width(a)), dtype=torch.float32, device=x.device)
-        if a.rows:
-            a.g = saved.data_ptr()
-            a.u = a.g + 2 * saved.numel()
-    _call("GatedMLP", a, x.device)
+        saved = torch.empty((2, rows, (hidden + 7) // 8 * 8), dtype=torch.float32, device=x.device)
+        if rows:
+            g = saved.data_ptr()
+            u = g + 2 * saved.numel()
+    _call("GatedMLP", GatedMLPArgs(
+        x=x2.data_ptr(), ldx=_ld(x2), gate=gate.data_ptr(), ldgate=_ld(gate), up=up.data_ptr(), ldup=_ld(up), down=down.data_ptr(),
+        lddown=_ld(down), y=y.data_ptr(), ldy=width, g=g, u=u, rows=rows, width=width, hidden=hidden, type=_TYPES[x.dtype], act=act,
+        coef=coef), x.device)
     return y, saved
 
 
@@ -251,20 +253,22 @@ def gated_mlp_forward(x, gate, up, down, activation="silu"):
 
 def gated_mlp_backward(grad, x, gate, up, down, saved, activation="silu"):
     """(dx, dgate, dup, ddown)."""
-    a, held = _mlp_args(x, gate, up, down, activation)
-    g2 = _rows(grad, a.width, "grad", x)
-    _need(g2.shape[0] == a.rows, f"grad: {g2.shape[0]} rows, not {a.rows}")
-    _need(tuple(saved.shape) == (2, a.rows, _saved_width(a)) and saved.dtype == torch.float32 and saved.device == x.device
+    x2, gate, up, down = _mlp_tensors(x, gate, up, down)
+    act, coef = _act(activation)
+    rows, hidden, width = x2.shape[0], gate.shape[0], gate.shape[1]
+    g2 = _rows(grad, width, "grad", x)
+    if g2.shape[0] != rows:
+        raise ValueError(f"grad: {g2.shape[0]} rows, not {rows}")
+    _need(tuple(saved.shape) == (2, rows, (hidden + 7) // 8 * 8) and saved.dtype == torch.float32 and saved.device == x.device
           and saved.is_contiguous(), "saved: not what the forward call returned")
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dgate, dup, ddown = (torch.empty(w.shape, dtype=x.dtype, device=x.device) for w in (gate, up, down))
-    a.dy, a.lddy = g2.data_ptr(), _ld(g2)
-    a.dx, a.lddx = dx.data_ptr(), a.width
-    if a.rows:
-        a.g = saved.data_ptr()
-        a.u = a.g + 2 * saved.numel()
-    a.dgate, a.dup, a.ddown = dgate.data_ptr(), dup.data_ptr(), ddown.data_ptr()
-    _call("GatedMLPGrad", a, x.device)
+    g = saved.data_ptr() if rows else None
+    _call("GatedMLPGrad", GatedMLPArgs(
+        x=x2.data_ptr(), ldx=_ld(x2), gate=gate.data_ptr(), ldgate=_ld(gate), up=up.data_ptr(), ldup=_ld(up), down=down.data_ptr(),
+        lddown=_ld(down), g=g, u=g + 2 * saved.numel() if rows else None, dy=g2.data_ptr(), lddy=_ld(g2), dx=dx.data_ptr(), lddx=width,
+        dgate=dgate.data_ptr(), dup=dup.data_ptr(), ddown=ddown.data_ptr(), rows=rows, width=width, hidden=hidden,
+        type=_TYPES[x.dtype], act=act, coef=coef), x.device)
     return dx, dgate, dup, ddown
 
 
@@ -294,42 +298,40 @@ def gated_mlp(x, gate, up, down, activation="silu"):
 # ---- softmax cross entropy against a table ------------------------------------------------
 
 
-def _loss_args(x, table, target, ignore_index):
+def _loss_tensors(x, table, target):
     _need(table.dim() == 2 and table.shape[0] >= 1 and table.shape[1] >= 1, "table: not a matrix with elements")
-    vocab, width = table.shape
-    x2 = _rows(x, width, "x")
-    table = _rows(table, width, "table", x)
-    target = _vector(target.reshape(-1), x2.shape[0], "target", torch.int64, x.device)
-    a = CrossEntropyArgs()
-    a.x, a.ldx = x2.data_ptr(), _ld(x2)
-    a.table, a.ldtable = table.data_ptr(), _ld(table)
-    a.target = target.data_ptr()
-    a.rows, a.width, a.vocab, a.ignore, a.type = x2.shape[0], width, vocab, ignore_index, _TYPES[x.dtype]
-    return a, (x2, table, target)
+    x2 = _rows(x, table.shape[1], "x")
+    target = _vector(target.reshape(-1) if target.dim() != 1 else target, x2.shape[0], "target", torch.int64, x.device)
+    return x2, _rows(table, table.shape[1], "table", x), target
 
 
 def cross_entropy_forward(x, table, target, ignore_index=-100):
     """(losses, lse), float32 for each row: the softmax cross entropy of x's products with the table's rows, and the
     logarithm of the softmax's sum.  Rows whose target is `ignore_index` have 0 for both; a target outside the table
     gives NaN.  The logits are never in memory."""
-    a, held = _loss_args(x, table, target, ignore_index)
-    losses, lse = torch.empty((2, a.rows), dtype=torch.float32, device=x.device)
-    a.loss, a.lse = losses.data_ptr(), lse.data_ptr()
-    _call("CrossEntropy", a, x.device)
-    return losses.view(x.shape[:-1]), lse.view(x.shape[:-1])
+    x2, table, target = _loss_tensors(x, table, target)
+    losses = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    lse = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _call("CrossEntropy", CrossEntropyArgs(
+        x=x2.data_ptr(), ldx=_ld(x2), table=table.data_ptr(), ldtable=_ld(table), target=target.data_ptr(), loss=losses.data_ptr(),
+        lse=lse.data_ptr(), rows=x2.shape[0], width=table.shape[1], vocab=table.shape[0], ignore=ignore_index,
+        type=_TYPES[x.dtype]), x.device)
+    return losses, lse
 
 
 def cross_entropy_backward(grad, x, table, target, lse, ignore_index=-100):
     """(dx, dtable) for the gradient `grad` of the losses (float32); lse as the forward call gave it.  The logits are
     computed again, a piece of the table at a time."""
-    a, held = _loss_args(x, table, target, ignore_index)
-    grad = _vector(grad.reshape(-1), a.rows, "grad", torch.float32, x.device)
-    lse = _vector(lse.reshape(-1), a.rows, "lse", torch.float32, x.device)
+    x2, table, target = _loss_tensors(x, table, target)
+    rows, width = x2.shape
+    grad = _vector(grad.reshape(-1), rows, "grad", torch.float32, x.device)
+    lse = _vector(lse.reshape(-1), rows, "lse", torch.float32, x.device)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dtable = torch.empty(table.shape, dtype=x.dtype, device=x.device)
-    a.dloss, a.lse = grad.data_ptr(), lse.data_ptr()
-    a.dx, a.lddx, a.dtable = dx.data_ptr(), a.width, dtable.data_ptr()
-    _call("CrossEntropyGrad", a, x.device)
+    _call("CrossEntropyGrad", CrossEntropyArgs(
+        x=x2.data_ptr(), ldx=_ld(x2), table=table.data_ptr(), ldtable=_ld(table), target=target.data_ptr(), lse=lse.data_ptr(),
+        dloss=grad.data_ptr(), dx=dx.data_ptr(), lddx=width, dtable=dtable.data_ptr(), rows=rows, width=width, vocab=table.shape[0],
+        ignore=ignore_index, type=_TYPES[x.dtype]), x.device)
     return dx, dtable
 
 

@@ -5,6 +5,7 @@
 #include "cleartext.h"
 #include "norm.h"
 #include "products.h"
+#include "skinny.h"
 #include "../../include/helrm_hip.h"
 
 namespace {
@@ -117,7 +118,33 @@ int add_pairs(ProductArgs& p, const Held& a, const Held& b, const Held* b2 = nul
 // The scratch of the largest of an operator's products, which use it in turn.
 float* scratch(Arena& m, std::initializer_list<size_t> sizes) { return m.take<float>(std::max(sizes) / sizeof(float)); }
 
+// Single vectors: two kernels that read the weights once.
+size_t mlp_skinny(const GatedMLPArgs* a, bool count, hipStream_t st) {
+  Arena m{count ? nullptr : (char*)a->workspace};
+  const long ldh = up8(a->hidden);
+  void* h = m.bytes((size_t)a->rows * ldh * dtype_size(a->type));
+  if (count) return m.used;
+  SkinnyArgs p{};
+  p.dtype = a->type;
+  p.T = (int)a->rows; p.N = a->hidden; p.K = a->width;
+  p.x = a->x; p.ldx = a->ldx;
+  p.w = a->gate; p.ldw = a->ldgate;
+  p.w2 = a->up; p.ldw2 = a->ldup;
+  p.out = h; p.ldout = ldh;
+  p.g = a->g; p.u = a->u; p.ldg = ldh;
+  p.act = a->act;
+  for (int i = 0; i < 4; i++) p.coef[i] = a->coef[i];
+  skinny_gate(p, st);
+  p.N = a->width; p.K = a->hidden;
+  p.x = h; p.ldx = ldh;
+  p.w = a->down; p.ldw = a->lddown;
+  p.out = a->y; p.ldout = a->ldy;
+  skinny_store(p, st);
+  return m.used;
+}
+
 size_t mlp_forward(const GatedMLPArgs* a, bool count, hipStream_t st) {
+  if (a->rows <= skinny_rows(a->type)) return mlp_skinny(a, count, st);
   Arena m{count ? nullptr : (char*)a->workspace};
   const int type = a->type;
   const bool same = a->ldgate == a->ldup;
@@ -207,7 +234,23 @@ void check_ce_tensors(const CrossEntropyArgs* a) {
   require(a->lse || !a->rows, "CrossEntropy: lse");
 }
 
+size_t ce_skinny(const CrossEntropyArgs* a, bool count, hipStream_t st) {
+  Arena m{count ? nullptr : (char*)a->workspace};
+  SkinnyArgs p{};
+  p.dtype = a->type;
+  p.T = (int)a->rows; p.N = a->vocab; p.K = a->width;
+  p.x = a->x; p.ldx = a->ldx;
+  p.w = a->table; p.ldw = a->ldtable;
+  p.target = a->target;
+  p.picked = m.take<float>(a->rows);
+  p.part = m.take<float2>((size_t)a->rows * skinny_softmax_parts(a->vocab));
+  if (count) return m.used;
+  skinny_softmax(p, a->ignore, a->loss, a->lse, st);
+  return m.used;
+}
+
 size_t ce_forward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
+  if (a->rows <= skinny_rows(a->type)) return ce_skinny(a, count, st);
   Arena m{count ? nullptr : (char*)a->workspace};
   const long n = a->rows;
   const int parts = softmax_parts(n, a->vocab, a->width, a->type == DT_F32 ? 6 : 1);

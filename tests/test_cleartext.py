@@ -95,7 +95,7 @@ def test_workspaces(lib):
         assert need > 0
         assert size(ctypes.byref(make(rows=5000))) > need        # rows, width and type lie where the library reads them
         if make is not mlp:                                       # the block's takes the hidden values alone
-            assert size(ctypes.byref(make(width=5000))) > need
+            assert size(ctypes.byref(make(rows=500, width=5000))) > size(ctypes.byref(make(rows=500)))
         assert size(ctypes.byref(make(type=3))) == -1
         a = make(workspace=SOME, workspaceBytes=need - 1)
         refused(lib, call, a, "workspace too small")
