@@ -31,53 +31,54 @@ from .backend import CrossEntropyArgs, GatedMLPArgs, HipError, LayerNormArgs, lo
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {"silu": 0, "gelu": 1}
 
-_lib = None
 # the handle of the current stream, without making a Stream object of it (a microsecond of a small call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+# entry point -> (the call, its workspace's size or None), once the library is there
+_calls = {}
+
+
 def _library():
-    global _lib
-    if _lib is None:
-        lib = load_library()
-        # a stream or pointer of one HIP runtime means nothing to another one: torch brings its own, and the
-        # library takes that one if it is there when the library is loaded
-        with open("/proc/self/maps") as f:
-            runtimes = {line.split()[-1] for line in f if "libamdhip64.so" in line}
-        if len(runtimes) > 1:
-            raise HipError("two HIP runtimes in one process (" + ", ".join(sorted(runtimes))
-                           + "): import torch before the library is loaded")
-        for name in ("LayerNorm", "LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad"):
-            call = getattr(lib, name)
-            call.argtypes, call.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
-        for name in ("LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad"):
-            size = getattr(lib, name + "Workspace")
+    lib = load_library()
+    # a stream or pointer of one HIP runtime means nothing to another one: torch brings its own, and the
+    # library takes that one if it is there when the library is loaded
+    with open("/proc/self/maps") as f:
+        runtimes = {line.split()[-1] for line in f if "libamdhip64.so" in line}
+    if len(runtimes) > 1:
+        raise HipError("two HIP runtimes in one process (" + ", ".join(sorted(runtimes))
+                       + "): import torch before the library is loaded")
+    for name in ("LayerNorm", "LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad"):
+        call, size = getattr(lib, name), getattr(lib, name + "Workspace") if name != "LayerNorm" else None
+        call.argtypes, call.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
+        if size is not None:
             size.argtypes, size.restype = [ctypes.c_void_p], ctypes.c_long
-        _lib = lib
-    return _lib
+        _calls[name] = call, size
 
 
-def _refused(lib):
-    raise HipError(lib.GetLastError().decode())
+def _refused():
+    raise HipError(load_library().GetLastError().decode())
 
 
-def _call(name, args, device, sized=True):
-    """Queue one entry point on the current stream, with a workspace of the size it asks for."""
-    lib = _lib or _library()
+def _call(name, args, device):
+    """Queue one entry point on the current stream; a workspace of the size it asks for is there while it runs."""
+    if not _calls:
+        _library()
+    call, size = _calls[name]
     index = device.index
     if index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return _call(name, args, device, sized)
+            return _call(name, args, device)
     ref = ctypes.byref(args)
     space = None
-    if sized:
-        need = getattr(lib, name + "Workspace")(ref)
+    if size is not None and not args.workspace:
+        need = size(ref)
         if need < 0:
-            _refused(lib)
+            _refused()
         space = torch.empty(need, dtype=torch.uint8, device=device)
         args.workspace, args.workspaceBytes = space.data_ptr(), need
-    if getattr(lib, name)(ref, _raw_stream(index)):
-        _refused(lib)
+    if call(ref, _raw_stream(index)):
+        _refused()
 
 
 def _need(ok, what):
@@ -144,7 +145,7 @@ def _norm_forward(x, weight, bias, eps, keep):
     _call("LayerNorm", LayerNormArgs(
         x=x2.data_ptr(), ldx=_ld(x2), weight=weight.data_ptr(), bias=None if bias is None else bias.data_ptr(),
         y=y.data_ptr(), ldy=width, mean=mean.data_ptr() if keep else None, rstd=rstd.data_ptr() if keep else None,
-        rows=rows, width=width, type=_TYPES[x.dtype], paramType=_TYPES[weight.dtype], eps=eps), x.device, sized=False)
+        rows=rows, width=width, type=_TYPES[x.dtype], paramType=_TYPES[weight.dtype], eps=eps), x.device)
     return y, mean, rstd
 
 

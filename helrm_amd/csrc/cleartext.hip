@@ -90,15 +90,21 @@ Held hold(Arena& m, long rows, long width, int type) {
   const long ld = up8(width), part = rows * ld;
   return {m.take<uint16_t>((size_t)part * (type == DT_F32 ? 3 : 1)), ld, part};
 }
-// Where alignment, an odd width or float32 does not let the tiles be loaded
-// from the matrix itself it is copied first: a pass over it, which a product
-// of more than a few rows reads many times.
-Held held(Arena& m, const void* p, long ld, long rows, long width, int type, hipStream_t st, bool same_ld_as_next = true) {
-  if (fits(p, ld, rows, width, type) && same_ld_as_next) return {(const uint16_t*)p, rows > 1 ? ld : width, 0};
-  Held h = hold(m, rows, width, type);
-  if (m.base) lay_out(p, ld, type, (void*)h.p, h.ld, h.part, nullptr, nullptr, rows, (int)width, st);
-  return h;
-}
+// Matrices that are copied first, all in one launch: where alignment, an odd
+// width or float32 does not let the tiles be loaded from a matrix itself.  A
+// pass over it; a product of more than a few rows reads it many times.
+struct Copies {
+  LayOut j[8];
+  int n = 0;
+  const Held& add(const Held& h, const void* p, long ld, long rows, long width, const int* at = nullptr, const int* count = nullptr) {
+    j[n++] = {p, ld, (void*)h.p, h.ld, h.part, at, count, rows, (int)width};
+    return h;
+  }
+  Held held(Arena& m, const void* p, long ld, long rows, long width, int type, bool same_ld = true) {
+    if (fits(p, ld, rows, width, type) && same_ld) return {(const uint16_t*)p, rows > 1 ? ld : width, 0};
+    return add(hold(m, rows, width, type), p, ld, rows, width);
+  }
+};
 // The pairs of parts whose products make one product: of three parts of 8 bits
 // each those above 2^-24, smallest first.
 int add_pairs(ProductArgs& p, const Held& a, const Held& b, const Held* b2 = nullptr) {
@@ -116,7 +122,7 @@ int add_pairs(ProductArgs& p, const Held& a, const Held& b, const Held* b2 = nul
 }
 
 // The scratch of the largest of an operator's products, which use it in turn.
-float* scratch(Arena& m, std::initializer_list<size_t> sizes) { return m.take<float>(std::max(sizes) / sizeof(float)); }
+float* scratch(Arena& m, std::initializer_list<size_t> sizes) { return (float*)m.bytes(std::max(sizes)); }
 
 // Single vectors: two kernels that read the weights once.
 size_t mlp_skinny(const GatedMLPArgs* a, bool count, hipStream_t st) {
@@ -149,18 +155,21 @@ size_t mlp_forward(const GatedMLPArgs* a, bool count, hipStream_t st) {
   const int type = a->type;
   const bool same = a->ldgate == a->ldup;
   const Held h = hold(m, a->rows, a->hidden, type);
-  const Held x = held(m, a->x, a->ldx, a->rows, a->width, type, st);
-  const Held gate = held(m, a->gate, a->ldgate, a->hidden, a->width, type, st, same && fits(a->up, a->ldup, a->hidden, a->width, type));
-  const Held up = held(m, a->up, a->ldup, a->hidden, a->width, type, st, same && fits(a->gate, a->ldgate, a->hidden, a->width, type));
-  const Held down = held(m, a->down, a->lddown, a->width, a->hidden, type, st);
+  Copies copy;
+  const Held x = copy.held(m, a->x, a->ldx, a->rows, a->width, type);
+  const Held gate = copy.held(m, a->gate, a->ldgate, a->hidden, a->width, type, same && fits(a->up, a->ldup, a->hidden, a->width, type));
+  const Held up = copy.held(m, a->up, a->ldup, a->hidden, a->width, type, same && fits(a->gate, a->ldgate, a->hidden, a->width, type));
+  const Held down = copy.held(m, a->down, a->lddown, a->width, a->hidden, type);
   const int parts = type == DT_F32 ? 6 : 1;
-  float* partial = scratch(m, {product_scratch(a->rows, a->width, a->hidden, parts)});
+  float* partial = scratch(m, {product_scratch({{a->rows, a->hidden}}, a->width, parts, true), product_scratch({{a->rows, a->width}}, a->hidden, parts)});
   if (count) return m.used;
+  lay_out(copy.j, copy.n, type, st);
   ProductArgs p{};
   p.dtype = type;
   p.M = (int)a->rows; p.N = a->hidden; p.K = a->width;
   add_pairs(p, x, gate, &up);
   p.g = a->g; p.u = a->u; p.h = (void*)h.p; p.ldh = h.ld; p.hpart = h.part;
+  p.partial = partial;
   set_act(p, a);
   product_gate(p, st);
   ProductArgs q{};
@@ -178,20 +187,24 @@ size_t mlp_backward(const GatedMLPArgs* a, bool count, hipStream_t st) {
   const int type = a->type;
   const bool same = a->ldgate == a->ldup;
   const Held dg = hold(m, a->rows, a->hidden, type), du = hold(m, a->rows, a->hidden, type), h = hold(m, a->rows, a->hidden, type);
-  const Held x = held(m, a->x, a->ldx, a->rows, a->width, type, st), dy = held(m, a->dy, a->lddy, a->rows, a->width, type, st);
-  const Held gate = held(m, a->gate, a->ldgate, a->hidden, a->width, type, st, same && fits(a->up, a->ldup, a->hidden, a->width, type));
-  const Held up = held(m, a->up, a->ldup, a->hidden, a->width, type, st, same && fits(a->gate, a->ldgate, a->hidden, a->width, type));
-  const Held down = held(m, a->down, a->lddown, a->width, a->hidden, type, st);
+  Copies copy;
+  const Held x = copy.held(m, a->x, a->ldx, a->rows, a->width, type), dy = copy.held(m, a->dy, a->lddy, a->rows, a->width, type);
+  const Held gate = copy.held(m, a->gate, a->ldgate, a->hidden, a->width, type, same && fits(a->up, a->ldup, a->hidden, a->width, type));
+  const Held up = copy.held(m, a->up, a->ldup, a->hidden, a->width, type, same && fits(a->gate, a->ldgate, a->hidden, a->width, type));
+  const Held down = copy.held(m, a->down, a->lddown, a->width, a->hidden, type);
   const int parts = type == DT_F32 ? 6 : 1;
-  float* partial = scratch(m, {product_scratch(a->rows, a->width, a->hidden, 2 * parts), product_scratch(a->hidden, a->width, a->rows, parts),
-                               product_scratch(a->width, a->hidden, a->rows, parts)});
+  const Shape in{a->hidden, a->width}, out{a->width, a->hidden};
+  float* partial = scratch(m, {product_scratch({{a->rows, a->hidden}}, a->width, parts), product_scratch({{a->rows, a->width}}, a->hidden, 2 * parts),
+                               product_scratch({in, in, out}, a->rows, parts)});
   if (count) return m.used;
+  lay_out(copy.j, copy.n, type, st);
   // dh = dy down, and through the product and the activation
   ProductArgs p{};
   p.dtype = type;
   p.M = (int)a->rows; p.N = a->hidden; p.K = a->width;
   add_pairs(p, dy, down);
   p.g = a->g; p.u = a->u; p.h = (void*)h.p; p.dg = (void*)dg.p; p.du = (void*)du.p; p.ldh = h.ld; p.hpart = h.part;
+  p.partial = partial;
   set_act(p, a);
   product_gate_grad(p, st);
   // dx = dg gate + du up
@@ -204,18 +217,16 @@ size_t mlp_backward(const GatedMLPArgs* a, bool count, hipStream_t st) {
   q.c = a->dx; q.ldc = a->lddx;
   product_nn(q, st);
   // the weights' gradients: sums over the rows
-  auto weight = [&](const Held& l, const Held& r, long rows, long cols, void* out) {
+  auto weight = [&](const Held& l, const Held& r, const Shape& s, void* to) {
     ProductArgs w{};
     w.dtype = w.ctype = type;
-    w.M = (int)rows; w.N = (int)cols; w.K = (int)a->rows;
+    w.M = (int)s.M; w.N = (int)s.N; w.K = (int)a->rows;
     add_pairs(w, l, r);
     w.partial = partial;
-    w.c = out; w.ldc = cols;
-    product_tn(w, st);
+    w.c = to; w.ldc = s.N;
+    return w;
   };
-  weight(dg, x, a->hidden, a->width, a->dgate);
-  weight(du, x, a->hidden, a->width, a->dup);
-  weight(dy, h, a->width, a->hidden, a->ddown);
+  product_tn(weight(dg, x, in, a->dgate), weight(du, x, in, a->dup), weight(dy, h, out, a->ddown), st);
   return m.used;
 }
 
@@ -259,10 +270,12 @@ size_t ce_forward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
   r.picked = m.take<float>(n); r.loss = a->loss; r.lse = a->lse;
   const Held x = hold(m, n, a->width, a->type);
   float2* part = m.take<float2>((size_t)n * parts);
-  const Held table = held(m, a->table, a->ldtable, a->vocab, a->width, a->type, st);
+  Copies copy;
+  copy.add(x, a->x, a->ldx, n, a->width, r.rows, r.count);
+  const Held table = copy.held(m, a->table, a->ldtable, a->vocab, a->width, a->type);
   if (count) return m.used;
   kept_rows(r, st);
-  lay_out(a->x, a->ldx, a->type, (void*)x.p, x.ld, x.part, r.rows, r.count, n, a->width, st);
+  lay_out(copy.j, copy.n, a->type, st);
   ProductArgs p{};
   p.dtype = a->type;
   p.M = (int)n; p.N = a->vocab; p.K = a->width;
@@ -292,12 +305,14 @@ size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
   const Held x = hold(m, n, a->width, a->type), dl = hold(m, n, piece, a->type);
   float* acc = m.take<float>((size_t)n * D);
   const int parts = a->type == DT_F32 ? 6 : 1, last = a->vocab % piece ? a->vocab % piece : piece;
-  float* partial = scratch(m, {product_scratch(n, D, piece, parts), product_scratch(n, D, last, parts), product_scratch(piece, D, n, parts),
-                               product_scratch(last, D, n, parts)});
-  const Held table = held(m, a->table, a->ldtable, a->vocab, a->width, a->type, st);
+  float* partial = scratch(m, {product_scratch({{n, D}}, piece, parts), product_scratch({{n, D}}, last, parts), product_scratch({{piece, D}}, n, parts),
+                               product_scratch({{last, D}}, n, parts)});
+  Copies copy;
+  copy.add(x, a->x, a->ldx, n, a->width, r.rows, r.count);
+  const Held table = copy.held(m, a->table, a->ldtable, a->vocab, a->width, a->type);
   if (count) return m.used;
   kept_rows(r, st);
-  lay_out(a->x, a->ldx, a->type, (void*)x.p, x.ld, x.part, r.rows, r.count, n, a->width, st);
+  lay_out(copy.j, copy.n, a->type, st);
   for (long v0 = 0; v0 < a->vocab; v0 += piece) {
     const int len = (int)std::min<long>(piece, a->vocab - v0);
     const Held rows{table.p + v0 * table.ld, table.ld, table.part};

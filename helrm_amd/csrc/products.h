@@ -1,6 +1,7 @@
 // products.h -- launches of products.hip: the matrix products of the gated
 // block and of the cross entropy, with what follows each done on the tile.
 #pragma once
+#include <initializer_list>
 #include "cleartext.h"
 
 // act(g): silu g/(1 + e^-g), gelu g Phi(g), cubic ((c3 g + c2) g + c1) g + c0
@@ -20,9 +21,9 @@ struct ProductArgs {
   int dtype;                 // of the operator; the factors of a float32 one are its bfloat16 parts
   const int* count;          // on the device, may be null: the rows present, in the place of M
   bool count_k;              // in the place of K
-  // store
-  float* partial;            // product_scratch bytes
+  float* partial;            // product_scratch bytes (but softmax)
   int splits;                // (of the launch)
+  // store
   void* c; long ldc; int ctype; bool add;  // add: c (float32) += the product
   const float* unscale;      // the product is divided by this, where there is one
   // gate
@@ -43,11 +44,13 @@ struct ProductArgs {
 void product_gate(const ProductArgs& p, hipStream_t st);
 // v = A B, A's rows along k, B's along n: dg = v u act'(g), du = v act(g), h = act(g) u
 void product_gate_grad(const ProductArgs& p, hipStream_t st);
-// Bytes that the next three need of a product's shape at `partial`.
-size_t product_scratch(long M, long N, long K, int pairs);
+// Bytes that a product (softmax but) of these shapes needs at `partial`, or products in one launch together.
+struct Shape { long M, N; };
+size_t product_scratch(std::initializer_list<Shape> shapes, long K, int pairs, bool gate = false);
 void product_nt(const ProductArgs& p, hipStream_t st);  // A B^T
 void product_nn(const ProductArgs& p, hipStream_t st);  // A B
 void product_tn(const ProductArgs& p, hipStream_t st);  // A^T B
+void product_tn(ProductArgs a, ProductArgs b, ProductArgs c, hipStream_t st);  // three of the same K in one launch, a.partial of all
 // the products of rows of A with rows of the table go into part and picked
 void product_softmax(const ProductArgs& p, hipStream_t st);
 // (exp(A B^T - lse) - onehot(target)) grad into c, in the layout of a factor
@@ -55,9 +58,16 @@ void product_softmax_grad(const ProductArgs& p, hipStream_t st);
 // pieces of a row that product_softmax leaves
 int softmax_parts(long M, long N, long K, int pairs);
 
-// A factor in the layout above: row rows[i] (or i) of `from` to row i of `to`, for i < *count (or n); a float32 one
-// as three parts `part` elements apart.
-void lay_out(const void* from, long ld, int dtype, void* to, long ldto, long part, const int* rows, const int* count, long n, int width, hipStream_t st);
+// Matrices into the layout above, up to 8 in one launch: row rows[i] (or i) of
+// `from` to row i of `to`, for i < *count (or n); a float32 one as three parts
+// `part` elements apart.
+struct LayOut {
+  const void* from; long ld;
+  void* to; long ldto, part;
+  const int* rows; const int* count;
+  long n; int width;
+};
+void lay_out(const LayOut* jobs, int n, int dtype, hipStream_t st);
 
 // Rows whose target is not `ignore`, in order: rows[], tgt[] (-1: outside [0,
 // vocab)), *count.  Forward (loss): picked[] = NaN, and loss and lse of the

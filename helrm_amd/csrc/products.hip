@@ -27,6 +27,13 @@ namespace {
 
 constexpr int STEP = 64;                 // k of a step
 constexpr int XCDS = 8;
+// Products of one launch, in the order of their workgroups.
+struct Batch {
+  ProductArgs p[3];
+  int first[3];
+  int count;
+  __device__ __forceinline__ int which(int block) const { return count > 2 && block >= first[2] ? 2 : count > 1 && block >= first[1] ? 1 : 0; }
+};
 constexpr unsigned OUTSIDE = 0x80000000u;  // an offset past every descriptor's bound
 
 enum Epi { EPI_STORE, EPI_GATE, EPI_GATE_GRAD, EPI_SOFTMAX, EPI_SOFTMAX_GRAD };
@@ -209,6 +216,56 @@ __device__ __forceinline__ void softmax_piece(const ProductArgs& p, const f32x4 
   }
 }
 
+// What becomes of four neighbouring columns of a row, n columns from the end
+// of the matrix (`left`), at element first + at of the results (gate: v of the
+// gate, u of the up projection).
+struct RowValues { float lse, grad; int target; };
+template <class T, int EPI>
+__device__ __forceinline__ void emit4(const ProductArgs& p, long first, unsigned at, int left, const RowValues& row, float v[4], float u[4]) {
+  if (left < 4) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) if (e >= left) v[e] = u[e] = 0.0f;   // the columns that fill a row up are 0
+  }
+  if (EPI == EPI_STORE) {
+    store4<T>(p, first + at, left, v);
+  } else if (EPI == EPI_GATE) {
+    float a[4], d[4];
+    act4(p.act, p.coef, v, a, d);
+#pragma unroll
+    for (int e = 0; e < 4; e++) a[e] *= u[e];
+    if (p.g) {   // (read again in the backward pass only: past the caches they are written twice as fast)
+      __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, (f32x4*)(p.g + first + at));
+      __builtin_nontemporal_store(f32x4{u[0], u[1], u[2], u[3]}, (f32x4*)(p.u + first + at));
+    }
+    put_held<T>((u16*)p.h + first + at, p.dtype, p.hpart, a);
+  } else if (EPI == EPI_GATE_GRAD) {
+    float g[4], a[4], d[4];
+    get4(p.g + first + at, g);
+    get4(p.u + first + at, u);
+    act4(p.act, p.coef, g, a, d);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {   // (g, u and v are 0 in the columns that fill a row up)
+      d[e] *= v[e] * u[e];
+      v[e] *= a[e];
+      a[e] *= u[e];
+    }
+    put_held<T>((u16*)p.dg + first + at, p.dtype, p.hpart, d);
+    put_held<T>((u16*)p.du + first + at, p.dtype, p.hpart, v);
+    put_held<T>((u16*)p.h + first + at, p.dtype, p.hpart, a);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = e < left ? (__expf(v[e] - row.lse) - (row.target == e ? 1.0f : 0.0f)) * row.grad : 0.0f;
+    put_held<T>((u16*)p.c + first + at, p.dtype, p.hpart, v);
+  }
+}
+
+// Elements from one row of the results to the next, and of a split product's sums (gate: the gate's, then the up projection's).
+template <int EPI> __device__ __host__ __forceinline__ long result_ld(const ProductArgs& p) {
+  return EPI == EPI_STORE || EPI == EPI_SOFTMAX_GRAD ? p.ldc : p.ldh;
+}
+template <int EPI> __device__ __host__ __forceinline__ long sum_cols(const ProductArgs& p) { return EPI == EPI_STORE ? (p.N + 3) & ~3 : p.ldh; }
+template <int EPI> __device__ __host__ __forceinline__ long sum_ld(const ProductArgs& p) { return sum_cols<EPI>(p) * (EPI == EPI_GATE ? 2 : 1); }
+
 // A wave's accumulators go through its own part of LDS, 64 rows of 64 float32
 // columns at a time (16 bytes c of row r at c ^ (r & 15)), so that what is
 // stored are whole lines of a row and the code of it is there once.  A place is
@@ -220,23 +277,21 @@ __device__ __forceinline__ void emit(const ProductArgs& p, const f32x4 (&acc)[FM
   const int lane = threadIdx.x & 63, col = lane % LANES;
   // gate: the columns are 16 of the gate, the same 16 of the up projection, 16 of the gate, ...
   const int c = EPI == EPI_GATE ? (col >> 2) * 8 + (col & 3) : col;
-  const bool sums = EPI == EPI_STORE && p.splits > 1;
-  const unsigned ld = sums ? (p.N + 3) & ~3 : EPI == EPI_STORE || EPI == EPI_SOFTMAX_GRAD ? (unsigned)p.ldc : (unsigned)p.ldh;
-  const long first = mw * ld + nw;
+  const bool sums = EPI != EPI_SOFTMAX_GRAD && p.splits > 1;
+  const unsigned ld = (unsigned)(sums ? sum_ld<EPI>(p) : result_ld<EPI>(p));
+  const long first = (sums ? (long)split * p.M * ld : 0) + mw * ld + nw;
+  const unsigned second = EPI == EPI_GATE ? (unsigned)sum_cols<EPI>(p) : 0;
   // columns that there are from the lane's first one on, and columns with the zeros that fill an intermediate's row up
   const int left = (int)min((long)p.N - nw, 64L) - col * 4;
   const int room = EPI == EPI_STORE ? left : (int)min(((p.N + 7L) & ~7L) - nw, 64L) - col * 4;
-  float* const sum_at = sums ? p.partial + (long)split * p.M * ld + first : nullptr;
-  u16* const h = (u16*)(EPI == EPI_SOFTMAX_GRAD ? p.c : p.h) + first;
 #pragma unroll
   for (int part = 0; part < FM / 4; part++) {
-    float lse = 0, grad = 0;   // of row `lane` of the 64
-    int target = 0;
+    RowValues mine{};   // of row `lane` of the 64
     if (EPI == EPI_SOFTMAX_GRAD && mw + part * 64 + lane < M) {
       const long m = mw + part * 64 + lane;
-      target = p.target[m];
-      lse = p.lse[m];
-      grad = target < 0 ? NAN : p.grad[m] * (p.scale ? *p.scale : 1.0f);
+      mine.target = p.target[m];
+      mine.lse = p.lse[m];
+      mine.grad = mine.target < 0 ? NAN : p.grad[m] * (p.scale ? *p.scale : 1.0f);
     }
 #pragma unroll
     for (int i = 0; i < 4; i++)
@@ -252,45 +307,15 @@ __device__ __forceinline__ void emit(const ProductArgs& p, const f32x4 (&acc)[FM
       float v[4], u[4] = {0, 0, 0, 0};
       get4(lds + r * 64 + ((c ^ (r & 15)) * 4), v);
       if (EPI == EPI_GATE) get4(lds + r * 64 + (((c + 4) ^ (r & 15)) * 4), u);
-      const float row_lse = EPI == EPI_SOFTMAX_GRAD ? __shfl(lse, r) : 0.0f, row_grad = EPI == EPI_SOFTMAX_GRAD ? __shfl(grad, r) : 0.0f;
-      const int t = EPI == EPI_SOFTMAX_GRAD ? __shfl(target, r) - (int)(p.n0 + nw) - col * 4 : 0;
+      RowValues row{};
+      if (EPI == EPI_SOFTMAX_GRAD) row = {__shfl(mine.lse, r), __shfl(mine.grad, r), __shfl(mine.target, r) - (int)(p.n0 + nw) - col * 4};
       if (r >= rows || room <= 0) continue;
       const unsigned at = (part * 64 + r) * ld + col * 4;
-      if (left < 4) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) if (e >= left) v[e] = u[e] = 0.0f;
-      }
-      if (EPI == EPI_STORE) {
-        if (sums) *(float4*)(sum_at + at) = make_float4(v[0], v[1], v[2], v[3]);
-        else store4<T>(p, first + at, left, v);
-      } else if (EPI == EPI_GATE) {
-        float a[4], d[4];
-        act4(p.act, p.coef, v, a, d);
-#pragma unroll
-        for (int e = 0; e < 4; e++) a[e] *= u[e];
-        if (p.g) {
-          __builtin_nontemporal_store(f32x4{v[0], v[1], v[2], v[3]}, (f32x4*)(p.g + first + at));
-          __builtin_nontemporal_store(f32x4{u[0], u[1], u[2], u[3]}, (f32x4*)(p.u + first + at));
-        }
-        put_held<T>(h + at, p.dtype, p.hpart, a);
-      } else if (EPI == EPI_GATE_GRAD) {
-        float g[4], a[4], d[4];
-        get4(p.g + first + at, g);
-        get4(p.u + first + at, u);
-        act4(p.act, p.coef, g, a, d);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {   // (g, u and v are 0 in the columns that fill a row up)
-          d[e] *= v[e] * u[e];
-          v[e] *= a[e];
-          a[e] *= u[e];
-        }
-        put_held<T>((u16*)p.dg + first + at, p.dtype, p.hpart, d);
-        put_held<T>((u16*)p.du + first + at, p.dtype, p.hpart, v);
-        put_held<T>(h + at, p.dtype, p.hpart, a);
+      if (sums) {
+        *(float4*)(p.partial + first + at) = make_float4(v[0], v[1], v[2], v[3]);
+        if (EPI == EPI_GATE) *(float4*)(p.partial + first + second + at) = make_float4(u[0], u[1], u[2], u[3]);
       } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = e < left ? (__expf(v[e] - row_lse) - (t == e ? 1.0f : 0.0f)) * row_grad : 0.0f;
-        put_held<T>(h + at, p.dtype, p.hpart, v);
+        emit4<T, EPI>(p, first, at, left, row, v, u);
       }
     }
   }
@@ -321,7 +346,10 @@ template <int READS, int MULS> __device__ __forceinline__ void spread() {
 }
 
 template <class T, int BM, int BN, int WM, int WN, bool A_K, bool B_K, int EPI>
-__global__ __launch_bounds__(WM* WN * 64) void product_kernel(const ProductArgs p) {
+__global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Batch batch) {
+  const int which = batch.which(blockIdx.x);
+  const ProductArgs& p = batch.p[which];
+  const int id = blockIdx.x - batch.first[which];
   constexpr int W = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
   constexpr int COLS = EPI == EPI_GATE ? BN / 2 : BN;   // columns of C in a tile
   // Arrays of their own, not one: only so does the compiler see that a load into one does not concern reads of another.
@@ -329,9 +357,9 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const ProductArgs 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave_m = wave / WN, wave_n = wave % WN;
   const int nm = (p.M + BM - 1) / BM, nn = (p.N + COLS - 1) / COLS;
-  const int split = blockIdx.x / (nm * nn);
+  const int split = id / (nm * nn);
   int tile_m, tile_n;
-  tile_of(blockIdx.x - split * nm * nn, nm * nn, nm, nn, tile_m, tile_n);
+  tile_of(id - split * nm * nn, nm * nn, nm, nn, tile_m, tile_n);
   const long m0 = (long)tile_m * BM, n0 = (long)tile_n * COLS;
   int M = p.M, K = p.K;
   if (p.count) { if (p.count_k) K = *p.count; else M = *p.count; }
@@ -470,36 +498,51 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const ProductArgs 
   }
 }
 
-// The sums of a split product, four columns a thread.
-template <class T>
-__global__ __launch_bounds__(256) void join_kernel(const ProductArgs p) {
-  const long cols = (p.N + 3) / 4, i = blockIdx.x * 256L + threadIdx.x;
+// The sums of split products, four columns a thread, and what becomes of them.
+template <class T, int EPI>
+__global__ __launch_bounds__(256) void join_kernel(const Batch batch) {
+  const int which = batch.which(blockIdx.x);
+  const ProductArgs& p = batch.p[which];
+  const long cols = sum_cols<EPI>(p) / 4, i = (blockIdx.x - batch.first[which]) * 256L + threadIdx.x;
   const long m = i / cols, n = (i - m * cols) * 4;
   if (m >= (p.count && !p.count_k ? *p.count : p.M)) return;
-  float v[4] = {0, 0, 0, 0};
+  float v[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
+#pragma unroll 4
   for (int s = 0; s < p.splits; s++) {
+    const float* at = p.partial + ((long)s * p.M + m) * sum_ld<EPI>(p) + n;
     float t[4];
-    get4(p.partial + ((long)s * p.M + m) * (cols * 4) + n, t);
+    get4(at, t);
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] += t[e];
+    if (EPI == EPI_GATE) {
+      get4(at + cols * 4, t);
+#pragma unroll
+      for (int e = 0; e < 4; e++) u[e] += t[e];
+    }
   }
-  store4<T>(p, m * p.ldc + n, (int)min(p.N - n, 4L), v);
+  emit4<T, EPI>(p, m * result_ld<EPI>(p) + n, 0, (int)min(p.N - n, 4L), RowValues{}, v, u);
 }
 
-// The tile and the splits of a product: the least time of its rounds over the
-// 256 CUs, which hold one 256 x 256 tile or two 128 x 128 ones (whose steps
-// and ends overlap).  Microseconds, measured: a step 1.6 and 1.0, the end of a
-// tile 10 and 6. The large tile has half the traffic for each product, the
-// small one fills the GPU with a quarter of the rows.
+// The tile and the splits of products in one launch: the least time of their
+// rounds over the 256 CUs, which hold one 256 x 256 tile or two 128 x 128 ones
+// (whose steps and ends overlap).  Microseconds, measured: a step 1.6 and 1.0,
+// the end of a tile 10 and 6.  The large tile has half the traffic for each
+// product, the small one fills the GPU with a quarter of the rows.
 struct Plan { bool big; int splits; };
-Plan plan_of(long M, long N, long steps, bool gate, bool may_split) {
+Plan plan_of(std::initializer_list<Shape> shapes, long steps, bool gate, bool may_split) {
   Plan best{};
   double least = 1e30;
   for (int big = 0; big < 2; big++) {
-    const long size = big ? 256 : 128, tiles = clr::ceil_div(M, size) * clr::ceil_div(N, gate ? size / 2 : size);
+    const long size = big ? 256 : 128;
+    long tiles = 0;
+    double results = 0;
+    for (const Shape& s : shapes) {
+      tiles += clr::ceil_div(s.M, size) * clr::ceil_div(s.N, gate ? size / 2 : size);
+      results += (double)s.M * s.N * (gate ? 2 : 1);
+    }
     for (int s = 1; s <= (may_split ? 16 : 1); s++) {
       if (s > 1 && steps / s < 4) break;
-      const double sums = s > 1 ? 4.0 + (s + 1) * (double)M * N * 4 / 3e6 : 0.0;   // of a kernel more, and its traffic
+      const double sums = s > 1 ? 4.0 + (s + 1) * results * 4 / 3e6 : 0.0;   // of a kernel more, and its traffic
       const long rounds = clr::ceil_div(tiles * s, 256), each = clr::ceil_div(steps, s);
       const double t = (big ? rounds * (each * 1.6 + 10) : (rounds + 1) / 2 * (each * 1.0 + 6) * (rounds == 1 ? 0.6 : 1.0)) + sums;
       if (t < least) { least = t; best = {big != 0, s}; }
@@ -507,40 +550,81 @@ Plan plan_of(long M, long N, long steps, bool gate, bool may_split) {
   }
   return best;
 }
-Plan plan_of(const ProductArgs& p, bool gate, bool may_split) {
-  return plan_of(p.M, p.N, clr::ceil_div(p.K, STEP) * p.pairs, gate, may_split);
-}
+long steps_of(long K, int pairs) { return clr::ceil_div(K, STEP) * pairs; }
 
-template <class T, bool A_K, bool B_K, int EPI> void launch_type(ProductArgs p, hipStream_t st) {
-  if (p.M <= 0 || p.N <= 0) return;
-  constexpr int half = EPI == EPI_GATE ? 2 : 1;
-  const Plan plan = plan_of(p, EPI == EPI_GATE, EPI == EPI_STORE);
-  p.splits = plan.splits;
-  const long size = plan.big ? 256 : 128, n = clr::ceil_div(p.M, size) * clr::ceil_div(p.N, size / half) * p.splits;
-  if (plan.big) product_kernel<T, 256, 256, 2, 4, A_K, B_K, EPI><<<(unsigned)n, 512, 0, st>>>(p);
-  else product_kernel<T, 128, 128, 2, 2, A_K, B_K, EPI><<<(unsigned)n, 256, 0, st>>>(p);
-  if (p.splits > 1) join_kernel<T><<<(unsigned)clr::ceil_div((long)p.M * clr::ceil_div(p.N, 4), 256), 256, 0, st>>>(p);
+template <class T, bool A_K, bool B_K, int EPI> void launch_type(Batch b, const Plan& plan, hipStream_t st) {
+  const long size = plan.big ? 256 : 128;
+  long tiles = 0, sums = 0;
+  Batch j = b;
+  for (int i = 0; i < b.count; i++) {
+    ProductArgs& p = b.p[i];
+    p.splits = j.p[i].splits = plan.splits;
+    b.first[i] = (int)tiles;
+    j.first[i] = (int)sums;
+    tiles += clr::ceil_div(p.M, size) * clr::ceil_div(p.N, EPI == EPI_GATE ? size / 2 : size) * p.splits;
+    sums += clr::ceil_div((long)p.M * (sum_cols<EPI>(p) / 4), 256);
+  }
+  if (plan.big) product_kernel<T, 256, 256, 2, 4, A_K, B_K, EPI><<<(unsigned)tiles, 512, 0, st>>>(b);
+  else product_kernel<T, 128, 128, 2, 2, A_K, B_K, EPI><<<(unsigned)tiles, 256, 0, st>>>(b);
+  if constexpr (EPI == EPI_STORE || EPI == EPI_GATE || EPI == EPI_GATE_GRAD)
+    if (plan.splits > 1) join_kernel<T, EPI><<<(unsigned)sums, 256, 0, st>>>(j);
+}
+template <bool A_K, bool B_K, int EPI> void launch(std::initializer_list<ProductArgs> products, const Plan& plan, hipStream_t st) {
+  Batch b{};
+  for (const ProductArgs& p : products) if (p.M > 0 && p.N > 0) b.p[b.count++] = p;
+  if (!b.count) return;
+  if (b.p[0].dtype == DT_F16) launch_type<_Float16, A_K, B_K, EPI>(b, plan, st);
+  else launch_type<__bf16, A_K, B_K, EPI>(b, plan, st);
 }
 template <bool A_K, bool B_K, int EPI> void launch(const ProductArgs& p, hipStream_t st) {
-  if (p.dtype == DT_F16) launch_type<_Float16, A_K, B_K, EPI>(p, st);
-  else launch_type<__bf16, A_K, B_K, EPI>(p, st);
+  constexpr bool may_split = EPI == EPI_STORE || EPI == EPI_GATE || EPI == EPI_GATE_GRAD;
+  launch<A_K, B_K, EPI>({p}, plan_of({{p.M, p.N}}, steps_of(p.K, p.pairs), EPI == EPI_GATE, may_split), st);
 }
 
-// A factor in the layout that the tiles are loaded from: rows[i] (or i) of
-// `from` to row i, filled up with zeros to ldto; float32 as three parts.
+// Up to 8 matrices into the layout that the tiles are loaded from, one launch:
+// rows[i] (or i) of `from` to row i of `to`, filled up with zeros to ldto;
+// float32 as three parts.
+struct LayOuts { LayOut j[8]; int first[8]; int count; };
 template <class T>
-__global__ __launch_bounds__(256) void lay_out_kernel(const T* from, long ld, u16* to, long ldto, long part, const int* rows, const int* count, int width) {
-  const long i = blockIdx.x;
-  if (count && i >= *count) return;
-  const T* f = from + (rows ? (long)rows[i] : i) * ld;
-  for (int k = blockIdx.y * 256 + threadIdx.x; k < ldto; k += gridDim.y * 256) {
-    const T v = k < width ? f[k] : (T)0.0f;
+__global__ __launch_bounds__(256) void lay_out_kernel(const LayOuts all) {
+  int which = 0;
+  while (which + 1 < all.count && (int)blockIdx.x >= all.first[which + 1]) which++;
+  const LayOut& j = all.j[which];
+  const long i = blockIdx.x - all.first[which];
+  if (j.count && i >= *j.count) return;
+  const T* f = (const T*)j.from + (j.rows ? (long)j.rows[i] : i) * j.ld;
+  u16* to = (u16*)j.to + i * j.ldto;
+  constexpr int V = 16 / sizeof(T);
+  if (((uintptr_t)f & 15) == 0 && j.width % V == 0) {
+    for (int k = threadIdx.x * V; k < j.ldto; k += 256 * V) {
+      T v[V];
+      if (k < j.width) __builtin_memcpy(v, __builtin_assume_aligned(f + k, 16), 16);
+      else for (int e = 0; e < V; e++) v[e] = (T)0.0f;
+      if constexpr (sizeof(T) == 4) {
+        float q[3][4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          __bf16 s[3];
+          split3(v[e], s);
+#pragma unroll
+          for (int t = 0; t < 3; t++) q[t][e] = (float)s[t];
+        }
+#pragma unroll
+        for (int t = 0; t < 3; t++) *(uint2*)(to + t * j.part + k) = pack4<__bf16>(q[t]);
+      } else {
+        __builtin_memcpy(__builtin_assume_aligned(to + k, 16), v, 16);
+      }
+    }
+    return;
+  }
+  for (int k = threadIdx.x; k < j.ldto; k += 256) {
+    const T v = k < j.width ? f[k] : (T)0.0f;
     if constexpr (sizeof(T) == 4) {
       __bf16 s[3];
       split3(v, s);
-      for (int j = 0; j < 3; j++) to[j * part + i * ldto + k] = bits(s[j]);
+      for (int t = 0; t < 3; t++) to[t * j.part + k] = bits(s[t]);
     } else {
-      to[i * ldto + k] = bits(v);
+      to[k] = bits(v);
     }
   }
 }
@@ -625,30 +709,43 @@ __global__ void zero_kernel(uint16_t* p, size_t n) {
 
 }  // namespace
 
-size_t product_scratch(long M, long N, long K, int pairs) {
-  const Plan plan = plan_of(M, N, clr::ceil_div(K, STEP) * pairs, false, true);
-  return plan.splits > 1 ? (size_t)plan.splits * M * ((N + 3) & ~3L) * sizeof(float) : 0;
+size_t product_scratch(std::initializer_list<Shape> shapes, long K, int pairs, bool gate) {
+  const Plan plan = plan_of(shapes, steps_of(K, pairs), gate, true);
+  size_t n = 0;
+  if (plan.splits > 1)
+    for (const Shape& s : shapes) n += (size_t)plan.splits * s.M * ((s.N + 7) & ~7L) * (gate ? 2 : 1);
+  return n * sizeof(float);
 }
 int softmax_parts(long M, long N, long K, int pairs) {
-  return (int)clr::ceil_div(N, plan_of(M, N, clr::ceil_div(K, STEP) * pairs, false, false).big ? 256 : 128);
+  return (int)clr::ceil_div(N, plan_of({{M, N}}, steps_of(K, pairs), false, false).big ? 256 : 128);
 }
 void product_gate(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_GATE>(p, st); }
 void product_gate_grad(const ProductArgs& p, hipStream_t st) { launch<true, false, EPI_GATE_GRAD>(p, st); }
 void product_nt(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_STORE>(p, st); }
 void product_nn(const ProductArgs& p, hipStream_t st) { launch<true, false, EPI_STORE>(p, st); }
 void product_tn(const ProductArgs& p, hipStream_t st) { launch<false, false, EPI_STORE>(p, st); }
+void product_tn(ProductArgs a, ProductArgs b, ProductArgs c, hipStream_t st) {
+  const Plan plan = plan_of({{a.M, a.N}, {b.M, b.N}, {c.M, c.N}}, steps_of(a.K, a.pairs), false, true);
+  auto sums = [&](const ProductArgs& p) { return (size_t)plan.splits * p.M * ((p.N + 7) & ~7L); };
+  b.partial = a.partial + (plan.splits > 1 ? sums(a) : 0);
+  c.partial = b.partial + (plan.splits > 1 ? sums(b) : 0);
+  launch<false, false, EPI_STORE>({a, b, c}, plan, st);
+}
 void product_softmax(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_SOFTMAX>(p, st); }
 void product_softmax_grad(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_SOFTMAX_GRAD>(p, st); }
 
-void kept_rows(const RowsArgs& a, hipStream_t st) { kept_rows_kernel<<<1, ROWS_BLOCK, 0, st>>>(a); }
-void lay_out(const void* from, long ld, int dtype, void* to, long ldto, long part, const int* rows, const int* count, long n, int width, hipStream_t st) {
-  if (!n) return;
-  const dim3 grid((unsigned)n, (unsigned)std::min<long>(16, clr::ceil_div(ldto, 256)));
-  clr::with_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    lay_out_kernel<T><<<grid, 256, 0, st>>>((const T*)from, ld, (u16*)to, ldto, part, rows, count, width);
-  });
+void lay_out(const LayOut* jobs, int n, int dtype, hipStream_t st) {
+  LayOuts all{};
+  long blocks = 0;
+  for (int i = 0; i < n; i++)
+    if (jobs[i].n > 0) {
+      all.first[all.count] = (int)blocks;
+      all.j[all.count++] = jobs[i];
+      blocks += jobs[i].n;
+    }
+  if (blocks) clr::with_type(dtype, [&](auto t) { lay_out_kernel<decltype(t)><<<(unsigned)blocks, 256, 0, st>>>(all); });
 }
+void kept_rows(const RowsArgs& a, hipStream_t st) { kept_rows_kernel<<<1, ROWS_BLOCK, 0, st>>>(a); }
 void softmax_finish(const float2* part, int parts, const float* picked, const int* rows, const int* count, long n, float* loss, float* lse, hipStream_t st) {
   if (n) finish_kernel<<<(unsigned)clr::ceil_div(n, 4), 256, 0, st>>>(part, parts, picked, rows, count, loss, lse);
 }

@@ -13,7 +13,7 @@ struct SkinnyArgs {
   float* g; float* u; long ldg;      // gate: [T][ldg] kept projections, 0 past N; may be null
   int act; float coef[4];
   const long long* target; float* picked; float2* part;   // softmax: [T], [T], [T][parts]
-  int parts, groups;                 // (of the launch)
+  int parts, groups; bool alone;     // (of the launch)
 };
 // out = act(X W^T) * (X W2^T)
 void skinny_gate(SkinnyArgs p, hipStream_t st);

@@ -71,7 +71,9 @@ template <class T> __device__ __forceinline__ f32x4 dot8(const Eight<T>& w, cons
   }
 }
 
-// A workgroup takes `groups` times 16 rows of W.  Lane l of a wave holds, of a
+// A workgroup takes `groups` times 16 rows of W; or, where there are rows
+// enough to keep every wave loading, each of its waves does (`alone`), which
+// saves the exchange of sums.  Lane l of a wave holds, of a
 // group, row l % 16 and the k 16 (l / 16) + 0..15 of 64; its sums are row t = l % 16
 // of X and the columns 4 (l / 16) + 0..3.
 template <class T, bool ALIGNED, int NB> constexpr int most_waves() { return sizeof(T) == 2 && ALIGNED && NB == 1 ? 16 : 8; }
@@ -79,13 +81,15 @@ template <class T, bool ALIGNED, int NB, int EPI>
 __global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_kernel(const SkinnyArgs p) {
   constexpr int MATS = EPI == SKINNY_GATE ? 2 : 1, TURNS = !ALIGNED ? 1 : sizeof(T) == 4 ? 2 : 4;
   extern __shared__ float lds[];   // [waves][MATS * NB][64][4]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, own = threadIdx.x >> 6;
+  const int wave = p.alone ? 0 : own, waves = p.alone ? 1 : blockDim.x >> 6;   // of those that share k
+  const long team = p.alone ? (long)blockIdx.x * (blockDim.x >> 6) + own : blockIdx.x;
   const int t = lane & 15, quad = lane >> 4;
-  float2 run[NB];   // softmax: the workgroup's piece of row t (of wave b)
+  float2 run[NB];   // softmax: the team's piece of row t (of wave b)
 #pragma unroll
   for (int b = 0; b < NB; b++) run[b] = make_float2(-INFINITY, 0.0f);
   for (int group = 0; group < p.groups; group++) {
-    const long n0 = ((long)blockIdx.x * p.groups + group) * 16;
+    const long n0 = (team * p.groups + group) * 16;
     if (n0 >= p.N) break;
     const bool in = n0 + t < p.N;
     const T* w[2] = {(const T*)p.w + (n0 + t) * p.ldw, MATS == 2 ? (const T*)p.w2 + (n0 + t) * p.ldw2 : nullptr};
@@ -178,7 +182,7 @@ __global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_ke
   if (EPI == SKINNY_SOFTMAX) {
 #pragma unroll
     for (int b = 0; b < NB; b++)
-      if (b % waves == wave && lane < 16 && b * 16 + t < p.T) p.part[(long)(b * 16 + t) * p.parts + blockIdx.x] = run[b];
+      if (b % waves == wave && lane < 16 && b * 16 + t < p.T && team < p.parts) p.part[(long)(b * 16 + t) * p.parts + team] = run[b];
   }
 }
 
@@ -213,7 +217,8 @@ int waves_of(int N, int K, int type, int most) {
 
 template <int EPI> void launch(SkinnyArgs p, hipStream_t st) {
   if (p.T <= 0 || p.N <= 0) return;
-  const unsigned grid = (unsigned)clr::ceil_div(p.N, 16L * p.groups);
+  const long teams = clr::ceil_div(p.N, 16L * p.groups);
+  p.alone = teams >= 2048;
   clr::with_type(p.dtype, [&](auto type) {
     using T = decltype(type);
     const long v = 16 / sizeof(T);
@@ -221,7 +226,8 @@ template <int EPI> void launch(SkinnyArgs p, hipStream_t st) {
     const bool aligned = p.K % 8 == 0 && fits(p.x, p.ldx) && fits(p.w, p.ldw) && (EPI != SKINNY_GATE || fits(p.w2, p.ldw2));
     auto go = [&](auto nb) {
       constexpr int NB = decltype(nb)::value;
-      const int waves = waves_of(p.N, p.K, p.dtype, aligned ? most_waves<T, true, NB>() : most_waves<T, false, NB>());
+      const int waves = p.alone ? 4 : waves_of(p.N, p.K, p.dtype, aligned ? most_waves<T, true, NB>() : most_waves<T, false, NB>());
+      const unsigned grid = (unsigned)(p.alone ? clr::ceil_div(teams, 4) : teams);
       const size_t lds = (size_t)waves * (EPI == SKINNY_GATE ? 2 : 1) * NB * 1024;
       if (aligned) skinny_kernel<T, true, NB, EPI><<<grid, waves * 64, lds, st>>>(p);
       else skinny_kernel<T, false, NB, EPI><<<grid, waves * 64, lds, st>>>(p);
@@ -238,8 +244,8 @@ template <int EPI> void launch(SkinnyArgs p, hipStream_t st) {
 
 void skinny_gate(SkinnyArgs p, hipStream_t st) { p.groups = 1; launch<SKINNY_GATE>(p, st); }
 void skinny_store(SkinnyArgs p, hipStream_t st) { p.groups = 1; launch<SKINNY_STORE>(p, st); }
-// Groups of 16 rows a workgroup takes one after another: as many as leave 2,048 workgroups.
-static int softmax_groups(int N) { return (int)std::max<long>(1, N / 16 / 2048); }
+// Groups of 16 rows a team takes one after another: as many as leave 4,096 teams.
+static int softmax_groups(int N) { return (int)std::max<long>(1, N / 16 / 4096); }
 int skinny_softmax_parts(int N) { return (int)clr::ceil_div(N, 16L * softmax_groups(N)); }
 void skinny_softmax(SkinnyArgs p, long long ignore, float* loss, float* lse, hipStream_t st) {
   p.groups = softmax_groups(p.N);

@@ -550,9 +550,10 @@ def test_workspace_refusals(ct):
     dx, dw = torch.empty_like(x), torch.empty_like(w)
     a = LayerNormArgs(x=x.data_ptr(), ldx=8, weight=w.data_ptr(), mean=mean.data_ptr(), rstd=rstd.data_ptr(), dy=x.data_ptr(), lddy=8,
                       dx=dx.data_ptr(), lddx=8, dweight=dw.data_ptr(), rows=4, width=8)
-    with pytest.raises(HipError, match="workspace too small"):
-        ct._call("LayerNormGrad", a, x.device, sized=False)
     space = torch.empty(1 << 20, dtype=torch.uint8, device=DEV)
+    a.workspace, a.workspaceBytes = space.data_ptr(), 16
+    with pytest.raises(HipError, match="workspace too small"):
+        ct._call("LayerNormGrad", a, x.device)
     a.workspace, a.workspaceBytes = space.data_ptr() + 8, space.numel() - 8
     with pytest.raises(HipError, match="aligned"):
-        ct._call("LayerNormGrad", a, x.device, sized=False)
+        ct._call("LayerNormGrad", a, x.device)
