@@ -128,7 +128,7 @@ float* scratch(Arena& m, std::initializer_list<size_t> sizes) { return (float*)m
 size_t mlp_skinny(const GatedMLPArgs* a, bool count, hipStream_t st) {
   Arena m{count ? nullptr : (char*)a->workspace};
   const long ldh = up8(a->hidden);
-  void* h = m.bytes((size_t)a->rows * ldh * dtype_size(a->type));
+  float* h = m.take<float>((size_t)a->rows * ldh);
   if (count) return m.used;
   SkinnyArgs p{};
   p.dtype = a->type;

@@ -198,9 +198,9 @@ __global__ __launch_bounds__(MANY ? 512 : BLOCK) void norm_backward(const T* dy,
   }
 }
 
-// dw and db: the sums over the workgroups' parts, 32 columns a workgroup, in
+// dw and db: the sums over the workgroups' parts, 16 columns a workgroup, in
 // a fixed order (no atomics: the gradient is the same on every run).
-constexpr int SUM_COLS = 32, SUM_ROWS = 32;
+constexpr int SUM_COLS = 16, SUM_ROWS = 64;
 template <class P>
 __global__ __launch_bounds__(SUM_COLS* SUM_ROWS) void norm_param_sum(const float* part, P* dw, P* db, int parts, int width) {
   __shared__ float lds[SUM_ROWS][SUM_COLS + 1];

@@ -182,26 +182,31 @@ __device__ __forceinline__ void softmax_piece(const ProductArgs& p, const f32x4 
                                               float2* lds) {
   const int lane = threadIdx.x & 63, quad = lane >> 4;
   const int left = (int)min((long)p.N - n0 - wave_n * FN * 16, 1L << 20) - 4 * quad;   // columns from the lane's first one on
-  const bool whole = left >= FN * 16;
+  const bool whole = (long)p.N - n0 - wave_n * FN * 16 >= FN * 16;   // of the wave: no bounds
 #pragma unroll
   for (int i = 0; i < FM; i++) {
     const int r = (wave_m * FM + i) * 16 + (lane & 15);
     const long m = m0 + r;
     const int t = m < M ? p.target[m] - (int)(n0 + wave_n * FN * 16 + 4 * quad) : -1;   // the target's place from there
-    float v[FN * 4], top = -INFINITY, sum = 0;
-#pragma unroll
-    for (int c = 0; c < FN * 4; c++) {
-      v[c] = whole || 16 * (c >> 2) + (c & 3) < left ? acc[i][c >> 2][c & 3] : -INFINITY;
-      top = fmaxf(top, v[c]);
-    }
     if (t >= 0 && t < FN * 16) {   // (seldom: one tile has it)
 #pragma unroll
-      for (int c = 0; c < FN * 4; c++) if (16 * (c >> 2) + (c & 3) == t) p.picked[m] = v[c];
+      for (int c = 0; c < FN * 4; c++) if (16 * (c >> 2) + (c & 3) == t) p.picked[m] = acc[i][c >> 2][c & 3];
     }
+    float top = -INFINITY, sum = 0;
     // fmaxf passes over a NaN; its exponential is one again
-    const float base = top == -INFINITY ? 0.0f : top;
+    if (whole) {
 #pragma unroll
-    for (int c = 0; c < FN * 4; c++) sum += __expf(v[c] - base);
+      for (int c = 0; c < FN * 4; c++) top = fmaxf(top, acc[i][c >> 2][c & 3]);
+      const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int c = 0; c < FN * 4; c++) sum += __expf(acc[i][c >> 2][c & 3] - base);
+    } else {
+#pragma unroll
+      for (int c = 0; c < FN * 4; c++) if (16 * (c >> 2) + (c & 3) < left) top = fmaxf(top, acc[i][c >> 2][c & 3]);
+      const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int c = 0; c < FN * 4; c++) if (16 * (c >> 2) + (c & 3) < left) sum += __expf(acc[i][c >> 2][c & 3] - base);
+    }
     float2 run = make_float2(top, sum);
 #pragma unroll
     for (int o = 16; o < 64; o <<= 1) run = join(run, make_float2(__shfl_xor(run.x, o), __shfl_xor(run.y, o)));
@@ -254,7 +259,17 @@ __device__ __forceinline__ void emit4(const ProductArgs& p, long first, unsigned
     put_held<T>((u16*)p.h + first + at, p.dtype, p.hpart, a);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = e < left ? (__expf(v[e] - row.lse) - (row.target == e ? 1.0f : 0.0f)) * row.grad : 0.0f;
+    for (int e = 0; e < 4; e++) v[e] = __expf(v[e] - row.lse);
+    if (row.target >= 0 && row.target < 4) {   // (seldom)
+#pragma unroll
+      for (int e = 0; e < 4; e++) if (row.target == e) v[e] -= 1.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] *= row.grad;
+    if (left < 4) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) if (e >= left) v[e] = 0.0f;
+    }
     put_held<T>((u16*)p.c + first + at, p.dtype, p.hpart, v);
   }
 }

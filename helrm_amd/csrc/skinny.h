@@ -5,11 +5,11 @@
 inline long skinny_rows(int dtype) { return dtype == DT_F32 ? 64 : 16; }   // the most rows of X
 
 struct SkinnyArgs {
-  const void* x; long ldx;           // [T][K]
+  const void* x; long ldx;           // [T][K]; float32 for skinny_store
   const void* w; long ldw;           // [N][K]
   const void* w2; long ldw2;         // gate: the up projection
   int T, N, K, dtype;                // of x, w and out; any alignment
-  void* out; long ldout;             // [T][N]
+  void* out; long ldout;             // [T][N]; float32 of skinny_gate
   float* g; float* u; long ldg;      // gate: [T][ldg] kept projections, 0 past N; may be null
   int act; float coef[4];
   const long long* target; float* picked; float2* part;   // softmax: [T], [T], [T][parts]

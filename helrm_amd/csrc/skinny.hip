@@ -71,13 +71,31 @@ template <class T> __device__ __forceinline__ f32x4 dot8(const Eight<T>& w, cons
   }
 }
 
+// The hidden values of a 16-bit block stay float32 here: they are few, and in
+// two parts of 8 (11) bits they multiply as exactly as the weights deserve.
+template <class T> struct Two {
+  typename Vec8<T>::type v[2];
+};
+template <class T> __device__ __forceinline__ Two<T> two(const Raw<float>& r) {
+  Two<T> o;
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const T first = (T)r.e[e];
+    o.v[0][e] = first;
+    o.v[1][e] = (T)(fabsf((float)first) < INFINITY ? r.e[e] - (float)first : 0.0f);
+  }
+  return o;
+}
+template <class T> __device__ __forceinline__ f32x4 dot8(const Eight<T>& w, const Two<T>& x, f32x4 c) { return mfma(w.v[0], x.v[0], mfma(w.v[0], x.v[1], c)); }
+
 // A workgroup takes `groups` times 16 rows of W; or, where there are rows
 // enough to keep every wave loading, each of its waves does (`alone`), which
 // saves the exchange of sums.  Lane l of a wave holds, of a
 // group, row l % 16 and the k 16 (l / 16) + 0..15 of 64; its sums are row t = l % 16
 // of X and the columns 4 (l / 16) + 0..3.
 template <class T, bool ALIGNED, int NB> constexpr int most_waves() { return sizeof(T) == 2 && ALIGNED && NB == 1 ? 16 : 8; }
-template <class T, bool ALIGNED, int NB, int EPI>
+// X: the type of x, T or float.
+template <class T, class X, bool ALIGNED, int NB, int EPI>
 __global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_kernel(const SkinnyArgs p) {
   constexpr int MATS = EPI == SKINNY_GATE ? 2 : 1, TURNS = !ALIGNED ? 1 : sizeof(T) == 4 ? 2 : 4;
   extern __shared__ float lds[];   // [waves][MATS * NB][64][4]
@@ -112,9 +130,16 @@ __global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_ke
 #pragma unroll
           for (int b = 0; b < NB; b++) {
             const int row = b * 16 + t;
-            const Eight<T> x = eight(load8<T, ALIGNED>((const T*)p.x + (long)row * p.ldx, k0 + u * waves * 64 + quad * 16 + s * 8, p.K, row < p.T));
+            const Raw<X> rx = load8<X, ALIGNED>((const X*)p.x + (long)row * p.ldx, k0 + u * waves * 64 + quad * 16 + s * 8, p.K, row < p.T);
+            if constexpr (sizeof(X) == sizeof(T)) {
+              const Eight<T> x = eight(rx);
 #pragma unroll
-            for (int m = 0; m < MATS; m++) acc[m][b] = dot8(f[m], x, acc[m][b]);
+              for (int m = 0; m < MATS; m++) acc[m][b] = dot8(f[m], x, acc[m][b]);
+            } else {
+              const Two<T> x = two<T>(rx);
+#pragma unroll
+              for (int m = 0; m < MATS; m++) acc[m][b] = dot8(f[m], x, acc[m][b]);
+            }
           }
         }
     }
@@ -176,7 +201,11 @@ __global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_ke
         for (int e = 0; e < 4; e++) v[e] = a[e] * u[e];
       }
 #pragma unroll
-      for (int e = 0; e < 4; e++) if (e < left) ((T*)p.out)[row * p.ldout + n + e] = (T)v[e];
+      for (int e = 0; e < 4; e++) {
+        if (e >= left) continue;
+        if (EPI == SKINNY_GATE) ((float*)p.out)[row * p.ldout + n + e] = v[e];
+        else ((T*)p.out)[row * p.ldout + n + e] = (T)v[e];
+      }
     }
   }
   if (EPI == SKINNY_SOFTMAX) {
@@ -187,19 +216,20 @@ __global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_ke
 }
 
 // A workgroup a row: the loss and lse of its pieces, 0 for an ignored row.
-__global__ __launch_bounds__(256) void skinny_finish_kernel(const float2* part, int parts, const float* picked, const long long* target, long long ignore,
+constexpr int FINISH = 1024;
+__global__ __launch_bounds__(FINISH) void skinny_finish_kernel(const float2* part, int parts, const float* picked, const long long* target, long long ignore,
                                                             int vocab, float* loss, float* lse) {
-  __shared__ float2 lds[4];
+  __shared__ float2 lds[FINISH / 64];
   const int row = blockIdx.x;
   part += (long)row * parts;
   float2 run = make_float2(-INFINITY, 0.0f);
-#pragma unroll 8
-  for (int k = threadIdx.x; k < parts; k += 256) run = join(run, part[k]);
+#pragma unroll 4
+  for (int k = threadIdx.x; k < parts; k += FINISH) run = join(run, part[k]);
   for (int o = 32; o; o >>= 1) run = join(run, make_float2(__shfl_xor(run.x, o), __shfl_xor(run.y, o)));
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = run;
   __syncthreads();
   if (threadIdx.x) return;
-  for (int k = 1; k < 4; k++) run = join(run, lds[k]);
+  for (int k = 1; k < FINISH / 64; k++) run = join(run, lds[k]);
   const long long t = target[row];
   const float l = run.x + logf(run.y);
   lse[row] = t == ignore ? 0.0f : l;
@@ -222,6 +252,7 @@ template <int EPI> void launch(SkinnyArgs p, hipStream_t st) {
   clr::with_type(p.dtype, [&](auto type) {
     using T = decltype(type);
     const long v = 16 / sizeof(T);
+    using X = std::conditional_t<EPI == SKINNY_STORE, float, T>;
     auto fits = [&](const void* q, long ld) { return (uintptr_t)q % 16 == 0 && ld % v == 0; };
     const bool aligned = p.K % 8 == 0 && fits(p.x, p.ldx) && fits(p.w, p.ldw) && (EPI != SKINNY_GATE || fits(p.w2, p.ldw2));
     auto go = [&](auto nb) {
@@ -229,8 +260,8 @@ template <int EPI> void launch(SkinnyArgs p, hipStream_t st) {
       const int waves = p.alone ? 4 : waves_of(p.N, p.K, p.dtype, aligned ? most_waves<T, true, NB>() : most_waves<T, false, NB>());
       const unsigned grid = (unsigned)(p.alone ? clr::ceil_div(teams, 4) : teams);
       const size_t lds = (size_t)waves * (EPI == SKINNY_GATE ? 2 : 1) * NB * 1024;
-      if (aligned) skinny_kernel<T, true, NB, EPI><<<grid, waves * 64, lds, st>>>(p);
-      else skinny_kernel<T, false, NB, EPI><<<grid, waves * 64, lds, st>>>(p);
+      if (aligned) skinny_kernel<T, X, true, NB, EPI><<<grid, waves * 64, lds, st>>>(p);
+      else skinny_kernel<T, X, false, NB, EPI><<<grid, waves * 64, lds, st>>>(p);
     };
     if (p.T <= 16) go(std::integral_constant<int, 1>{});
     if constexpr (sizeof(T) == 4) {
@@ -251,5 +282,5 @@ void skinny_softmax(SkinnyArgs p, long long ignore, float* loss, float* lse, hip
   p.groups = softmax_groups(p.N);
   p.parts = skinny_softmax_parts(p.N);
   launch<SKINNY_SOFTMAX>(p, st);
-  skinny_finish_kernel<<<(unsigned)p.T, 256, 0, st>>>(p.part, p.parts, p.picked, p.target, ignore, p.N, loss, lse);
+  skinny_finish_kernel<<<(unsigned)p.T, FINISH, 0, st>>>(p.part, p.parts, p.picked, p.target, ignore, p.N, loss, lse);
 }
