@@ -8,7 +8,7 @@ import math
 import torch
 
 U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
-CUBIC = (-0.0320, 0.2195, 0.5706, 0.2048)   # the encrypted model's activation, lowest degree first
+CUBIC = (-0.0320, 0.2195, 0.5706, 0.2048)   # lowest degree first
 
 
 def d(t):

@@ -114,3 +114,17 @@ def test_tensors_on_the_host():
         ct.gated_mlp(x, torch.zeros(3, 4), torch.zeros(3, 4), torch.zeros(4, 3))
     with pytest.raises(ValueError, match="not on the GPU"):
         ct.cross_entropy(x, torch.zeros(3, 4), torch.zeros(2, dtype=torch.int64))
+
+
+def test_a_second_hip_runtime_is_refused():
+    """The library loaded first brings its own HIP runtime, torch then another one: their streams and pointers mean
+    nothing to each other, so the operators refuse to start.  With torch first there is one runtime."""
+    import subprocess
+    import sys
+    pytest.importorskip("torch")
+    code = "{}\nfrom helrm_amd import cleartext\ntry:\n    cleartext._library()\n    print('one')\nexcept Exception as e:\n    print(type(e).__name__, e)"
+    first = "from helrm_amd.backend import load_library\nload_library()\nimport torch"
+    root = __file__.rsplit("/", 2)[0]
+    said = [subprocess.run([sys.executable, "-c", code.format(s)], capture_output=True, text=True, cwd=root).stdout for s in (first, "import torch")]
+    assert said[1].strip() == "one", said
+    assert "two HIP runtimes" in said[0] or said[0].strip() == "one", said     # (one file for both: nothing to refuse)
