@@ -176,7 +176,7 @@ __device__ __forceinline__ void tile_of(int id, int total, int nm, int nn, int& 
 
 // A row's maximum and sum over the tile's columns: over the lane's, over the
 // four lanes that share the row, over the waves beside one another.  acc[i][j][e]
-// is (m, n) = (mw + 16 i + lane % 16, nw + 16 j + 4 (lane / 16) + e).
+// is (m, n) = (mw + 16 i + lane % 16, n_wave + 16 j + 4 (lane / 16) + e).
 template <int FM, int FN, int WAVES_M, int WAVES_N>
 __device__ __forceinline__ void softmax_piece(const ProductArgs& p, const f32x4 (&acc)[FM][FN], int M, long m0, long n0, int wave_m, int wave_n, int tile_n,
                                               float2* lds) {
@@ -224,15 +224,19 @@ __device__ __forceinline__ void softmax_piece(const ProductArgs& p, const f32x4 
 // What becomes of four neighbouring columns of a row, n columns from the end
 // of the matrix (`left`), at element first + at of the results (gate: v of the
 // gate, u of the up projection).
+// WHOLE: all four columns are there and, of a store, the place takes one vector.
 struct RowValues { float lse, grad; int target; };
-template <class T, int EPI>
-__device__ __forceinline__ void emit4(const ProductArgs& p, long first, unsigned at, int left, const RowValues& row, float v[4], float u[4]) {
-  if (left < 4) {
+template <class T, int EPI, bool WHOLE>
+__device__ __forceinline__ void emit4(const ProductArgs& p, long first, unsigned at, int left, const RowValues& row, float v[4], float u[4],
+                                      const float (&held)[2][4]) {
+  if (!WHOLE && left < 4) {
 #pragma unroll
     for (int e = 0; e < 4; e++) if (e >= left) v[e] = u[e] = 0.0f;   // the columns that fill a row up are 0
   }
   if (EPI == EPI_STORE) {
-    store4<T>(p, first + at, left, v);
+    if (!WHOLE) store4<T>(p, first + at, left, v);
+    else if (p.ctype == DT_F32) *(float4*)((float*)p.c + first + at) = make_float4(v[0], v[1], v[2], v[3]);
+    else *(uint2*)((u16*)p.c + first + at) = pack4<T>(v);
   } else if (EPI == EPI_GATE) {
     float a[4], d[4];
     act4(p.act, p.coef, v, a, d);
@@ -244,15 +248,13 @@ __device__ __forceinline__ void emit4(const ProductArgs& p, long first, unsigned
     }
     put_held<T>((u16*)p.h + first + at, p.dtype, p.hpart, a);
   } else if (EPI == EPI_GATE_GRAD) {
-    float g[4], a[4], d[4];
-    get4(p.g + first + at, g);
-    get4(p.u + first + at, u);
-    act4(p.act, p.coef, g, a, d);
+    float a[4], d[4];
+    act4(p.act, p.coef, held[0], a, d);
 #pragma unroll
     for (int e = 0; e < 4; e++) {   // (g, u and v are 0 in the columns that fill a row up)
-      d[e] *= v[e] * u[e];
+      d[e] *= v[e] * held[1][e];
       v[e] *= a[e];
-      a[e] *= u[e];
+      a[e] *= held[1][e];
     }
     put_held<T>((u16*)p.dg + first + at, p.dtype, p.hpart, d);
     put_held<T>((u16*)p.du + first + at, p.dtype, p.hpart, v);
@@ -266,7 +268,7 @@ __device__ __forceinline__ void emit4(const ProductArgs& p, long first, unsigned
     }
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] *= row.grad;
-    if (left < 4) {
+    if (!WHOLE && left < 4) {
 #pragma unroll
       for (int e = 0; e < 4; e++) if (e >= left) v[e] = 0.0f;
     }
@@ -286,53 +288,74 @@ template <int EPI> __device__ __host__ __forceinline__ long sum_ld(const Product
 // stored are whole lines of a row and the code of it is there once.  A place is
 // a 32-bit offset from the wave's first element (rows are under 2^21 elements).
 template <class T, int EPI, int FM, int FN>
-__device__ __forceinline__ void emit(const ProductArgs& p, const f32x4 (&acc)[FM][FN], int M, long mw, long nw, int split, float* lds) {
-  static_assert(FN == 4 && FM % 4 == 0, "64 x 64 a time");
+__device__ __forceinline__ void emit(const ProductArgs& p, const f32x4 (&acc)[FM][FN], int M, long mw, long n_wave, int split, float* own) {
   constexpr int LANES = EPI == EPI_GATE ? 8 : 16, ROWS = 64 / LANES;   // of a row; rows a time
+  constexpr int GROUP = 4;   // places a lane reads before it writes them: its waits are shared
   const int lane = threadIdx.x & 63, col = lane % LANES;
   // gate: the columns are 16 of the gate, the same 16 of the up projection, 16 of the gate, ...
   const int c = EPI == EPI_GATE ? (col >> 2) * 8 + (col & 3) : col;
   const bool sums = EPI != EPI_SOFTMAX_GRAD && p.splits > 1;
   const unsigned ld = (unsigned)(sums ? sum_ld<EPI>(p) : result_ld<EPI>(p));
-  const long first = (sums ? (long)split * p.M * ld : 0) + mw * ld + nw;
   const unsigned second = EPI == EPI_GATE ? (unsigned)sum_cols<EPI>(p) : 0;
-  // columns that there are from the lane's first one on, and columns with the zeros that fill an intermediate's row up
-  const int left = (int)min((long)p.N - nw, 64L) - col * 4;
-  const int room = EPI == EPI_STORE ? left : (int)min(((p.N + 7L) & ~7L) - nw, 64L) - col * 4;
+  // a store of whole vectors, nothing to add or divide by
+  const bool plain = EPI != EPI_STORE || sums || (!p.add && !p.unscale && p.ldc % 4 == 0 && (uintptr_t)p.c % 16 == 0);
+  static_assert(FN == 4 && FM % 4 == 0, "64 x 64 a time");
 #pragma unroll
   for (int part = 0; part < FM / 4; part++) {
-    RowValues mine{};   // of row `lane` of the 64
-    if (EPI == EPI_SOFTMAX_GRAD && mw + part * 64 + lane < M) {
-      const long m = mw + part * 64 + lane;
-      mine.target = p.target[m];
-      mine.lse = p.lse[m];
-      mine.grad = mine.target < 0 ? NAN : p.grad[m] * (p.scale ? *p.scale : 1.0f);
-    }
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const int r = i * 16 + (lane & 15), at = j * 4 + (lane >> 4);
-        *(f32x4*)(lds + r * 64 + ((at ^ (r & 15)) * 4)) = acc[part * 4 + i][j];
+        *(f32x4*)(own + r * 64 + ((at ^ (r & 15)) * 4)) = acc[part * 4 + i][j];
       }
+    const long first = (sums ? (long)split * p.M * ld : 0) + mw * ld + n_wave;
+    // columns that there are from the lane's first one on, and columns with the zeros that fill an intermediate's row up
+    const int left = (int)min((long)p.N - n_wave, 64L) - col * 4;
+    const int room = EPI == EPI_STORE ? left : (int)min(((p.N + 7L) & ~7L) - n_wave, 64L) - col * 4;
     const int rows = (int)min(M - mw - part * 64, 64L);
-#pragma unroll 4
-    for (int r0 = 0; r0 < 64; r0 += ROWS) {
-      const int r = r0 + lane / LANES;
-      float v[4], u[4] = {0, 0, 0, 0};
-      get4(lds + r * 64 + ((c ^ (r & 15)) * 4), v);
-      if (EPI == EPI_GATE) get4(lds + r * 64 + (((c + 4) ^ (r & 15)) * 4), u);
-      RowValues row{};
-      if (EPI == EPI_SOFTMAX_GRAD) row = {__shfl(mine.lse, r), __shfl(mine.grad, r), __shfl(mine.target, r) - (int)(p.n0 + nw) - col * 4};
-      if (r >= rows || room <= 0) continue;
-      const unsigned at = (part * 64 + r) * ld + col * 4;
-      if (sums) {
-        *(float4*)(p.partial + first + at) = make_float4(v[0], v[1], v[2], v[3]);
-        if (EPI == EPI_GATE) *(float4*)(p.partial + first + second + at) = make_float4(u[0], u[1], u[2], u[3]);
-      } else {
-        emit4<T, EPI>(p, first, at, left, row, v, u);
-      }
+    RowValues mine{};   // of row `lane` of the 64
+    if (EPI == EPI_SOFTMAX_GRAD && lane < rows) {
+      const long m = mw + part * 64 + lane;
+      mine.target = p.target[m];
+      mine.lse = p.lse[m];
+      mine.grad = mine.target < 0 ? NAN : p.grad[m] * (p.scale ? *p.scale : 1.0f);
     }
+    auto places = [&](auto whole_) __attribute__((always_inline)) {
+      constexpr bool WHOLE = decltype(whole_)::value;
+#pragma unroll 1
+      for (int r0 = 0; r0 < 64; r0 += ROWS * GROUP) {
+        float v[GROUP][4], u[GROUP][4] = {}, held[GROUP][2][4] = {};
+        RowValues row[GROUP] = {};
+#pragma unroll
+        for (int g = 0; g < GROUP; g++) {
+          const int r = r0 + g * ROWS + lane / LANES;
+          get4(own + r * 64 + ((c ^ (r & 15)) * 4), v[g]);
+          if (EPI == EPI_GATE) get4(own + r * 64 + (((c + 4) ^ (r & 15)) * 4), u[g]);
+          if (EPI == EPI_SOFTMAX_GRAD)
+            row[g] = {__shfl(mine.lse, r), __shfl(mine.grad, r), __shfl(mine.target, r) - (int)(p.n0 + n_wave) - col * 4};
+          if (EPI == EPI_GATE_GRAD && !sums && (WHOLE || (r < rows && room > 0))) {
+            const unsigned at = (part * 64 + r) * ld + col * 4;
+            get4(p.g + first + at, held[g][0]);
+            get4(p.u + first + at, held[g][1]);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < GROUP; g++) {
+          const int r = r0 + g * ROWS + lane / LANES;
+          if (!WHOLE && (r >= rows || room <= 0)) continue;
+          const unsigned at = (part * 64 + r) * ld + col * 4;
+          if (sums) {
+            *(float4*)(p.partial + first + at) = make_float4(v[g][0], v[g][1], v[g][2], v[g][3]);
+            if (EPI == EPI_GATE) *(float4*)(p.partial + first + second + at) = make_float4(u[g][0], u[g][1], u[g][2], u[g][3]);
+          } else {
+            emit4<T, EPI, WHOLE>(p, first, at, left, row[g], v[g], u[g], held[g]);
+          }
+        }
+      }
+    };
+    if (plain && rows == 64 && p.N - n_wave >= (EPI == EPI_GATE ? 32 : 64)) places(std::true_type{});
+    else places(std::false_type{});
   }
 }
 
@@ -535,7 +558,13 @@ __global__ __launch_bounds__(256) void join_kernel(const Batch batch) {
       for (int e = 0; e < 4; e++) u[e] += t[e];
     }
   }
-  emit4<T, EPI>(p, m * result_ld<EPI>(p) + n, 0, (int)min(p.N - n, 4L), RowValues{}, v, u);
+  const long at = m * result_ld<EPI>(p) + n;
+  float held[2][4] = {};
+  if (EPI == EPI_GATE_GRAD) {
+    get4(p.g + at, held[0]);
+    get4(p.u + at, held[1]);
+  }
+  emit4<T, EPI, false>(p, at, 0, (int)min(p.N - n, 4L), RowValues{}, v, u, held);
 }
 
 // The tile and the splits of products in one launch: the least time of their
