@@ -570,7 +570,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Batch batch) {
 // The tile and the splits of products in one launch: the least time of their
 // rounds over the 256 CUs, which hold one 256 x 256 tile or two 128 x 128 ones
 // (whose steps and ends overlap).  Microseconds, measured: a step 1.6 and 1.0,
-// the end of a tile 10 and 6.  The large tile has half the traffic for each
+// the end of a tile 8.5 and 6.  The large tile has half the traffic for each
 // product, the small one fills the GPU with a quarter of the rows.
 struct Plan { bool big; int splits; };
 Plan plan_of(std::initializer_list<Shape> shapes, long steps, bool gate, bool may_split) {
@@ -588,7 +588,7 @@ Plan plan_of(std::initializer_list<Shape> shapes, long steps, bool gate, bool ma
       if (s > 1 && steps / s < 4) break;
       const double sums = s > 1 ? 4.0 + (s + 1) * results * 4 / 3e6 : 0.0;   // of a kernel more, and its traffic
       const long rounds = clr::ceil_div(tiles * s, 256), each = clr::ceil_div(steps, s);
-      const double t = (big ? rounds * (each * 1.6 + 10) : (rounds + 1) / 2 * (each * 1.0 + 6) * (rounds == 1 ? 0.6 : 1.0)) + sums;
+      const double t = (big ? rounds * (each * 1.6 + 8.5) : (rounds + 1) / 2 * (each * 1.0 + 6) * (rounds == 1 ? 0.6 : 1.0)) + sums;
       if (t < least) { least = t; best = {big != 0, s}; }
     }
   }

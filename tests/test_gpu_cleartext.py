@@ -158,6 +158,15 @@ def test_gated_mlp(ct, dtype, rows, width, hidden):
     mlp_check(ct, x, gate, up, down, dy, acts[(rows + hidden) % 3])
 
 
+# each product of the block in large tiles, whole and in sums split along k, none of the sizes a multiple of a tile
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width,hidden", [(2051, 4099, 33), (1541, 33, 2565), (2051, 33, 4099), (33, 1027, 2565), (131, 4099, 2565),
+                                               (131, 2565, 4099), (131, 4099, 1285), (2565, 131, 1541)])
+def test_gated_mlp_large_tiles(ct, dtype, rows, width, hidden):
+    x, gate, up, down, dy = mlp_tensors(seeded(rows + width), rows, width, hidden, dtype)
+    mlp_check(ct, x, gate, up, down, dy, "gelu")
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", ref.CUBIC])
 @pytest.mark.parametrize("rows", [1, 40])
 def test_gated_mlp_activations(ct, act, rows):
@@ -253,6 +262,21 @@ def ce_tensors(gen, rows, width, vocab, dtype, ignored=0.0, lean=2.0):
                                               (50, 100, 257), (65, 416, 1300), (130, 24, 2500), (257, 136, 512), (600, 16, 100)])
 def test_cross_entropy(ct, dtype, rows, width, vocab):
     x, table, target, grad = ce_tensors(seeded(rows + vocab), rows, width, vocab, dtype)
+    ce_check(ct, x, table, target, grad)
+
+
+# each product of the loss in large tiles, whole and split; the last: a table in two pieces in float32
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width,vocab", [(261, 33, 24001), (33, 261, 24001), (2051, 4099, 515), (131, 4099, 4099), (1027, 131, 8197),
+                                              (4099, 33, 12001)])
+def test_cross_entropy_large_tiles(ct, dtype, rows, width, vocab):
+    x, table, target, grad = ce_tensors(seeded(rows + vocab), rows, width, vocab, dtype, ignored=0.2)
+    ce_check(ct, x, table, target, grad)
+
+
+def test_cross_entropy_of_two_pieces_of_16_bits(ct):
+    x, table, target, grad = ce_tensors(seeded(8), 2100, 24, 64100, torch.bfloat16)
+    target[:3] = torch.tensor([63487, 63488, 64099])     # beside the cut, and the last row
     ce_check(ct, x, table, target, grad)
 
 
