@@ -156,13 +156,17 @@ __global__ __launch_bounds__(MANY ? 512 : BLOCK) void norm_backward(const T* dy,
     const float mu = mean[row], r = rstd[row];
     float2 s = make_float2(0, 0);
 #pragma unroll
-    for (int i = 0; i < E; i++) {   // (past the end of the row d and c are 0)
-      h[i] = (h[i] - mu) * r;
-      sw[i] += d[i] * h[i];
-      sb[i] += d[i];
-      d[i] *= c[i];
-      s.x += d[i];
-      s.y += d[i] * h[i];
+    for (int j = 0; j < N; j++) {
+      const float m = (j * n + lane) * V < width ? mu : 0.0f;   // past the end of the row d, c and h are 0, also where mu r overflows
+#pragma unroll
+      for (int i = j * V; i < (j + 1) * V; i++) {
+        h[i] = (h[i] - m) * r;
+        sw[i] += d[i] * h[i];
+        sb[i] += d[i];
+        d[i] *= c[i];
+        s.x += d[i];
+        s.y += d[i] * h[i];
+      }
     }
     s = row_sum<MANY>(s, wave, waves, lds[turn]);
     s.x /= width;

@@ -106,6 +106,19 @@ def test_layer_norm_of_a_nan_row_stays_in_its_row(ct):
     assert torch.isfinite(y[[0, 1, 4]]).all()
 
 
+@pytest.mark.parametrize("width", [7, 520, 1032])
+def test_layer_norm_of_equal_values_whose_mean_overflows_times_rstd(ct, width):
+    # 2^114 and its sum are exact, h is 0: dx = r (w dy - mean(w dy)), r = 10^6
+    x = torch.full((3, width), 2.0 ** 114, device=DEV)
+    w, dy = torch.ones(width, device=DEV), normal(seeded(7), 3, width)
+    y, mean, rstd = ct.layer_norm_forward(x, w, None, 1e-12)
+    assert (y == 0).all() and (mean == 2.0 ** 114).all()
+    dx, dw, _ = ct.layer_norm_backward(dy, x, w, mean, rstd, has_bias=False)
+    assert (dw == 0).all()
+    t = ref.d(dy)
+    ref.check(dx, 1e6 * (t - t.mean(1, keepdim=True)), 1e6 * (t.abs() + t.abs().mean(1, keepdim=True)), (width + 30) * F32, "dx")
+
+
 def test_layer_norm_offsets_beyond_32_bits(ct):
     rows, width = (1 << 31) // 4096 + 5, 4096
     x = torch.zeros(rows, width, dtype=torch.bfloat16, device=DEV)
