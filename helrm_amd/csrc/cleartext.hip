@@ -298,7 +298,7 @@ size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
   const long n = a->rows, D = a->width;
   const int piece = piece_rows(a);
   RowsArgs r{a->target, a->dloss, n, a->ignore, a->vocab};
-  r.rows = m.take<int>(n); r.tgt = m.take<int>(n); r.count = m.take<int>(1);
+  r.rows = m.take<int>(n); r.tgt = m.take<int>(n); r.place = m.take<int>(n); r.count = m.take<int>(1);
   float* scale = m.take<float>(1);
   if (a->type == DT_F16) r.scale = scale;
   r.lse = a->lse; r.lse_kept = m.take<float>(n); r.grad_kept = m.take<float>(n);
@@ -339,7 +339,7 @@ size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
     w.unscale = r.scale;
     product_tn(w, st);
   }
-  scatter_rows(acc, D, r.rows, r.count, r.scale, a->dx, a->lddx, n, a->width, a->type, st);
+  scatter_rows(acc, D, r.place, r.scale, a->dx, a->lddx, n, a->width, a->type, st);
   return m.used;
 }
 

@@ -7,6 +7,11 @@
 // rows far from zero lose nothing.  Bound by memory: a row is read once, by 1
 // to 8 waves that hold 16 values a lane, and the backward pass adds its rows
 // to the weights' gradients in registers while it has them.
+//
+// Measured (a copy here: 4.95 TB/s): 32,768 x 4,096 bfloat16 forward 110 us =
+// 4.9 TB/s, backward 176 us = 4.6 TB/s and 8 us for the sums of the weights'
+// gradients; 8,192 x 1,024 bfloat16 9 + 13 + 4 us; 4,097 x 1,001 float32, an
+// element a load, 8 + 15 + 4 us; 1 x 512 2 us.
 #include <algorithm>
 #include "cleartext.h"
 #include "norm.h"
@@ -203,7 +208,8 @@ __global__ __launch_bounds__(MANY ? 512 : BLOCK) void norm_backward(const T* dy,
 }
 
 // dw and db: the sums over the workgroups' parts, 16 columns a workgroup, in
-// a fixed order (no atomics: the gradient is the same on every run).
+// a fixed order (no atomics: the gradient is the same on every run).  Bound by
+// latency: 512 parts of 4,096 columns, 17 MB from the last-level cache, 8 us.
 constexpr int SUM_COLS = 16, SUM_ROWS = 64;
 template <class P>
 __global__ __launch_bounds__(SUM_COLS* SUM_ROWS) void norm_param_sum(const float* part, P* dw, P* db, int parts, int width) {
@@ -223,7 +229,8 @@ __global__ __launch_bounds__(SUM_COLS* SUM_ROWS) void norm_param_sum(const float
   out[i] = (P)s;
 }
 
-// ---- rows of more than MOST_WAVES * 64 * HOLD values: one workgroup a row, which it reads once for every sum ----
+// ---- rows of more than MOST_WAVES * 64 * HOLD values: one workgroup a row, which it reads once for every sum (from its
+// caches after the first: a row is at least 16 KiB).  The simple form: no model here has rows that long. ----
 __device__ __forceinline__ float block_sum(float v, float* lds) {
   v = wave_sum(make_float2(v, 0)).x;
   __syncthreads();

@@ -76,13 +76,13 @@ void lay_out(const LayOut* jobs, int n, int dtype, hipStream_t st);
 struct RowsArgs {
   const long long* target; const float* grad;
   long n; long long ignore; int vocab;
-  int* rows; int* tgt; int* count;
+  int* rows; int* tgt; int* count;   // of the rows that count: each one's row, its target (-1 outside the table), and how many they are
+  int* place;                        // of each row: where it is among them, or -1
   float* picked; float* loss; float* lse; float* lse_kept; float* grad_kept; float* scale;
 };
 void kept_rows(const RowsArgs& a, hipStream_t st);
 // loss[row] = lse - picked, lse = the logarithm of the parts' sum
 void softmax_finish(const float2* part, int parts, const float* picked, const int* rows, const int* count, long n, float* loss, float* lse, hipStream_t st);
-// out[row] = acc[i] / *scale, 0 for rows that are not kept
-void scatter_rows(const float* acc, long ldacc, const int* rows, const int* count, const float* scale, void* out, long ldout, long n, int width, int dtype,
-                  hipStream_t st);
+// out[row] = acc[place[row]] / *scale, 0 for rows that are not kept
+void scatter_rows(const float* acc, long ldacc, const int* place, const float* scale, void* out, long ldout, long n, int width, int dtype, hipStream_t st);
 void fill_zero(void* p, size_t bytes, hipStream_t st);  // bytes: a multiple of 2

@@ -20,6 +20,19 @@
 // as [64 k][row] and read through the transposing LDS load, four k of 16 rows
 // for 16 lanes; 32 bytes p of row k are at p ^ h(k), h(k) = (k & 3) | (k >> 1 & 4),
 // so that the eight k rows that 32 lanes read lie in all banks.
+//
+// Measured, bfloat16, random values (a library product of 8192 x 8192 x 2048
+// here: 1364 TFLOP/s of A B^T, 1180 of A B):
+//   A B^T    8192 x 2048 x 8192           204 us   1350 TFLOP/s
+//   A B      8192 x 2048 x (8192 + 8192)  412      1335
+//   A^T B    3 of 8192 x 2048 x 8192      649      1271
+//   gate     8192 x 8192 x 2048, twice    534      1029 (670 MB of results)
+//   its gradient  8192 x 8192 x 2048      425       647 (940 MB in and out: 190 us of a copy)
+//   softmax  8192 x 131072 x 2048        3555      1237
+// Bound by power first: with zeros for data the same instructions reach 1500
+// TFLOP/s, with random values the clock falls to 1.57 GHz and the matrix units
+// are busy 64 % of the time.  The gate and its gradient are bound by memory at
+// the end of a tile, when a CU does nothing else.
 #include "products.h"
 #include "tiles.h"
 
@@ -537,6 +550,9 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Batch batch)
 }
 
 // The sums of split products, four columns a thread, and what becomes of them.
+// In the order of the splits, so that a result does not depend on which
+// workgroup ends first.  Bound by memory and its launch: 1537 x 1000 over k =
+// 2 x 2736 takes 56 us in one piece, 38 in two, 5 of them here.
 template <class T, int EPI>
 __global__ __launch_bounds__(256) void join_kernel(const Batch batch) {
   const int which = batch.which(blockIdx.x);
@@ -570,8 +586,10 @@ __global__ __launch_bounds__(256) void join_kernel(const Batch batch) {
 // The tile and the splits of products in one launch: the least time of their
 // rounds over the 256 CUs, which hold one 256 x 256 tile or two 128 x 128 ones
 // (whose steps and ends overlap).  Microseconds, measured: a step 1.6 and 1.0,
-// the end of a tile 8.5 and 6.  The large tile has half the traffic for each
-// product, the small one fills the GPU with a quarter of the rows.
+// the end of a tile 8.5 and 6, a small tile alone on its CU 0.55 of that.  The
+// large tile has half the traffic for each product, the small one fills the
+// GPU with a quarter of the rows.  8192 x 4096 over 4096, gate gradient: 323 us
+// large, 349 small; 2048 x 8192 over 512, gate: 67 us large, 54 small.
 struct Plan { bool big; int splits; };
 Plan plan_of(std::initializer_list<Shape> shapes, long steps, bool gate, bool may_split) {
   Plan best{};
@@ -588,7 +606,7 @@ Plan plan_of(std::initializer_list<Shape> shapes, long steps, bool gate, bool ma
       if (s > 1 && steps / s < 4) break;
       const double sums = s > 1 ? 4.0 + (s + 1) * results * 4 / 3e6 : 0.0;   // of a kernel more, and its traffic
       const long rounds = clr::ceil_div(tiles * s, 256), each = clr::ceil_div(steps, s);
-      const double t = (big ? rounds * (each * 1.6 + 8.5) : (rounds + 1) / 2 * (each * 1.0 + 6) * (rounds == 1 ? 0.6 : 1.0)) + sums;
+      const double t = (big ? rounds * (each * 1.6 + 8.5) : (rounds + 1) / 2 * (each * 1.0 + 6) * (rounds == 1 ? 0.55 : 1.0)) + sums;
       if (t < least) { least = t; best = {big != 0, s}; }
     }
   }
@@ -627,7 +645,8 @@ template <bool A_K, bool B_K, int EPI> void launch(const ProductArgs& p, hipStre
 
 // Up to 8 matrices into the layout that the tiles are loaded from, one launch:
 // rows[i] (or i) of `from` to row i of `to`, filled up with zeros to ldto;
-// float32 as three parts.
+// float32 as three parts.  Bound by memory: 50,021 x 416 float32, 208 MB read
+// and written, 45 us = 4.7 TB/s.
 struct LayOuts { LayOut j[8]; int first[8]; int count; };
 template <class T>
 __global__ __launch_bounds__(256) void lay_out_kernel(const LayOuts all) {
@@ -675,7 +694,8 @@ __global__ __launch_bounds__(256) void lay_out_kernel(const LayOuts all) {
 
 constexpr int ROWS_BLOCK = 1024;
 
-// One workgroup: the rows that count, in order.
+// One workgroup: the rows that count, in order.  Bound by latency (a loop of 1,024 rows a turn): 14 us for 8,192 rows,
+// 0.1 % of the loss that so leaves the others out of its products.
 __global__ __launch_bounds__(ROWS_BLOCK) void kept_rows_kernel(RowsArgs a) {
   __shared__ int sums[ROWS_BLOCK / 64];
   __shared__ float tops[ROWS_BLOCK / 64];
@@ -698,8 +718,10 @@ __global__ __launch_bounds__(ROWS_BLOCK) void kept_rows_kernel(RowsArgs a) {
       if (a.lse_kept) { a.lse_kept[i] = a.lse[r]; a.grad_kept[i] = a.grad[r]; }
       if (a.picked) a.picked[i] = NAN;
       if (a.scale) top = fmaxf(top, fabsf(a.grad[r]));
+      if (a.place) a.place[r] = i;
     } else if (r < a.n) {
       if (a.loss) { a.loss[r] = 0.0f; a.lse[r] = 0.0f; }
+      if (a.place) a.place[r] = -1;
     }
     base += all;
     __syncthreads();
@@ -718,6 +740,7 @@ __global__ __launch_bounds__(ROWS_BLOCK) void kept_rows_kernel(RowsArgs a) {
   if (threadIdx.x == 0) *a.count = base;
 }
 
+// A wave a row joins its tiles' pieces: 8,192 rows of 512 pieces, 34 MB, 11 us (twice its memory time; one launch of the loss).
 __global__ void finish_kernel(const float2* part, int parts, const float* picked, const int* rows, const int* count, float* loss, float* lse) {
   const long i = blockIdx.x * 4L + (threadIdx.x >> 6);
   if (i >= *count) return;
@@ -732,19 +755,26 @@ __global__ void finish_kernel(const float2* part, int parts, const float* picked
   }
 }
 
-
+// A workgroup a row, its sums from where kept_rows put it, or zeros: a run of ignored rows is as parallel as any.
+// Bound by memory: 8,192 x 2,048 from float32 to bfloat16, 100 MB, 18 us = 5.4 TB/s.
 template <class T>
-__global__ void scatter_kernel(const float* acc, long ldacc, const int* rows, const int* count, const float* scale, T* out, long ldout, long n, int width) {
-  // the rows between one kept row and the next belong to the first of them
-  const long i = blockIdx.x;
-  const int kept = *count;
-  if (i > kept) return;
-  const long first = i < kept ? rows[i] : n, before = i ? rows[i - 1] + 1 : 0;
-  for (long r = before; r < first; r++)
-    for (int k = threadIdx.x; k < width; k += blockDim.x) out[r * ldout + k] = (T)0.0f;
-  if (i == kept) return;
+__global__ __launch_bounds__(256) void scatter_kernel(const float* acc, long ldacc, const int* place, const float* scale, T* out, long ldout, int width) {
+  const long r = blockIdx.x, i = place[r];
   const float s = scale ? 1.0f / *scale : 1.0f;
-  for (int k = threadIdx.x; k < width; k += blockDim.x) out[first * ldout + k] = (T)(acc[i * ldacc + k] * s);
+  T* o = out + r * ldout;
+  const float* v = acc + i * ldacc;
+  if (width % 4 == 0 && (uintptr_t)o % (4 * sizeof(T)) == 0) {   // (ldacc is the width)
+    for (int k = threadIdx.x * 4; k < width; k += 1024) {
+      float t[4] = {0, 0, 0, 0};
+      if (i >= 0) get4(v + k, t);
+      T q[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) q[e] = (T)(t[e] * s);
+      __builtin_memcpy(__builtin_assume_aligned(o + k, 4 * sizeof(T)), q, sizeof(q));
+    }
+  } else {
+    for (int k = threadIdx.x; k < width; k += 256) o[k] = i < 0 ? (T)0.0f : (T)(v[k] * s);
+  }
 }
 
 __global__ void zero_kernel(uint16_t* p, size_t n) {
@@ -793,11 +823,10 @@ void kept_rows(const RowsArgs& a, hipStream_t st) { kept_rows_kernel<<<1, ROWS_B
 void softmax_finish(const float2* part, int parts, const float* picked, const int* rows, const int* count, long n, float* loss, float* lse, hipStream_t st) {
   if (n) finish_kernel<<<(unsigned)clr::ceil_div(n, 4), 256, 0, st>>>(part, parts, picked, rows, count, loss, lse);
 }
-void scatter_rows(const float* acc, long ldacc, const int* rows, const int* count, const float* scale, void* out, long ldout, long n, int width, int dtype,
-                  hipStream_t st) {
-  clr::with_type(dtype, [&](auto t) {
+void scatter_rows(const float* acc, long ldacc, const int* place, const float* scale, void* out, long ldout, long n, int width, int dtype, hipStream_t st) {
+  if (n) clr::with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    scatter_kernel<T><<<(unsigned)(n + 1), 256, 0, st>>>(acc, ldacc, rows, count, scale, (T*)out, ldout, n, width);
+    scatter_kernel<T><<<(unsigned)n, 256, 0, st>>>(acc, ldacc, place, scale, (T*)out, ldout, width);
   });
 }
 void fill_zero(void* p, size_t bytes, hipStream_t st) {

@@ -12,6 +12,10 @@
 // Nothing is laid out first: unaligned matrices are read an element at a time,
 // float32 ones are split into three bfloat16 parts in registers and multiplied
 // as in products.hip.
+//
+// Measured: one row against 65,536 x 1,024 bfloat16, 134 MB, 28 us = 4.8 TB/s
+// (a copy: 4.95); the gate and up projections of one row, 17 MB, 8 to 11 us,
+// and the down projection, 8 MB, 7 us, which are launch and latency.
 #include "skinny.h"
 #include "tiles.h"
 
