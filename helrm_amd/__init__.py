@@ -4,7 +4,9 @@ The compute path is libhelrm_hip.so (hand-written HIP for gfx950, built from
 helrm_amd/csrc by helrm_amd.build).  `HipLibrary` binds it with the method
 names of Orion's Lattigo backend; `orion_host` holds the host-side callers of
 the path (hybrid diagonal packing, the block loop + rescale, the output fold
-and bias, the HE-LRM selector).
+and bias, the HE-LRM selector).  `cleartext` holds the operators that train
+and score a model in the clear, on torch tensors; it is imported by itself,
+since it needs torch.
 """
 import os
 

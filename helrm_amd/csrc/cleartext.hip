@@ -78,7 +78,8 @@ void set_act(ProductArgs& p, const GatedMLPArgs* a) {
 // A matrix as the products take it: where it is, or a copy in the workspace.
 struct Held {
   const uint16_t* p;
-  long ld, part;             // part: elements from one part of a float32 matrix to the next
+  long ld, part;             // part: elements from one part to the next
+  int parts = 1;             // three of a float32 matrix, two of a 16-bit intermediate of few rows
   const uint16_t* at(int k) const { return p + k * part; }
 };
 long up8(long n) { return (n + 7) & ~7L; }
@@ -86,10 +87,20 @@ bool fits(const void* p, long ld, long rows, long width, int type) {
   return type != DT_F32 && (uintptr_t)p % 16 == 0 && width % 8 == 0 && (rows <= 1 || ld % 8 == 0) && ld < MAX_LD;
 }
 // An intermediate of the operator's own.
-Held hold(Arena& m, long rows, long width, int type) {
+Held hold(Arena& m, long rows, long width, int type, bool exact = false) {
   const long ld = up8(width), part = rows * ld;
-  return {m.take<uint16_t>((size_t)part * (type == DT_F32 ? 3 : 1)), ld, part};
+  const int parts = type == DT_F32 ? 3 : exact ? 2 : 1;
+  return {m.take<uint16_t>((size_t)part * parts), ld, parts > 1 ? part : 0, parts};
 }
+// Where a 16-bit operator has so few rows, its intermediates are held in two
+// parts.  Rounded to one, each result has two roundings, sqrt(2) times the
+// error of its own; over many rows that is what it stays, in a sum over few of
+// them one value's rounding may be all there is (up to 2.5 times, seen 1.6).
+// The products are bound by the weights there, not by the matrix units, and up
+// to 64 rows are one step of k in the weights' gradients: 64 x 1,024 x 4,096,
+// forward and backward, 82 us with two parts and 75 with one; the loss of 64 x
+// 1,024 against 65,536 172 and 165.
+bool few_rows(long rows, int type) { return type != DT_F32 && rows <= 64; }
 // Matrices that are copied first, all in one launch: where alignment, an odd
 // width or float32 does not let the tiles be loaded from a matrix itself.  A
 // pass over it; a product of more than a few rows reads it many times.
@@ -101,17 +112,18 @@ struct Copies {
     return h;
   }
   Held held(Arena& m, const void* p, long ld, long rows, long width, int type, bool same_ld = true) {
-    if (fits(p, ld, rows, width, type) && same_ld) return {(const uint16_t*)p, rows > 1 ? ld : width, 0};
+    if (fits(p, ld, rows, width, type) && same_ld) return {(const uint16_t*)p, rows > 1 ? ld : width, 0, 1};
     return add(hold(m, rows, width, type), p, ld, rows, width);
   }
 };
-// The pairs of parts whose products make one product: of three parts of 8 bits
-// each those above 2^-24, smallest first.
+// The pairs of parts whose products make one product, smallest first: of three
+// parts of 8 bits each those above 2^-24, of two parts of one factor both.
 int add_pairs(ProductArgs& p, const Held& a, const Held& b, const Held* b2 = nullptr) {
   static const int part_a[6] = {0, 1, 2, 0, 1, 0}, part_b[6] = {2, 1, 0, 1, 0, 0};
-  const int n = p.dtype == DT_F32 ? 6 : 1;
+  const bool f32 = p.dtype == DT_F32;
+  const int n = f32 ? 6 : std::max(a.parts, b.parts);
   for (int k = 0; k < n; k++) {
-    const int ia = n == 1 ? 0 : part_a[k], ib = n == 1 ? 0 : part_b[k];
+    const int ia = f32 ? part_a[k] : std::min(n - 1 - k, a.parts - 1), ib = f32 ? part_b[k] : std::min(n - 1 - k, b.parts - 1);
     p.a[p.pairs] = a.at(ia);
     p.b[p.pairs] = b.at(ib);
     if (b2) p.b2[p.pairs] = b2->at(ib);
@@ -154,14 +166,16 @@ size_t mlp_forward(const GatedMLPArgs* a, bool count, hipStream_t st) {
   Arena m{count ? nullptr : (char*)a->workspace};
   const int type = a->type;
   const bool same = a->ldgate == a->ldup;
-  const Held h = hold(m, a->rows, a->hidden, type);
+  const bool few = few_rows(a->rows, type);
+  const Held h = hold(m, a->rows, a->hidden, type, few);
   Copies copy;
   const Held x = copy.held(m, a->x, a->ldx, a->rows, a->width, type);
   const Held gate = copy.held(m, a->gate, a->ldgate, a->hidden, a->width, type, same && fits(a->up, a->ldup, a->hidden, a->width, type));
   const Held up = copy.held(m, a->up, a->ldup, a->hidden, a->width, type, same && fits(a->gate, a->ldgate, a->hidden, a->width, type));
   const Held down = copy.held(m, a->down, a->lddown, a->width, a->hidden, type);
   const int parts = type == DT_F32 ? 6 : 1;
-  float* partial = scratch(m, {product_scratch({{a->rows, a->hidden}}, a->width, parts, true), product_scratch({{a->rows, a->width}}, a->hidden, parts)});
+  float* partial = scratch(m, {product_scratch({{a->rows, a->hidden}}, a->width, parts, true),
+                               product_scratch({{a->rows, a->width}}, a->hidden, parts * (few ? 2 : 1))});
   if (count) return m.used;
   lay_out(copy.j, copy.n, type, st);
   ProductArgs p{};
@@ -186,7 +200,8 @@ size_t mlp_backward(const GatedMLPArgs* a, bool count, hipStream_t st) {
   Arena m{count ? nullptr : (char*)a->workspace};
   const int type = a->type;
   const bool same = a->ldgate == a->ldup;
-  const Held dg = hold(m, a->rows, a->hidden, type), du = hold(m, a->rows, a->hidden, type), h = hold(m, a->rows, a->hidden, type);
+  const bool few = few_rows(a->rows, type);
+  const Held dg = hold(m, a->rows, a->hidden, type, few), du = hold(m, a->rows, a->hidden, type, few), h = hold(m, a->rows, a->hidden, type, few);
   Copies copy;
   const Held x = copy.held(m, a->x, a->ldx, a->rows, a->width, type), dy = copy.held(m, a->dy, a->lddy, a->rows, a->width, type);
   const Held gate = copy.held(m, a->gate, a->ldgate, a->hidden, a->width, type, same && fits(a->up, a->ldup, a->hidden, a->width, type));
@@ -194,8 +209,9 @@ size_t mlp_backward(const GatedMLPArgs* a, bool count, hipStream_t st) {
   const Held down = copy.held(m, a->down, a->lddown, a->width, a->hidden, type);
   const int parts = type == DT_F32 ? 6 : 1;
   const Shape in{a->hidden, a->width}, out{a->width, a->hidden};
-  float* partial = scratch(m, {product_scratch({{a->rows, a->hidden}}, a->width, parts), product_scratch({{a->rows, a->width}}, a->hidden, 2 * parts),
-                               product_scratch({in, in, out}, a->rows, parts)});
+  const int held = parts * (few ? 2 : 1);   // pairs of a product with an intermediate
+  float* partial = scratch(m, {product_scratch({{a->rows, a->hidden}}, a->width, parts), product_scratch({{a->rows, a->width}}, a->hidden, 2 * held),
+                               product_scratch({in, in, out}, a->rows, held)});
   if (count) return m.used;
   lay_out(copy.j, copy.n, type, st);
   // dh = dy down, and through the product and the activation
@@ -289,7 +305,7 @@ size_t ce_forward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
 // Rows of the table whose gradients of the logits are held at a time: those
 // of all rows of x take at most 256 MiB, what the last-level cache holds.
 int piece_rows(const CrossEntropyArgs* a) {
-  const long most = (256L << 20) / (std::max<long>(a->rows, 1) * (a->type == DT_F32 ? 6 : 2));
+  const long most = (256L << 20) / (std::max<long>(a->rows, 1) * (a->type == DT_F32 ? 6 : few_rows(a->rows, a->type) ? 4 : 2));
   return (int)std::min<long>(up8(a->vocab), std::max<long>(1024, most / 1024 * 1024));
 }
 
@@ -302,11 +318,14 @@ size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
   float* scale = m.take<float>(1);
   if (a->type == DT_F16) r.scale = scale;
   r.lse = a->lse; r.lse_kept = m.take<float>(n); r.grad_kept = m.take<float>(n);
-  const Held x = hold(m, n, a->width, a->type), dl = hold(m, n, piece, a->type);
-  float* acc = m.take<float>((size_t)n * D);
-  const int parts = a->type == DT_F32 ? 6 : 1, last = a->vocab % piece ? a->vocab % piece : piece;
-  float* partial = scratch(m, {product_scratch({{n, D}}, piece, parts), product_scratch({{n, D}}, last, parts), product_scratch({{piece, D}}, n, parts),
-                               product_scratch({{last, D}}, n, parts)});
+  const bool few = few_rows(n, a->type);
+  const Held x = hold(m, n, a->width, a->type), dl = hold(m, n, piece, a->type, few);
+  // two parts are twice as many rows for dx, in a tile that has room for them (the table is read once); scatter_rows adds them
+  const long stacked = few ? 2 * n : n;
+  float* acc = m.take<float>((size_t)stacked * D);
+  const int parts = a->type == DT_F32 ? 6 : 1, sums = parts * (few ? 2 : 1), last = a->vocab % piece ? a->vocab % piece : piece;
+  float* partial = scratch(m, {product_scratch({{stacked, D}}, piece, parts), product_scratch({{stacked, D}}, last, parts),
+                               product_scratch({{piece, D}}, n, sums), product_scratch({{last, D}}, n, sums)});
   Copies copy;
   copy.add(x, a->x, a->ldx, n, a->width, r.rows, r.count);
   const Held table = copy.held(m, a->table, a->ldtable, a->vocab, a->width, a->type);
@@ -315,7 +334,7 @@ size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
   lay_out(copy.j, copy.n, a->type, st);
   for (long v0 = 0; v0 < a->vocab; v0 += piece) {
     const int len = (int)std::min<long>(piece, a->vocab - v0);
-    const Held rows{table.p + v0 * table.ld, table.ld, table.part};
+    const Held rows{table.p + v0 * table.ld, table.ld, table.part, table.parts};
     ProductArgs p{};
     p.dtype = a->type; p.count = r.count;
     p.M = (int)n; p.N = len; p.K = a->width;
@@ -324,9 +343,9 @@ size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
     p.n0 = (int)v0; p.target = r.tgt; p.lse = r.lse_kept; p.grad = r.grad_kept; p.scale = r.scale;
     product_softmax_grad(p, st);
     ProductArgs q{};
-    q.dtype = a->type; q.ctype = DT_F32; q.count = r.count;
-    q.M = (int)n; q.N = a->width; q.K = len;
-    add_pairs(q, dl, rows);
+    q.dtype = a->type; q.ctype = DT_F32; q.count = few ? nullptr : r.count;   // (few: rows past the count are anything, and are not looked at)
+    q.M = (int)stacked; q.N = a->width; q.K = len;
+    add_pairs(q, {dl.p, dl.ld, dl.part, few ? 1 : dl.parts}, rows);
     q.partial = partial;
     q.c = acc; q.ldc = D; q.add = v0 > 0;
     product_nn(q, st);
@@ -339,7 +358,7 @@ size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
     w.unscale = r.scale;
     product_tn(w, st);
   }
-  scatter_rows(acc, D, r.place, r.scale, a->dx, a->lddx, n, a->width, a->type, st);
+  scatter_rows(acc, D, few ? n * D : 0, r.place, r.scale, a->dx, a->lddx, n, a->width, a->type, st);
   return m.used;
 }
 

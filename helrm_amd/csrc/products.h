@@ -28,7 +28,7 @@ struct ProductArgs {
   const float* unscale;      // the product is divided by this, where there is one
   // gate
   float* g; float* u;        // [M][ldh] float32, kept for the backward pass; may be null
-  void* h; void* dg; void* du;  // [M][ldh], `hpart` elements from one part to the next
+  void* h; void* dg; void* du;  // [M][ldh], `hpart` elements from one part to the next (0: one part)
   long ldh, hpart;           // (hpart also of the c of softmax_grad)
   int act; float coef[4];
   // softmax: table rows n0 .. n0 + N
@@ -83,6 +83,7 @@ struct RowsArgs {
 void kept_rows(const RowsArgs& a, hipStream_t st);
 // loss[row] = lse - picked, lse = the logarithm of the parts' sum
 void softmax_finish(const float2* part, int parts, const float* picked, const int* rows, const int* count, long n, float* loss, float* lse, hipStream_t st);
-// out[row] = acc[place[row]] / *scale, 0 for rows that are not kept
-void scatter_rows(const float* acc, long ldacc, const int* place, const float* scale, void* out, long ldout, long n, int width, int dtype, hipStream_t st);
+// out[row] = (acc[place[row]], and what is `second` elements behind it) / *scale, 0 for rows that are not kept
+void scatter_rows(const float* acc, long ldacc, long second, const int* place, const float* scale, void* out, long ldout, long n, int width, int dtype,
+                  hipStream_t st);
 void fill_zero(void* p, size_t bytes, hipStream_t st);  // bytes: a multiple of 2

@@ -59,7 +59,8 @@ template <class T> __device__ __forceinline__ uint2 pack4(const float v[4]) {
   return __builtin_bit_cast(uint2, __builtin_convertvector(f, T4));
 }
 // Four neighbouring elements into an intermediate in the layout of a factor
-// (8-byte aligned; a float32 operator's: three parts, `part` elements apart).
+// (8-byte aligned; a float32 operator's: three parts, `part` elements apart; of
+// 16 bits: two parts, or one and no `part`).
 template <class T> __device__ __forceinline__ void put_held(u16* o, int type, long part, const float v[4]) {
   *(uint2*)o = pack4<T>(v);
   if (type == DT_F32) {
@@ -73,6 +74,14 @@ template <class T> __device__ __forceinline__ void put_held(u16* o, int type, lo
     }
 #pragma unroll
     for (int k = 0; k < 2; k++) *(uint2*)(o + (k + 1) * part) = pack4<__bf16>(r[k]);
+  } else if (part) {
+    float r[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float first = (float)(T)v[e];
+      r[e] = isfinite(first) ? v[e] - first : 0.0f;
+    }
+    *(uint2*)(o + part) = pack4<T>(r);
   }
 }
 // The first n of four neighbouring elements of a tensor of the caller's.
@@ -758,7 +767,8 @@ __global__ void finish_kernel(const float2* part, int parts, const float* picked
 // A workgroup a row, its sums from where kept_rows put it, or zeros: a run of ignored rows is as parallel as any.
 // Bound by memory: 8,192 x 2,048 from float32 to bfloat16, 100 MB, 18 us = 5.4 TB/s.
 template <class T>
-__global__ __launch_bounds__(256) void scatter_kernel(const float* acc, long ldacc, const int* place, const float* scale, T* out, long ldout, int width) {
+__global__ __launch_bounds__(256) void scatter_kernel(const float* acc, long ldacc, long second, const int* place, const float* scale, T* out, long ldout,
+                                                      int width) {
   const long r = blockIdx.x, i = place[r];
   const float s = scale ? 1.0f / *scale : 1.0f;
   T* o = out + r * ldout;
@@ -767,13 +777,19 @@ __global__ __launch_bounds__(256) void scatter_kernel(const float* acc, long lda
     for (int k = threadIdx.x * 4; k < width; k += 1024) {
       float t[4] = {0, 0, 0, 0};
       if (i >= 0) get4(v + k, t);
+      if (i >= 0 && second) {
+        float l[4];
+        get4(v + second + k, l);
+#pragma unroll
+        for (int e = 0; e < 4; e++) t[e] += l[e];
+      }
       T q[4];
 #pragma unroll
       for (int e = 0; e < 4; e++) q[e] = (T)(t[e] * s);
       __builtin_memcpy(__builtin_assume_aligned(o + k, 4 * sizeof(T)), q, sizeof(q));
     }
   } else {
-    for (int k = threadIdx.x; k < width; k += 256) o[k] = i < 0 ? (T)0.0f : (T)(v[k] * s);
+    for (int k = threadIdx.x; k < width; k += 256) o[k] = i < 0 ? (T)0.0f : (T)((v[k] + (second ? v[second + k] : 0.0f)) * s);
   }
 }
 
@@ -823,10 +839,11 @@ void kept_rows(const RowsArgs& a, hipStream_t st) { kept_rows_kernel<<<1, ROWS_B
 void softmax_finish(const float2* part, int parts, const float* picked, const int* rows, const int* count, long n, float* loss, float* lse, hipStream_t st) {
   if (n) finish_kernel<<<(unsigned)clr::ceil_div(n, 4), 256, 0, st>>>(part, parts, picked, rows, count, loss, lse);
 }
-void scatter_rows(const float* acc, long ldacc, const int* place, const float* scale, void* out, long ldout, long n, int width, int dtype, hipStream_t st) {
+void scatter_rows(const float* acc, long ldacc, long second, const int* place, const float* scale, void* out, long ldout, long n, int width, int dtype,
+                  hipStream_t st) {
   if (n) clr::with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    scatter_kernel<T><<<(unsigned)n, 256, 0, st>>>(acc, ldacc, place, scale, (T*)out, ldout, width);
+    scatter_kernel<T><<<(unsigned)n, 256, 0, st>>>(acc, ldacc, second, place, scale, (T*)out, ldout, width);
   });
 }
 void fill_zero(void* p, size_t bytes, hipStream_t st) {

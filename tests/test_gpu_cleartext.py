@@ -180,6 +180,20 @@ def test_gated_mlp_large_tiles(ct, dtype, rows, width, hidden):
     mlp_check(ct, x, gate, up, down, dy, "gelu")
 
 
+# up to 64 rows the intermediates are held in two parts, off by u^2: only the result is rounded to its type
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,width,hidden", [(1, 72, 64), (3, 264, 1000), (17, 64, 72), (40, 100, 301), (64, 520, 128)])
+def test_gated_mlp_of_few_rows_rounds_once(ct, dtype, rows, width, hidden):
+    x, gate, up, down, dy = mlp_tensors(seeded(rows + hidden), rows, width, hidden, dtype)
+    u, least = ref.U[dtype], 2.0 ** -24 * (1 + hidden + rows) * 4 if dtype == torch.float16 else 0.0
+    tol = 2 * (2 * width + hidden + rows + 40) * F32 + 2 * u * u
+    y, saved = ct.gated_mlp_forward(x, gate, up, down, "silu")
+    got = (y, *ct.gated_mlp_backward(dy, x, gate, up, down, saved, "silu"))
+    want = (ref.mlp(x, gate, up, down, "silu"), *ref.mlp_grad(dy, x, gate, up, down, "silu"))
+    for name, g, r, size in zip(("y", "dx", "dgate", "dup", "ddown"), got, want, ref.mlp_sizes(dy, x, gate, up, down, "silu")):
+        ref.check(g, r, u * r.abs() + 1.01 * (size * tol + least), 1.0, name)
+
+
 @pytest.mark.parametrize("act", ["silu", "gelu", ref.CUBIC])
 @pytest.mark.parametrize("rows", [1, 40])
 def test_gated_mlp_activations(ct, act, rows):
@@ -285,6 +299,19 @@ def test_cross_entropy(ct, dtype, rows, width, vocab):
 def test_cross_entropy_large_tiles(ct, dtype, rows, width, vocab):
     x, table, target, grad = ce_tensors(seeded(rows + vocab), rows, width, vocab, dtype, ignored=0.2)
     ce_check(ct, x, table, target, grad)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,width,vocab", [(1, 72, 264), (3, 264, 1000), (17, 64, 4096), (40, 100, 301), (64, 520, 1300)])
+def test_cross_entropy_of_few_rows_rounds_once(ct, dtype, rows, width, vocab):
+    x, table, target, grad = ce_tensors(seeded(rows + vocab), rows, width, vocab, dtype)
+    _, lse = ct.cross_entropy_forward(x, table, target)
+    u, least = ref.U[dtype], 2.0 ** -24 if dtype == torch.float16 else 2.0 ** -126
+    logit = (width + 12) * F32 * (ref.d(x).abs() @ ref.d(table).abs().T).amax().item()
+    tol, soft = (vocab + rows + 60) * F32 + 2 * u * u, 4 * logit + 8 * F32
+    dx64, dt64, sx, st, px, pt = ref.cross_entropy_grad(grad, x, table, target)
+    for name, g, r, size, p in zip(("dx", "dtable"), ct.cross_entropy_backward(grad, x, table, target, lse), (dx64, dt64), (sx, st), (px, pt)):
+        ref.check(g, r, u * r.abs() + 1.01 * (size * tol + p * soft + least), 1.0, name)
 
 
 def test_cross_entropy_of_two_pieces_of_16_bits(ct):
