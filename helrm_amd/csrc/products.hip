@@ -652,17 +652,24 @@ template <bool A_K, bool B_K, int EPI> void launch(const ProductArgs& p, hipStre
   launch<A_K, B_K, EPI>({p}, plan_of({{p.M, p.N}}, steps_of(p.K, p.pairs), EPI == EPI_GATE, may_split), st);
 }
 
+// A workgroup of 256 for each of n rows: a launch has less than 2^32 threads.
+template <class F> void in_launches(long n, F&& f) {
+  constexpr long MOST = 1L << 23;
+  for (long base = 0; base < n; base += MOST) f(base, (unsigned)std::min(MOST, n - base));
+}
+
 // Up to 8 matrices into the layout that the tiles are loaded from, one launch:
 // rows[i] (or i) of `from` to row i of `to`, filled up with zeros to ldto;
 // float32 as three parts.  Bound by memory: 50,021 x 416 float32, 208 MB read
 // and written, 45 us = 4.7 TB/s.
-struct LayOuts { LayOut j[8]; int first[8]; int count; };
+struct LayOuts { LayOut j[8]; long first[8]; int count; };
 template <class T>
-__global__ __launch_bounds__(256) void lay_out_kernel(const LayOuts all) {
+__global__ __launch_bounds__(256) void lay_out_kernel(const LayOuts all, long base) {
+  const long id = base + blockIdx.x;
   int which = 0;
-  while (which + 1 < all.count && (int)blockIdx.x >= all.first[which + 1]) which++;
+  while (which + 1 < all.count && id >= all.first[which + 1]) which++;
   const LayOut& j = all.j[which];
-  const long i = blockIdx.x - all.first[which];
+  const long i = id - all.first[which];
   if (j.count && i >= *j.count) return;
   const T* f = (const T*)j.from + (j.rows ? (long)j.rows[i] : i) * j.ld;
   u16* to = (u16*)j.to + i * j.ldto;
@@ -768,8 +775,8 @@ __global__ void finish_kernel(const float2* part, int parts, const float* picked
 // Bound by memory: 8,192 x 2,048 from float32 to bfloat16, 100 MB, 18 us = 5.4 TB/s.
 template <class T>
 __global__ __launch_bounds__(256) void scatter_kernel(const float* acc, long ldacc, long second, const int* place, const float* scale, T* out, long ldout,
-                                                      int width) {
-  const long r = blockIdx.x, i = place[r];
+                                                      int width, long base) {
+  const long r = base + blockIdx.x, i = place[r];
   const float s = scale ? 1.0f / *scale : 1.0f;
   T* o = out + r * ldout;
   const float* v = acc + i * ldacc;
@@ -829,11 +836,13 @@ void lay_out(const LayOut* jobs, int n, int dtype, hipStream_t st) {
   long blocks = 0;
   for (int i = 0; i < n; i++)
     if (jobs[i].n > 0) {
-      all.first[all.count] = (int)blocks;
+      all.first[all.count] = blocks;
       all.j[all.count++] = jobs[i];
       blocks += jobs[i].n;
     }
-  if (blocks) clr::with_type(dtype, [&](auto t) { lay_out_kernel<decltype(t)><<<(unsigned)blocks, 256, 0, st>>>(all); });
+  clr::with_type(dtype, [&](auto t) {
+    in_launches(blocks, [&](long base, unsigned n) { lay_out_kernel<decltype(t)><<<n, 256, 0, st>>>(all, base); });
+  });
 }
 void kept_rows(const RowsArgs& a, hipStream_t st) { kept_rows_kernel<<<1, ROWS_BLOCK, 0, st>>>(a); }
 void softmax_finish(const float2* part, int parts, const float* picked, const int* rows, const int* count, long n, float* loss, float* lse, hipStream_t st) {
@@ -841,9 +850,9 @@ void softmax_finish(const float2* part, int parts, const float* picked, const in
 }
 void scatter_rows(const float* acc, long ldacc, long second, const int* place, const float* scale, void* out, long ldout, long n, int width, int dtype,
                   hipStream_t st) {
-  if (n) clr::with_type(dtype, [&](auto t) {
+  clr::with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    scatter_kernel<T><<<(unsigned)n, 256, 0, st>>>(acc, ldacc, second, place, scale, (T*)out, ldout, width);
+    in_launches(n, [&](long base, unsigned k) { scatter_kernel<T><<<k, 256, 0, st>>>(acc, ldacc, second, place, scale, (T*)out, ldout, width, base); });
   });
 }
 void fill_zero(void* p, size_t bytes, hipStream_t st) {

@@ -442,6 +442,49 @@ def test_cross_entropy_table_offsets_beyond_32_bits(ct):
     ref.check(dx, p @ ref.d(table[-200:]), p.abs() @ ref.d(table[-200:]).abs(), 2.0 ** -6, "dx")
 
 
+def test_cross_entropy_of_more_rows_than_one_launch_has_workgroups(ct):
+    # a table of more than 2^24 rows that has to be laid out (bfloat16 of an odd width); equal logits but for a few rows
+    vocab, width, rows = (1 << 24) + 77, 3, 20
+    gen = seeded(2)
+    table = torch.zeros(vocab, width, dtype=torch.bfloat16, device=DEV)
+    table[-50:] = normal(gen, 50, width, dtype=torch.bfloat16)
+    x = normal(gen, rows, width, std=3.0, dtype=torch.bfloat16)
+    target = torch.arange(vocab - rows, vocab, device=DEV)
+    losses, lse = ct.cross_entropy_forward(x, table, target)
+    z = ref.d(x) @ ref.d(table[-50:]).T
+    s = torch.log(torch.exp(z).sum(1) + (vocab - 50))
+    at = torch.arange(rows)
+    ref.check(lse, s, torch.ones(rows), 1e-4, "lse")
+    ref.check(losses, s - z[at, 50 - rows + at], torch.ones(rows), 1e-4, "losses")
+    dx, dtable = ct.cross_entropy_backward(torch.ones(rows, device=DEV), x, table, target, lse)
+    p = torch.exp(z - s[:, None])
+    p[at, 50 - rows + at] -= 1
+    ref.check(dx, p @ ref.d(table[-50:]), p.abs() @ ref.d(table[-50:]).abs(), 2.0 ** -6, "dx")
+    ref.check(dtable[-50:], p.T @ ref.d(x), p.abs().T @ ref.d(x).abs(), 2.0 ** -6, "dtable")
+
+
+def test_cross_entropy_of_more_vectors_than_one_launch_has_workgroups(ct):
+    rows = (1 << 24) + 99
+    gen = seeded(3)
+    x = torch.zeros(rows, 1, dtype=torch.bfloat16, device=DEV)
+    x[-40:] = normal(gen, 40, 1, dtype=torch.bfloat16)
+    table = normal(gen, 2, 1, dtype=torch.bfloat16)
+    target = torch.zeros(rows, dtype=torch.int64, device=DEV)
+    losses, lse = ct.cross_entropy_forward(x, table, target)
+    z = ref.d(x[-40:]) @ ref.d(table).T
+    s = torch.logsumexp(z, 1)
+    ref.check(lse[-40:], s, torch.ones(40), 1e-5, "lse")
+    ref.check(losses[-40:], s - z[:, 0], torch.ones(40), 1e-5, "losses")
+    grad = torch.zeros(rows, device=DEV)
+    grad[-40:] = 1.0
+    dx, dtable = ct.cross_entropy_backward(grad, x, table, target, lse)
+    p = torch.exp(z - s[:, None])
+    p[:, 0] -= 1
+    ref.check(dx[-40:], p @ ref.d(table), p.abs() @ ref.d(table).abs(), 2.0 ** -6, "dx")
+    ref.check(dtable, p.T @ ref.d(x[-40:]), p.abs().T @ ref.d(x[-40:]).abs(), 2.0 ** -6, "dtable")
+    assert not dx[:-40].any()
+
+
 # ---- gradients against differences, autograd -------------------------------------------
 
 
