@@ -36,6 +36,11 @@ void check_matrix(const void* p, long ld, long rows, long width, const char* wha
 }
 constexpr long MAX_ROWS = 1L << 30;
 constexpr long MAX_LD = 1L << 21;  // 256 rows are within a buffer descriptor's 31-bit offsets
+// A result that the products store themselves: 128 of its rows are within 32-bit offsets.
+void check_result(const void* p, long ld, long rows, long width, const char* what) {
+  check_matrix(p, ld, rows, width, what);
+  require(rows <= 1 || ld < 1L << 24, what);
+}
 
 // ---- layer norm ----
 void check_norm(const LayerNormArgs* a) {
@@ -409,7 +414,7 @@ int GatedMLP(const GatedMLPArgs* a, void* stream) {
   return clr::guarded([&] {
     check_mlp(a);
     check_mlp_tensors(a);
-    check_matrix(a->y, a->ldy, a->rows, a->width, "GatedMLP: y");
+    check_result(a->y, a->ldy, a->rows, a->width, "GatedMLP: y");
     require(!a->g == !a->u, "GatedMLP: g and u are kept together");
     require(((uintptr_t)a->g | (uintptr_t)a->u) % 16 == 0, "GatedMLP: g and u are not aligned to 16 bytes");
     if (!a->rows) return;
@@ -425,7 +430,7 @@ int GatedMLPGrad(const GatedMLPArgs* a, void* stream) {
     check_mlp(a);
     check_mlp_tensors(a);
     check_matrix(a->dy, a->lddy, a->rows, a->width, "GatedMLPGrad: dy");
-    check_matrix(a->dx, a->lddx, a->rows, a->width, "GatedMLPGrad: dx");
+    check_result(a->dx, a->lddx, a->rows, a->width, "GatedMLPGrad: dx");
     require((a->g && a->u) || !a->rows, "GatedMLPGrad: g and u");
     require(((uintptr_t)a->g | (uintptr_t)a->u) % 16 == 0, "GatedMLPGrad: g and u are not aligned to 16 bytes");
     require(a->dgate && a->dup && a->ddown, "GatedMLPGrad: the weights' gradients");

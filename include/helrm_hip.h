@@ -306,13 +306,15 @@ int LayerNormGrad(const LayerNormArgs* args, void* stream);
 
 /* y = (act(x gate^T) * (x up^T)) down^T: the gated feed-forward block.
  * act 0: silu, 1: gelu (erf), 2: cubic, coef lowest degree first, the form
- * that EvaluatePolynomial takes. */
+ * that EvaluatePolynomial takes.  The products' factors act(g) u, dg and du are
+ * of the tensors' type (in two parts up to 64 rows): in float16 one beyond
+ * 65504 is infinite. */
 typedef struct {
   const void* x; long ldx;               /* [rows][width] */
   const void* gate; long ldgate;         /* [hidden][width] */
   const void* up; long ldup;             /* [hidden][width] */
   const void* down; long lddown;         /* [width][hidden] */
-  void* y; long ldy;                     /* [rows][width] */
+  void* y; long ldy;                     /* [rows][width]; ldy and lddx below 2^24 */
   float* g; float* u;                    /* x gate^T and x up^T, kept for the gradient (both or neither), 16-byte aligned:
                                             [rows][hidden rounded up to a multiple of 8] each, the rest of a row 0 */
   const void* dy; long lddy;             /* GatedMLPGrad */

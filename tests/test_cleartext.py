@@ -88,6 +88,15 @@ def test_missing_tensors(lib):
     refused(lib, "CrossEntropyGrad", loss(lse=None), "lse")
 
 
+def test_results_whose_rows_are_too_far_apart(lib):
+    """A tile's places in a result are 32-bit offsets from its first one."""
+    for ld in (1 << 24, 1 << 40):
+        refused(lib, "GatedMLP", mlp(ldy=ld), "GatedMLP: y")
+        refused(lib, "GatedMLPGrad", mlp(lddx=ld), "GatedMLPGrad: dx")
+    refused(lib, "GatedMLP", mlp(ldy=(1 << 24) - 1), "workspace too small")
+    refused(lib, "GatedMLP", mlp(rows=1, ldy=1 << 40), "workspace too small")
+
+
 def test_workspaces(lib):
     for call, make in (("LayerNormGrad", norm), ("GatedMLP", mlp), ("GatedMLPGrad", mlp), ("CrossEntropy", loss), ("CrossEntropyGrad", loss)):
         size = getattr(lib, call + "Workspace")
