@@ -302,7 +302,19 @@ size_t ce_forward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
   p.M = (int)n; p.N = a->vocab; p.K = a->width;
   add_pairs(p, x, table);
   p.count = r.count; p.target = r.tgt; p.picked = r.picked; p.part = part; p.parts = parts;
-  product_softmax(p, st);
+  // A launch has less than 2^32 threads, 512 for a tile of 256 x 256 (so many
+  // tiles are never the small ones): the table in equal pieces of 2^22 tiles
+  // or less, nearly always one.
+  const long launches = clr::ceil_div(clr::ceil_div(n, 256) * clr::ceil_div(a->vocab, 256), 1L << 22);
+  const long len = launches > 1 ? clr::ceil_div(clr::ceil_div(a->vocab, launches), 256) * 256 : a->vocab;
+  for (long v0 = 0; v0 < a->vocab; v0 += len) {
+    ProductArgs q = p;
+    q.n0 = (int)v0;
+    q.N = (int)std::min<long>(len, a->vocab - v0);
+    for (int k = 0; k < q.pairs; k++) q.b[k] += v0 * q.ldb;
+    q.part += v0 / 256;   // (v0 is not 0 with large tiles alone)
+    product_softmax(q, st);
+  }
   softmax_finish(part, parts, r.picked, r.rows, r.count, n, a->loss, a->lse, st);
   return m.used;
 }

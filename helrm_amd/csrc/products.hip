@@ -209,7 +209,7 @@ __device__ __forceinline__ void softmax_piece(const ProductArgs& p, const f32x4 
   for (int i = 0; i < FM; i++) {
     const int r = (wave_m * FM + i) * 16 + (lane & 15);
     const long m = m0 + r;
-    const int t = m < M ? p.target[m] - (int)(n0 + wave_n * FN * 16 + 4 * quad) : -1;   // the target's place from there
+    const int t = m < M ? p.target[m] - (int)(p.n0 + n0 + wave_n * FN * 16 + 4 * quad) : -1;   // the target's place from there
     if (t >= 0 && t < FN * 16) {   // (seldom: one tile has it)
 #pragma unroll
       for (int c = 0; c < FN * 4; c++) if (16 * (c >> 2) + (c & 3) == t) p.picked[m] = acc[i][c >> 2][c & 3];

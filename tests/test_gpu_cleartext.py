@@ -485,6 +485,23 @@ def test_cross_entropy_of_more_vectors_than_one_launch_has_workgroups(ct):
     assert not dx[:-40].any()
 
 
+def test_cross_entropy_of_more_tiles_than_one_launch_has(ct):
+    # 64 x 65538 tiles of 256 x 256: two launches
+    rows, vocab, width = 16384, (1 << 24) + 300, 8
+    gen = seeded(4)
+    table = torch.zeros(vocab, width, dtype=torch.bfloat16, device=DEV)
+    some = torch.cat([torch.arange(100, 120), torch.arange((1 << 23) - 300, (1 << 23) + 600, 15), torch.arange(vocab - 40, vocab)])
+    table[some.to(DEV)] = normal(gen, len(some), width, dtype=torch.bfloat16)
+    x = normal(gen, rows, width, std=2.0, dtype=torch.bfloat16)
+    at = torch.randint(len(some), (rows,), generator=gen)
+    losses, lse = ct.cross_entropy_forward(x, table, some[at].to(DEV))
+    z = ref.d(x) @ ref.d(table[some.to(DEV)]).T
+    top = z.amax(1).clamp(min=0)
+    s = top + torch.log(torch.exp(z - top[:, None]).sum(1) + (vocab - len(some)) * torch.exp(-top))
+    ref.check(lse, s, torch.ones(rows), 1e-4, "lse")
+    ref.check(losses, s - z[torch.arange(rows), at], torch.ones(rows), 1e-4, "losses")
+
+
 # ---- gradients against differences, autograd -------------------------------------------
 
 
