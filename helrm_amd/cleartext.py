@@ -48,12 +48,14 @@ def _library():
     if len(runtimes) > 1:
         raise HipError("two HIP runtimes in one process (" + ", ".join(sorted(runtimes))
                        + "): import torch before the library is loaded")
+    calls = {}
     for name in ("LayerNorm", "LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad"):
         call, size = getattr(lib, name), getattr(lib, name + "Workspace") if name != "LayerNorm" else None
         call.argtypes, call.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
         if size is not None:
             size.argtypes, size.restype = [ctypes.c_void_p], ctypes.c_long
-        _calls[name] = call, size
+        calls[name] = call, size
+    _calls.update(calls)   # all at once: another thread finds none of them or every one
 
 
 def _refused():
@@ -290,7 +292,8 @@ class _GatedMLP(torch.autograd.Function):
 def gated_mlp(x, gate, up, down, activation="silu"):
     """The gated feed-forward block (act(x gate^T) * (x up^T)) down^T: gate, up [hidden, width], down [width, hidden].
     activation: "silu", "gelu" or a cubic's four coefficients, lowest degree first, which the block can also be
-    evaluated with under encryption."""
+    evaluated with under encryption.  Hidden values and their gradients are factors of the next product, of x's type: in
+    float16 one beyond 65504 is infinite."""
     if _wants_grad(x, gate, up, down):
         return _GatedMLP.apply(x, gate, up, down, activation)
     return _mlp_forward(x, gate, up, down, activation, False)[0]
