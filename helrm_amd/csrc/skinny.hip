@@ -9,9 +9,10 @@
 // row and turn, and multiply up to four groups of 16 rows of X there
 // (v_mfma_f32_16x16x32).  The waves of a workgroup share out k and add their
 // sums through LDS, so that a short matrix still keeps every CU loading.
-// Nothing is laid out first: unaligned matrices are read an element at a time,
-// float32 ones are split into three bfloat16 parts in registers and multiplied
-// as in products.hip.
+// Nothing is laid out first: rows of any alignment are read 16 bytes at a time,
+// but for a row's last odd elements (one row against 65,536 x 1,001: bfloat16 46
+// us, 98 an element at a time; float32 60 and 124), and float32 ones are split
+// into three bfloat16 parts in registers and multiplied as in products.hip.
 //
 // Measured: one row against 65,536 x 1,024 bfloat16, 134 MB, 28 us = 4.8 TB/s
 // (a copy: 4.95); the gate and up projections of one row, 17 MB, 8 to 11 us,
@@ -41,9 +42,11 @@ template <class T, bool ALIGNED> __device__ __forceinline__ Raw<T> load8(const T
       for (int i = 0; i < (int)sizeof(T) / 2; i++) q[i] = ((const uint4*)(p + k))[i];
       __builtin_memcpy(&r, q, sizeof(r));
     }
-  } else {
+  } else if (in && k + 8 <= K) {
+    __builtin_memcpy(&r, p + k, sizeof(r));   // (global loads of 16 bytes need no alignment)
+  } else if (in) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) if (in && k + e < K) r.e[e] = p[k + e];
+    for (int e = 0; e < 8; e++) if (k + e < K) r.e[e] = p[k + e];
   }
   return r;
 }
@@ -101,7 +104,7 @@ template <class T, bool ALIGNED, int NB> constexpr int most_waves() { return siz
 // X: the type of x, T or float.
 template <class T, class X, bool ALIGNED, int NB, int EPI>
 __global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_kernel(const SkinnyArgs p) {
-  constexpr int MATS = EPI == SKINNY_GATE ? 2 : 1, TURNS = !ALIGNED ? 1 : sizeof(T) == 4 ? 2 : 4;
+  constexpr int MATS = EPI == SKINNY_GATE ? 2 : 1, TURNS = !ALIGNED || sizeof(T) == 4 ? 2 : 4;
   extern __shared__ float lds[];   // [waves][MATS * NB][64][4]
   const int lane = threadIdx.x & 63, own = threadIdx.x >> 6;
   const int wave = p.alone ? 0 : own, waves = p.alone ? 1 : blockDim.x >> 6;   // of those that share k
