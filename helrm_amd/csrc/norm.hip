@@ -25,21 +25,27 @@ constexpr int MOST_WAVES = 8;        // of a row: 8,192 values; longer rows are 
 template <class T, int V> struct Pack { T v[V]; };
 
 // A row's values, V neighbours at a time: lane l of n takes packs l, l + n, ...
-template <class T, int V, int N>
+// ODD: rows start anywhere and the last pack may be cut short.
+template <class T, int V, int N, bool ODD>
 __device__ __forceinline__ void load_row(const T* p, int lane, int n, int width, float (&v)[N * V]) {
 #pragma unroll
   for (int j = 0; j < N; j++) {
     const int i = (j * n + lane) * V;
     Pack<T, V> t{};
-    if (i < width) {
-      if constexpr (V * sizeof(T) == 16) { const uint4 raw = *(const uint4*)(p + i); t = __builtin_bit_cast(decltype(t), raw); }
-      else t.v[0] = p[i];
+    if constexpr (ODD) {
+      if (i + V <= width) __builtin_memcpy(&t, p + i, sizeof(t));   // (global loads of 16 bytes need no alignment)
+      else
+#pragma unroll
+        for (int e = 0; e < V; e++) if (i + e < width) t.v[e] = p[i + e];
+    } else if (i < width) {
+      const uint4 raw = *(const uint4*)(p + i);
+      t = __builtin_bit_cast(decltype(t), raw);
     }
 #pragma unroll
     for (int e = 0; e < V; e++) v[j * V + e] = (float)t.v[e];
   }
 }
-template <class T, int V, int N>
+template <class T, int V, int N, bool ODD>
 __device__ __forceinline__ void store_row(T* p, int lane, int n, int width, const float (&v)[N * V]) {
 #pragma unroll
   for (int j = 0; j < N; j++) {
@@ -48,26 +54,29 @@ __device__ __forceinline__ void store_row(T* p, int lane, int n, int width, cons
     Pack<T, V> t;
 #pragma unroll
     for (int e = 0; e < V; e++) t.v[e] = (T)v[j * V + e];
-    if constexpr (V * sizeof(T) == 16) *(uint4*)(p + i) = __builtin_bit_cast(uint4, t);
-    else p[i] = t.v[0];
+    if constexpr (!ODD) *(uint4*)(p + i) = __builtin_bit_cast(uint4, t);
+    else if (i + V <= width) __builtin_memcpy(p + i, &t, sizeof(t));
+    else
+#pragma unroll
+      for (int e = 0; e < V; e++) if (i + e < width) p[i + e] = t.v[e];
   }
 }
 // The weights of the same places, 0 past the end of the row.
-template <class P, int V, int N>
+template <class P, int V, int N, bool ODD>
 __device__ __forceinline__ void load_param(const P* p, int lane, int n, int width, float (&v)[N * V]) {
 #pragma unroll
   for (int j = 0; j < N; j++) {
     const int i = (j * n + lane) * V;
     Pack<P, V> t{};
     if (i < width) {
-      if constexpr (V * sizeof(P) % 16 == 0) {
+      if constexpr (!ODD && V * sizeof(P) % 16 == 0) {
         uint4 raw[V * sizeof(P) / 16];
 #pragma unroll
         for (int k = 0; k < (int)(V * sizeof(P) / 16); k++) raw[k] = ((const uint4*)(p + i))[k];
         __builtin_memcpy(&t, raw, sizeof(t));
       } else {
 #pragma unroll
-        for (int e = 0; e < V; e++) t.v[e] = p[i + e];
+        for (int e = 0; e < V; e++) if (!ODD || i + e < width) t.v[e] = p[i + e];
       }
     }
 #pragma unroll
@@ -94,7 +103,7 @@ template <bool MANY> __device__ __forceinline__ float2 row_sum(float2 v, int wav
 // MANY: the workgroup has one row at a time; otherwise each of its waves has
 // one.  It takes every gridDim.x-th (of four): the weights stay in registers,
 // where 32-bit ones of their own would be twice the traffic of a 16-bit row.
-template <class T, class P, int V, int N, bool MANY>
+template <class T, class P, int V, int N, bool ODD, bool MANY>
 __global__ __launch_bounds__(MANY ? 512 : BLOCK) void norm_forward(const T* x, long ldx, const P* w, const P* b, T* y, long ldy, float* mean,
                                                                      float* rstd, long rows, int width, float eps) {
   __shared__ float2 lds[4][MOST_WAVES];
@@ -102,8 +111,8 @@ __global__ __launch_bounds__(MANY ? 512 : BLOCK) void norm_forward(const T* x, l
   const int lane = MANY ? threadIdx.x : threadIdx.x & 63, n = waves * 64;
   const long per = MANY ? 1 : BLOCK / 64;
   float c[N * V], o[N * V];
-  load_param<P, V, N>(w, lane, n, width, c);
-  if (b) load_param<P, V, N>(b, lane, n, width, o);
+  load_param<P, V, N, ODD>(w, lane, n, width, c);
+  if (b) load_param<P, V, N, ODD>(b, lane, n, width, o);
   else {
 #pragma unroll
     for (int i = 0; i < N * V; i++) o[i] = 0.0f;
@@ -111,7 +120,7 @@ __global__ __launch_bounds__(MANY ? 512 : BLOCK) void norm_forward(const T* x, l
   int turn = 0;
   for (long row = blockIdx.x * per + (MANY ? 0 : threadIdx.x >> 6); row < rows; row += gridDim.x * per, turn ^= 2) {
     float v[N * V];
-    load_row<T, V, N>(x + row * ldx, lane, n, width, v);
+    load_row<T, V, N, ODD>(x + row * ldx, lane, n, width, v);
     float s = 0;
 #pragma unroll
     for (int i = 0; i < N * V; i++) s += v[i];
@@ -121,14 +130,14 @@ __global__ __launch_bounds__(MANY ? 512 : BLOCK) void norm_forward(const T* x, l
     for (int j = 0; j < N; j++)
 #pragma unroll
       for (int e = 0; e < V; e++) {
-        const float d = (j * n + lane) * V < width ? v[j * V + e] - mu : 0.0f;
+        const float d = (j * n + lane) * V + (ODD ? e : 0) < width ? v[j * V + e] - mu : 0.0f;
         v[j * V + e] = d;
         q += d * d;
       }
     const float r = 1.0f / sqrtf(row_sum<MANY>(make_float2(q, 0), wave, waves, lds[turn + 1]).x / width + eps);
 #pragma unroll
     for (int i = 0; i < N * V; i++) v[i] = v[i] * r * c[i] + o[i];
-    store_row<T, V, N>(y + row * ldy, lane, n, width, v);
+    store_row<T, V, N, ODD>(y + row * ldy, lane, n, width, v);
     if (lane == 0) {
       if (mean) mean[row] = mu;
       if (rstd) rstd[row] = r;
@@ -139,7 +148,7 @@ __global__ __launch_bounds__(MANY ? 512 : BLOCK) void norm_forward(const T* x, l
 // A workgroup takes every gridDim.x-th row (MANY), or four of them at a time,
 // one a wave, and leaves the sums of dy h and dy over its rows in
 // part[blockIdx.x][2][width].
-template <class T, class P, int V, int N, bool MANY>
+template <class T, class P, int V, int N, bool ODD, bool MANY>
 __global__ __launch_bounds__(MANY ? 512 : BLOCK) void norm_backward(const T* dy, long lddy, const T* x, long ldx, const P* w, const float* mean,
                                                                      const float* rstd, T* dx, long lddx, float* part, long rows, int width) {
   constexpr int E = N * V;
@@ -150,21 +159,22 @@ __global__ __launch_bounds__(MANY ? 512 : BLOCK) void norm_backward(const T* dy,
   const int mine = MANY ? 0 : threadIdx.x >> 6;
   const long per = MANY ? 1 : BLOCK / 64;
   float c[E], sw[E], sb[E];
-  load_param<P, V, N>(w, lane, n, width, c);
+  load_param<P, V, N, ODD>(w, lane, n, width, c);
 #pragma unroll
   for (int i = 0; i < E; i++) sw[i] = sb[i] = 0;
   int turn = 0;
   for (long row = blockIdx.x * per + mine; row < rows; row += gridDim.x * per, turn ^= 1) {
     float h[E], d[E];
-    load_row<T, V, N>(x + row * ldx, lane, n, width, h);
-    load_row<T, V, N>(dy + row * lddy, lane, n, width, d);
+    load_row<T, V, N, ODD>(x + row * ldx, lane, n, width, h);
+    load_row<T, V, N, ODD>(dy + row * lddy, lane, n, width, d);
     const float mu = mean[row], r = rstd[row];
     float2 s = make_float2(0, 0);
 #pragma unroll
     for (int j = 0; j < N; j++) {
-      const float m = (j * n + lane) * V < width ? mu : 0.0f;   // past the end of the row d, c and h are 0, also where mu r overflows
 #pragma unroll
       for (int i = j * V; i < (j + 1) * V; i++) {
+        // past the end of the row d, c and h are 0, also where mu r overflows
+        const float m = (j * n + lane) * V + (ODD ? i - j * V : 0) < width ? mu : 0.0f;
         h[i] = (h[i] - m) * r;
         sw[i] += d[i] * h[i];
         sb[i] += d[i];
@@ -178,7 +188,7 @@ __global__ __launch_bounds__(MANY ? 512 : BLOCK) void norm_backward(const T* dy,
     s.y /= width;
 #pragma unroll
     for (int i = 0; i < E; i++) d[i] = r * (d[i] - s.x - h[i] * s.y);
-    store_row<T, V, N>(dx + row * lddx, lane, n, width, d);
+    store_row<T, V, N, ODD>(dx + row * lddx, lane, n, width, d);
   }
   float* out = part + (long)blockIdx.x * 2 * width;
 #pragma unroll
@@ -309,15 +319,23 @@ int part_count(long rows, int width) {
   return (int)std::max<long>(1, std::min<long>(512, clr::ceil_div(rows, per)));
 }
 
-// f(V, N): how a row is loaded -- 16 bytes at a time where every row of every tensor starts at a multiple of 16 bytes
-// and holds a whole number of them, else an element -- and how many of these a lane takes; the weights start at such a multiple then
+// f(V, N, ODD): how a row is loaded -- V elements at a time, N times a lane -- and whether not every row of every tensor
+// (and the weights) starts at a multiple of 16 bytes and holds a whole number of them.  Then 16-bit rows are still read 16
+// bytes at a time (32,768 x 4,095 bfloat16 forward 204 us, 335 an element at a time, backward 327 and 966; 4,097 x 1,001
+// backward 19 and 38), except forward with a whole row of 513 to 1,024 in one wave, where the cut pack holds the wave up
+// (4,097 x 1,001 14 us, 10 an element at a time), and float32 an element at a time (4,097 x 1,001 10 + 17 us, 14 + 18 in packs).
 template <int V> struct Int { static constexpr int value = V; };
-template <class T, class F> void with_packs(bool aligned, int width, int waves, F&& f) {
+template <class T, class F> void with_packs(bool aligned, bool forward, int width, int waves, F&& f) {
   constexpr int V = 16 / sizeof(T);
-  const int n = (int)clr::ceil_div(width, waves * 64 * V);
-  if (!aligned) f(Int<1>{}, Int<HOLD>{});
-  else if (n <= HOLD / V / 2) f(Int<V>{}, Int<HOLD / V / 2>{});
-  else f(Int<V>{}, Int<HOLD / V>{});
+  const bool half = clr::ceil_div(width, waves * 64 * V) <= HOLD / V / 2;
+  auto go = [&](auto odd) {
+    if (half) f(Int<V>{}, Int<HOLD / V / 2>{}, odd);
+    else f(Int<V>{}, Int<HOLD / V>{}, odd);
+  };
+  if (aligned) return go(std::false_type{});
+  if constexpr (sizeof(T) == 2)
+    if (!forward || waves > 1 || half) return go(std::true_type{});
+  f(Int<1>{}, Int<HOLD>{}, std::true_type{});
 }
 bool packs(const void* p, long ld, long rows, int width, int dtype) {
   const int v = 16 / dtype_size(dtype);
@@ -340,12 +358,12 @@ void norm_forward_launch(const NormArgs& a, hipStream_t st) {
                                                                     a.rstd, a.width, a.eps);
         return;
       }
-      with_packs<T>(aligned, a.width, waves, [&](auto v, auto n) {
+      with_packs<T>(aligned, true, a.width, waves, [&](auto v, auto n, auto odd) {
         if (waves > 1)
-          norm_forward<T, P, decltype(v)::value, decltype(n)::value, true><<<(unsigned)std::min<long>(a.rows, MOST_GROUPS), waves * 64, 0, st>>>(
+          norm_forward<T, P, decltype(v)::value, decltype(n)::value, decltype(odd)::value, true><<<(unsigned)std::min<long>(a.rows, MOST_GROUPS), waves * 64, 0, st>>>(
               (const T*)a.x, a.ldx, (const P*)a.weight, (const P*)a.bias, (T*)a.y, a.ldy, a.mean, a.rstd, a.rows, a.width, a.eps);
         else
-          norm_forward<T, P, decltype(v)::value, decltype(n)::value, false><<<(unsigned)std::min(clr::ceil_div(a.rows, BLOCK / 64), MOST_GROUPS), BLOCK, 0, st>>>(
+          norm_forward<T, P, decltype(v)::value, decltype(n)::value, decltype(odd)::value, false><<<(unsigned)std::min(clr::ceil_div(a.rows, BLOCK / 64), MOST_GROUPS), BLOCK, 0, st>>>(
               (const T*)a.x, a.ldx, (const P*)a.weight, (const P*)a.bias, (T*)a.y, a.ldy, a.mean, a.rstd, a.rows, a.width, a.eps);
       });
     };
@@ -372,12 +390,12 @@ void norm_backward_launch(const NormArgs& a, hipStream_t st) {
           norm_backward_long<T, P><<<(unsigned)a.rows, BLOCK, 0, st>>>((const T*)a.y, a.ldy, (const T*)a.x, a.ldx, (const P*)a.weight, a.mean, a.rstd,
                                                                        (T*)a.dx, a.lddx, a.width);
       } else {
-        with_packs<T>(aligned, a.width, waves, [&](auto v, auto n) {
+        with_packs<T>(aligned, false, a.width, waves, [&](auto v, auto n, auto odd) {
           if (waves > 1)
-            norm_backward<T, P, decltype(v)::value, decltype(n)::value, true><<<parts, waves * 64, 0, st>>>(
+            norm_backward<T, P, decltype(v)::value, decltype(n)::value, decltype(odd)::value, true><<<parts, waves * 64, 0, st>>>(
                 (const T*)a.y, a.ldy, (const T*)a.x, a.ldx, (const P*)a.weight, a.mean, a.rstd, (T*)a.dx, a.lddx, part, a.rows, a.width);
           else
-            norm_backward<T, P, decltype(v)::value, decltype(n)::value, false><<<parts, BLOCK, 0, st>>>(
+            norm_backward<T, P, decltype(v)::value, decltype(n)::value, decltype(odd)::value, false><<<parts, BLOCK, 0, st>>>(
                 (const T*)a.y, a.ldy, (const T*)a.x, a.ldx, (const P*)a.weight, a.mean, a.rstd, (T*)a.dx, a.lddx, part, a.rows, a.width);
         });
       }
