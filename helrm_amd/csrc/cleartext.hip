@@ -47,6 +47,8 @@ void check_norm(const LayerNormArgs* a) {
   require(a, "no arguments");
   check_type(a->type);
   check_type(a->paramType);
+  // the kernels read and write parameters as one of these two: another type has elements of another size
+  require(a->paramType == a->type || a->paramType == DT_F32, "LayerNorm: paramType is neither type nor float32");
   require(a->rows >= 0 && a->rows < INT_MAX, "LayerNorm: bad number of rows");
   require(a->width >= 1, "LayerNorm: bad width");
 }

@@ -297,7 +297,7 @@ typedef struct {
   void* dweight; void* dbias;            /* [width], of paramType; dbias may be NULL */
   void* workspace; size_t workspaceBytes; /* LayerNormGrad only */
   long rows; int width;
-  int type; int paramType;
+  int type; int paramType;               /* paramType: type, or float32 */
   float eps;
 } LayerNormArgs;
 int LayerNorm(const LayerNormArgs* args, void* stream);
