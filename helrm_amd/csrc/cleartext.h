@@ -7,6 +7,7 @@
 #include <stdint.h>
 #include <stdexcept>
 #include <string>
+#include "plan.h"
 
 // The element types of an operator's tensors, as the C ABI numbers them.
 enum DType { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
@@ -27,7 +28,6 @@ template <class F> int guarded(F&& f) {
   catch (const std::exception& e) { return report_error(e.what()); }
   catch (...) { return report_error("unknown error"); }
 }
-inline long ceil_div(long a, long b) { return (a + b - 1) / b; }
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // f(T{}) with T the C++ type of a DType

@@ -287,12 +287,12 @@ size_t ce_forward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
   if (a->rows <= skinny_rows(a->type)) return ce_skinny(a, count, st);
   Arena m{count ? nullptr : (char*)a->workspace};
   const long n = a->rows;
-  const int parts = softmax_parts(n, a->vocab, a->width, a->type == DT_F32 ? 6 : 1);
+  const clr::SoftmaxPlan plan = clr::softmax_plan(n, a->vocab, a->width, a->type == DT_F32 ? 6 : 1);
   RowsArgs r{a->target, nullptr, n, a->ignore, a->vocab};
   r.rows = m.take<int>(n); r.tgt = m.take<int>(n); r.count = m.take<int>(1);
   r.picked = m.take<float>(n); r.loss = a->loss; r.lse = a->lse;
   const Held x = hold(m, n, a->width, a->type);
-  float2* part = m.take<float2>((size_t)n * parts);
+  float2* part = m.take<float2>((size_t)n * plan.parts);
   Copies copy;
   copy.add(x, a->x, a->ldx, n, a->width, r.rows, r.count);
   const Held table = copy.held(m, a->table, a->ldtable, a->vocab, a->width, a->type);
@@ -303,21 +303,9 @@ size_t ce_forward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
   p.dtype = a->type;
   p.M = (int)n; p.N = a->vocab; p.K = a->width;
   add_pairs(p, x, table);
-  p.count = r.count; p.target = r.tgt; p.picked = r.picked; p.part = part; p.parts = parts;
-  // A launch has less than 2^32 threads, 512 for a tile of 256 x 256 (so many
-  // tiles are never the small ones): the table in equal pieces of 2^22 tiles
-  // or less, nearly always one.
-  const long launches = clr::ceil_div(clr::ceil_div(n, 256) * clr::ceil_div(a->vocab, 256), 1L << 22);
-  const long len = launches > 1 ? clr::ceil_div(clr::ceil_div(a->vocab, launches), 256) * 256 : a->vocab;
-  for (long v0 = 0; v0 < a->vocab; v0 += len) {
-    ProductArgs q = p;
-    q.n0 = (int)v0;
-    q.N = (int)std::min<long>(len, a->vocab - v0);
-    for (int k = 0; k < q.pairs; k++) q.b[k] += v0 * q.ldb;
-    q.part += v0 / 256;   // (v0 is not 0 with large tiles alone)
-    product_softmax(q, st);
-  }
-  softmax_finish(part, parts, r.picked, r.rows, r.count, n, a->loss, a->lse, st);
+  p.count = r.count; p.target = r.tgt; p.picked = r.picked; p.part = part;
+  product_softmax(p, plan, st);
+  softmax_finish(part, plan.parts, r.picked, r.rows, r.count, n, a->loss, a->lse, st);
   return m.used;
 }
 

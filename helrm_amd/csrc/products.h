@@ -3,6 +3,7 @@
 #pragma once
 #include <initializer_list>
 #include "cleartext.h"
+#include "plan.h"
 
 // act(g): silu g/(1 + e^-g), gelu g Phi(g), cubic ((c3 g + c2) g + c1) g + c0
 enum Act { ACT_SILU = 0, ACT_GELU = 1, ACT_CUBIC = 2 };
@@ -45,18 +46,16 @@ void product_gate(const ProductArgs& p, hipStream_t st);
 // v = A B, A's rows along k, B's along n: dg = v u act'(g), du = v act(g), h = act(g) u
 void product_gate_grad(const ProductArgs& p, hipStream_t st);
 // Bytes that a product (softmax but) of these shapes needs at `partial`, or products in one launch together.
-struct Shape { long M, N; };
+using clr::Shape;
 size_t product_scratch(std::initializer_list<Shape> shapes, long K, int pairs, bool gate = false);
 void product_nt(const ProductArgs& p, hipStream_t st);  // A B^T
 void product_nn(const ProductArgs& p, hipStream_t st);  // A B
 void product_tn(const ProductArgs& p, hipStream_t st);  // A^T B
 void product_tn(ProductArgs a, ProductArgs b, ProductArgs c, hipStream_t st);  // three of the same K in one launch, a.partial of all
-// the products of rows of A with rows of the table go into part and picked
-void product_softmax(const ProductArgs& p, hipStream_t st);
+// the products of rows of A with the N rows of the table go into part, plan.parts pieces a row, and picked
+void product_softmax(const ProductArgs& p, const clr::SoftmaxPlan& plan, hipStream_t st);
 // (exp(A B^T - lse) - onehot(target)) grad into c, in the layout of a factor
 void product_softmax_grad(const ProductArgs& p, hipStream_t st);
-// pieces of a row that product_softmax leaves
-int softmax_parts(long M, long N, long K, int pairs);
 
 // Matrices into the layout above, up to 8 in one launch: row rows[i] (or i) of
 // `from` to row i of `to`, for i < *count (or n); a float32 one as three parts

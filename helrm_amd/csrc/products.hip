@@ -38,7 +38,7 @@
 
 namespace {
 
-constexpr int STEP = 64;                 // k of a step
+using clr::STEP;
 constexpr int XCDS = 8;
 // Products of one launch, in the order of their workgroups.
 struct Batch {
@@ -592,39 +592,12 @@ __global__ __launch_bounds__(256) void join_kernel(const Batch batch) {
   emit4<T, EPI, false>(p, at, 0, (int)min(p.N - n, 4L), RowValues{}, v, u, held);
 }
 
-// The tile and the splits of products in one launch: the least time of their
-// rounds over the 256 CUs, which hold one 256 x 256 tile or two 128 x 128 ones
-// (whose steps and ends overlap).  Microseconds, measured: a step 1.6 and 1.0,
-// the end of a tile 8.5 and 6, a small tile alone on its CU 0.55 of that.  The
-// large tile has half the traffic for each product, the small one fills the
-// GPU with a quarter of the rows.  8192 x 4096 over 4096, gate gradient: 323 us
-// large, 349 small; 2048 x 8192 over 512, gate: 67 us large, 54 small.
-struct Plan { bool big; int splits; };
-Plan plan_of(std::initializer_list<Shape> shapes, long steps, bool gate, bool may_split) {
-  Plan best{};
-  double least = 1e30;
-  for (int big = 0; big < 2; big++) {
-    const long size = big ? 256 : 128;
-    long tiles = 0;
-    double results = 0;
-    for (const Shape& s : shapes) {
-      tiles += clr::ceil_div(s.M, size) * clr::ceil_div(s.N, gate ? size / 2 : size);
-      results += (double)s.M * s.N * (gate ? 2 : 1);
-    }
-    for (int s = 1; s <= (may_split ? 16 : 1); s++) {
-      if (s > 1 && steps / s < 4) break;
-      const double sums = s > 1 ? 4.0 + (s + 1) * results * 4 / 3e6 : 0.0;   // of a kernel more, and its traffic
-      const long rounds = clr::ceil_div(tiles * s, 256), each = clr::ceil_div(steps, s);
-      const double t = (big ? rounds * (each * 1.6 + 8.5) : (rounds + 1) / 2 * (each * 1.0 + 6) * (rounds == 1 ? 0.55 : 1.0)) + sums;
-      if (t < least) { least = t; best = {big != 0, s}; }
-    }
-  }
-  return best;
-}
-long steps_of(long K, int pairs) { return clr::ceil_div(K, STEP) * pairs; }
+using clr::Plan;
+using clr::plan_of;
+using clr::steps_of;
 
 template <class T, bool A_K, bool B_K, int EPI> void launch_type(Batch b, const Plan& plan, hipStream_t st) {
-  const long size = plan.big ? 256 : 128;
+  const long size = plan.tile();
   long tiles = 0, sums = 0;
   Batch j = b;
   for (int i = 0; i < b.count; i++) {
@@ -813,9 +786,6 @@ size_t product_scratch(std::initializer_list<Shape> shapes, long K, int pairs, b
     for (const Shape& s : shapes) n += (size_t)plan.splits * s.M * ((s.N + 7) & ~7L) * (gate ? 2 : 1);
   return n * sizeof(float);
 }
-int softmax_parts(long M, long N, long K, int pairs) {
-  return (int)clr::ceil_div(N, plan_of({{M, N}}, steps_of(K, pairs), false, false).big ? 256 : 128);
-}
 void product_gate(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_GATE>(p, st); }
 void product_gate_grad(const ProductArgs& p, hipStream_t st) { launch<true, false, EPI_GATE_GRAD>(p, st); }
 void product_nt(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_STORE>(p, st); }
@@ -828,7 +798,17 @@ void product_tn(ProductArgs a, ProductArgs b, ProductArgs c, hipStream_t st) {
   c.partial = b.partial + (plan.splits > 1 ? sums(b) : 0);
   launch<false, false, EPI_STORE>({a, b, c}, plan, st);
 }
-void product_softmax(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_SOFTMAX>(p, st); }
+void product_softmax(const ProductArgs& p, const clr::SoftmaxPlan& plan, hipStream_t st) {
+  for (long v0 = 0; v0 < p.N; v0 += plan.columns) {
+    ProductArgs q = p;
+    q.n0 = (int)v0;
+    q.N = (int)std::min(plan.columns, p.N - v0);
+    for (int k = 0; k < q.pairs; k++) q.b[k] += v0 * q.ldb;
+    q.parts = plan.parts;
+    q.part += v0 / plan.plan.tile();
+    launch<true, true, EPI_SOFTMAX>({q}, plan.plan, st);
+  }
+}
 void product_softmax_grad(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_SOFTMAX_GRAD>(p, st); }
 
 void lay_out(const LayOut* jobs, int n, int dtype, hipStream_t st) {

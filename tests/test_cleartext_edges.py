@@ -2,6 +2,8 @@
 points refuse on the host before anything is launched, and the sizes that
 their plans come to."""
 import ctypes
+import os
+import subprocess
 
 import pytest
 
@@ -33,3 +35,47 @@ def test_a_norms_parameters_are_of_its_type_or_float32(lib, type, params):
     assert lib.LayerNormGradWorkspace(ctypes.byref(a)) > 0
     a.paramType = 0
     assert lib.LayerNormGradWorkspace(ctypes.byref(a)) > 0
+
+
+# ---- the launches of the loss --------------------------------------------------------
+
+# rows, table rows, width, products a product is made of: small tiles in several launches (few rows; 257 to 384 of float32), a
+# short last piece, several launches of large ones, one launch
+LOSSES = [(17, (1 << 30) + 300, 8, 1), (65, (1 << 30) + 1, 8, 1), (128, (1 << 31) - 1, 1000, 1), (129, (1 << 31) - 1, 8, 1), (300, (1 << 29) + 300, 8, 6),
+          (257, (1 << 30) - 1, 40, 6), (384, (1 << 29) + 1, 8, 6), ((1 << 26) - 256, 57700, 8, 6), (16384, (1 << 24) + 300, 8, 1),
+          ((1 << 30) - 1, 1, 1, 1), ((1 << 30) - 1, 700, 1, 6), ((1 << 29) + 1, 257, 300, 1), (65, 300, 8, 6), (8192, 131072, 2048, 1)]
+
+
+def test_the_pieces_of_all_launches_are_every_piece_once(tmp_path):
+    source = tmp_path / "pieces.cpp"
+    source.write_text("""
+#include <cstdio>
+#include "plan.h"
+int main() {
+  long m, n, k;
+  int pairs;
+  while (scanf("%ld %ld %ld %d", &m, &n, &k, &pairs) == 4) {
+    const clr::SoftmaxPlan s = clr::softmax_plan(m, n, k, pairs);
+    printf("%d %ld %d %d\\n", s.parts, s.columns, s.plan.tile(), s.plan.threads());
+  }
+}
+""")
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "helrm_amd", "csrc")
+    program = tmp_path / "pieces"
+    subprocess.run(["g++", "-std=c++17", "-I", csrc, str(source), "-o", str(program)], check=True)
+    said = subprocess.run([str(program)], input="\n".join(" ".join(map(str, s)) for s in LOSSES), capture_output=True, text=True, check=True).stdout
+    tiles = set()
+    for (rows, vocab, _, _), line in zip(LOSSES, said.splitlines(), strict=True):
+        parts, columns, tile, threads = map(int, line.split())
+        assert threads == {128: 256, 256: 512}[tile]
+        several = columns < vocab
+        tiles.add((tile, several))
+        assert columns % tile == 0 and 0 < columns < 1 << 31
+        at = 0
+        for first in range(0, vocab, columns):              # a launch's pieces are its columns' tiles, and lie where they belong
+            assert first // tile == at
+            here = -(-min(columns, vocab - first) // tile)
+            assert -(-rows // tile) * here * threads < 1 << 32
+            at += here
+        assert at == parts
+    assert tiles == {(128, False), (128, True), (256, False), (256, True)}
