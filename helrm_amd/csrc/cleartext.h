@@ -28,6 +28,16 @@ template <class F> int guarded(F&& f) {
   catch (const std::exception& e) { return report_error(e.what()); }
   catch (...) { return report_error("unknown error"); }
 }
+// Workgroups of a launch: one of 2^32 threads or more runs what is left of them beyond, and reports no error.
+inline unsigned groups_of(long groups, int threads) {
+  require(groups * threads < 1L << 32, "more threads than a launch has");
+  return (unsigned)groups;
+}
+// f(first, n) for up to 2^31 threads' workgroups at a time
+template <class F> void in_launches(long groups, int threads, F&& f) {
+  const long most = (1L << 31) / threads;
+  for (long first = 0; first < groups; first += most) f(first, (unsigned)(groups - first < most ? groups - first : most));
+}
 inline size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // f(T{}) with T the C++ type of a DType

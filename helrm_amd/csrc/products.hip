@@ -608,10 +608,10 @@ template <class T, bool A_K, bool B_K, int EPI> void launch_type(Batch b, const 
     tiles += clr::ceil_div(p.M, size) * clr::ceil_div(p.N, EPI == EPI_GATE ? size / 2 : size) * p.splits;
     sums += clr::ceil_div((long)p.M * (sum_cols<EPI>(p) / 4), 256);
   }
-  if (plan.big) product_kernel<T, 256, 256, 2, 4, A_K, B_K, EPI><<<(unsigned)tiles, 512, 0, st>>>(b);
-  else product_kernel<T, 128, 128, 2, 2, A_K, B_K, EPI><<<(unsigned)tiles, 256, 0, st>>>(b);
+  if (plan.big) product_kernel<T, 256, 256, 2, 4, A_K, B_K, EPI><<<clr::groups_of(tiles, 512), 512, 0, st>>>(b);
+  else product_kernel<T, 128, 128, 2, 2, A_K, B_K, EPI><<<clr::groups_of(tiles, 256), 256, 0, st>>>(b);
   if constexpr (EPI == EPI_STORE || EPI == EPI_GATE || EPI == EPI_GATE_GRAD)
-    if (plan.splits > 1) join_kernel<T, EPI><<<(unsigned)sums, 256, 0, st>>>(j);
+    if (plan.splits > 1) join_kernel<T, EPI><<<clr::groups_of(sums, 256), 256, 0, st>>>(j);
 }
 template <bool A_K, bool B_K, int EPI> void launch(std::initializer_list<ProductArgs> products, const Plan& plan, hipStream_t st) {
   Batch b{};
@@ -623,12 +623,6 @@ template <bool A_K, bool B_K, int EPI> void launch(std::initializer_list<Product
 template <bool A_K, bool B_K, int EPI> void launch(const ProductArgs& p, hipStream_t st) {
   constexpr bool may_split = EPI == EPI_STORE || EPI == EPI_GATE || EPI == EPI_GATE_GRAD;
   launch<A_K, B_K, EPI>({p}, plan_of({{p.M, p.N}}, steps_of(p.K, p.pairs), EPI == EPI_GATE, may_split), st);
-}
-
-// A workgroup of 256 for each of n rows: a launch has less than 2^32 threads.
-template <class F> void in_launches(long n, F&& f) {
-  constexpr long MOST = 1L << 23;
-  for (long base = 0; base < n; base += MOST) f(base, (unsigned)std::min(MOST, n - base));
 }
 
 // Up to 8 matrices into the layout that the tiles are loaded from, one launch:
@@ -730,8 +724,8 @@ __global__ __launch_bounds__(ROWS_BLOCK) void kept_rows_kernel(RowsArgs a) {
 }
 
 // A wave a row joins its tiles' pieces: 8,192 rows of 512 pieces, 34 MB, 11 us (twice its memory time; one launch of the loss).
-__global__ void finish_kernel(const float2* part, int parts, const float* picked, const int* rows, const int* count, float* loss, float* lse) {
-  const long i = blockIdx.x * 4L + (threadIdx.x >> 6);
+__global__ void finish_kernel(const float2* part, int parts, const float* picked, const int* rows, const int* count, float* loss, float* lse, long first) {
+  const long i = (first + blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (i >= *count) return;
   const int lane = threadIdx.x & 63;
   float2 run = make_float2(-INFINITY, 0.0f);
@@ -821,18 +815,20 @@ void lay_out(const LayOut* jobs, int n, int dtype, hipStream_t st) {
       blocks += jobs[i].n;
     }
   clr::with_type(dtype, [&](auto t) {
-    in_launches(blocks, [&](long base, unsigned n) { lay_out_kernel<decltype(t)><<<n, 256, 0, st>>>(all, base); });
+    clr::in_launches(blocks, 256, [&](long base, unsigned n) { lay_out_kernel<decltype(t)><<<n, 256, 0, st>>>(all, base); });
   });
 }
 void kept_rows(const RowsArgs& a, hipStream_t st) { kept_rows_kernel<<<1, ROWS_BLOCK, 0, st>>>(a); }
 void softmax_finish(const float2* part, int parts, const float* picked, const int* rows, const int* count, long n, float* loss, float* lse, hipStream_t st) {
-  if (n) finish_kernel<<<(unsigned)clr::ceil_div(n, 4), 256, 0, st>>>(part, parts, picked, rows, count, loss, lse);
+  clr::in_launches(clr::ceil_div(n, 4), 256, [&](long first, unsigned k) {
+    finish_kernel<<<k, 256, 0, st>>>(part, parts, picked, rows, count, loss, lse, first);
+  });
 }
 void scatter_rows(const float* acc, long ldacc, long second, const int* place, const float* scale, void* out, long ldout, long n, int width, int dtype,
                   hipStream_t st) {
   clr::with_type(dtype, [&](auto t) {
     using T = decltype(t);
-    in_launches(n, [&](long base, unsigned k) { scatter_kernel<T><<<k, 256, 0, st>>>(acc, ldacc, second, place, scale, (T*)out, ldout, width, base); });
+    clr::in_launches(n, 256, [&](long base, unsigned k) { scatter_kernel<T><<<k, 256, 0, st>>>(acc, ldacc, second, place, scale, (T*)out, ldout, width, base); });
   });
 }
 void fill_zero(void* p, size_t bytes, hipStream_t st) {

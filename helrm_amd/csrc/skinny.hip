@@ -265,7 +265,7 @@ template <int EPI> void launch(SkinnyArgs p, hipStream_t st) {
     auto go = [&](auto nb) {
       constexpr int NB = decltype(nb)::value;
       const int waves = p.alone ? 4 : waves_of(p.N, p.K, p.dtype, aligned ? most_waves<T, true, NB>() : most_waves<T, false, NB>());
-      const unsigned grid = (unsigned)(p.alone ? clr::ceil_div(teams, 4) : teams);
+      const unsigned grid = clr::groups_of(p.alone ? clr::ceil_div(teams, 4) : teams, waves * 64);
       const size_t lds = (size_t)waves * (EPI == SKINNY_GATE ? 2 : 1) * NB * 1024;
       if (aligned) skinny_kernel<T, X, true, NB, EPI><<<grid, waves * 64, lds, st>>>(p);
       else skinny_kernel<T, X, false, NB, EPI><<<grid, waves * 64, lds, st>>>(p);

@@ -24,3 +24,22 @@ def test_cross_entropy_of_small_tiles_in_several_launches(ct):  # noqa: F811
     s = torch.logsumexp(torch.cat([z, torch.full((rows, 1), float(vocab - len(some)), dtype=torch.float64).log()], 1), 1)
     ref.check(lse, s, torch.ones(rows), 1e-4, "lse")
     ref.check(losses, s - z[torch.arange(rows), at], torch.ones(rows), 1e-4, "losses")
+
+
+def test_cross_entropy_of_more_vectors_than_one_launch_has_waves(ct):  # noqa: F811
+    # a wave a row would be 2^32 threads and some
+    rows = (1 << 26) + 37
+    gen = seeded(6)
+    x = torch.zeros(rows, 1, dtype=torch.bfloat16, device=DEV)
+    table = normal(gen, 2, 1, dtype=torch.bfloat16)
+    some = torch.cat([torch.arange(70), torch.arange((1 << 25) - 10, (1 << 25) + 10), torch.arange(rows - 70, rows)])
+    x[some.to(DEV)] = normal(gen, len(some), 1, dtype=torch.bfloat16)
+    target = torch.ones(rows, dtype=torch.int64, device=DEV)
+    losses, lse = ct.cross_entropy_forward(x, table, target)
+    z = ref.d(x[some.to(DEV)]) @ ref.d(table).T
+    s = torch.logsumexp(z, 1)
+    ref.check(lse[some.to(DEV)], s, torch.ones(len(some)), 1e-5, "lse")
+    ref.check(losses[some.to(DEV)], s - z[:, 1], torch.ones(len(some)), 1e-5, "losses")
+    empty = torch.ones(rows, dtype=torch.bool, device=DEV)
+    empty[some.to(DEV)] = False
+    assert ((losses[empty] - 0.6931472).abs() < 1e-6).all() and ((lse[empty] - 0.6931472).abs() < 1e-6).all()
