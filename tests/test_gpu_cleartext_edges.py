@@ -9,6 +9,26 @@ from test_gpu_cleartext import DEV, F32, ce_tensors, ct, mlp_tensors, normal, se
 pytestmark = pytest.mark.gpu
 
 
+@pytest.mark.parametrize("rows", [1, 2])
+def test_layer_norm_of_more_columns_than_one_launch_sums(ct, rows):  # noqa: F811
+    # the sums of the weights' gradients, 1,024 threads for 16 columns, would be 2^32 threads and some
+    width = (1 << 26) + 9
+    gen = torch.Generator(DEV).manual_seed(rows)
+    x, dy = (torch.randn(rows, width, generator=gen, device=DEV).bfloat16() for _ in range(2))
+    w = (1 + 0.1 * torch.randn(width, generator=gen, device=DEV)).bfloat16()
+    y, mean, rstd = ct.layer_norm_forward(x, w, w)
+    dx, dw, db = ct.layer_norm_backward(dy, x, w, mean, rstd)
+    x, w, dy = x.double(), w.double(), dy.double()
+    var, mu = torch.var_mean(x, dim=1, correction=0, keepdim=True)
+    r = (var + 1e-5).rsqrt()
+    h, t = (x - mu) * r, dy * w
+    slop, u = (width / 256 + 30) * F32, ref.U[torch.bfloat16]      # 256 threads' sums
+    want = r * (t - t.mean(1, keepdim=True) - h * (t * h).mean(1, keepdim=True))
+    for name, got, value, size in (("y", y, h * w + w, (1 + h.abs()) * w.abs()), ("dx", dx, want, t.abs() + 1 + h.abs()),
+                                   ("dw", dw, (dy * h).sum(0), (dy.abs() * (1 + h.abs())).sum(0)), ("db", db, dy.sum(0), dy.abs().sum(0) * F32)):
+        assert ((got.double() - value).abs() <= size * slop + u * value.abs()).all(), name
+
+
 def test_cross_entropy_of_small_tiles_in_several_launches(ct):  # noqa: F811
     # 17 rows take tiles of 128 x 128, 2^23 and 3 of them, in three launches; equal logits but for a few rows
     rows, vocab, width = 17, (1 << 30) + 300, 8
