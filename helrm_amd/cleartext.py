@@ -88,6 +88,12 @@ def _need(ok, what):
         raise ValueError(what)
 
 
+def _sized(n, name):
+    # (a C int takes a larger size modulo 2^32, without an error)
+    if n >= 1 << 31:
+        raise ValueError(f"{name}: {n}, the most is 2^31 - 1")
+
+
 def _rows(t, width, name, like=None):
     """[rows, width] of a tensor whose last dimension is the vector, in a layout that the kernels take."""
     shape = t.shape
@@ -127,6 +133,7 @@ def _vector(t, n, name, dtype, device):
 def _norm_tensors(x, weight, bias):
     _need(x.dim() >= 1 and x.shape[-1] >= 1, "x: no last dimension")
     width = x.shape[-1]
+    _sized(width, "x: the last dimension")
     x2 = _rows(x, width, "x")
     if weight.dtype != x.dtype and weight.dtype != torch.float32:
         raise ValueError(f"weight: {weight.dtype}, neither {x.dtype} nor float32")
@@ -211,6 +218,8 @@ def _mlp_tensors(x, gate, up, down):
     _need(gate.dim() == 2 and up.dim() == 2 and down.dim() == 2, "gate, up and down are matrices")
     hidden, width = gate.shape
     _need(hidden >= 1 and width >= 1, "gate: no elements")
+    _sized(hidden, "gate: rows")
+    _sized(width, "gate: the last dimension")
     x2 = _rows(x, width, "x")
     gate, up, down = _rows(gate, width, "gate", x), _rows(up, width, "up", x), _rows(down, hidden, "down", x)
     if up.shape[0] != hidden:
@@ -302,8 +311,11 @@ def gated_mlp(x, gate, up, down, activation="silu"):
 # ---- softmax cross entropy against a table ------------------------------------------------
 
 
-def _loss_tensors(x, table, target):
+def _loss_tensors(x, table, target, ignore_index):
     _need(table.dim() == 2 and table.shape[0] >= 1 and table.shape[1] >= 1, "table: not a matrix with elements")
+    _sized(table.shape[0], "table: rows")
+    _sized(table.shape[1], "table: the last dimension")
+    _need(-(1 << 63) <= ignore_index < 1 << 63, "ignore_index: not an int64")
     x2 = _rows(x, table.shape[1], "x")
     target = _vector(target.reshape(-1) if target.dim() != 1 else target, x2.shape[0], "target", torch.int64, x.device)
     return x2, _rows(table, table.shape[1], "table", x), target
@@ -313,7 +325,7 @@ def cross_entropy_forward(x, table, target, ignore_index=-100):
     """(losses, lse), float32 for each row: the softmax cross entropy of x's products with the table's rows, and the
     logarithm of the softmax's sum.  Rows whose target is `ignore_index` have 0 for both; a target outside the table
     gives NaN.  The logits are never in memory."""
-    x2, table, target = _loss_tensors(x, table, target)
+    x2, table, target = _loss_tensors(x, table, target, ignore_index)
     losses = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     lse = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     _call("CrossEntropy", CrossEntropyArgs(
@@ -326,7 +338,7 @@ def cross_entropy_forward(x, table, target, ignore_index=-100):
 def cross_entropy_backward(grad, x, table, target, lse, ignore_index=-100):
     """(dx, dtable) for the gradient `grad` of the losses (float32); lse as the forward call gave it.  The logits are
     computed again, a piece of the table at a time."""
-    x2, table, target = _loss_tensors(x, table, target)
+    x2, table, target = _loss_tensors(x, table, target, ignore_index)
     rows, width = x2.shape
     grad = _vector(grad.reshape(-1), rows, "grad", torch.float32, x.device)
     lse = _vector(lse.reshape(-1), rows, "lse", torch.float32, x.device)

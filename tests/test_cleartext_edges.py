@@ -37,6 +37,29 @@ def test_a_norms_parameters_are_of_its_type_or_float32(lib, type, params):
     assert lib.LayerNormGradWorkspace(ctypes.byref(a)) > 0
 
 
+# ---- sizes ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n", [1 << 31, (1 << 32) + 5])
+def test_sizes_beyond_a_c_int_are_refused(n):
+    # (tensors of one element, expanded; with sizes modulo 2^32 a table of 2^32 + 5 rows would be one of 5)
+    torch = pytest.importorskip("torch")
+    from helrm_amd import cleartext as ct
+    one = torch.zeros(1, 1)
+    wide, tall, row, target = one.expand(1, n), one.expand(n, 1), one[0].expand(n), torch.zeros(1, dtype=torch.int64)
+    for call in (lambda: ct.layer_norm(wide, row), lambda: ct.layer_norm_forward(wide, row), lambda: ct.layer_norm_backward(wide, wide, row, row, row),
+                 lambda: ct.gated_mlp(wide, wide, wide, tall), lambda: ct.gated_mlp(one, tall, tall, wide),
+                 lambda: ct.gated_mlp_backward(one, one, tall, tall, wide, one), lambda: ct.cross_entropy(one, tall, target),
+                 lambda: ct.cross_entropy(wide, wide, target), lambda: ct.cross_entropy_backward(row[:1], one, tall, target, row[:1])):
+        with pytest.raises(ValueError, match=f"{n}, the most is"):
+            call()
+    with pytest.raises(ValueError, match="not on the GPU"):
+        ct.layer_norm(one.expand(1, (1 << 31) - 1), one[0].expand((1 << 31) - 1))
+    for index in (1 << 63, -(1 << 63) - 1):
+        with pytest.raises(ValueError, match="ignore_index"):
+            ct.cross_entropy(one, one, target, ignore_index=index)
+
+
 # ---- the launches of the loss --------------------------------------------------------
 
 # rows, table rows, width, products a product is made of: small tiles in several launches (few rows; 257 to 384 of float32), a
