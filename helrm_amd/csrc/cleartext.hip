@@ -50,7 +50,8 @@ void check_norm(const LayerNormArgs* a) {
   // the kernels read and write parameters as one of these two: another type has elements of another size
   require(a->paramType == a->type || a->paramType == DT_F32, "LayerNorm: paramType is neither type nor float32");
   require(a->rows >= 0 && a->rows < INT_MAX, "LayerNorm: bad number of rows");
-  require(a->width >= 1, "LayerNorm: bad width");
+  // (a long row's indices are ints that a workgroup's stride is added to)
+  require(a->width >= 1 && a->width <= INT_MAX - 1024, "LayerNorm: bad width");
 }
 NormArgs norm_args(const LayerNormArgs* a) {
   NormArgs n{};

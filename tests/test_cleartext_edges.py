@@ -60,6 +60,20 @@ def test_sizes_beyond_a_c_int_are_refused(n):
             ct.cross_entropy(one, one, target, ignore_index=index)
 
 
+def test_norms_so_wide_that_an_index_would_overflow_are_refused(lib):
+    # a long row's kernels step past its end by up to 1,024 before they compare
+    top = (1 << 31) - 1
+    for width in (top, top - 255, top - 1023):
+        a = LayerNormArgs(x=SOME, ldx=top, y=SOME, ldy=top, weight=SOME, mean=SOME, rstd=SOME, dy=SOME, lddy=top, dx=SOME, lddx=top, dweight=SOME,
+                          rows=1, width=width, type=1, paramType=1)
+        assert lib.LayerNormGradWorkspace(ctypes.byref(a)) == -1
+        for call in (lib.LayerNorm, lib.LayerNormGrad):
+            assert call(ctypes.byref(a), None) == -1
+            assert "width" in lib.GetLastError().decode()
+    a.width = top - 1024
+    assert lib.LayerNormGradWorkspace(ctypes.byref(a)) == 2 * 4 * a.width
+
+
 # ---- the launches of the loss --------------------------------------------------------
 
 # rows, table rows, width, products a product is made of: small tiles in several launches (few rows; 257 to 384 of float32), a
