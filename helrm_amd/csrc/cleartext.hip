@@ -125,16 +125,20 @@ struct Copies {
   }
 };
 // The pairs of parts whose products make one product, smallest first: of three
-// parts of 8 bits each those above 2^-24, of two parts of one factor both.
+// parts of 8 bits each those above 2^-24, of two parts of one factor both.  All
+// but the last, the first parts', are corrections, and come before the last
+// pairs of other products of the same sum.
 int add_pairs(ProductArgs& p, const Held& a, const Held& b, const Held* b2 = nullptr) {
   static const int part_a[6] = {0, 1, 2, 0, 1, 0}, part_b[6] = {2, 1, 0, 1, 0, 0};
   const bool f32 = p.dtype == DT_F32;
   const int n = f32 ? 6 : std::max(a.parts, b.parts);
   for (int k = 0; k < n; k++) {
     const int ia = f32 ? part_a[k] : std::min(n - 1 - k, a.parts - 1), ib = f32 ? part_b[k] : std::min(n - 1 - k, b.parts - 1);
-    p.a[p.pairs] = a.at(ia);
-    p.b[p.pairs] = b.at(ib);
-    if (b2) p.b2[p.pairs] = b2->at(ib);
+    const int at = k < n - 1 ? p.corrections++ : p.pairs;
+    for (int i = p.pairs; i > at; i--) { p.a[i] = p.a[i - 1]; p.b[i] = p.b[i - 1]; }
+    p.a[at] = a.at(ia);
+    p.b[at] = b.at(ib);
+    if (b2) p.b2[at] = b2->at(ib);   // (one product: none is moved)
     p.pairs++;
   }
   p.lda = a.ld; p.ldb = b.ld;

@@ -9,14 +9,15 @@
 enum Act { ACT_SILU = 0, ACT_GELU = 1, ACT_CUBIC = 2 };
 
 // C[m][n] = sum over k of A(m, k) B(n, k), for up to 12 pairs of factors that
-// are added.  Factors are 16-bit, 16-byte aligned, their rows `ld` elements
+// are added, of which the first `corrections` are settled (tiles.h) before the
+// others.  Factors are 16-bit, 16-byte aligned, their rows `ld` elements
 // (a multiple of 8) apart and filled up with zeros to a multiple of 8
 // elements.  Whether a factor's rows run along k or along m (n) goes by the
 // product.
 struct ProductArgs {
   const uint16_t* a[12]; const uint16_t* b[12];
   const uint16_t* b2[6];     // gate: the up projection's
-  int pairs;
+  int pairs, corrections;
   long lda, ldb;
   int M, N, K;
   int dtype;                 // of the operator; the factors of a float32 one are its bfloat16 parts

@@ -4,7 +4,11 @@
 // of 16-bit elements are exact and every sum is float32.  A float32 factor
 // is three bfloat16 parts of 8 bits each, x = x0 + x1 + x2, and a product the
 // six of their nine products above 2^-24 of it, smallest first; that is as
-// exact as a float32 multiplication, on a unit 16 times as fast.
+// exact as a float32 multiplication, on a unit 16 times as fast.  Infinite
+// factors and overflows come out as float32's do: the sums of the five smaller
+// products are left out where they are not finite, before x0 y0 is added
+// (a product within 2^-7 of the largest float32 may already be infinite).
+// That takes 1 to 3 % of a float32 product, in kernels of its own.
 //
 // A workgroup has a BM x BN tile of C, k advances by 64.  Both factors' tiles
 // go from memory to LDS directly (16 bytes a lane, no registers), into one of
@@ -62,19 +66,21 @@ template <class T> __device__ __forceinline__ uint2 pack4(const float v[4]) {
 // (8-byte aligned; a float32 operator's: three parts, `part` elements apart; of
 // 16 bits: two parts, or one and no `part`).
 template <class T> __device__ __forceinline__ void put_held(u16* o, int type, long part, const float v[4]) {
-  *(uint2*)o = pack4<T>(v);
   if (type == DT_F32) {
-    float r[2][4];
+    float r[3][4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       __bf16 s[3];
       split3(v[e], s);
-      r[0][e] = (float)s[1];
-      r[1][e] = (float)s[2];
+#pragma unroll
+      for (int k = 0; k < 3; k++) r[k][e] = (float)s[k];
     }
 #pragma unroll
-    for (int k = 0; k < 2; k++) *(uint2*)(o + (k + 1) * part) = pack4<__bf16>(r[k]);
-  } else if (part) {
+    for (int k = 0; k < 3; k++) *(uint2*)(o + k * part) = pack4<__bf16>(r[k]);
+    return;
+  }
+  *(uint2*)o = pack4<T>(v);
+  if (part) {
     float r[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -405,7 +411,8 @@ template <int READS, int MULS> __device__ __forceinline__ void spread() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-template <class T, int BM, int BN, int WM, int WN, bool A_K, bool B_K, int EPI>
+// PARTS: the first pairs of factors are corrections.
+template <class T, int BM, int BN, int WM, int WN, bool A_K, bool B_K, int EPI, bool PARTS>
 __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Batch batch) {
   const int which = batch.which(blockIdx.x);
   const ProductArgs& p = batch.p[which];
@@ -531,6 +538,14 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Batch batch)
     multiply(3, 1);
     spread<READ_B, MULS>();
   };
+  // steps of corrections, from the first one here
+  const int corrections = steps_of * p.corrections - from;
+  auto settle = [&] {
+#pragma unroll
+    for (int i = 0; i < FM; i++)
+#pragma unroll
+      for (int j = 0; j < FN; j++) acc[i][j] = settled(acc[i][j]);
+  };
   const int total = (to - from + 1) / 2;
   if (total) {
 #pragma unroll
@@ -545,9 +560,12 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Batch batch)
     read_b(b0, 0);
   }
   for (int t = 0; t < total; t++) {
+    if (PARTS && t > 0 && corrections == 2 * t) settle();
     step(a0, b0, a1, b1);
+    if (PARTS && corrections == 2 * t + 1) settle();
     step(a1, b1, a0, b0);
   }
+  if (PARTS && corrections >= to - from) settle();
   arrive<0>();   // no load may still write LDS when it is used again, or given away
   if constexpr (EPI == EPI_SOFTMAX) {
     softmax_piece<FM, FN, WM, WN>(p, acc, M, m0, n0, wave_m, wave_n, tile_n, (float2*)a0);
@@ -608,8 +626,20 @@ template <class T, bool A_K, bool B_K, int EPI> void launch_type(Batch b, const 
     tiles += clr::ceil_div(p.M, size) * clr::ceil_div(p.N, EPI == EPI_GATE ? size / 2 : size) * p.splits;
     sums += clr::ceil_div((long)p.M * (sum_cols<EPI>(p) / 4), 256);
   }
-  if (plan.big) product_kernel<T, 256, 256, 2, 4, A_K, B_K, EPI><<<clr::groups_of(tiles, 512), 512, 0, st>>>(b);
-  else product_kernel<T, 128, 128, 2, 2, A_K, B_K, EPI><<<clr::groups_of(tiles, 256), 256, 0, st>>>(b);
+  auto go = [&](auto parts) {
+    constexpr bool PARTS = decltype(parts)::value;
+    if (plan.big) product_kernel<T, 256, 256, 2, 4, A_K, B_K, EPI, PARTS><<<clr::groups_of(tiles, 512), 512, 0, st>>>(b);
+    else product_kernel<T, 128, 128, 2, 2, A_K, B_K, EPI, PARTS><<<clr::groups_of(tiles, 256), 256, 0, st>>>(b);
+  };
+  // (float16 factors have two parts only where the product is stored)
+  bool parts = false;
+  for (int i = 0; i < b.count; i++) parts |= b.p[i].corrections > 0;
+  if constexpr (EPI == EPI_STORE || std::is_same_v<T, __bf16>) {
+    if (parts) go(std::true_type{});
+    else go(std::false_type{});
+  } else {
+    go(std::false_type{});
+  }
   if constexpr (EPI == EPI_STORE || EPI == EPI_GATE || EPI == EPI_GATE_GRAD)
     if (plan.splits > 1) join_kernel<T, EPI><<<clr::groups_of(sums, 256), 256, 0, st>>>(j);
 }
@@ -755,7 +785,7 @@ __global__ __launch_bounds__(256) void scatter_kernel(const float* acc, long lda
         float l[4];
         get4(v + second + k, l);
 #pragma unroll
-        for (int e = 0; e < 4; e++) t[e] += l[e];
+        for (int e = 0; e < 4; e++) t[e] += settled(l[e]);
       }
       T q[4];
 #pragma unroll
@@ -763,7 +793,7 @@ __global__ __launch_bounds__(256) void scatter_kernel(const float* acc, long lda
       __builtin_memcpy(__builtin_assume_aligned(o + k, 4 * sizeof(T)), q, sizeof(q));
     }
   } else {
-    for (int k = threadIdx.x; k < width; k += 256) o[k] = i < 0 ? (T)0.0f : (T)((v[k] + (second ? v[second + k] : 0.0f)) * s);
+    for (int k = threadIdx.x; k < width; k += 256) o[k] = i < 0 ? (T)0.0f : (T)((v[k] + (second ? settled(v[second + k]) : 0.0f)) * s);
   }
 }
 

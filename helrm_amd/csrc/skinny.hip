@@ -65,17 +65,16 @@ template <class T> __device__ __forceinline__ Eight<T> eight(const Raw<T>& r) {
   }
   return o;
 }
-template <class T> __device__ __forceinline__ f32x4 dot8(const Eight<T>& w, const Eight<T>& x, f32x4 c) {
+// The first parts' products are added to c, the corrections to r (settled at the end).
+template <class T> __device__ __forceinline__ void dot8(const Eight<T>& w, const Eight<T>& x, f32x4& c, f32x4& r) {
   if constexpr (sizeof(T) == 4) {
-    c = mfma(w.v[0], x.v[2], c);
-    c = mfma(w.v[1], x.v[1], c);
-    c = mfma(w.v[2], x.v[0], c);
-    c = mfma(w.v[0], x.v[1], c);
-    c = mfma(w.v[1], x.v[0], c);
-    return mfma(w.v[0], x.v[0], c);
-  } else {
-    return mfma(w.v[0], x.v[0], c);
+    r = mfma(w.v[0], x.v[2], r);
+    r = mfma(w.v[1], x.v[1], r);
+    r = mfma(w.v[2], x.v[0], r);
+    r = mfma(w.v[0], x.v[1], r);
+    r = mfma(w.v[1], x.v[0], r);
   }
+  c = mfma(w.v[0], x.v[0], c);
 }
 
 // The hidden values of a 16-bit block stay float32 here: they are few, and in
@@ -93,7 +92,10 @@ template <class T> __device__ __forceinline__ Two<T> two(const Raw<float>& r) {
   }
   return o;
 }
-template <class T> __device__ __forceinline__ f32x4 dot8(const Eight<T>& w, const Two<T>& x, f32x4 c) { return mfma(w.v[0], x.v[0], mfma(w.v[0], x.v[1], c)); }
+template <class T> __device__ __forceinline__ void dot8(const Eight<T>& w, const Two<T>& x, f32x4& c, f32x4& r) {
+  r = mfma(w.v[0], x.v[1], r);
+  c = mfma(w.v[0], x.v[0], c);
+}
 
 // A workgroup takes `groups` times 16 rows of W; or, where there are rows
 // enough to keep every wave loading, each of its waves does (`alone`), which
@@ -118,7 +120,7 @@ __global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_ke
     if (n0 >= p.N) break;
     const bool in = n0 + t < p.N;
     const T* w[2] = {(const T*)p.w + (n0 + t) * p.ldw, MATS == 2 ? (const T*)p.w2 + (n0 + t) * p.ldw2 : nullptr};
-    f32x4 acc[MATS][NB] = {};
+    f32x4 acc[MATS][NB] = {}, rest[MATS][NB] = {};
     for (int k0 = wave * 64; k0 < p.K; k0 += waves * 64 * TURNS) {
       Raw<T> raw[MATS][TURNS][2];
 #pragma unroll
@@ -141,14 +143,20 @@ __global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_ke
             if constexpr (sizeof(X) == sizeof(T)) {
               const Eight<T> x = eight(rx);
 #pragma unroll
-              for (int m = 0; m < MATS; m++) acc[m][b] = dot8(f[m], x, acc[m][b]);
+              for (int m = 0; m < MATS; m++) dot8(f[m], x, acc[m][b], rest[m][b]);
             } else {
               const Two<T> x = two<T>(rx);
 #pragma unroll
-              for (int m = 0; m < MATS; m++) acc[m][b] = dot8(f[m], x, acc[m][b]);
+              for (int m = 0; m < MATS; m++) dot8(f[m], x, acc[m][b], rest[m][b]);
             }
           }
         }
+    }
+    if constexpr (sizeof(X) == 4) {
+#pragma unroll
+      for (int m = 0; m < MATS; m++)
+#pragma unroll
+        for (int b = 0; b < NB; b++) acc[m][b] += settled(rest[m][b]);
     }
     if (waves > 1) {
       if (group) __syncthreads();   // the sums of the group before have been read

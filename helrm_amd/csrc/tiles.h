@@ -51,12 +51,25 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
   return make_float2(m, a.y * __expf(a.x - m) + b.y * __expf(b.x - m));
 }
 
-// The parts of a float32 value; what is not finite is in the first alone.
+// The parts of a float32 value, x = x0 + x1 + x2.  x0 is x (1 - 2^-9) rounded:
+// what 8 bits hold is its own first part, and no finite x has an infinite one
+// (the largest float32 rounds to infinity).  So x1 is up to 1.5 2^-8 of x and
+// x2 up to 2^-16; both are NaN of an infinite x.
 __device__ __forceinline__ void split3(float v, __bf16 out[3]) {
-  out[0] = (__bf16)v;
-  const float r = fabsf((float)out[0]) < INFINITY ? v - (float)out[0] : 0.0f;
+  out[0] = (__bf16)(v * 0x1.ffp-1f);
+  const float r = v - (float)out[0];
   out[1] = (__bf16)r;
   out[2] = (__bf16)(r - (float)out[1]);
+}
+
+// A sum of parts' products as what the first parts' are corrected by.  Those
+// alone know what an infinite factor or an overflow comes to: the other parts
+// are NaN or of either sign there, and the correction is left out.
+__device__ __forceinline__ float settled(float v) { return fabsf(v) < INFINITY ? v : 0.0f; }
+__device__ __forceinline__ f32x4 settled(f32x4 v) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) v[e] = settled(v[e]);
+  return v;
 }
 
 }  // namespace

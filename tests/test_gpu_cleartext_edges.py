@@ -63,3 +63,114 @@ def test_cross_entropy_of_more_vectors_than_one_launch_has_waves(ct):  # noqa: F
     empty = torch.ones(rows, dtype=torch.bool, device=DEV)
     empty[some.to(DEV)] = False
     assert ((losses[empty] - 0.6931472).abs() < 1e-6).all() and ((lse[empty] - 0.6931472).abs() < 1e-6).all()
+
+
+# ---- infinities, the types' lowest values, overflow ------------------------------------
+
+
+def special_check(got, want, size, tol, what):
+    """The infinities and NaN of `want`; what is finite there within tol * size."""
+    got, want = ref.d(got), want.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), f"{what}: NaN in the wrong places"
+    assert torch.equal(torch.where(torch.isinf(got), got, 0), torch.where(torch.isinf(want), want, 0)), f"{what}: infinities"
+    fine = torch.isfinite(want)
+    ref.check(torch.where(fine, got, 0), torch.where(fine, want, 0), torch.where(fine, size, 0), tol, what)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [3, 40, 70, 300])
+@pytest.mark.parametrize("mask", ["-inf", "lowest", "near"])
+def test_cross_entropy_of_table_rows_masked_through_a_constant_coordinate(ct, dtype, rows, mask):  # noqa: F811
+    width, vocab, column = 33, 700, 7
+    x, table, target, grad = ce_tensors(seeded(rows), rows, width, vocab, dtype)
+    low = torch.finfo(dtype).min
+    value = {"-inf": float("-inf"), "lowest": low, "near": low * (1 - 2.0 ** -12) if dtype == torch.float32 else low / 2}[mask]
+    gone = torch.arange(vocab) % 3 == 1
+    x[:, column] = 1.0
+    table[:, column] = 0
+    table[gone.to(DEV), column] = value
+    target = target // 3 * 3
+    losses, lse = ct.cross_entropy_forward(x, table, target)
+    dx, dtable = ct.cross_entropy_backward(grad, x, table, target, lse)
+    # the same without the masked rows
+    left = table.cpu()[~gone]
+    at = (torch.cumsum(~gone, 0) - 1)[target.cpu()]
+    l64, s64 = ref.cross_entropy(x, left, at)
+    logit = (width + 12) * F32 * (ref.d(x).abs() @ ref.d(left).abs().T).amax().item()
+    off = logit * 2 + (12 + vocab / 64) * F32 * (1 + s64.abs())
+    ref.check(losses, l64, off, 1.0, "losses")
+    ref.check(lse, s64, off, 1.0, "lse")
+    dx64, dt64, sx, st, px, pt = ref.cross_entropy_grad(grad, x, left, at)
+    tol, soft = (vocab + rows + 60) * F32 + 2.1 * ref.U[dtype], 4 * logit + 8 * F32
+    least = 2.0 ** -24 if dtype == torch.float16 else 2.0 ** -126
+    assert not dtable.cpu()[gone].any()
+    ref.check(dtable.cpu()[~gone], dt64, st * tol + pt * soft + least, 1.0, "dtable")
+    if mask == "-inf":      # 0 times an infinity
+        assert torch.isnan(dx[:, column]).all()
+        dx[:, column] = 0
+        dx64[:, column] = 0
+    ref.check(dx, dx64, sx * tol + px * soft + least, 1.0, "dx")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 17, 40, 70, 300])
+@pytest.mark.parametrize("where", ["gate", "up", "down", "x", "grad"])
+def test_gated_mlp_with_one_infinite_factor(ct, dtype, rows, where):  # noqa: F811
+    x, gate, up, down, dy = mlp_tensors(seeded(rows), rows, 24, 40, dtype)
+    x[:, 5] = x[:, 5].abs() + 0.5
+    {"gate": gate, "up": up, "down": down, "x": x, "grad": dy}[where][min(rows - 1, 2) if where in ("x", "grad") else 2, 5] = float("inf")
+    y, saved = ct.gated_mlp_forward(x, gate, up, down, "silu")
+    got = (y, *ct.gated_mlp_backward(dy, x, gate, up, down, saved, "silu"))
+    want = (ref.mlp(x, gate, up, down, "silu"), *ref.mlp_grad(dy, x, gate, up, down, "silu"))
+    u = ref.U[dtype]
+    tol = 2 * (2 * 24 + 40 + rows + 40) * F32 + 2.1 * u
+    least = 2.0 ** -24 * (1 + 40 + rows) * 4 / (2.1 * u) if dtype == torch.float16 else 0.0
+    for name, g, w, size in zip(("y", "dx", "dgate", "dup", "ddown"), got, want, ref.mlp_sizes(dy, x, gate, up, down, "silu")):
+        special_check(g, w, size + least, tol, name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 17, 40, 70, 300])
+def test_gated_mlp_with_a_weight_of_the_types_largest_value(ct, dtype, rows):  # noqa: F811
+    x, gate, up, down, dy = mlp_tensors(seeded(rows), rows, 24, 40, dtype)
+    x *= 0.25
+    down[2, 5] = torch.finfo(dtype).max
+    y = ct.gated_mlp(x, gate, up, down, "silu")
+    assert torch.isfinite(y).all()
+    ref.check(y, ref.mlp(x, gate, up, down, "silu"), ref.mlp_sizes(dy, x, gate, up, down, "silu")[0], 2 * (2 * 24 + 40 + 40) * F32 + 2.1 * ref.U[dtype], "y")
+
+
+@pytest.mark.parametrize("rows", [3, 40, 70, 300])
+def test_products_beyond_float32_are_infinite(ct, rows):  # noqa: F811
+    # 10^30 times weights of 10^15 and less: the corrections overflow too, with either sign
+    x, gate, up, down, _ = mlp_tensors(seeded(rows), rows, 24, 40, torch.float32)
+    x[:, 4] *= 1e30
+    gate[::2, 4] *= 1e15
+    gate[1::4, 4] *= 1e8
+    _, saved = ct.gated_mlp_forward(x, gate, up, down, "silu")
+    want = ref.d(x) @ ref.d(gate).T
+    want[want.abs() > torch.finfo(torch.float32).max] *= float("inf")
+    assert torch.isinf(want).any() and torch.isfinite(want).any()
+    special_check(saved[0], want, ref.d(x).abs() @ ref.d(gate).abs().T, 2.0 ** -20, "g")
+
+
+@pytest.mark.parametrize("rows", [3, 40, 70, 136, 300])
+def test_float32_products_are_as_exact_as_float32s(ct, rows):  # noqa: F811
+    """One term in every sum but dx's: each of the products' six parts counts.  A product is off by what the three left
+    out come to, 1.5 2^-23 at most, and two roundings; y and the weights' gradients are three products behind one another."""
+    n = 136
+    gen = seeded(rows)
+    x, dy, down = torch.zeros(rows, n), torch.zeros(rows, n), torch.zeros(n, n)
+    x[torch.arange(rows), torch.randint(n, (rows,), generator=gen)] = torch.randn(rows, generator=gen)
+    dy[rows // 2] = torch.randn(n, generator=gen)
+    down[torch.arange(n), torch.randperm(n, generator=gen)] = torch.randn(n, generator=gen)
+    gate, up = normal(gen, n, n), normal(gen, n, n)
+    x, dy, down, act = x.to(DEV), dy.to(DEV), down.to(DEV), (8.0, 0.25, 0.0, 0.0)
+    y, saved = ct.gated_mlp_forward(x, gate, up, down, act)
+    for got, w in zip(saved, (gate, up)):
+        want = ref.d(x) @ ref.d(w).T
+        ref.check(got, want, want.abs(), 1.25 * 2.0 ** -22, "a projection")
+    _, *got = ct.gated_mlp_backward(dy, x, gate, up, down, saved, act)
+    _, *want = ref.mlp_grad(dy, x, gate, up, down, act)
+    for name, g, w in zip(("y", "dgate", "dup", "ddown"), (y, *got), (ref.mlp(x, gate, up, down, act), *want)):
+        ref.check(g, w, w.abs(), 2.0 ** -19, name)
