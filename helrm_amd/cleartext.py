@@ -19,12 +19,13 @@ for it.  Outputs and workspaces come from torch's allocator; a tensor that
 another stream made or still writes has to be waited for by the caller, as
 with torch's own operators.  A layout that the kernels do not take (a last
 dimension that is not contiguous, rows that overlap) is copied first.
-Shapes and types that do not fit raise ValueError; HipError holds what the
-library refuses.
+Shapes and types that do not fit raise ValueError, tensors with a forward-mode
+tangent NotImplementedError; HipError holds what the library refuses.
 """
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from .backend import CrossEntropyArgs, GatedMLPArgs, HipError, LayerNormArgs, load_library
 
@@ -94,8 +95,16 @@ def _sized(n, name):
         raise ValueError(f"{name}: {n}, the most is 2^31 - 1")
 
 
+def _no_tangent(t, name):
+    # (a kernel reads the storage, where a dual tensor's tangent is not: it would be lost without a word)
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{name}: has a tangent, and there are no forward-mode derivatives")
+
+
 def _rows(t, width, name, like=None):
     """[rows, width] of a tensor whose last dimension is the vector, in a layout that the kernels take."""
+    if forward_ad._current_level >= 0:
+        _no_tangent(t, name)
     shape = t.shape
     if not shape or shape[-1] != width:
         raise ValueError(f"{name}: the last dimension is {list(shape)[-1:]}, not {width}")
@@ -120,6 +129,8 @@ def _ld(t):
 
 
 def _vector(t, n, name, dtype, device):
+    if forward_ad._current_level >= 0:
+        _no_tangent(t, name)
     if t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name}: {list(t.shape)}, not [{n}]")
     if t.dtype != dtype or t.device != device:

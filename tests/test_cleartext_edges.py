@@ -74,6 +74,28 @@ def test_norms_so_wide_that_an_index_would_overflow_are_refused(lib):
     assert lib.LayerNormGradWorkspace(ctypes.byref(a)) == 2 * 4 * a.width
 
 
+# ---- derivatives that there are not -----------------------------------------------------
+
+
+def test_tensors_with_a_tangent_are_refused():
+    # (the tangent was lost: an output without one is a constant)
+    torch = pytest.importorskip("torch")
+    from torch.autograd import forward_ad
+
+    from helrm_amd import cleartext as ct
+    x, w, m, target = torch.ones(2, 4), torch.ones(4), torch.ones(4, 4), torch.zeros(2, dtype=torch.int64)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in (lambda: ct.layer_norm(d, w), lambda: ct.layer_norm_forward(d, w), lambda: ct.gated_mlp(d, m, m, m),
+                             lambda: ct.cross_entropy(d, m, target), lambda: ct.cross_entropy_forward(d, m, target)):
+                    with pytest.raises(NotImplementedError, match="x: has a tangent"):
+                        call()
+        with pytest.raises(ValueError, match="not on the GPU"):      # none of these has one
+            ct.layer_norm(x, w)
+
+
 # ---- the launches of the loss --------------------------------------------------------
 
 # rows, table rows, width, products a product is made of: small tiles in several launches (few rows; 257 to 384 of float32), a

@@ -174,3 +174,25 @@ def test_float32_products_are_as_exact_as_float32s(ct, rows):  # noqa: F811
     _, *want = ref.mlp_grad(dy, x, gate, up, down, act)
     for name, g, w in zip(("y", "dgate", "dup", "ddown"), (y, *got), (ref.mlp(x, gate, up, down, act), *want)):
         ref.check(g, w, w.abs(), 2.0 ** -19, name)
+
+
+# ---- forward mode -----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("which", range(12))
+def test_no_tensor_with_a_tangent_is_taken(ct, which):  # noqa: F811
+    from torch.autograd import forward_ad
+    x, gate, up, down, dy = mlp_tensors(seeded(1), 4, 8, 12, torch.float32)
+    w, b = normal(seeded(2), 8), normal(seeded(3), 8)
+    target = torch.zeros(4, dtype=torch.int64, device=DEV)
+    _, mean, rstd = ct.layer_norm_forward(x, w, b)
+    _, saved = ct.gated_mlp_forward(x, gate, up, down)
+    losses, lse = ct.cross_entropy_forward(x, gate, target)
+    calls = [(ct.layer_norm, [x, w, b]), (ct.gated_mlp, [x, gate, up, down]), (ct.cross_entropy, [x, gate, target]),
+             (lambda g: ct.layer_norm_backward(g, x, w, mean, rstd), [dy]), (lambda g: ct.gated_mlp_backward(g, x, gate, up, down, saved), [dy]),
+             (lambda g: ct.cross_entropy_backward(g, x, gate, target, lse), [losses])]
+    call, args, k = [(f, a, k) for f, a in calls for k in range(len(a)) if a[k] is not target][which % 12]
+    with forward_ad.dual_level():
+        args[k] = forward_ad.make_dual(args[k], torch.ones_like(args[k]))
+        with pytest.raises(NotImplementedError, match="tangent"):
+            call(*args)
