@@ -12,7 +12,8 @@ Each has a `_forward` and a `_backward` call, which a training loop of one's
 own makes, and a form for torch's autograd.  The matrices' last dimension is
 the vector; leading dimensions are rows.  Types: float32, bfloat16, float16,
 one for all of an operator's tensors (a norm's weight and bias may be float32
-beside any); sums and softmax statistics are float32.
+beside any); sums and softmax statistics are float32.  Tensors of the same rows
+have the same leading dimensions, or the rows in one.
 
 Work goes to torch's current stream of the tensors' device and nothing waits
 for it.  Outputs and workspaces come from torch's allocator; a tensor that
@@ -124,6 +125,14 @@ def _rows(t, width, name, like=None):
     return t
 
 
+def _same_order(lead, like, name):
+    """Leading dimensions of a tensor beside x's, `like`: the same, or rows in a line beside either."""
+    if len(lead) > 1 and lead != like:
+        a, b = [n for n in lead if n != 1], [n for n in like if n != 1]
+        if a != b and len(a) > 1 and len(b) > 1:
+            raise ValueError(f"{name}: leading dimensions {list(lead)}, not {list(like)}")
+
+
 def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
@@ -178,6 +187,7 @@ def layer_norm_backward(grad, x, weight, mean, rstd, has_bias=True):
     """(dx, dweight, dbias) of the norm; dbias is None without a bias."""
     x2, weight, _ = _norm_tensors(x, weight, None)
     rows, width = x2.shape
+    _same_order(grad.shape[:-1], x.shape[:-1], "grad")
     g2 = _rows(grad, width, "grad", x)
     if g2.shape[0] != rows:
         raise ValueError(f"grad: {g2.shape[0]} rows, not {rows}")
@@ -279,6 +289,7 @@ def gated_mlp_backward(grad, x, gate, up, down, saved, activation="silu"):
     x2, gate, up, down = _mlp_tensors(x, gate, up, down)
     act, coef = _act(activation)
     rows, hidden, width = x2.shape[0], gate.shape[0], gate.shape[1]
+    _same_order(grad.shape[:-1], x.shape[:-1], "grad")
     g2 = _rows(grad, width, "grad", x)
     if g2.shape[0] != rows:
         raise ValueError(f"grad: {g2.shape[0]} rows, not {rows}")
@@ -327,6 +338,7 @@ def _loss_tensors(x, table, target, ignore_index):
     _sized(table.shape[0], "table: rows")
     _sized(table.shape[1], "table: the last dimension")
     _need(-(1 << 63) <= ignore_index < 1 << 63, "ignore_index: not an int64")
+    _same_order(target.shape, x.shape[:-1], "target")
     x2 = _rows(x, table.shape[1], "x")
     target = _vector(target.reshape(-1) if target.dim() != 1 else target, x2.shape[0], "target", torch.int64, x.device)
     return x2, _rows(table, table.shape[1], "table", x), target
@@ -351,6 +363,8 @@ def cross_entropy_backward(grad, x, table, target, lse, ignore_index=-100):
     computed again, a piece of the table at a time."""
     x2, table, target = _loss_tensors(x, table, target, ignore_index)
     rows, width = x2.shape
+    _same_order(grad.shape, x.shape[:-1], "grad")
+    _same_order(lse.shape, x.shape[:-1], "lse")
     grad = _vector(grad.reshape(-1), rows, "grad", torch.float32, x.device)
     lse = _vector(lse.reshape(-1), rows, "lse", torch.float32, x.device)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)

@@ -74,6 +74,23 @@ def test_norms_so_wide_that_an_index_would_overflow_are_refused(lib):
     assert lib.LayerNormGradWorkspace(ctypes.byref(a)) == 2 * 4 * a.width
 
 
+def test_tensors_of_the_same_rows_have_them_in_the_same_order():
+    torch = pytest.importorskip("torch")
+    from helrm_amd import cleartext as ct
+    x, m = torch.zeros(9, 5, 4), torch.zeros(4, 4)
+    refused = [torch.Size(s) for s in ((5, 9), (3, 15), (5, 3, 3), (1, 5, 9))]
+    for s in refused:
+        with pytest.raises(ValueError, match="target: leading dimensions"):
+            ct.cross_entropy(x, m, torch.zeros(s, dtype=torch.int64))
+        with pytest.raises(ValueError, match="target: leading dimensions"):
+            ct.cross_entropy_backward(torch.zeros(45), x, m, torch.zeros(s, dtype=torch.int64), torch.zeros(45))
+    for s in ((9, 5), (45,), (9, 1, 5), (45, 1), (1, 45)):          # (the next check is the one for the GPU)
+        with pytest.raises(ValueError, match="not on the GPU"):
+            ct.cross_entropy(x, m, torch.zeros(s, dtype=torch.int64))
+        with pytest.raises(ValueError, match="not on the GPU"):
+            ct.cross_entropy(x.view(45, 4), m, torch.zeros(s, dtype=torch.int64))
+
+
 # ---- derivatives that there are not -----------------------------------------------------
 
 

@@ -196,3 +196,29 @@ def test_no_tensor_with_a_tangent_is_taken(ct, which):  # noqa: F811
         args[k] = forward_ad.make_dual(args[k], torch.ones_like(args[k]))
         with pytest.raises(NotImplementedError, match="tangent"):
             call(*args)
+
+
+# ---- leading dimensions -----------------------------------------------------------------
+
+
+def test_gradients_of_other_leading_dimensions(ct):  # noqa: F811
+    x, gate, up, down, dy = mlp_tensors(seeded(1), 45, 8, 12, torch.float32)
+    w, target = normal(seeded(2), 8), torch.arange(45, device=DEV) % 12
+    _, mean, rstd = ct.layer_norm_forward(x, w)
+    _, saved = ct.gated_mlp_forward(x, gate, up, down)
+    losses, lse = ct.cross_entropy_forward(x, gate, target)
+
+    def calls(x, dy, losses, lse):
+        return [lambda: ct.layer_norm_backward(dy, x, w, mean, rstd), lambda: ct.gated_mlp_backward(dy, x, gate, up, down, saved),
+                lambda: ct.cross_entropy_backward(losses, x, gate, target, lse)]
+
+    want = [call() for call in calls(x, dy, losses, lse)]
+    for lead in ((9, 5), (45,), (1, 45), (9, 1, 5)):
+        for other in (lead, (45,)):
+            for got, w_ in zip(calls(x.view(*other, 8), dy.view(*lead, 8), losses.view(lead), lse.view(lead)), want):
+                got = got()
+                assert got[0].shape == (*other, 8) and all(torch.equal(a.reshape(b.shape), b) for a, b in zip(got, w_))
+    x = x.view(9, 5, 8)
+    for call in calls(x, dy.view(5, 9, 8), losses.view(5, 9), lse) + [lambda: ct.cross_entropy_backward(losses, x, gate, target, lse.view(5, 9))]:
+        with pytest.raises(ValueError, match="leading dimensions"):
+            call()
