@@ -24,7 +24,12 @@ inline void check_hip(hipError_t e, const char* what) {
   if (e != hipSuccess) throw Error(std::string("HIP error: ") + hipGetErrorString(e) + " at " + what);
 }
 template <class F> int guarded(F&& f) {
-  try { f(); check_hip(hipGetLastError(), "a kernel launch"); return 0; }
+  try {
+    (void)hipGetLastError();   // (of an earlier call, an allocation that failed say: not this one's)
+    f();
+    check_hip(hipGetLastError(), "a kernel launch");
+    return 0;
+  }
   catch (const std::exception& e) { return report_error(e.what()); }
   catch (...) { return report_error("unknown error"); }
 }

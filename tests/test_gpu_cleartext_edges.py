@@ -1,5 +1,7 @@
 """The cleartext operators at the limits of a launch and of a type, against
 plain 64-bit implementations.  Bounds as in cleartext_ref."""
+import ctypes
+
 import pytest
 import torch
 
@@ -222,3 +224,21 @@ def test_gradients_of_other_leading_dimensions(ct):  # noqa: F811
     for call in calls(x, dy.view(5, 9, 8), losses.view(5, 9), lse) + [lambda: ct.cross_entropy_backward(losses, x, gate, target, lse.view(5, 9))]:
         with pytest.raises(ValueError, match="leading dimensions"):
             call()
+
+
+# ---- errors of others -------------------------------------------------------------------
+
+
+def test_an_error_of_an_earlier_call_is_not_the_operators(ct):  # noqa: F811
+    # an allocation that fails leaves its error behind until somebody asks for the last one
+    # (torch's own kernels, copies among them, ask for it, and so there are none in these calls)
+    x, w, down = normal(seeded(1), 4, 8), normal(seeded(2), 8), normal(seeded(3), 8, 4)
+    want = ct.layer_norm(x, w)
+    with open("/proc/self/maps") as f:
+        hip = ctypes.CDLL(next(line.split()[-1] for line in f if "libamdhip64.so" in line))
+    hip.hipMalloc.argtypes = [ctypes.c_void_p, ctypes.c_size_t]
+    for call in (lambda: ct.layer_norm(x, w), lambda: ct.gated_mlp(x, x, x, down)):
+        pointer = ctypes.c_void_p()
+        assert hip.hipMalloc(ctypes.byref(pointer), 1 << 60) != 0
+        call()
+    assert torch.equal(ct.layer_norm(x, w), want)
