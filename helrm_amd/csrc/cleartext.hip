@@ -315,9 +315,12 @@ size_t ce_forward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
 }
 
 // Rows of the table whose gradients of the logits are held at a time: those
-// of all rows of x take at most 256 MiB, what the last-level cache holds.
+// of all rows of x take at most 256 MiB, what the last-level cache holds, or
+// there are 1,024 of them.
+constexpr long PIECE_BYTES = 256L << 20;
+static_assert(PIECE_BYTES < 1L << 31 && 256 * 1024 * 2 < 1L << 31, "the rows of a tile of dl are within 31-bit offsets, whatever their number and width");
 int piece_rows(const CrossEntropyArgs* a) {
-  const long most = (256L << 20) / (std::max<long>(a->rows, 1) * (a->type == DT_F32 ? 6 : few_rows(a->rows, a->type) ? 4 : 2));
+  const long most = PIECE_BYTES / (std::max<long>(a->rows, 1) * (a->type == DT_F32 ? 6 : few_rows(a->rows, a->type) ? 4 : 2));
   return (int)std::min<long>(up8(a->vocab), std::max<long>(1024, most / 1024 * 1024));
 }
 

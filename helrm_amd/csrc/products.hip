@@ -132,7 +132,8 @@ template <class T> __device__ __forceinline__ void store4(const ProductArgs& p, 
 // tile, W waves; every wave issues R / 8 / W loads of 1 KiB.
 template <bool ALONG_K, int R, int W> struct Loader {
   static constexpr int N = R / 8 / W;
-  unsigned off[N];   // of the lane's 16 bytes, from the step's first element
+  unsigned off[N];   // of the lane's 16 bytes, from the step's first element: under 2^31, since factors' rows are under 2^21
+                     // elements apart, or (dl) all within 2^28 bytes
   int kk;            // the lane's first k (ALONG_K) -- or, of load j, kk + j * PER
   static constexpr int PER = 512 / R;
 
@@ -314,7 +315,10 @@ template <int EPI> __device__ __host__ __forceinline__ long sum_ld(const Product
 // A wave's accumulators go through its own part of LDS, 64 rows of 64 float32
 // columns at a time (16 bytes c of row r at c ^ (r & 15)), so that what is
 // stored are whole lines of a row and the code of it is there once.  A place is
-// a 32-bit offset from the wave's first element (rows are under 2^21 elements).
+// a 32-bit offset from the wave's first element: of up to 128 rows, which are
+// under 2^24 elements apart in a caller's result, 2^21 in an intermediate, 2^22
+// in split sums; all the rows of a loss's dl are under 2^27 elements, or 2^10
+// apart.
 template <class T, int EPI, int FM, int FN>
 __device__ __forceinline__ void emit(const ProductArgs& p, const f32x4 (&acc)[FM][FN], int M, long mw, long n_wave, int split, float* own) {
   constexpr int LANES = EPI == EPI_GATE ? 8 : 16, ROWS = 64 / LANES;   // of a row; rows a time
