@@ -324,7 +324,7 @@ def gated_mlp(x, gate, up, down, activation="silu"):
     """The gated feed-forward block (act(x gate^T) * (x up^T)) down^T: gate, up [hidden, width], down [width, hidden].
     activation: "silu", "gelu" or a cubic's four coefficients, lowest degree first, which the block can also be
     evaluated with under encryption.  Hidden values and their gradients are factors of the next product, of x's type: in
-    float16 one beyond 65504 is infinite."""
+    float16 one beyond 65504 is infinite, and gradients below 2^-14 lose bits unless the loss is scaled."""
     if _wants_grad(x, gate, up, down):
         return _GatedMLP.apply(x, gate, up, down, activation)
     return _mlp_forward(x, gate, up, down, activation, False)[0]

@@ -106,8 +106,10 @@ Held hold(Arena& m, long rows, long width, int type, bool exact = false) {
 // them one value's rounding may be all there is (up to 2.5 times, seen 1.6).
 // The products are bound by the weights there, not by the matrix units, and up
 // to 64 rows are one step of k in the weights' gradients: 64 x 1,024 x 4,096,
-// forward and backward, 82 us with two parts and 75 with one; the loss of 64 x
-// 1,024 against 65,536 172 and 165.
+// forward and backward, 81 us with two parts and 73 with one; the loss of 64 x
+// 1,024 against 65,536 172 and 162.  The parts are of the operator's type, with
+// its range: float16 hidden values and their gradients are infinite beyond 65504
+// and lose bits below 2^-14 (a loss in float16 is scaled; dl is by itself).
 bool few_rows(long rows, int type) { return type != DT_F32 && rows <= 64; }
 // Matrices that are copied first, all in one launch: where alignment, an odd
 // width or float32 does not let the tiles be loaded from a matrix itself.  A

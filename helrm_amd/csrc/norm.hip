@@ -323,7 +323,9 @@ int part_count(long rows, int width) {
 // (and the weights) starts at a multiple of 16 bytes and holds a whole number of them.  Then 16-bit rows are still read 16
 // bytes at a time (32,768 x 4,095 bfloat16 forward 204 us, 335 an element at a time, backward 327 and 966; 4,097 x 1,001
 // backward 19 and 38), except forward with a whole row of 513 to 1,024 in one wave, where the cut pack holds the wave up
-// (4,097 x 1,001 14 us, 10 an element at a time), and float32 an element at a time (4,097 x 1,001 10 + 17 us, 14 + 18 in packs).
+// (4,097 x 1,001 14 us, 10 an element at a time), and float32 an element at a time (4,097 x 1,001 10 + 18.7 us, 14 + 18.7 in
+// packs; 32,768 x 1,535 79 + 151 and 89 + 215; 32,768 x 4,095 202 + 313 and 224 + 324).  Not the faster at every size: 32,768 x
+// 333 float32 backward 39 us, 34.5 in packs; 32,768 x 767 bfloat16 forward 50 us, 41 in packs.
 template <int V> struct Int { static constexpr int value = V; };
 template <class T, class F> void with_packs(bool aligned, bool forward, int width, int waves, F&& f) {
   constexpr int V = 16 / sizeof(T);

@@ -3,7 +3,7 @@
 //
 // C[t][n] = sum_k X(t, k) W(n, k) for up to 16 rows t, 64 of float32 (more of
 // 16 bits are faster through the tiles: 33 rows against 65,536 x 1,024 bfloat16
-// 71 us here and 35 there; of float32, which the tiles need laid out, 152 us
+// 71 us here and 35 there; of float32, which the tiles need laid out, 148 us
 // here and 339 there).  Bound by memory: 16
 // rows of W go straight from memory to the registers of a wave, 128 bytes a
 // row and turn, and multiply up to four groups of 16 rows of X there
@@ -15,8 +15,9 @@
 // into three bfloat16 parts in registers and multiplied as in products.hip.
 //
 // Measured: one row against 65,536 x 1,024 bfloat16, 134 MB, 28 us = 4.8 TB/s
-// (a copy: 4.95); the gate and up projections of one row, 17 MB, 8 to 11 us,
-// and the down projection, 8 MB, 7 us, which are launch and latency.
+// (a copy: 4.95); the gate and up projections of one row of 1,024 to 4,096, 17
+// MB, 6.5 us; the down projection, 8 MB, 10.7 us: its 1,024 results are 64
+// workgroups, on a quarter of the CUs.
 #include "skinny.h"
 #include "tiles.h"
 

@@ -283,7 +283,8 @@ unsigned long long StopLiveHeapSampler(void);
  * by its call is done.  Element types: 0 float32, 1 bfloat16, 2 float16; sums,
  * means and softmax statistics are float32 for each.  A matrix's rows are
  * contiguous and `ld...` elements apart.  Outputs do not overlap inputs
- * except where said. */
+ * except where said.  float32 products are as exact as float32 multiplications,
+ * and infinite where those are. */
 #define HELRM_F32 0
 #define HELRM_BF16 1
 #define HELRM_F16 2
@@ -308,7 +309,7 @@ int LayerNormGrad(const LayerNormArgs* args, void* stream);
  * act 0: silu, 1: gelu (erf), 2: cubic, coef lowest degree first, the form
  * that EvaluatePolynomial takes.  The products' factors act(g) u, dg and du are
  * of the tensors' type (in two parts up to 64 rows): in float16 one beyond
- * 65504 is infinite. */
+ * 65504 is infinite, one below 2^-14 loses bits.  width, hidden below 2^21. */
 typedef struct {
   const void* x; long ldx;               /* [rows][width] */
   const void* gate; long ldgate;         /* [hidden][width] */
