@@ -65,6 +65,11 @@ class CrossEntropyArgs(ctypes.Structure):
                 ("type", ctypes.c_int)]
 
 
+class LossTotalArgs(ctypes.Structure):
+    _fields_ = [("loss", ctypes.c_void_p), ("target", ctypes.c_void_p), ("total", ctypes.c_void_p), ("factor", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspaceBytes", ctypes.c_size_t), ("rows", ctypes.c_long), ("ignore", ctypes.c_longlong)]
+
+
 _ARRAY_TYPES = (ArrayResultInt, ArrayResultFloat, ArrayResultUInt64)
 
 
@@ -323,6 +328,8 @@ _SIGNATURES = {
     "CrossEntropy": ([_c.c_void_p, _c.c_void_p], _I),
     "CrossEntropyGradWorkspace": ([_c.c_void_p], _c.c_long),
     "CrossEntropyGrad": ([_c.c_void_p, _c.c_void_p], _I),
+    "LossTotalWorkspace": ([_c.c_void_p], _c.c_long),
+    "LossTotal": ([_c.c_void_p, _c.c_void_p], _I),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -28,7 +28,7 @@ import ctypes
 import torch
 from torch.autograd import forward_ad
 
-from .backend import CrossEntropyArgs, GatedMLPArgs, HipError, LayerNormArgs, load_library
+from .backend import CrossEntropyArgs, GatedMLPArgs, HipError, LayerNormArgs, LossTotalArgs, load_library
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {"silu": 0, "gelu": 1}
@@ -51,7 +51,7 @@ def _library():
         raise HipError("two HIP runtimes in one process (" + ", ".join(sorted(runtimes))
                        + "): import torch before the library is loaded")
     calls = {}
-    for name in ("LayerNorm", "LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad"):
+    for name in ("LayerNorm", "LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad", "LossTotal"):
         call, size = getattr(lib, name), getattr(lib, name + "Workspace") if name != "LayerNorm" else None
         call.argtypes, call.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
         if size is not None:
@@ -390,15 +390,39 @@ class _CrossEntropy(torch.autograd.Function):
         return cross_entropy_backward(grad, *ctx.saved_tensors, ctx.ignore_index) + (None, None)
 
 
+def _total(losses, target, ignore_index):
+    """(the losses' sum, or with a target their mean; what each one's gradient is of it).  (torch's sum of many values
+    clears memory first, which a captured graph does not repeat.)"""
+    total, factor = (torch.empty((), dtype=torch.float32, device=losses.device) for _ in "ab")
+    if target is not None:
+        target = target.reshape(-1).contiguous()
+    _call("LossTotal", LossTotalArgs(
+        loss=losses.data_ptr(), target=None if target is None else target.data_ptr(), total=total.data_ptr(), factor=factor.data_ptr(),
+        rows=losses.numel(), ignore=ignore_index), losses.device)
+    return total, factor
+
+
+class _Total(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, losses, target, ignore_index):
+        total, factor = _total(losses, target, ignore_index)
+        ctx.save_for_backward(factor)
+        ctx.shape = losses.shape
+        return total
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return (grad * ctx.saved_tensors[0]).expand(ctx.shape), None, None
+
+
 def cross_entropy(x, table, target, ignore_index=-100, reduction="mean"):
     """Softmax cross entropy of x [..., width] against table [vocab, width]: the mean over the rows that have a target
     (0 where none has one), their "sum", or "none" for a loss a row."""
     _need(reduction in ("mean", "sum", "none"), f"reduction {reduction!r}: neither mean, sum nor none")
-    if _wants_grad(x, table):
-        losses = _CrossEntropy.apply(x, table, target, ignore_index)
-    else:
-        losses = cross_entropy_forward(x, table, target, ignore_index)[0]
+    grad = _wants_grad(x, table)
+    losses = _CrossEntropy.apply(x, table, target, ignore_index) if grad else cross_entropy_forward(x, table, target, ignore_index)[0]
     if reduction == "none":
         return losses
-    total = losses.sum()
-    return total if reduction == "sum" else total / (target != ignore_index).sum().clamp(min=1)
+    target = target if reduction == "mean" else None
+    return _Total.apply(losses, target, ignore_index) if grad else _total(losses, target, ignore_index)[0]

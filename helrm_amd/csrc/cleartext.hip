@@ -379,6 +379,11 @@ size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
   return m.used;
 }
 
+void check_total(const LossTotalArgs* a) {
+  require(a, "no arguments");
+  require(a->rows >= 0 && a->rows < MAX_ROWS, "LossTotal: bad number of rows");
+}
+
 template <class F> long sized(F&& f) {
   try { return (long)f(); } catch (const std::exception& e) { return report_error(e.what()); }
 }
@@ -485,6 +490,19 @@ int CrossEntropyGrad(const CrossEntropyArgs* a, void* stream) {
     }
     check_space(a->workspace, a->workspaceBytes, ce_backward(a, true, nullptr));
     ce_backward(a, false, (hipStream_t)stream);
+  });
+}
+
+long LossTotalWorkspace(const LossTotalArgs* a) {
+  return sized([&] { check_total(a); return loss_total_bytes(a->rows); });
+}
+int LossTotal(const LossTotalArgs* a, void* stream) {
+  return clr::guarded([&] {
+    check_total(a);
+    require(a->loss || !a->rows, "LossTotal: loss");
+    require(a->total && a->factor, "LossTotal: total and factor");
+    check_space(a->workspace, a->workspaceBytes, loss_total_bytes(a->rows));
+    loss_total(a->loss, a->target, a->ignore, a->rows, a->workspace, a->total, a->factor, (hipStream_t)stream);
   });
 }
 

@@ -86,4 +86,7 @@ void softmax_finish(const float2* part, int parts, const float* picked, const in
 // out[row] = (acc[place[row]], and what is `second` elements behind it) / *scale, 0 for rows that are not kept
 void scatter_rows(const float* acc, long ldacc, long second, const int* place, const float* scale, void* out, long ldout, long n, int width, int dtype,
                   hipStream_t st);
+// total[0] = the sum of n losses, or (target) their mean over the rows whose target is not `ignore`; factor[0] = 1, or one over their number
+size_t loss_total_bytes(long n);
+void loss_total(const float* loss, const long long* target, long long ignore, long n, void* workspace, float* total, float* factor, hipStream_t st);
 void fill_zero(void* p, size_t bytes, hipStream_t st);  // bytes: a multiple of 2

@@ -354,6 +354,20 @@ int CrossEntropy(const CrossEntropyArgs* args, void* stream);
 long CrossEntropyGradWorkspace(const CrossEntropyArgs* args);
 int CrossEntropyGrad(const CrossEntropyArgs* args, void* stream);
 
+/* total = the sum of the losses, or with `target` their mean over the rows that
+ * have one other than `ignore` (0 where none has); factor = what the gradient of
+ * every such loss is of total's: 1, or one over their number. */
+typedef struct {
+  const float* loss;                     /* [rows] */
+  const long long* target;               /* [rows], or NULL: the sum */
+  float* total; float* factor;
+  void* workspace; size_t workspaceBytes;
+  long rows;
+  long long ignore;
+} LossTotalArgs;
+long LossTotalWorkspace(const LossTotalArgs* args);
+int LossTotal(const LossTotalArgs* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,7 +7,7 @@ import subprocess
 
 import pytest
 
-from helrm_amd.backend import LayerNormArgs, load_library
+from helrm_amd.backend import LayerNormArgs, LossTotalArgs, load_library
 
 SOME = 1 << 20      # a pointer that is not followed
 
@@ -15,9 +15,10 @@ SOME = 1 << 20      # a pointer that is not followed
 @pytest.fixture(scope="module")
 def lib():
     lib = load_library()
-    for name in ("LayerNorm", "LayerNormGrad"):
+    for name in ("LayerNorm", "LayerNormGrad", "LossTotal"):
         getattr(lib, name).argtypes, getattr(lib, name).restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
-    lib.LayerNormGradWorkspace.argtypes, lib.LayerNormGradWorkspace.restype = [ctypes.c_void_p], ctypes.c_long
+    for name in ("LayerNormGradWorkspace", "LossTotalWorkspace"):
+        getattr(lib, name).argtypes, getattr(lib, name).restype = [ctypes.c_void_p], ctypes.c_long
     return lib
 
 
@@ -89,6 +90,18 @@ def test_tensors_of_the_same_rows_have_them_in_the_same_order():
             ct.cross_entropy(x, m, torch.zeros(s, dtype=torch.int64))
         with pytest.raises(ValueError, match="not on the GPU"):
             ct.cross_entropy(x.view(45, 4), m, torch.zeros(s, dtype=torch.int64))
+
+
+def test_what_a_total_refuses(lib):
+    assert lib.LossTotal(None, None) == -1 and "no arguments" in lib.GetLastError().decode()
+    for message, change in (("number of rows", dict(rows=-1)), ("number of rows", dict(rows=1 << 30)), (": loss", dict(loss=None)),
+                            ("total and factor", dict(factor=None)), ("workspace too small", dict(rows=1 << 20))):
+        a = LossTotalArgs(loss=SOME, target=SOME, total=SOME, factor=SOME, rows=100, ignore=-100)
+        for k, v in change.items():
+            setattr(a, k, v)
+        assert lib.LossTotal(ctypes.byref(a), None) == -1
+        assert message in lib.GetLastError().decode()
+    assert lib.LossTotalWorkspace(ctypes.byref(a)) == 256 * 16
 
 
 # ---- derivatives that there are not -----------------------------------------------------

@@ -242,3 +242,70 @@ def test_an_error_of_an_earlier_call_is_not_the_operators(ct):  # noqa: F811
         assert hip.hipMalloc(ctypes.byref(pointer), 1 << 60) != 0
         call()
     assert torch.equal(ct.layer_norm(x, w), want)
+
+
+# ---- the mean and the sum of the losses -----------------------------------------------------
+
+
+@pytest.mark.parametrize("rows", [0, 1, 5, 4095, 8191, 8192, 300001, (1 << 21) + 3])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_cross_entropy_totals(ct, rows, reduction):  # noqa: F811
+    # 64-bit sums, one rounding (the losses as the operator leaves them)
+    x, table, target, _ = ce_tensors(seeded(rows), rows, 8, 16, torch.float32, 0.3)
+    losses = ct.cross_entropy(x, table, target, reduction="none")
+    got = ct.cross_entropy(x.view(rows, 1, 8), table, target.view(rows, 1), reduction=reduction)
+    n = max(1, int((target != -100).sum())) if reduction == "mean" else 1
+    want = ref.d(losses).sum() / n
+    ref.check(got, want, want.abs(), 2.0 ** -24 + 2.0 ** -40, reduction)
+    x, table = x.requires_grad_(), table.requires_grad_()
+    total = ct.cross_entropy(x, table, target, reduction=reduction)
+    assert torch.equal(total, got)
+    (2.0 * total).backward()
+    lse = ct.cross_entropy_forward(x.detach(), table.detach(), target)[1]
+    grad = torch.full((rows,), 2.0 / n, dtype=torch.float64, device=DEV).float()
+    for a, b in zip((x.grad, table.grad), ct.cross_entropy_backward(grad, x.detach(), table.detach(), target, lse)):
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-9)
+
+
+def test_cross_entropy_totals_of_nothing_and_of_nan(ct):  # noqa: F811
+    x, table, target, _ = ce_tensors(seeded(1), 20000, 8, 16, torch.float32)
+    gone = torch.full_like(target, -100)
+    for reduction in ("mean", "sum"):
+        assert ct.cross_entropy(x, table, gone, reduction=reduction).item() == 0.0
+        target[777] = 16                       # outside the table
+        assert torch.isnan(ct.cross_entropy(x, table, target, reduction=reduction))
+        assert ct.cross_entropy(x, table, gone, ignore_index=-100, reduction=reduction).item() == 0.0
+
+
+@pytest.mark.parametrize("rows", [1000, 70000, 300000, 3000000])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_cross_entropy_totals_in_a_graph(ct, rows, reduction):  # noqa: F811
+    # (with torch's sum every replay after the first had the first one's value, from some 100,000 rows on)
+    x, table, target, _ = ce_tensors(seeded(rows), rows, 8, 16, torch.float32, 0.2)
+    x, table = x.requires_grad_(), table.requires_grad_()
+
+    def step():
+        total = ct.cross_entropy(x, table, target, reduction=reduction)
+        return (total, *torch.autograd.grad(total, (x, table)))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(4):
+        with torch.no_grad():
+            x.mul_(0.9)
+            target[k::5] = -100
+        want = step()
+        torch.randn(1 << 22, device=DEV).sum()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), k
