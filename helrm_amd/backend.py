@@ -70,6 +70,14 @@ class LossTotalArgs(ctypes.Structure):
                 ("workspace", ctypes.c_void_p), ("workspaceBytes", ctypes.c_size_t), ("rows", ctypes.c_long), ("ignore", ctypes.c_longlong)]
 
 
+class EmbeddingArgs(ctypes.Structure):
+    _fields_ = [("ids", ctypes.c_void_p), ("table", ctypes.c_void_p), ("ldtable", ctypes.c_long), ("y", ctypes.c_void_p),
+                ("ldy", ctypes.c_long), ("dy", ctypes.c_void_p), ("lddy", ctypes.c_long), ("dtable", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspaceBytes", ctypes.c_size_t),
+                ("tokens", ctypes.c_long), ("width", ctypes.c_int), ("vocab", ctypes.c_int), ("ignore", ctypes.c_longlong),
+                ("type", ctypes.c_int), ("scale", ctypes.c_float)]
+
+
 _ARRAY_TYPES = (ArrayResultInt, ArrayResultFloat, ArrayResultUInt64)
 
 
@@ -330,6 +338,9 @@ _SIGNATURES = {
     "CrossEntropyGrad": ([_c.c_void_p, _c.c_void_p], _I),
     "LossTotalWorkspace": ([_c.c_void_p], _c.c_long),
     "LossTotal": ([_c.c_void_p, _c.c_void_p], _I),
+    "Embedding": ([_c.c_void_p, _c.c_void_p], _I),
+    "EmbeddingGradWorkspace": ([_c.c_void_p], _c.c_long),
+    "EmbeddingGrad": ([_c.c_void_p, _c.c_void_p], _I),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -7,6 +7,7 @@ that training and of scoring beside it, on the same card:
     layer_norm      y = (x - mean) / sqrt(var + eps) * weight + bias
     gated_mlp       y = (act(x gate^T) * (x up^T)) down^T
     cross_entropy   log sum_v exp <x, table[v]> - <x, table[target]>
+    embedding       y[i] = scale * table[ids[i]]
 
 Each has a `_forward` and a `_backward` call, which a training loop of one's
 own makes, and a form for torch's autograd.  The matrices' last dimension is
@@ -28,7 +29,7 @@ import ctypes
 import torch
 from torch.autograd import forward_ad
 
-from .backend import CrossEntropyArgs, GatedMLPArgs, HipError, LayerNormArgs, LossTotalArgs, load_library
+from .backend import CrossEntropyArgs, EmbeddingArgs, GatedMLPArgs, HipError, LayerNormArgs, LossTotalArgs, load_library
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {"silu": 0, "gelu": 1}
@@ -51,8 +52,9 @@ def _library():
         raise HipError("two HIP runtimes in one process (" + ", ".join(sorted(runtimes))
                        + "): import torch before the library is loaded")
     calls = {}
-    for name in ("LayerNorm", "LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad", "LossTotal"):
-        call, size = getattr(lib, name), getattr(lib, name + "Workspace") if name != "LayerNorm" else None
+    for name in ("LayerNorm", "LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad", "LossTotal", "Embedding",
+                 "EmbeddingGrad"):
+        call, size = getattr(lib, name), getattr(lib, name + "Workspace", None)
         call.argtypes, call.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
         if size is not None:
             size.argtypes, size.restype = [ctypes.c_void_p], ctypes.c_long
@@ -426,3 +428,69 @@ def cross_entropy(x, table, target, ignore_index=-100, reduction="mean"):
         return losses
     target = target if reduction == "mean" else None
     return _Total.apply(losses, target, ignore_index) if grad else _total(losses, target, ignore_index)[0]
+
+
+# ---- rows of a table for ids -----------------------------------------------------------------
+
+
+def _embedding_ids(ids, vocab, ignore_index, device):
+    _need(vocab >= 1, "table: no rows")
+    _need(-(1 << 63) <= ignore_index < 1 << 63, "ignore_index: not an int64")
+    if ids.dtype != torch.int64 or ids.device != device:
+        raise ValueError(f"ids: {ids.dtype} on {ids.device}, not {torch.int64} on {device}")
+    return ids.reshape(-1).contiguous()
+
+
+def embedding_forward(ids, table, scale=1.0, ignore_index=-100):
+    """table[ids] * scale, [..., width]: rows of zeros where an id is `ignore_index`, of NaN where another one is outside the table."""
+    _need(table.dim() == 2 and table.shape[1] >= 1, "table: not a matrix with elements")
+    vocab, width = table.shape
+    _sized(vocab, "table: rows")
+    _sized(width, "table: the last dimension")
+    t2 = _rows(table, width, "table")
+    flat = _embedding_ids(ids, vocab, ignore_index, table.device)
+    y = torch.empty((*ids.shape, width), dtype=table.dtype, device=table.device)
+    _call("Embedding", EmbeddingArgs(
+        ids=flat.data_ptr(), table=t2.data_ptr(), ldtable=_ld(t2), y=y.data_ptr(), ldy=width, tokens=flat.shape[0], width=width,
+        vocab=vocab, ignore=ignore_index, type=_TYPES[table.dtype], scale=scale), table.device)
+    return y
+
+
+def embedding_backward(grad, ids, vocab, scale=1.0, ignore_index=-100):
+    """dtable [vocab, width] for the gradient `grad` [..., width] of the rows of `ids`, of grad's type: what ids outside the table
+    and ignored ones have in grad goes nowhere."""
+    _need(grad.dim() >= 1 and grad.shape[-1] >= 1, "grad: no last dimension")
+    width = grad.shape[-1]
+    _sized(width, "grad: the last dimension")
+    _sized(vocab, "table: rows")
+    _same_order(grad.shape[:-1], ids.shape, "grad")
+    g2 = _rows(grad, width, "grad")
+    flat = _embedding_ids(ids, vocab, ignore_index, grad.device)
+    if flat.shape[0] != g2.shape[0]:
+        raise ValueError(f"grad: {g2.shape[0]} rows, not {flat.shape[0]}")
+    dtable = torch.empty((vocab, width), dtype=grad.dtype, device=grad.device)
+    _call("EmbeddingGrad", EmbeddingArgs(
+        ids=flat.data_ptr(), dy=g2.data_ptr(), lddy=_ld(g2), dtable=dtable.data_ptr(), tokens=flat.shape[0], width=width, vocab=vocab,
+        ignore=ignore_index, type=_TYPES[grad.dtype], scale=scale), grad.device)
+    return dtable
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, table, scale, ignore_index):
+        ctx.save_for_backward(ids)
+        ctx.rest = table.shape[0], scale, ignore_index
+        return embedding_forward(ids, table, scale, ignore_index)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        return None, embedding_backward(grad, *ctx.saved_tensors, *ctx.rest), None, None
+
+
+def embedding(ids, table, scale=1.0, ignore_index=-100):
+    """Rows of table [vocab, width] for ids of any shape, times `scale`: [..., width].  The table's gradient is the sum of its ids'
+    rows in float32, rounded once, and the same on every run."""
+    if _wants_grad(table):
+        return _Embedding.apply(ids, table, scale, ignore_index)
+    return embedding_forward(ids, table, scale, ignore_index)

@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <climits>
 #include "cleartext.h"
+#include "embedding.h"
 #include "norm.h"
 #include "products.h"
 #include "skinny.h"
@@ -384,6 +385,26 @@ void check_total(const LossTotalArgs* a) {
   require(a->rows >= 0 && a->rows < MAX_ROWS, "LossTotal: bad number of rows");
 }
 
+// ---- embedding ----
+void check_embedding(const EmbeddingArgs* a) {
+  require(a, "no arguments");
+  check_type(a->type);
+  require(a->tokens >= 0 && a->tokens < MAX_ROWS, "Embedding: bad number of tokens");
+  // (indices of a row's elements are ints)
+  require(a->width >= 1 && a->width <= INT_MAX - 1024, "Embedding: bad width");
+  require(a->vocab >= 1, "Embedding: bad number of table rows");
+}
+EmbedArgs embed_args(const EmbeddingArgs* a) {
+  EmbedArgs e{};
+  e.ids = a->ids;
+  e.tokens = a->tokens; e.width = a->width; e.vocab = a->vocab;
+  e.ignore = a->ignore;
+  e.dtype = a->type;
+  e.scale = a->scale;
+  return e;
+}
+size_t embedding_space(const EmbeddingArgs* a) { return embedding_grad_workspace(a->tokens, a->width, a->vocab, a->type); }
+
 template <class F> long sized(F&& f) {
   try { return (long)f(); } catch (const std::exception& e) { return report_error(e.what()); }
 }
@@ -503,6 +524,36 @@ int LossTotal(const LossTotalArgs* a, void* stream) {
     require(a->total && a->factor, "LossTotal: total and factor");
     check_space(a->workspace, a->workspaceBytes, loss_total_bytes(a->rows));
     loss_total(a->loss, a->target, a->ignore, a->rows, a->workspace, a->total, a->factor, (hipStream_t)stream);
+  });
+}
+
+int Embedding(const EmbeddingArgs* a, void* stream) {
+  return clr::guarded([&] {
+    check_embedding(a);
+    require(a->ids || !a->tokens, "Embedding: ids");
+    check_matrix(a->table, a->ldtable, a->vocab, a->width, "Embedding: table");
+    check_matrix(a->y, a->ldy, a->tokens, a->width, "Embedding: y");
+    EmbedArgs e = embed_args(a);
+    e.table = a->table; e.ldtable = a->ldtable;
+    e.y = a->y; e.ldy = a->ldy;
+    embedding_launch(e, (hipStream_t)stream);
+  });
+}
+long EmbeddingGradWorkspace(const EmbeddingArgs* a) {
+  return sized([&] { check_embedding(a); return embedding_space(a); });
+}
+int EmbeddingGrad(const EmbeddingArgs* a, void* stream) {
+  return clr::guarded([&] {
+    check_embedding(a);
+    require(a->ids || !a->tokens, "EmbeddingGrad: ids");
+    check_matrix(a->dy, a->lddy, a->tokens, a->width, "EmbeddingGrad: dy");
+    require(a->dtable, "EmbeddingGrad: dtable");
+    check_space(a->workspace, a->workspaceBytes, embedding_space(a));
+    EmbedArgs e = embed_args(a);
+    e.y = const_cast<void*>(a->dy); e.ldy = a->lddy;
+    e.dtable = a->dtable;
+    e.workspace = a->workspace;
+    embedding_grad_launch(e, (hipStream_t)stream);
   });
 }
 

@@ -368,6 +368,28 @@ typedef struct {
 long LossTotalWorkspace(const LossTotalArgs* args);
 int LossTotal(const LossTotalArgs* args, void* stream);
 
+/* y[i] = scale table[ids[i]]: rows of a table, and the table's gradient
+ * dtable[v] = scale * the sum of dy[i] over ids[i] = v, 0 for rows that no id
+ * names.  Sums are float32, rounded once, in an order that only the ids decide.
+ * An id that is `ignore` gives a row of zeros and takes nothing back, whatever
+ * its row of dy holds; another one outside [0, vocab) gives a row of NaN and
+ * takes nothing back. */
+typedef struct {
+  const long long* ids;                  /* [tokens] */
+  const void* table; long ldtable;       /* [vocab][width]; Embedding */
+  void* y; long ldy;                     /* [tokens][width]; Embedding */
+  const void* dy; long lddy;             /* [tokens][width]; EmbeddingGrad */
+  void* dtable;                          /* [vocab][width], contiguous */
+  void* workspace; size_t workspaceBytes; /* EmbeddingGrad only */
+  long tokens; int width; int vocab;
+  long long ignore;
+  int type;
+  float scale;
+} EmbeddingArgs;
+int Embedding(const EmbeddingArgs* args, void* stream);
+long EmbeddingGradWorkspace(const EmbeddingArgs* args);
+int EmbeddingGrad(const EmbeddingArgs* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
