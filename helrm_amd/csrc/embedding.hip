@@ -2,13 +2,22 @@
 //
 //   y[i] = scale table[ids[i]],  dtable[v] = scale sum over i with ids[i] = v of dy[i]
 //
-// The gradient has no atomics: ids are sorted (a stable radix sort, so that
-// equal ids keep their order), the sorted ids are cut into pieces of equal
+// The gradient adds nothing atomically: ids are sorted (a stable radix sort, so
+// that equal ids keep their order), the sorted ids are cut into pieces of equal
 // length, and each piece adds the rows of its runs of equal ids in registers.  A
 // run inside a piece is a row of the gradient; what a run has in each of several
-// pieces is added in order by a second launch.  So a frequent id is as parallel
+// pieces is added in order by a second launch.  So a common id is as parallel
 // as any, and a result is the same on every run.  Sums are float32, scaled and
-// rounded once.
+// rounded once.  Rows that no id names are cleared by workgroups beside the
+// sort's, which so costs nothing where the table is large.
+//
+// Bound by memory where rows are long (a copy here: 4.95 TB/s), by launches
+// where they are few.  131,072 ids x 2,048 against 131,072 rows bfloat16: rows
+// 120-186 us (537 MB written, the common ids' rows come from the caches),
+// gradient 245: 94 for 537 MB cleared beside the sort, 132 for the sums (537
+// MB read, 155 written), 20 for the runs over several pieces.  16,384 x 1,024
+// against 65,536 rows: rows 8-10 us, gradient 33 + 13 + 9.  53,248 x 16 float32: 3
+// us, and 24 + 6 + 5 of short launches.
 #include <algorithm>
 #include "embedding.h"
 
@@ -18,18 +27,31 @@ constexpr int BLOCK = 256;
 
 // V neighbouring elements of a row, 16 bytes or one element (rows of any
 // alignment: global accesses of 16 bytes need none).
+typedef unsigned Wide __attribute__((ext_vector_type(4), aligned(2)));
 template <class T, int V> struct Pack { T v[V]; };
 template <class T, int V> __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   Pack<T, V> t;
   __builtin_memcpy(&t, p, sizeof(t));
   return t;
 }
-template <class T, int V> __device__ __forceinline__ void store_pack(T* p, const float (&v)[V]) {
+// ... that are read once
+template <class T, int V> __device__ __forceinline__ Pack<T, V> stream_pack(const T* p) {
+  if constexpr (V == 1) return load_pack<T, V>(p);
+  else return __builtin_bit_cast(Pack<T, V>, __builtin_nontemporal_load((const Wide*)p));
+}
+// STREAM: past the caches
+template <bool STREAM, class T, int V> __device__ __forceinline__ void store_pack(T* p, const float (&v)[V]) {
   Pack<T, V> t;
 #pragma unroll
   for (int e = 0; e < V; e++) t.v[e] = (T)v[e];
-  __builtin_memcpy(p, &t, sizeof(t));
+  if constexpr (V == 1 || !STREAM) __builtin_memcpy(p, &t, sizeof(t));
+  else __builtin_nontemporal_store(__builtin_bit_cast(Wide, t), (Wide*)p);
 }
+// Results larger than the last-level cache go past it, so that it keeps the
+// common ids' rows: 131,072 x 2,048 bfloat16, both directions, 446 us, 480 with
+// ordinary stores; of 16,384 x 1,024, whose reader finds them in the cache, 66 and 63.
+bool streams(long rows, int width, int dtype) { return rows * width * dtype_size(dtype) > 256L << 20; }
+
 // First element of a row's pack: the last one begins earlier, where the width is not a multiple, and holds some elements again.
 template <int V> __device__ __forceinline__ int pack_at(int pack, int width) { return min(pack * V, width - V); }
 
@@ -50,25 +72,31 @@ struct Places {
 
 constexpr int TURNS = 4;   // packs a thread
 
-template <class T, int V>
+template <class A> __device__ __forceinline__ bool inside(const A& a, long long id) { return id >= 0 && id < a.vocab && id != a.ignore; }
+
+template <class T, int V, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void embed_kernel(const EmbedArgs a, int packs, long items, long base) {
   const long first = (base + blockIdx.x) * (BLOCK * TURNS);
   const Places places(first, packs);
+  const int last = (int)min(items - first, (long)BLOCK * TURNS) - 1;   // (the last workgroup's threads do that one again)
+  long row[TURNS], id[TURNS];
+  int at[TURNS];
+  Pack<T, V> t[TURNS];
 #pragma unroll
   for (int u = 0; u < TURNS; u++) {
-    const int j = u * BLOCK + threadIdx.x;
-    if (first + j >= items) break;
-    long row;
-    int pack;
-    places.of(j, row, pack);
-    const int at = pack_at<V>(pack, a.width);
-    const long long id = a.ids[row];
-    const bool in = id >= 0 && id < a.vocab && id != a.ignore;
-    const Pack<T, V> t = load_pack<T, V>((const T*)a.table + (in ? id : 0) * a.ldtable + at);
+    places.of(min(u * BLOCK + (int)threadIdx.x, last), row[u], at[u]);
+    at[u] = pack_at<V>(at[u], a.width);
+    id[u] = a.ids[row[u]];
+  }
+#pragma unroll
+  for (int u = 0; u < TURNS; u++) t[u] = load_pack<T, V>((const T*)a.table + (inside(a, id[u]) ? id[u] : 0) * a.ldtable + at[u]);
+#pragma unroll
+  for (int u = 0; u < TURNS; u++) {
+    const bool in = inside(a, id[u]);
     float v[V];
 #pragma unroll
-    for (int e = 0; e < V; e++) v[e] = in ? (float)t.v[e] * a.scale : id == a.ignore ? 0.0f : NAN;
-    store_pack<T, V>((T*)a.y + row * a.ldy + at, v);
+    for (int e = 0; e < V; e++) v[e] = in ? (float)t[u].v[e] * a.scale : id[u] == a.ignore ? 0.0f : NAN;
+    store_pack<STREAM, T, V>((T*)a.y + row[u] * a.ldy + at[u], v);
   }
 }
 
@@ -76,8 +104,9 @@ __global__ __launch_bounds__(BLOCK) void embed_kernel(const EmbedArgs a, int pac
 // Keys are ids, `vocab` of an id that has no row (sorted last); values are the ids' places.
 
 constexpr int SORT = 1024, WAVES = SORT / 64, MOST_BITS = 9, MOST_DIGITS = 1 << MOST_BITS;
-constexpr int ONE_ITEMS = 8, TILE_ITEMS = 4;
-constexpr long ONE = SORT * ONE_ITEMS, TILE = SORT * TILE_ITEMS;   // the most that one workgroup sorts alone; a workgroup's share otherwise
+constexpr long ONE = SORT * 8;   // the most ids that one workgroup sorts alone
+// Ids a thread of a workgroup's share otherwise: as few as leave 32 tiles, whose counts every workgroup adds up.
+int items_of(long tokens) { return tokens <= 32 * SORT ? 1 : tokens <= 64 * SORT ? 2 : 4; }
 
 struct SortArgs {
   const long long* ids;                     // of the first pass
@@ -89,7 +118,7 @@ struct SortArgs {
 };
 __device__ __forceinline__ unsigned key_of(const SortArgs& a, int i) {
   const long long id = a.ids[i];
-  return id >= 0 && id < a.vocab && id != a.ignore ? (unsigned)id : (unsigned)a.vocab;
+  return inside(a, id) ? (unsigned)id : (unsigned)a.vocab;
 }
 
 // Item j of a lane is number wave * 64 ITEMS + 64 j + lane of the tile; the
@@ -104,19 +133,22 @@ __device__ __forceinline__ void rank_items(const unsigned (&key)[ITEMS], int n, 
   for (int j = 0; j < ITEMS; j++) {
     const bool there = (wave * ITEMS + j) * 64 + lane < n;
     const unsigned digit = key[j] >> shift & ((1u << bits) - 1);
-    unsigned long long same = __ballot(there);
-    for (int b = 0; b < bits; b++) {
-      const bool bit = digit >> b & 1;
+    const unsigned long long all = __ballot(there);
+    unsigned low = (unsigned)all, high = (unsigned)(all >> 32);   // lanes with the same digit
+#pragma unroll
+    for (int b = 0; b < MOST_BITS; b++) {   // (bits that no digit has are equal)
+      const int bit = __builtin_amdgcn_sbfe(digit, b, 1);
       const unsigned long long set = __ballot(bit);
-      same &= bit ? set : ~set;
+      low &= ~((unsigned)set ^ bit);
+      high &= ~((unsigned)(set >> 32) ^ bit);
     }
-    const int before = __popcll(same & ((1ull << lane) - 1));
+    const int before = __builtin_amdgcn_mbcnt_hi(high, __builtin_amdgcn_mbcnt_lo(low, 0));
     rank[j] = 0;
     if (there) rank[j] = counts[wave][digit] + before;
     // (a wave's accesses to LDS are in order; the compiler may not keep a count that another lane writes)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
-    if (there && before == 0) counts[wave][digit] += __popcll(same);
+    if (there && before == 0) counts[wave][digit] += __popc(low) + __popc(high);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_wave_barrier();
   }
@@ -124,12 +156,16 @@ __device__ __forceinline__ void rank_items(const unsigned (&key)[ITEMS], int n, 
 // counts[wave][digit] becomes what the waves before have; the result, of thread `digit`, what all have.
 __device__ __forceinline__ int over_waves(int digits, int (*counts)[MOST_DIGITS]) {
   int sum = 0;
-  if ((int)threadIdx.x < digits)
+  if ((int)threadIdx.x < digits) {
+    int c[WAVES];
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) c[w] = counts[w][threadIdx.x];
+#pragma unroll
     for (int w = 0; w < WAVES; w++) {
-      const int c = counts[w][threadIdx.x];
       counts[w][threadIdx.x] = sum;
-      sum += c;
+      sum += c[w];
     }
+  }
   return sum;
 }
 // The sum of v over the threads before this one.  Two barriers.
@@ -143,66 +179,101 @@ __device__ __forceinline__ int before_me(int v, int* lds) {
   }
   if (lane == 63) lds[wave] = s;
   __syncthreads();
-  for (int w = 0; w < wave; w++) s += lds[w];
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) s += w < wave ? lds[w] : 0;
   __syncthreads();
   return s - v;
 }
 
-// The whole sort of up to ONE ids.
-__global__ __launch_bounds__(SORT) void sort_one_kernel(const SortArgs a) {
-  __shared__ int counts[WAVES][MOST_DIGITS], start[MOST_DIGITS], sums[WAVES];
-  __shared__ unsigned keys[ONE], ats[ONE];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  unsigned key[ONE_ITEMS], at[ONE_ITEMS];
-  int rank[ONE_ITEMS];
+// What a launch of the sort does beside it: workgroups behind those of the sort
+// clear a share of the table's gradient, which takes longer than the sort where
+// the table is large.
+struct Clear {
+  char* table;
+  long first, last;   // places of 16 bytes, or of 2 where a row has less than 16; the last ones of a row overlap
+  int packs, groups;
+  long row;           // bytes of a row
+  bool stream;
+};
+template <int BYTES> __device__ __forceinline__ void clear_places(const Clear& c, int group) {
+  constexpr int EACH = 4;
+  for (long first = c.first + (long)group * SORT * EACH; first < c.last; first += (long)c.groups * SORT * EACH) {
+    const Places places(first, c.packs);
 #pragma unroll
-  for (int j = 0; j < ONE_ITEMS; j++) {
-    const int i = (wave * ONE_ITEMS + j) * 64 + lane;
+    for (int u = 0; u < EACH; u++) {
+      const int j = u * SORT + threadIdx.x;
+      if (first + j >= c.last) continue;
+      long r;
+      int pack;
+      places.of(j, r, pack);
+      char* p = c.table + r * c.row;
+      if constexpr (BYTES == 2) *(uint16_t*)(p + pack * 2) = 0;
+      else {
+        Wide* to = (Wide*)(p + min((long)pack * 16, c.row - 16));
+        if (c.stream) __builtin_nontemporal_store(Wide{0, 0, 0, 0}, to);
+        else *to = Wide{0, 0, 0, 0};
+      }
+    }
+  }
+}
+__device__ __forceinline__ void clear_share(const Clear& c, int group) {
+  if (c.row >= 16) clear_places<16>(c, group);
+  else clear_places<2>(c, group);
+}
+
+// The whole sort of up to SORT * ITEMS ids.
+template <int ITEMS>
+__global__ __launch_bounds__(SORT) void sort_one_kernel(const SortArgs a, const Clear c) {
+  __shared__ int counts[WAVES][MOST_DIGITS], start[MOST_DIGITS], sums[WAVES];
+  __shared__ unsigned keys[SORT * ITEMS], ats[SORT * ITEMS];
+  if (blockIdx.x) return clear_share(c, blockIdx.x - 1);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  unsigned key[ITEMS], at[ITEMS];
+  int rank[ITEMS];
+#pragma unroll
+  for (int j = 0; j < ITEMS; j++) {
+    const int i = (wave * ITEMS + j) * 64 + lane;
     key[j] = i < a.n ? key_of(a, i) : 0;
     at[j] = i;
   }
   for (int pass = 0; pass < a.passes; pass++) {
     const int shift = pass * a.bits;
-    rank_items<ONE_ITEMS>(key, a.n, shift, a.bits, rank, counts);
+    rank_items<ITEMS>(key, a.n, shift, a.bits, rank, counts);
     __syncthreads();
     const int base = before_me(over_waves(1 << a.bits, counts), sums);
     if ((int)threadIdx.x < 1 << a.bits) start[threadIdx.x] = base;
     __syncthreads();
+    const bool last = pass == a.passes - 1;
 #pragma unroll
-    for (int j = 0; j < ONE_ITEMS; j++)
-      if ((wave * ONE_ITEMS + j) * 64 + lane < a.n) {
+    for (int j = 0; j < ITEMS; j++)
+      if ((wave * ITEMS + j) * 64 + lane < a.n) {
         const unsigned digit = key[j] >> shift & ((1u << a.bits) - 1);
         const int to = start[digit] + counts[wave][digit] + rank[j];
-        keys[to] = key[j];
-        ats[to] = at[j];
+        (last ? a.to : keys)[to] = key[j];
+        (last ? a.to_at : ats)[to] = at[j];
       }
+    if (last) break;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < ONE_ITEMS; j++) {
-      const int i = (wave * ONE_ITEMS + j) * 64 + lane;
+    for (int j = 0; j < ITEMS; j++) {
+      const int i = (wave * ITEMS + j) * 64 + lane;
       key[j] = i < a.n ? keys[i] : 0;
       at[j] = i < a.n ? ats[i] : 0;
     }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int j = 0; j < ONE_ITEMS; j++) {
-    const int i = (wave * ONE_ITEMS + j) * 64 + lane;
-    if (i < a.n) {
-      a.to[i] = key[j];
-      a.to_at[i] = at[j];
-    }
+    // (the next pass writes them after three barriers)
   }
 }
 
 // One pass over many tiles: how often each digit is in a tile, ...
-__global__ __launch_bounds__(SORT) void count_kernel(const SortArgs a) {
+template <int ITEMS>
+__global__ __launch_bounds__(SORT) void count_kernel(const SortArgs a, const Clear c) {
   __shared__ int counts[MOST_DIGITS];
-  const int digits = 1 << a.bits, first = blockIdx.x * (int)TILE;
+  if ((int)blockIdx.x >= a.tiles) return clear_share(c, blockIdx.x - a.tiles);
+  const int digits = 1 << a.bits, first = blockIdx.x * SORT * ITEMS;
   for (int k = threadIdx.x; k < digits; k += SORT) counts[k] = 0;
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < TILE_ITEMS; j++) {
+  for (int j = 0; j < ITEMS; j++) {
     const int i = first + j * SORT + threadIdx.x;
     if (i < a.n) atomicAdd(&counts[(a.shift ? a.from[i] : key_of(a, i)) >> a.shift & (digits - 1)], 1);
   }
@@ -234,43 +305,53 @@ __global__ __launch_bounds__(SORT) void scan_kernel(const SortArgs a) {
   if (wave == WAVES - 1) a.counts[(long)a.tiles * digits + digit] = sum;
 }
 // ... and every item to its place.
-__global__ __launch_bounds__(SORT) void scatter_kernel(const SortArgs a) {
-  __shared__ int counts[WAVES][MOST_DIGITS], start[MOST_DIGITS], sums[WAVES];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, digits = 1 << a.bits, tile = blockIdx.x, first = tile * (int)TILE;
-  unsigned key[TILE_ITEMS], at[TILE_ITEMS];
-  int rank[TILE_ITEMS];
-  const int n = min((int)TILE, a.n - first);
+template <int ITEMS>
+__global__ __launch_bounds__(SORT) void scatter_kernel(const SortArgs a, const Clear c) {
+  __shared__ int counts[WAVES][MOST_DIGITS], start[MOST_DIGITS], sums[WAVES], others[2][MOST_DIGITS];
+  if ((int)blockIdx.x >= a.tiles) return clear_share(c, blockIdx.x - a.tiles);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, digits = 1 << a.bits, tile = blockIdx.x, first = tile * SORT * ITEMS;
+  unsigned key[ITEMS], at[ITEMS];
+  int rank[ITEMS];
+  const int n = min(SORT * ITEMS, a.n - first);
 #pragma unroll
-  for (int j = 0; j < TILE_ITEMS; j++) {
-    const int i = (wave * TILE_ITEMS + j) * 64 + lane;
+  for (int j = 0; j < ITEMS; j++) {
+    const int i = (wave * ITEMS + j) * 64 + lane;
     key[j] = i >= n ? 0 : a.shift ? a.from[first + i] : key_of(a, first + i);
     at[j] = i >= n ? 0 : a.shift ? a.from_at[first + i] : first + i;
   }
-  rank_items<TILE_ITEMS>(key, n, a.shift, a.bits, rank, counts);
+  // of thread t's digit t % 512: how many there are in half of the tiles, and in those of them before this one
+  const int digit = threadIdx.x & (MOST_DIGITS - 1), half = threadIdx.x / MOST_DIGITS;
   int before = 0, all = 0;
-  if ((int)threadIdx.x < digits) {
+  if (digit < digits) {
     if (a.tiles > FEW_TILES) {
-      before = a.counts[(long)tile * digits + threadIdx.x];
-      all = a.counts[(long)a.tiles * digits + threadIdx.x];
+      if (!half) {
+        before = a.counts[(long)tile * digits + digit];
+        all = a.counts[(long)a.tiles * digits + digit];
+      }
     } else {
 #pragma unroll 8
-      for (int t = 0; t < a.tiles; t++) {
-        const int c = a.counts[t * digits + threadIdx.x];
-        all += c;
-        if (t < tile) before += c;
+      for (int t = half; t < a.tiles; t += 2) {
+        const int k = a.counts[t * digits + digit];
+        all += k;
+        if (t < tile) before += k;
       }
     }
   }
+  if (half) {
+    others[0][digit] = before;
+    others[1][digit] = all;
+  }
+  rank_items<ITEMS>(key, n, a.shift, a.bits, rank, counts);
   __syncthreads();
   over_waves(digits, counts);
-  const int base = before_me(all, sums);
-  if ((int)threadIdx.x < digits) start[threadIdx.x] = base + before;
+  const int base = before_me(half ? 0 : all + others[1][digit], sums);
+  if (!half) start[digit] = base + before + others[0][digit];
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < TILE_ITEMS; j++)
-    if ((wave * TILE_ITEMS + j) * 64 + lane < n) {
-      const unsigned digit = key[j] >> a.shift & (digits - 1);
-      const int to = start[digit] + counts[wave][digit] + rank[j];
+  for (int j = 0; j < ITEMS; j++)
+    if ((wave * ITEMS + j) * 64 + lane < n) {
+      const unsigned d = key[j] >> a.shift & (digits - 1);
+      const int to = start[d] + counts[wave][d] + rank[j];
       a.to[to] = key[j];
       a.to_at[to] = at[j];
     }
@@ -286,6 +367,7 @@ struct SumArgs {
   int n, vocab, width, packs;
   int piece, pieces;           // length and number
   int lanes, blocks;           // of a team, which adds `lanes` packs of the rows of a piece; teams beside one another
+  int across;                  // lanes of a team that joins
   float scale;
 };
 
@@ -315,7 +397,7 @@ __global__ __launch_bounds__(BLOCK) void sum_kernel(const SumArgs a, long base) 
       float v[V];
 #pragma unroll
       for (int e = 0; e < V; e++) v[e] = sum[e] * a.scale;
-      store_pack<T, V>((T*)a.dtable + (long)cur * a.width + at, v);
+      store_pack<false, T, V>((T*)a.dtable + (long)cur * a.width + at, v);
     }
   };
   for (int i = from; i < to; i += AHEAD) {
@@ -325,7 +407,7 @@ __global__ __launch_bounds__(BLOCK) void sum_kernel(const SumArgs a, long base) 
     for (int u = 0; u < AHEAD; u++) {
       const int k = min(i + u, to - 1);
       key[u] = a.keys[k];
-      t[u] = load_pack<T, V>((const T*)a.dy + a.ats[k] * a.lddy + at);
+      t[u] = stream_pack<T, V>((const T*)a.dy + a.ats[k] * a.lddy + at);
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; u++) {
@@ -346,62 +428,58 @@ __global__ __launch_bounds__(BLOCK) void sum_kernel(const SumArgs a, long base) 
   else done();
 }
 
-// The runs that go on over pieces, each by the workgroups of the piece that it begins in: a column block each.
+// The runs that go on over pieces, a workgroup for the piece that one begins in:
+// most pieces have none, a common id's has thousands of sums behind it.
+constexpr int JOIN = 1024;   // the most threads
 template <class T, int V>
-__global__ __launch_bounds__(BLOCK) void join_kernel(const SumArgs a, long base) {
-  __shared__ float lds[BLOCK * V];
-  const unsigned id = (unsigned)(base + blockIdx.x), piece = id / a.blocks;
-  const int from = (int)piece * a.piece, to = from + a.piece;
+__global__ __launch_bounds__(JOIN) void join_kernel(const SumArgs a, long base) {
+  extern __shared__ float lds[];   // [threads][V]
+  const int piece = (int)(base + blockIdx.x), from = piece * a.piece, to = from + a.piece;
   if (to >= a.n) return;
   const unsigned key = a.keys[to];
   if (key >= (unsigned)a.vocab || a.keys[to - 1] != key || (from > 0 && a.keys[from - 1] == key)) return;
   // pieces that begin with the run: those behind this one, as long as there are any
   int more = 0;
-  for (int q = (int)piece + 1;; q += BLOCK) {
+  for (int q = piece + 1;; q += blockDim.x) {
     const int mine = q + threadIdx.x;
     const int n = __syncthreads_count(mine < a.pieces && a.keys[(long)mine * a.piece] == key);
     more += n;
-    if (n < BLOCK) break;
+    if (n < (int)blockDim.x) break;
   }
-  const int lane = threadIdx.x & (a.lanes - 1), team = threadIdx.x / a.lanes, teams = BLOCK / a.lanes;
-  const int pack = (int)(id - piece * a.blocks) * a.lanes + lane, at = pack_at<V>(pack, a.width);
-  float sum[V] = {};
-  if (pack < a.packs)
-#pragma unroll 4
-    for (int i = team; i <= more; i += teams) {
-      float v[V];
-      __builtin_memcpy(v, a.partial + (((long)piece + i) * 2 + (i == 0)) * a.width + at, sizeof(v));
+  const int lane = threadIdx.x & (a.across - 1), team = threadIdx.x / a.across, teams = blockDim.x / a.across;
+  for (int first = 0; first < a.packs; first += a.across) {
+    const int pack = first + lane, at = pack_at<V>(pack, a.width);
+    float sum[V] = {};
+    if (pack < a.packs)
+#pragma unroll 8
+      for (int i = team; i <= more; i += teams) {
+        float v[V];
+        __builtin_memcpy(v, a.partial + (((long)piece + i) * 2 + (i == 0)) * a.width + at, sizeof(v));
 #pragma unroll
-      for (int e = 0; e < V; e++) sum[e] += v[e];
+        for (int e = 0; e < V; e++) sum[e] += v[e];
+      }
+    if (teams > 1) {
+      if (first) __syncthreads();
+#pragma unroll
+      for (int e = 0; e < V; e++) lds[threadIdx.x * V + e] = sum[e];
+      __syncthreads();
     }
+    if (team || pack >= a.packs) continue;
+    for (int t = 1; t < min(teams, more + 1); t++)
 #pragma unroll
-  for (int e = 0; e < V; e++) lds[threadIdx.x * V + e] = sum[e];
-  __syncthreads();
-  if (team || pack >= a.packs) return;
-  for (int t = 1; t < min(teams, more + 1); t++)
+      for (int e = 0; e < V; e++) sum[e] += lds[(t * a.across + lane) * V + e];
 #pragma unroll
-    for (int e = 0; e < V; e++) sum[e] += lds[(t * a.lanes + lane) * V + e];
-#pragma unroll
-  for (int e = 0; e < V; e++) sum[e] *= a.scale;
-  store_pack<T, V>((T*)a.dtable + (long)key * a.width + at, sum);
-}
-
-template <class T, int V>
-__global__ __launch_bounds__(BLOCK) void clear_kernel(T* table, int width, int packs, long items, long base) {
-  const long first = (base + blockIdx.x) * (BLOCK * TURNS);
-  const Places places(first, packs);
-#pragma unroll
-  for (int u = 0; u < TURNS; u++) {
-    const int j = u * BLOCK + threadIdx.x;
-    if (first + j >= items) break;
-    long row;
-    int pack;
-    places.of(j, row, pack);
-    const float v[V] = {};
-    store_pack<T, V>(table + row * width + pack_at<V>(pack, width), v);
+    for (int e = 0; e < V; e++) sum[e] *= a.scale;
+    store_pack<false, T, V>((T*)a.dtable + (long)key * a.width + at, sum);
   }
 }
 
+template <class F> void with_items(int n, F&& f) {
+  if (n <= 1) f(std::integral_constant<int, 1>{});
+  else if (n <= 2) f(std::integral_constant<int, 2>{});
+  else if (n <= 4) f(std::integral_constant<int, 4>{});
+  else f(std::integral_constant<int, 8>{});
+}
 // f(T{}, V): packs of 16 bytes, or single elements of rows that have no 16 bytes
 template <class F> void with_packs(int dtype, int width, F&& f) {
   clr::with_type(dtype, [&](auto t) {
@@ -422,14 +500,14 @@ struct Space {
   float* partial;
   size_t bytes = 0;
 };
-// Ids of a piece: as few as leave 2,048 teams, of 16 to 64.
+// Ids of a piece: as many as leave 2,048 waves, of 16 to 64.
 int piece_of(long tokens, int blocks, int lanes) {
-  const long teams = tokens * blocks * lanes / 64 / 2048;
-  return teams >= 64 ? 64 : teams >= 32 ? 32 : 16;
+  const long waves = tokens * blocks * lanes / 64;
+  return waves >= 64 * 2048 ? 64 : waves >= 32 * 2048 ? 32 : 16;
 }
-int lanes_of(int packs) {
+int lanes_of(int packs, int most) {
   int n = 1;
-  while (n < 64 && n < packs) n *= 2;
+  while (n < most && n < packs) n *= 2;
   return n;
 }
 Space space_of(char* base, long tokens, int width, int vocab, int dtype) {
@@ -439,13 +517,13 @@ Space space_of(char* base, long tokens, int width, int vocab, int dtype) {
     s.bytes += clr::align256(n);
     return p;
   };
-  const int packs = packs_of(width, dtype), lanes = lanes_of(packs), blocks = (int)clr::ceil_div(packs, lanes);
+  const int packs = packs_of(width, dtype), lanes = lanes_of(packs, 64), blocks = (int)clr::ceil_div(packs, lanes);
   const bool one = tokens <= ONE;
   for (int i = 0; i < 2; i++) {
     s.keys[i] = i && one ? s.keys[0] : (unsigned*)take(tokens * 4);
     s.ats[i] = i && one ? s.ats[0] : (unsigned*)take(tokens * 4);
   }
-  s.counts = one ? nullptr : (int*)take((clr::ceil_div(tokens, TILE) + 1) * MOST_DIGITS * 4);
+  s.counts = one ? nullptr : (int*)take((clr::ceil_div(tokens, SORT * items_of(tokens)) + 1) * MOST_DIGITS * 4);
   s.partial = (float*)take(clr::ceil_div(tokens, piece_of(tokens, blocks, lanes)) * 2 * width * sizeof(float));
   return s;
 }
@@ -457,7 +535,12 @@ void embedding_launch(const EmbedArgs& a, hipStream_t st) {
   const long items = a.tokens * packs;
   with_packs(a.dtype, a.width, [&](auto t, auto v) {
     clr::in_launches(clr::ceil_div(items, BLOCK * TURNS), BLOCK,
-                     [&](long base, unsigned n) { embed_kernel<decltype(t), decltype(v)::value><<<n, BLOCK, 0, st>>>(a, packs, items, base); });
+                     [&](long base, unsigned n) {
+                       using T = decltype(t);
+                       constexpr int V = decltype(v)::value;
+                       if (streams(a.tokens, a.width, a.dtype)) embed_kernel<T, V, true><<<n, BLOCK, 0, st>>>(a, packs, items, base);
+                       else embed_kernel<T, V, false><<<n, BLOCK, 0, st>>>(a, packs, items, base);
+                     });
   });
 }
 
@@ -465,15 +548,6 @@ size_t embedding_grad_workspace(long tokens, int width, int vocab, int dtype) { 
 
 void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
   const Space space = space_of((char*)a.workspace, a.tokens, a.width, a.vocab, a.dtype);
-  const int packs = packs_of(a.width, a.dtype);
-  const long items = (long)a.vocab * packs;
-  with_packs(a.dtype, a.width, [&](auto t, auto v) {
-    clr::in_launches(clr::ceil_div(items, BLOCK * TURNS), BLOCK, [&](long base, unsigned n) {
-      using T = decltype(t);
-      clear_kernel<T, decltype(v)::value><<<n, BLOCK, 0, st>>>((T*)a.dtable, a.width, packs, items, base);
-    });
-  });
-  if (!a.tokens) return;
   SortArgs s{};
   s.ids = a.ids;
   s.ignore = a.ignore;
@@ -483,13 +557,29 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
   while (a.vocab >> bits) bits++;
   s.passes = (int)clr::ceil_div(bits, MOST_BITS);
   s.bits = (int)clr::ceil_div(bits, s.passes);
+  const bool one = a.tokens <= ONE;
+  const int items = items_of(a.tokens);
+  if (!one) s.tiles = (int)clr::ceil_div(a.tokens, SORT * items);
+  // the table's places, shared out by how long the launches take: a scatter twice as long as a count
+  Clear c{};
+  c.table = (char*)a.dtable;
+  c.row = (long)a.width * dtype_size(a.dtype);
+  c.packs = (int)(c.row >= 16 ? clr::ceil_div(c.row, 16) : c.row / 2);
+  c.stream = streams(a.vocab, a.width, a.dtype);
+  const long places = (long)a.vocab * c.packs;
+  auto clearing = [&](int part, int parts, int of) {
+    c.first = places * part / of;
+    c.last = places * (part + parts) / of;
+    c.groups = (int)std::min<long>(clr::ceil_div(c.last - c.first, SORT * 4), 1024);
+    return c.groups;
+  };
   int out = 0;
-  if (a.tokens <= ONE) {
+  if (one) {
     s.to = space.keys[0];
     s.to_at = space.ats[0];
-    sort_one_kernel<<<1, SORT, 0, st>>>(s);
+    const unsigned groups = 1 + clearing(0, 1, 1);
+    with_items((int)clr::ceil_div(a.tokens, SORT), [&](auto n) { sort_one_kernel<decltype(n)::value><<<groups, SORT, 0, st>>>(s, c); });
   } else {
-    s.tiles = (int)clr::ceil_div(a.tokens, TILE);
     s.counts = space.counts;
     for (int pass = 0; pass < s.passes; pass++) {
       out = pass & 1;
@@ -498,11 +588,15 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
       s.from_at = space.ats[1 - out];
       s.to = space.keys[out];
       s.to_at = space.ats[out];
-      count_kernel<<<s.tiles, SORT, 0, st>>>(s);
+      unsigned groups = s.tiles + clearing(3 * pass, 1, 3 * s.passes);
+      with_items(items, [&](auto n) { count_kernel<decltype(n)::value><<<groups, SORT, 0, st>>>(s, c); });
       if (s.tiles > FEW_TILES) scan_kernel<<<(unsigned)clr::ceil_div(1 << s.bits, 64), SORT, 0, st>>>(s);
-      scatter_kernel<<<s.tiles, SORT, 0, st>>>(s);
+      groups = s.tiles + clearing(3 * pass + 1, 2, 3 * s.passes);
+      with_items(items, [&](auto n) { scatter_kernel<decltype(n)::value><<<groups, SORT, 0, st>>>(s, c); });
     }
   }
+  if (!a.tokens) return;
+  const int packs = packs_of(a.width, a.dtype);
   SumArgs m{};
   m.keys = space.keys[out];
   m.ats = space.ats[out];
@@ -510,7 +604,9 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
   m.dtable = a.dtable;
   m.partial = space.partial;
   m.n = (int)a.tokens; m.vocab = a.vocab; m.width = a.width; m.packs = packs;
-  m.lanes = lanes_of(packs);
+  m.lanes = lanes_of(packs, 64);
+  m.across = lanes_of(packs, JOIN);
+  const int threads = std::min(std::max(4 * m.across, 256), JOIN);
   m.blocks = (int)clr::ceil_div(packs, m.lanes);
   m.piece = piece_of(a.tokens, m.blocks, m.lanes);
   m.pieces = (int)clr::ceil_div(a.tokens, m.piece);
@@ -524,6 +620,6 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
       else sum_kernel<T, V, false><<<n, BLOCK, 0, st>>>(m, base);
     });
     if (m.pieces > 1)
-      clr::in_launches(teams, BLOCK, [&](long base, unsigned n) { join_kernel<T, V><<<n, BLOCK, 0, st>>>(m, base); });
+      clr::in_launches(m.pieces, threads, [&](long base, unsigned n) { join_kernel<T, V><<<n, threads, threads * V * sizeof(float), st>>>(m, base); });
   });
 }
