@@ -70,6 +70,16 @@ class LossTotalArgs(ctypes.Structure):
                 ("workspace", ctypes.c_void_p), ("workspaceBytes", ctypes.c_size_t), ("rows", ctypes.c_long), ("ignore", ctypes.c_longlong)]
 
 
+class DistillationArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("ldx", ctypes.c_long), ("table", ctypes.c_void_p), ("ldtable", ctypes.c_long),
+                ("ids", ctypes.c_void_p), ("logits", ctypes.c_void_p), ("loss", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("kept", ctypes.c_void_p), ("scores", ctypes.c_void_p), ("probs", ctypes.c_void_p),
+                ("dloss", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("lddx", ctypes.c_long), ("dtable", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspaceBytes", ctypes.c_size_t),
+                ("rows", ctypes.c_long), ("width", ctypes.c_int), ("vocab", ctypes.c_int), ("top", ctypes.c_int),
+                ("type", ctypes.c_int), ("teacherType", ctypes.c_int), ("ignore", ctypes.c_longlong), ("temperature", ctypes.c_float)]
+
+
 class EmbeddingArgs(ctypes.Structure):
     _fields_ = [("ids", ctypes.c_void_p), ("table", ctypes.c_void_p), ("ldtable", ctypes.c_long), ("y", ctypes.c_void_p),
                 ("ldy", ctypes.c_long), ("dy", ctypes.c_void_p), ("lddy", ctypes.c_long), ("dtable", ctypes.c_void_p),
@@ -338,6 +348,10 @@ _SIGNATURES = {
     "CrossEntropyGrad": ([_c.c_void_p, _c.c_void_p], _I),
     "LossTotalWorkspace": ([_c.c_void_p], _c.c_long),
     "LossTotal": ([_c.c_void_p, _c.c_void_p], _I),
+    "DistillationWorkspace": ([_c.c_void_p], _c.c_long),
+    "Distillation": ([_c.c_void_p, _c.c_void_p], _I),
+    "DistillationGradWorkspace": ([_c.c_void_p], _c.c_long),
+    "DistillationGrad": ([_c.c_void_p, _c.c_void_p], _I),
     "Embedding": ([_c.c_void_p, _c.c_void_p], _I),
     "EmbeddingGradWorkspace": ([_c.c_void_p], _c.c_long),
     "EmbeddingGrad": ([_c.c_void_p, _c.c_void_p], _I),

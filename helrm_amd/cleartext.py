@@ -7,6 +7,7 @@ that training and of scoring beside it, on the same card:
     layer_norm      y = (x - mean) / sqrt(var + eps) * weight + bias
     gated_mlp       y = (act(x gate^T) * (x up^T)) down^T
     cross_entropy   log sum_v exp <x, table[v]> - <x, table[target]>
+    distillation    the divergence of a teacher's top logits from the softmax of <x, table[v]>
     embedding       y[i] = scale * table[ids[i]]
 
 Each has a `_forward` and a `_backward` call, which a training loop of one's
@@ -29,7 +30,7 @@ import ctypes
 import torch
 from torch.autograd import forward_ad
 
-from .backend import CrossEntropyArgs, EmbeddingArgs, GatedMLPArgs, HipError, LayerNormArgs, LossTotalArgs, load_library
+from .backend import CrossEntropyArgs, DistillationArgs, EmbeddingArgs, GatedMLPArgs, HipError, LayerNormArgs, LossTotalArgs, load_library
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {"silu": 0, "gelu": 1}
@@ -52,8 +53,8 @@ def _library():
         raise HipError("two HIP runtimes in one process (" + ", ".join(sorted(runtimes))
                        + "): import torch before the library is loaded")
     calls = {}
-    for name in ("LayerNorm", "LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad", "LossTotal", "Embedding",
-                 "EmbeddingGrad"):
+    for name in ("LayerNorm", "LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad", "LossTotal",
+                 "Distillation", "DistillationGrad", "Embedding", "EmbeddingGrad"):
         call, size = getattr(lib, name), getattr(lib, name + "Workspace", None)
         call.argtypes, call.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
         if size is not None:
@@ -428,6 +429,110 @@ def cross_entropy(x, table, target, ignore_index=-100, reduction="mean"):
         return losses
     target = target if reduction == "mean" else None
     return _Total.apply(losses, target, ignore_index) if grad else _total(losses, target, ignore_index)[0]
+
+
+# ---- distillation from a teacher's top logits ---------------------------------------------
+
+
+def _teach_tensors(x, table, ids, temperature, ignore_index):
+    _need(table.dim() == 2 and table.shape[0] >= 1 and table.shape[1] >= 1, "table: not a matrix with elements")
+    _sized(table.shape[0], "table: rows")
+    _sized(table.shape[1], "table: the last dimension")
+    _need(-(1 << 63) <= ignore_index < 1 << 63, "ignore_index: not an int64")
+    _need(2.0 ** -60 <= temperature <= 2.0 ** 60, f"temperature {temperature}: not positive, or out of range")
+    _need(ids.dim() >= 1 and 1 <= ids.shape[-1] <= 1024, f"ids: {list(ids.shape)}, not [..., top] with top from 1 to 1024")
+    _same_order(ids.shape[:-1], x.shape[:-1], "ids")
+    x2 = _rows(x, table.shape[1], "x")
+    if ids.dtype != torch.int64 or ids.device != x.device:
+        raise ValueError(f"ids: {ids.dtype} on {ids.device}, not {torch.int64} on {x.device}")
+    ids = ids.reshape(-1, ids.shape[-1]).contiguous()
+    if ids.shape[0] != x2.shape[0]:
+        raise ValueError(f"ids: {ids.shape[0]} rows, not {x2.shape[0]}")
+    return x2, _rows(table, table.shape[1], "table", x), ids
+
+
+def distillation_forward(x, table, ids, logits, temperature=1.0, ignore_index=-100):
+    """(losses, lse, saved), losses and lse float32 for each row: temperature^2 times the divergence of the teacher's softmax of
+    logits / temperature over `ids` [..., top] from the softmax of x's products with all of the table's rows / temperature, and the
+    logarithm of the latter's sum; saved is what the gradient needs.  An id that is `ignore_index` or has a logit of -inf is no
+    entry, one that is there twice has both probabilities.  Rows without entries have 0 for both; an id outside the table gives
+    NaN.  x's logits are never in memory."""
+    x2, table, ids2 = _teach_tensors(x, table, ids, temperature, ignore_index)
+    rows, top = ids2.shape
+    if logits.shape != ids.shape:
+        raise ValueError(f"logits: {list(logits.shape)}, not {list(ids.shape)}")
+    if logits.dtype not in (x.dtype, torch.float32) or logits.device != x.device:
+        raise ValueError(f"logits: {logits.dtype} on {logits.device}, neither {x.dtype} nor float32 on {x.device}")
+    if forward_ad._current_level >= 0:
+        _no_tangent(logits, "logits")
+    logits = logits.reshape(rows, top).contiguous()
+    losses = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    lse = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    kept = torch.empty(rows, dtype=torch.int64, device=x.device)
+    held = torch.empty((2, rows, top), dtype=torch.float32, device=x.device)
+    _call("Distillation", DistillationArgs(
+        x=x2.data_ptr(), ldx=_ld(x2), table=table.data_ptr(), ldtable=_ld(table), ids=ids2.data_ptr(), logits=logits.data_ptr(),
+        loss=losses.data_ptr(), lse=lse.data_ptr(), kept=kept.data_ptr(), scores=held.data_ptr(), probs=held.data_ptr() + 2 * held.numel(),
+        rows=rows, width=table.shape[1], vocab=table.shape[0], top=top, type=_TYPES[x.dtype], teacherType=_TYPES[logits.dtype],
+        ignore=ignore_index, temperature=temperature), x.device)
+    return losses, lse, (kept, held)
+
+
+def distillation_backward(grad, x, table, ids, lse, saved, temperature=1.0, ignore_index=-100):
+    """(dx, dtable) for the gradient `grad` of the losses (float32); lse and saved as the forward call gave them.  The logits are
+    computed again, a piece of the table at a time."""
+    x2, table, ids = _teach_tensors(x, table, ids, temperature, ignore_index)
+    rows, width = x2.shape
+    _same_order(grad.shape, x.shape[:-1], "grad")
+    _same_order(lse.shape, x.shape[:-1], "lse")
+    grad = _vector(grad.reshape(-1), rows, "grad", torch.float32, x.device)
+    lse = _vector(lse.reshape(-1), rows, "lse", torch.float32, x.device)
+    kept, held = saved
+    _need(tuple(kept.shape) == (rows,) and kept.dtype == torch.int64 and kept.device == x.device and kept.is_contiguous()
+          and tuple(held.shape) == (2, *ids.shape) and held.dtype == torch.float32 and held.device == x.device and held.is_contiguous(),
+          "saved: not what the forward call returned")
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dtable = torch.empty(table.shape, dtype=x.dtype, device=x.device)
+    _call("DistillationGrad", DistillationArgs(
+        x=x2.data_ptr(), ldx=_ld(x2), table=table.data_ptr(), ldtable=_ld(table), ids=ids.data_ptr(), lse=lse.data_ptr(), kept=kept.data_ptr(),
+        scores=held.data_ptr(), probs=held.data_ptr() + 2 * held.numel(), dloss=grad.data_ptr(), dx=dx.data_ptr(), lddx=width,
+        dtable=dtable.data_ptr(), rows=rows, width=width, vocab=table.shape[0], top=ids.shape[1], type=_TYPES[x.dtype],
+        teacherType=_TYPES[x.dtype], ignore=ignore_index, temperature=temperature), x.device)
+    return dx, dtable
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, table, ids, logits, temperature, ignore_index):
+        losses, lse, (kept, held) = distillation_forward(x, table, ids, logits, temperature, ignore_index)
+        ctx.save_for_backward(x, table, ids, lse, kept, held)
+        ctx.rest = temperature, ignore_index
+        ctx.mark_non_differentiable(kept)
+        return losses, kept
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):
+        x, table, ids, lse, kept, held = ctx.saved_tensors
+        return distillation_backward(grad, x, table, ids, lse, (kept, held), *ctx.rest) + (None, None, None, None)
+
+
+def distillation(x, table, ids, logits, temperature=1.0, ignore_index=-100, reduction="mean"):
+    """Divergence of a teacher from x [..., width] against table [vocab, width], of the teacher's top logits [..., top] and their
+    ids, both softmaxes at `temperature` and the loss times its square (distillation_forward has the formula): the mean over the
+    rows that have a teacher (0 where none has one), their "sum", or "none" for a loss a row.  The teacher's logits have no
+    gradient here."""
+    _need(reduction in ("mean", "sum", "none"), f"reduction {reduction!r}: neither mean, sum nor none")
+    _need(not _wants_grad(logits), "logits: require a gradient, and are the teacher's; detach them")
+    grad = _wants_grad(x, table)
+    if grad:
+        losses, kept = _Distillation.apply(x, table, ids, logits, temperature, ignore_index)
+    else:
+        losses, _, (kept, _) = distillation_forward(x, table, ids, logits, temperature, ignore_index)
+    if reduction == "none":
+        return losses
+    kept = kept if reduction == "mean" else None
+    return _Total.apply(losses, kept, 0) if grad else _total(losses, kept, 0)[0]
 
 
 # ---- rows of a table for ids -----------------------------------------------------------------

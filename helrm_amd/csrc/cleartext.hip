@@ -7,6 +7,7 @@
 #include "norm.h"
 #include "products.h"
 #include "skinny.h"
+#include "teacher.h"
 #include "../../include/helrm_hip.h"
 
 namespace {
@@ -322,16 +323,17 @@ size_t ce_forward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
 // there are 1,024 of them.
 constexpr long PIECE_BYTES = 256L << 20;
 static_assert(PIECE_BYTES < 1L << 31 && 256 * 1024 * 2 < 1L << 31, "the rows of a tile of dl are within 31-bit offsets, whatever their number and width");
-int piece_rows(const CrossEntropyArgs* a) {
-  const long most = PIECE_BYTES / (std::max<long>(a->rows, 1) * (a->type == DT_F32 ? 6 : few_rows(a->rows, a->type) ? 4 : 2));
-  return (int)std::min<long>(up8(a->vocab), std::max<long>(1024, most / 1024 * 1024));
+int piece_rows(long rows, int vocab, int type) {
+  const long most = PIECE_BYTES / (std::max<long>(rows, 1) * (type == DT_F32 ? 6 : few_rows(rows, type) ? 4 : 2));
+  return (int)std::min<long>(up8(vocab), std::max<long>(1024, most / 1024 * 1024));
 }
 
-size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
+// The gradients of a loss against a table, dx = dl table and dtable = dl^T x, from `logits_grad`, which leaves dl for
+// some of the table's rows.  The arguments' targets and gradients, of which `r` says which.
+template <class Args, class F> size_t table_backward(const Args* a, RowsArgs r, bool count, hipStream_t st, F&& logits_grad) {
   Arena m{count ? nullptr : (char*)a->workspace};
   const long n = a->rows, D = a->width;
-  const int piece = piece_rows(a);
-  RowsArgs r{a->target, a->dloss, n, a->ignore, a->vocab};
+  const int piece = piece_rows(a->rows, a->vocab, a->type);
   r.rows = m.take<int>(n); r.tgt = m.take<int>(n); r.place = m.take<int>(n); r.count = m.take<int>(1);
   float* scale = m.take<float>(1);
   if (a->type == DT_F16) r.scale = scale;
@@ -359,7 +361,7 @@ size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
     add_pairs(p, x, rows);
     p.c = (void*)dl.p; p.ldc = dl.ld; p.hpart = dl.part;
     p.n0 = (int)v0; p.target = r.tgt; p.lse = r.lse_kept; p.grad = r.grad_kept; p.scale = r.scale;
-    product_softmax_grad(p, st);
+    logits_grad(p, r, dl);
     ProductArgs q{};
     q.dtype = a->type; q.ctype = DT_F32; q.count = few ? nullptr : r.count;   // (few: rows past the count are anything, and are not looked at)
     q.M = (int)stacked; q.N = a->width; q.K = len;
@@ -378,6 +380,101 @@ size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
   }
   scatter_rows(acc, D, few ? n * D : 0, r.place, r.scale, a->dx, a->lddx, n, a->width, a->type, st);
   return m.used;
+}
+
+size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
+  return table_backward(a, RowsArgs{a->target, a->dloss, a->rows, a->ignore, a->vocab}, count, st,
+                        [&](const ProductArgs& p, const RowsArgs&, const Held&) { product_softmax_grad(p, st); });
+}
+
+// ---- distillation ----
+void check_teach(const DistillationArgs* a) {
+  require(a, "no arguments");
+  check_type(a->type);
+  check_type(a->teacherType);
+  require(a->teacherType == a->type || a->teacherType == DT_F32, "Distillation: teacherType is neither type nor float32");
+  require(a->rows >= 0 && a->rows < MAX_ROWS, "Distillation: bad number of rows");
+  require(a->width >= 1 && a->width < MAX_LD, "Distillation: bad width");
+  require(a->vocab >= 1, "Distillation: bad number of table rows");
+  require(a->top >= 1 && a->top <= MOST_TOP, "Distillation: bad number of a teacher's logits");
+  // (its square is a factor of the loss, its reciprocal of the logits)
+  require(a->temperature >= 0x1p-60f && a->temperature <= 0x1p60f, "Distillation: bad temperature");
+}
+void check_teach_tensors(const DistillationArgs* a) {
+  check_matrix(a->x, a->ldx, a->rows, a->width, "Distillation: x");
+  check_matrix(a->table, a->ldtable, a->vocab, a->width, "Distillation: table");
+  require(a->ids || !a->rows, "Distillation: ids");
+  require(a->lse || !a->rows, "Distillation: lse");
+  require((a->kept && a->scores && a->probs) || !a->rows, "Distillation: kept, scores and probs");
+}
+
+size_t teach_forward(const DistillationArgs* a, bool count, hipStream_t st) {
+  Arena m{count ? nullptr : (char*)a->workspace};
+  const long n = a->rows;
+  const float rate = 1.0f / a->temperature;
+  TeachArgs e{a->x, a->ldx, a->table, a->ldtable, a->ids, a->logits, a->scores, a->probs, a->kept, n, a->width, a->vocab, a->top, a->type,
+              a->teacherType, a->ignore, a->temperature, 0};
+  TeachFinish f{};
+  f.scores = a->scores; f.probs = a->probs; f.kept = a->kept;
+  f.loss = a->loss; f.lse = a->lse;
+  f.n = n; f.top = a->top;
+  f.temperature = a->temperature;
+  if (n <= skinny_rows(a->type)) {
+    SkinnyArgs p{};
+    p.dtype = a->type;
+    p.T = (int)n; p.N = a->vocab; p.K = a->width;
+    p.x = a->x; p.ldx = a->ldx;
+    p.w = a->table; p.ldw = a->ldtable;
+    p.rate = rate;
+    f.parts = skinny_softmax_parts(a->vocab);
+    f.part = p.part = m.take<float2>((size_t)n * f.parts);
+    if (count) return m.used;
+    teach_entries(e, st);
+    skinny_teach(p, st);
+    teach_finish(f, st);
+    return m.used;
+  }
+  const clr::SoftmaxPlan plan = clr::softmax_plan(n, a->vocab, a->width, a->type == DT_F32 ? 6 : 1);
+  RowsArgs r{a->kept, nullptr, n, TEACH_NONE, TEACH_OUTSIDE};
+  r.rows = m.take<int>(n); r.tgt = m.take<int>(n); r.count = m.take<int>(1);
+  r.loss = a->loss; r.lse = a->lse;
+  const Held x = hold(m, n, a->width, a->type);
+  float2* part = m.take<float2>((size_t)n * plan.parts);
+  Copies copy;
+  copy.add(x, a->x, a->ldx, n, a->width, r.rows, r.count);
+  const Held table = copy.held(m, a->table, a->ldtable, a->vocab, a->width, a->type);
+  if (count) return m.used;
+  teach_entries(e, st);
+  kept_rows(r, st);
+  lay_out(copy.j, copy.n, a->type, st);
+  ProductArgs p{};
+  p.dtype = a->type;
+  p.M = (int)n; p.N = a->vocab; p.K = a->width;
+  add_pairs(p, x, table);
+  p.count = r.count; p.part = part;
+  p.rate = rate;
+  product_teach(p, plan, st);
+  f.part = part; f.parts = plan.parts;
+  f.rows = r.rows; f.count = r.count;
+  teach_finish(f, st);
+  return m.used;
+}
+
+size_t teach_backward(const DistillationArgs* a, bool count, hipStream_t st) {
+  RowsArgs r{a->kept, a->dloss, a->rows, TEACH_NONE, TEACH_OUTSIDE};
+  r.factor = a->temperature;
+  return table_backward(a, r, count, st, [&](ProductArgs p, const RowsArgs& r, const Held& dl) {
+    p.rate = 1.0f / a->temperature;
+    product_teach_grad(p, st);
+    TeachPatch t{};
+    t.dl = (uint16_t*)dl.p; t.ld = dl.ld; t.part = dl.part;
+    t.rows = r.rows; t.tgt = r.tgt; t.count = r.count;
+    t.lse = r.lse_kept; t.grad = r.grad_kept; t.scale = r.scale;
+    t.ids = a->ids; t.scores = a->scores; t.probs = a->probs;
+    t.n = a->rows; t.top = a->top; t.dtype = a->type;
+    t.v0 = p.n0; t.len = p.N;
+    teach_patch(t, st);
+  });
 }
 
 void check_total(const LossTotalArgs* a) {
@@ -511,6 +608,39 @@ int CrossEntropyGrad(const CrossEntropyArgs* a, void* stream) {
     }
     check_space(a->workspace, a->workspaceBytes, ce_backward(a, true, nullptr));
     ce_backward(a, false, (hipStream_t)stream);
+  });
+}
+
+long DistillationWorkspace(const DistillationArgs* a) {
+  return sized([&] { check_teach(a); return teach_forward(a, true, nullptr); });
+}
+int Distillation(const DistillationArgs* a, void* stream) {
+  return clr::guarded([&] {
+    check_teach(a);
+    check_teach_tensors(a);
+    require(a->logits || !a->rows, "Distillation: logits");
+    require(a->loss || !a->rows, "Distillation: loss");
+    if (!a->rows) return;
+    check_space(a->workspace, a->workspaceBytes, teach_forward(a, true, nullptr));
+    teach_forward(a, false, (hipStream_t)stream);
+  });
+}
+long DistillationGradWorkspace(const DistillationArgs* a) {
+  return sized([&] { check_teach(a); return teach_backward(a, true, nullptr); });
+}
+int DistillationGrad(const DistillationArgs* a, void* stream) {
+  return clr::guarded([&] {
+    check_teach(a);
+    check_teach_tensors(a);
+    check_matrix(a->dx, a->lddx, a->rows, a->width, "DistillationGrad: dx");
+    require(a->dtable, "DistillationGrad: dtable");
+    require(a->dloss || !a->rows, "DistillationGrad: dloss");
+    if (!a->rows) {
+      fill_zero(a->dtable, (size_t)a->vocab * a->width * dtype_size(a->type), (hipStream_t)stream);
+      return;
+    }
+    check_space(a->workspace, a->workspaceBytes, teach_backward(a, true, nullptr));
+    teach_backward(a, false, (hipStream_t)stream);
   });
 }
 

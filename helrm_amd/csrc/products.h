@@ -40,6 +40,7 @@ struct ProductArgs {
   float* picked;             // the target's logit
   const float* lse; const float* grad;  // of row i of the tiles
   const float* scale;        // the gradient's factor in a 16-bit type
+  float rate;                // teach: of the logits, 1 / temperature
 };
 
 // h = act(A B^T) * (A B2^T); rows of all three run along k
@@ -57,6 +58,9 @@ void product_tn(ProductArgs a, ProductArgs b, ProductArgs c, hipStream_t st);  /
 void product_softmax(const ProductArgs& p, const clr::SoftmaxPlan& plan, hipStream_t st);
 // (exp(A B^T - lse) - onehot(target)) grad into c, in the layout of a factor
 void product_softmax_grad(const ProductArgs& p, hipStream_t st);
+// the same of rate A B^T, without a target's part in either (a row whose target is negative has NaN all over)
+void product_teach(const ProductArgs& p, const clr::SoftmaxPlan& plan, hipStream_t st);
+void product_teach_grad(const ProductArgs& p, hipStream_t st);
 
 // Matrices into the layout above, up to 8 in one launch: row rows[i] (or i) of
 // `from` to row i of `to`, for i < *count (or n); a float32 one as three parts
@@ -79,6 +83,7 @@ struct RowsArgs {
   int* rows; int* tgt; int* count;   // of the rows that count: each one's row, its target (-1 outside the table), and how many they are
   int* place;                        // of each row: where it is among them, or -1
   float* picked; float* loss; float* lse; float* lse_kept; float* grad_kept; float* scale;
+  float factor = 1.0f;               // of grad, in grad_kept
 };
 void kept_rows(const RowsArgs& a, hipStream_t st);
 // loss[row] = lse - picked, lse = the logarithm of the parts' sum

@@ -53,7 +53,9 @@ struct Batch {
 };
 constexpr unsigned OUTSIDE = 0x80000000u;  // an offset past every descriptor's bound
 
-enum Epi { EPI_STORE, EPI_GATE, EPI_GATE_GRAD, EPI_SOFTMAX, EPI_SOFTMAX_GRAD };
+enum Epi { EPI_STORE, EPI_GATE, EPI_GATE_GRAD, EPI_SOFTMAX, EPI_SOFTMAX_GRAD, EPI_TEACH, EPI_TEACH_GRAD };
+constexpr bool is_softmax(int epi) { return epi == EPI_SOFTMAX || epi == EPI_TEACH; }
+constexpr bool is_softmax_grad(int epi) { return epi == EPI_SOFTMAX_GRAD || epi == EPI_TEACH_GRAD; }
 
 __device__ __forceinline__ u16 bits(__bf16 v) { return __builtin_bit_cast(u16, v); }
 __device__ __forceinline__ u16 bits(_Float16 v) { return __builtin_bit_cast(u16, v); }
@@ -206,7 +208,8 @@ __device__ __forceinline__ void tile_of(int id, int total, int nm, int nn, int& 
 // A row's maximum and sum over the tile's columns: over the lane's, over the
 // four lanes that share the row, over the waves beside one another.  acc[i][j][e]
 // is (m, n) = (mw + 16 i + lane % 16, n_wave + 16 j + 4 (lane / 16) + e).
-template <int FM, int FN, int WAVES_M, int WAVES_N>
+// TEACH: of p.rate times them, which is positive.
+template <bool TEACH, int FM, int FN, int WAVES_M, int WAVES_N>
 __device__ __forceinline__ void softmax_piece(const ProductArgs& p, const f32x4 (&acc)[FM][FN], int M, long m0, long n0, int wave_m, int wave_n, int tile_n,
                                               float2* lds) {
   const int lane = threadIdx.x & 63, quad = lane >> 4;
@@ -216,25 +219,28 @@ __device__ __forceinline__ void softmax_piece(const ProductArgs& p, const f32x4 
   for (int i = 0; i < FM; i++) {
     const int r = (wave_m * FM + i) * 16 + (lane & 15);
     const long m = m0 + r;
-    const int t = m < M ? p.target[m] - (int)(p.n0 + n0 + wave_n * FN * 16 + 4 * quad) : -1;   // the target's place from there
+    const int t = !TEACH && m < M ? p.target[m] - (int)(p.n0 + n0 + wave_n * FN * 16 + 4 * quad) : -1;   // the target's place from there
     if (t >= 0 && t < FN * 16) {   // (seldom: one tile has it)
 #pragma unroll
       for (int c = 0; c < FN * 4; c++) if (16 * (c >> 2) + (c & 3) == t) p.picked[m] = acc[i][c >> 2][c & 3];
     }
     float top = -INFINITY, sum = 0;
+    auto of = [&](float v, float base) { return TEACH ? __expf(__builtin_fmaf(v, p.rate, -base)) : __expf(v - base); };
     // fmaxf passes over a NaN; its exponential is one again
     if (whole) {
 #pragma unroll
       for (int c = 0; c < FN * 4; c++) top = fmaxf(top, acc[i][c >> 2][c & 3]);
+      if (TEACH) top *= p.rate;
       const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-      for (int c = 0; c < FN * 4; c++) sum += __expf(acc[i][c >> 2][c & 3] - base);
+      for (int c = 0; c < FN * 4; c++) sum += of(acc[i][c >> 2][c & 3], base);
     } else {
 #pragma unroll
       for (int c = 0; c < FN * 4; c++) if (16 * (c >> 2) + (c & 3) < left) top = fmaxf(top, acc[i][c >> 2][c & 3]);
+      if (TEACH) top *= p.rate;
       const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-      for (int c = 0; c < FN * 4; c++) if (16 * (c >> 2) + (c & 3) < left) sum += __expf(acc[i][c >> 2][c & 3] - base);
+      for (int c = 0; c < FN * 4; c++) if (16 * (c >> 2) + (c & 3) < left) sum += of(acc[i][c >> 2][c & 3], base);
     }
     float2 run = make_float2(top, sum);
 #pragma unroll
@@ -290,8 +296,8 @@ __device__ __forceinline__ void emit4(const ProductArgs& p, long first, unsigned
     put_held<T>((u16*)p.h + first + at, p.dtype, p.hpart, a);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = __expf(v[e] - row.lse);
-    if (row.target >= 0 && row.target < 4) {   // (seldom)
+    for (int e = 0; e < 4; e++) v[e] = EPI == EPI_TEACH_GRAD ? __expf(__builtin_fmaf(v[e], p.rate, -row.lse)) : __expf(v[e] - row.lse);
+    if (EPI == EPI_SOFTMAX_GRAD && row.target >= 0 && row.target < 4) {   // (seldom)
 #pragma unroll
       for (int e = 0; e < 4; e++) if (row.target == e) v[e] -= 1.0f;
     }
@@ -307,7 +313,7 @@ __device__ __forceinline__ void emit4(const ProductArgs& p, long first, unsigned
 
 // Elements from one row of the results to the next, and of a split product's sums (gate: the gate's, then the up projection's).
 template <int EPI> __device__ __host__ __forceinline__ long result_ld(const ProductArgs& p) {
-  return EPI == EPI_STORE || EPI == EPI_SOFTMAX_GRAD ? p.ldc : p.ldh;
+  return EPI == EPI_STORE || is_softmax_grad(EPI) ? p.ldc : p.ldh;
 }
 template <int EPI> __device__ __host__ __forceinline__ long sum_cols(const ProductArgs& p) { return EPI == EPI_STORE ? (p.N + 3) & ~3 : p.ldh; }
 template <int EPI> __device__ __host__ __forceinline__ long sum_ld(const ProductArgs& p) { return sum_cols<EPI>(p) * (EPI == EPI_GATE ? 2 : 1); }
@@ -326,7 +332,7 @@ __device__ __forceinline__ void emit(const ProductArgs& p, const f32x4 (&acc)[FM
   const int lane = threadIdx.x & 63, col = lane % LANES;
   // gate: the columns are 16 of the gate, the same 16 of the up projection, 16 of the gate, ...
   const int c = EPI == EPI_GATE ? (col >> 2) * 8 + (col & 3) : col;
-  const bool sums = EPI != EPI_SOFTMAX_GRAD && p.splits > 1;
+  const bool sums = !is_softmax_grad(EPI) && p.splits > 1;
   const unsigned ld = (unsigned)(sums ? sum_ld<EPI>(p) : result_ld<EPI>(p));
   const unsigned second = EPI == EPI_GATE ? (unsigned)sum_cols<EPI>(p) : 0;
   // a store of whole vectors, nothing to add or divide by
@@ -347,7 +353,7 @@ __device__ __forceinline__ void emit(const ProductArgs& p, const f32x4 (&acc)[FM
     const int room = EPI == EPI_STORE ? left : (int)min(((p.N + 7L) & ~7L) - n_wave, 64L) - col * 4;
     const int rows = (int)min(M - mw - part * 64, 64L);
     RowValues mine{};   // of row `lane` of the 64
-    if (EPI == EPI_SOFTMAX_GRAD && lane < rows) {
+    if (is_softmax_grad(EPI) && lane < rows) {
       const long m = mw + part * 64 + lane;
       mine.target = p.target[m];
       mine.lse = p.lse[m];
@@ -364,7 +370,7 @@ __device__ __forceinline__ void emit(const ProductArgs& p, const f32x4 (&acc)[FM
           const int r = r0 + g * ROWS + lane / LANES;
           get4(own + r * 64 + ((c ^ (r & 15)) * 4), v[g]);
           if (EPI == EPI_GATE) get4(own + r * 64 + (((c + 4) ^ (r & 15)) * 4), u[g]);
-          if (EPI == EPI_SOFTMAX_GRAD)
+          if (is_softmax_grad(EPI))
             row[g] = {__shfl(mine.lse, r), __shfl(mine.grad, r), __shfl(mine.target, r) - (int)(p.n0 + n_wave) - col * 4};
           if (EPI == EPI_GATE_GRAD && !sums && (WHOLE || (r < rows && room > 0))) {
             const unsigned at = (part * 64 + r) * ld + col * 4;
@@ -571,8 +577,8 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Batch batch)
   }
   if (PARTS && corrections >= to - from) settle();
   arrive<0>();   // no load may still write LDS when it is used again, or given away
-  if constexpr (EPI == EPI_SOFTMAX) {
-    softmax_piece<FM, FN, WM, WN>(p, acc, M, m0, n0, wave_m, wave_n, tile_n, (float2*)a0);
+  if constexpr (is_softmax(EPI)) {
+    softmax_piece<EPI == EPI_TEACH, FM, FN, WM, WN>(p, acc, M, m0, n0, wave_m, wave_n, tile_n, (float2*)a0);
   } else {
     const int q = BM == 256 ? wave >> 1 : wave;   // 16 KiB a wave
     u16* mine = (q == 0 ? a0 : q == 1 ? b0 : q == 2 ? a1 : b1) + (BM == 256 ? (wave & 1) * 8192 : 0);
@@ -732,9 +738,9 @@ __global__ __launch_bounds__(ROWS_BLOCK) void kept_rows_kernel(RowsArgs a) {
       const int i = before + __popcll(mask & ((1ull << lane) - 1));
       a.rows[i] = (int)r;
       a.tgt[i] = t >= 0 && t < a.vocab ? (int)t : -1;
-      if (a.lse_kept) { a.lse_kept[i] = a.lse[r]; a.grad_kept[i] = a.grad[r]; }
+      if (a.lse_kept) { a.lse_kept[i] = a.lse[r]; a.grad_kept[i] = a.grad[r] * a.factor; }
       if (a.picked) a.picked[i] = NAN;
-      if (a.scale) top = fmaxf(top, fabsf(a.grad[r]));
+      if (a.scale) top = fmaxf(top, fabsf(a.grad[r] * a.factor));
       if (a.place) a.place[r] = i;
     } else if (r < a.n) {
       if (a.loss) { a.loss[r] = 0.0f; a.lse[r] = 0.0f; }
@@ -868,7 +874,7 @@ void product_tn(ProductArgs a, ProductArgs b, ProductArgs c, hipStream_t st) {
   c.partial = b.partial + (plan.splits > 1 ? sums(b) : 0);
   launch<false, false, EPI_STORE>({a, b, c}, plan, st);
 }
-void product_softmax(const ProductArgs& p, const clr::SoftmaxPlan& plan, hipStream_t st) {
+template <int EPI> static void softmax_launches(const ProductArgs& p, const clr::SoftmaxPlan& plan, hipStream_t st) {
   for (long v0 = 0; v0 < p.N; v0 += plan.columns) {
     ProductArgs q = p;
     q.n0 = (int)v0;
@@ -876,10 +882,13 @@ void product_softmax(const ProductArgs& p, const clr::SoftmaxPlan& plan, hipStre
     for (int k = 0; k < q.pairs; k++) q.b[k] += v0 * q.ldb;
     q.parts = plan.parts;
     q.part += v0 / plan.plan.tile();
-    launch<true, true, EPI_SOFTMAX>({q}, plan.plan, st);
+    launch<true, true, EPI>({q}, plan.plan, st);
   }
 }
+void product_softmax(const ProductArgs& p, const clr::SoftmaxPlan& plan, hipStream_t st) { softmax_launches<EPI_SOFTMAX>(p, plan, st); }
 void product_softmax_grad(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_SOFTMAX_GRAD>(p, st); }
+void product_teach(const ProductArgs& p, const clr::SoftmaxPlan& plan, hipStream_t st) { softmax_launches<EPI_TEACH>(p, plan, st); }
+void product_teach_grad(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_TEACH_GRAD>(p, st); }
 
 void lay_out(const LayOut* jobs, int n, int dtype, hipStream_t st) {
   LayOuts all{};

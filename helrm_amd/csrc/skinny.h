@@ -14,6 +14,7 @@ struct SkinnyArgs {
   int act; float coef[4];
   const long long* target; float* picked; float2* part;   // softmax: [T], [T], [T][parts]
   int parts, groups; bool alone;     // (of the launch)
+  float rate;                        // teach: of the products
 };
 // out = act(X W^T) * (X W2^T)
 void skinny_gate(SkinnyArgs p, hipStream_t st);
@@ -22,3 +23,5 @@ void skinny_store(SkinnyArgs p, hipStream_t st);
 // loss and lse of every row of X against the rows of W
 int skinny_softmax_parts(int N);
 void skinny_softmax(SkinnyArgs p, long long ignore, float* loss, float* lse, hipStream_t st);
+// the pieces of the softmax of rate X W^T, p.part, of every row of X
+void skinny_teach(SkinnyArgs p, hipStream_t st);

@@ -23,7 +23,8 @@
 
 namespace {
 
-enum Epi { SKINNY_STORE, SKINNY_GATE, SKINNY_SOFTMAX };
+enum Epi { SKINNY_STORE, SKINNY_GATE, SKINNY_SOFTMAX, SKINNY_TEACH };
+constexpr bool is_softmax(int epi) { return epi == SKINNY_SOFTMAX || epi == SKINNY_TEACH; }
 
 // Eight k of a row for one matrix instruction, or the parts of eight float32.
 template <class T> struct Eight {
@@ -180,13 +181,14 @@ __global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_ke
       const int row = b * 16 + t;
       const long n = n0 + 4 * quad;
       const int left = (int)min((long)p.N - n, 4L);
-      if (EPI == SKINNY_SOFTMAX) {
+      if (is_softmax(EPI)) {
         float top = -INFINITY, s = 0;
-        const long long target = row < p.T ? p.target[row] : -1;
+        const long long target = EPI == SKINNY_SOFTMAX && row < p.T ? p.target[row] : -1;
+        if (EPI == SKINNY_TEACH) sum[0] *= p.rate;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           if (e < left) top = fmaxf(top, sum[0][e]);
-          if (e < left && n + e == target) p.picked[row] = sum[0][e];
+          if (EPI == SKINNY_SOFTMAX && e < left && n + e == target) p.picked[row] = sum[0][e];
         }
         const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
@@ -224,7 +226,7 @@ __global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_ke
       }
     }
   }
-  if (EPI == SKINNY_SOFTMAX) {
+  if (is_softmax(EPI)) {
 #pragma unroll
     for (int b = 0; b < NB; b++)
       if (b % waves == wave && lane < 16 && b * 16 + t < p.T && team < p.parts) p.part[(long)(b * 16 + t) * p.parts + team] = run[b];
@@ -299,4 +301,9 @@ void skinny_softmax(SkinnyArgs p, long long ignore, float* loss, float* lse, hip
   p.parts = skinny_softmax_parts(p.N);
   launch<SKINNY_SOFTMAX>(p, st);
   skinny_finish_kernel<<<(unsigned)p.T, FINISH, 0, st>>>(p.part, p.parts, p.picked, p.target, ignore, p.N, loss, lse);
+}
+void skinny_teach(SkinnyArgs p, hipStream_t st) {
+  p.groups = softmax_groups(p.N);
+  p.parts = skinny_softmax_parts(p.N);
+  launch<SKINNY_TEACH>(p, st);
 }

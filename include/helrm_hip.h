@@ -368,6 +368,38 @@ typedef struct {
 long LossTotalWorkspace(const LossTotalArgs* args);
 int LossTotal(const LossTotalArgs* args, void* stream);
 
+/* Distillation from a teacher's `top` largest logits against a table of `vocab`
+ * rows.  An entry j of row i is an id other than `ignore` with a logit above -inf;
+ * with p the softmax of the row's entries' logits / temperature (an id that is there
+ * several times has the sum), z[v] = <x[i], table[v]> / temperature and lse = log
+ * sum_v exp z[v],
+ *     loss[i] = temperature^2 sum_j p[j] (log p[j] - (z[ids[j]] - lse)):
+ * the teacher's divergence from the model, without keeping the model's logits.  A
+ * row without entries has loss, lse and gradients 0, and nothing it holds reaches
+ * another row's; an entry whose id is outside [0, vocab) gives a loss and
+ * gradients of NaN.  kept, scores and probs are what the gradient and a mean over
+ * the rows with a teacher need (kept is 0 for the others).  dtable is contiguous. */
+typedef struct {
+  const void* x; long ldx;               /* [rows][width] */
+  const void* table; long ldtable;       /* [vocab][width] */
+  const long long* ids; const void* logits; /* [rows][top]; Distillation reads logits, of teacherType */
+  float* loss; float* lse;               /* [rows]; DistillationGrad reads lse */
+  long long* kept;                       /* [rows]; written by Distillation, as the next two */
+  float* scores; float* probs;           /* [rows][top]: z, and p or -1 */
+  const float* dloss;                    /* [rows] */
+  void* dx; long lddx;                   /* [rows][width] */
+  void* dtable;                          /* [vocab][width] */
+  void* workspace; size_t workspaceBytes;
+  long rows; int width; int vocab; int top; /* top up to 1024 */
+  int type; int teacherType;             /* teacherType: type, or float32 */
+  long long ignore;
+  float temperature;
+} DistillationArgs;
+long DistillationWorkspace(const DistillationArgs* args);
+int Distillation(const DistillationArgs* args, void* stream);
+long DistillationGradWorkspace(const DistillationArgs* args);
+int DistillationGrad(const DistillationArgs* args, void* stream);
+
 /* y[i] = scale table[ids[i]]: rows of a table, and the table's gradient
  * dtable[v] = scale * the sum of dy[i] over ids[i] = v, 0 for rows that no id
  * names.  Sums are float32, rounded once, in an order that only the ids decide.
