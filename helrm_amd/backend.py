@@ -88,6 +88,16 @@ class EmbeddingArgs(ctypes.Structure):
                 ("type", ctypes.c_int), ("scale", ctypes.c_float)]
 
 
+class PreferenceArgs(ctypes.Structure):
+    _fields_ = [("loss", ctypes.c_void_p), ("ldloss", ctypes.c_long), ("reference", ctypes.c_void_p), ("ldreference", ctypes.c_long),
+                ("target", ctypes.c_void_p), ("ldtarget", ctypes.c_long), ("offsets", ctypes.c_void_p), ("value", ctypes.c_void_p),
+                ("ratio", ctypes.c_void_p), ("slope", ctypes.c_void_p), ("kept", ctypes.c_void_p), ("dvalue", ctypes.c_void_p),
+                ("dloss", ctypes.c_void_p), ("lddloss", ctypes.c_long),
+                ("workspace", ctypes.c_void_p), ("workspaceBytes", ctypes.c_size_t),
+                ("pairs", ctypes.c_long), ("length", ctypes.c_long), ("ignore", ctypes.c_longlong), ("kind", ctypes.c_int),
+                ("average", ctypes.c_int), ("beta", ctypes.c_float), ("margin", ctypes.c_float), ("smoothing", ctypes.c_float)]
+
+
 _ARRAY_TYPES = (ArrayResultInt, ArrayResultFloat, ArrayResultUInt64)
 
 
@@ -355,6 +365,9 @@ _SIGNATURES = {
     "Embedding": ([_c.c_void_p, _c.c_void_p], _I),
     "EmbeddingGradWorkspace": ([_c.c_void_p], _c.c_long),
     "EmbeddingGrad": ([_c.c_void_p, _c.c_void_p], _I),
+    "PreferenceWorkspace": ([_c.c_void_p], _c.c_long),
+    "Preference": ([_c.c_void_p, _c.c_void_p], _I),
+    "PreferenceGrad": ([_c.c_void_p, _c.c_void_p], _I),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

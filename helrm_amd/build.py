@@ -16,7 +16,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "libhelrm_hip.so")
 SOURCES = ["kernels.hip", "ntt.hip", "encoder.hip", "runtime.hip", "norm.hip", "products.hip", "skinny.hip",
-           "embedding.hip", "teacher.hip", "cleartext.hip"]
+           "embedding.hip", "teacher.hip", "preference.hip", "cleartext.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 FLAGS = [

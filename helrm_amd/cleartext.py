@@ -8,6 +8,7 @@ that training and of scoring beside it, on the same card:
     gated_mlp       y = (act(x gate^T) * (x up^T)) down^T
     cross_entropy   log sum_v exp <x, table[v]> - <x, table[target]>
     distillation    the divergence of a teacher's top logits from the softmax of <x, table[v]>
+    preference      log(1 + exp -m) of the difference m of two sequences' log ratios to a reference
     embedding       y[i] = scale * table[ids[i]]
 
 Each has a `_forward` and a `_backward` call, which a training loop of one's
@@ -26,11 +27,13 @@ Shapes and types that do not fit raise ValueError, tensors with a forward-mode
 tangent NotImplementedError; HipError holds what the library refuses.
 """
 import ctypes
+import math
 
 import torch
 from torch.autograd import forward_ad
 
-from .backend import CrossEntropyArgs, DistillationArgs, EmbeddingArgs, GatedMLPArgs, HipError, LayerNormArgs, LossTotalArgs, load_library
+from .backend import (CrossEntropyArgs, DistillationArgs, EmbeddingArgs, GatedMLPArgs, HipError, LayerNormArgs, LossTotalArgs, PreferenceArgs,
+                      load_library)
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTS = {"silu": 0, "gelu": 1}
@@ -54,7 +57,7 @@ def _library():
                        + "): import torch before the library is loaded")
     calls = {}
     for name in ("LayerNorm", "LayerNormGrad", "GatedMLP", "GatedMLPGrad", "CrossEntropy", "CrossEntropyGrad", "LossTotal",
-                 "Distillation", "DistillationGrad", "Embedding", "EmbeddingGrad"):
+                 "Distillation", "DistillationGrad", "Preference", "PreferenceGrad", "Embedding", "EmbeddingGrad"):
         call, size = getattr(lib, name), getattr(lib, name + "Workspace", None)
         call.argtypes, call.restype = [ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int
         if size is not None:
@@ -533,6 +536,143 @@ def distillation(x, table, ids, logits, temperature=1.0, ignore_index=-100, redu
         return losses
     kept = kept if reduction == "mean" else None
     return _Total.apply(losses, kept, 0) if grad else _total(losses, kept, 0)[0]
+
+
+# ---- pairs of sequences of which one is preferred ------------------------------------------
+
+
+_KINDS = {"logistic": 0, "hinge": 1}
+
+
+def _lines(t, shape, name, dtype, device, packed):
+    """Token values as the kernels take them, [2 pairs, length] or [length]."""
+    if forward_ad._current_level >= 0:
+        _no_tangent(t, name)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name}: {list(t.shape)}, not {list(shape)}")
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name}: {t.dtype} on {t.device}, not {dtype} on {device}")
+    if packed:
+        return t.contiguous()
+    rows, length = math.prod(shape[:-1]), shape[-1]
+    t = t.reshape(rows, length)
+    if (length > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < length):
+        t = t.contiguous()
+    return t
+
+
+def _pairs(losses, target, offsets, ignore_index):
+    """(leading dimensions of a pair, number of pairs, length, target, offsets)."""
+    _need(-(1 << 63) <= ignore_index < 1 << 63, "ignore_index: not an int64")
+    if losses.dtype != torch.float32:
+        raise ValueError(f"losses: {losses.dtype}, not {torch.float32}")
+    if offsets is None:
+        _need(losses.dim() >= 2 and losses.shape[-2] == 2, f"losses: {list(losses.shape)}, not [..., 2, length]")
+        lead = losses.shape[:-2]
+        pairs = math.prod(lead)
+    else:
+        _need(losses.dim() == 1, f"losses: {list(losses.shape)}, not [tokens] beside offsets")
+        _need(offsets.dim() == 1 and offsets.shape[0] % 2 == 1, f"offsets: {list(offsets.shape)}, not [2 * pairs + 1]")
+        pairs = offsets.shape[0] // 2
+        lead = (pairs,)
+    if not losses.is_cuda:
+        raise ValueError("losses: not on the GPU")
+    if offsets is not None:
+        offsets = _vector(offsets, 2 * pairs + 1, "offsets", torch.int64, losses.device)
+    if target is not None:
+        target = _lines(target, losses.shape, "target", torch.int64, losses.device, offsets is not None)
+    return lead, pairs, losses.shape[-1], target, offsets
+
+
+def _line_ld(t, packed):
+    return 0 if t is None or packed else t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _pointer(t):
+    return None if t is None else t.data_ptr()
+
+
+def _preference_forward(losses, reference, target, offsets, beta, margin, kind, smoothing, average, ignore_index):
+    _need(kind in _KINDS, f"kind {kind!r}: neither logistic nor hinge")
+    _need(math.isfinite(beta) and math.isfinite(margin), "beta and margin are not finite")
+    _need(0.0 <= smoothing <= (1.0 if kind == "logistic" else 0.0), f"smoothing {smoothing}: not from 0 to 1, or not 0 with the hinge")
+    lead, pairs, length, target, offsets = _pairs(losses, target, offsets, ignore_index)
+    packed, shape, device = offsets is not None, losses.shape, losses.device
+    losses = _lines(losses, shape, "losses", torch.float32, device, packed)
+    if reference is not None:
+        reference = _lines(reference, shape, "reference", torch.float32, device, packed)
+    values = torch.empty(lead, dtype=torch.float32, device=device)
+    ratios, slopes = (torch.empty((*lead, 2), dtype=torch.float32, device=device) for _ in "ab")
+    kept = torch.empty(pairs, dtype=torch.int64, device=device)
+    _call("Preference", PreferenceArgs(
+        loss=losses.data_ptr(), ldloss=_line_ld(losses, packed), reference=_pointer(reference), ldreference=_line_ld(reference, packed),
+        target=_pointer(target), ldtarget=_line_ld(target, packed), offsets=_pointer(offsets), value=values.data_ptr(), ratio=ratios.data_ptr(),
+        slope=slopes.data_ptr(), kept=kept.data_ptr(), pairs=pairs, length=length, ignore=ignore_index, kind=_KINDS[kind], average=bool(average),
+        beta=beta, margin=margin, smoothing=smoothing), device)
+    return values, ratios, slopes, kept
+
+
+def preference_forward(losses, reference=None, target=None, offsets=None, beta=0.1, margin=0.0, kind="logistic", smoothing=0.0, average=False,
+                       ignore_index=-100):
+    """(values, ratios, slopes) of pairs of sequences whose first one is preferred: the pairs' losses [...], and for both sequences
+    [..., 2] the sum of reference - losses over the tokens that count (their mean with `average`) and the derivative of the pair's
+    value by each of those losses.  losses [..., 2, length] are the tokens' (float32, as cross_entropy gives them); or [tokens],
+    sequence s the tokens from offsets[s] to offsets[s + 1].  Tokens whose target is `ignore_index` count in nothing.
+    With m = beta * (ratio of the first - of the second) - margin: "logistic" (1 - smoothing) log(1 + exp -m) + smoothing log(1 +
+    exp m), "hinge" max(0, 1 - m).  A pair without tokens that count has 0; offsets that descend or leave the tokens give NaN."""
+    return _preference_forward(losses, reference, target, offsets, beta, margin, kind, smoothing, average, ignore_index)[:3]
+
+
+def preference_backward(grad, losses, slopes, target=None, offsets=None, ignore_index=-100):
+    """The gradient of every token's loss, of losses' shape, for the gradient `grad` of the values; slopes as the forward call gave
+    them.  Tokens that count in nothing have 0."""
+    lead, pairs, length, target, offsets = _pairs(losses, target, offsets, ignore_index)
+    packed, device = offsets is not None, losses.device
+    if tuple(grad.shape) != tuple(lead):
+        raise ValueError(f"grad: {list(grad.shape)}, not {list(lead)}")
+    grad = _vector(grad.reshape(-1), pairs, "grad", torch.float32, device)
+    if tuple(slopes.shape) != (*lead, 2):
+        raise ValueError(f"slopes: {list(slopes.shape)}, not {[*lead, 2]}")
+    slopes = _vector(slopes.reshape(-1), 2 * pairs, "slopes", torch.float32, device)
+    d = torch.empty(losses.shape, dtype=torch.float32, device=device)
+    _call("PreferenceGrad", PreferenceArgs(
+        target=_pointer(target), ldtarget=_line_ld(target, packed), offsets=_pointer(offsets), slope=slopes.data_ptr(), dvalue=grad.data_ptr(),
+        dloss=d.data_ptr(), lddloss=length, pairs=pairs, length=length, ignore=ignore_index), device)
+    return d
+
+
+class _Preference(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, losses, reference, target, offsets, ignore_index, rest):
+        values, _, slopes, kept = _preference_forward(losses, reference, target, offsets, *rest, ignore_index)
+        ctx.save_for_backward(losses, slopes, target, offsets)
+        ctx.ignore_index = ignore_index
+        ctx.mark_non_differentiable(kept)
+        return values, kept
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):
+        return (preference_backward(grad, *ctx.saved_tensors, ctx.ignore_index),) + (None,) * 5
+
+
+def preference(losses, reference=None, target=None, offsets=None, beta=0.1, margin=0.0, kind="logistic", smoothing=0.0, average=False,
+               ignore_index=-100, reduction="mean"):
+    """Loss of pairs of sequences of which the first is preferred, from their tokens' losses and those of a reference model
+    (preference_forward has the arguments and the formula): the mean over the pairs that have a token (0 where none has one), their
+    "sum", or "none" for a loss a pair.  The reference has no gradient here."""
+    _need(reduction in ("mean", "sum", "none"), f"reduction {reduction!r}: neither mean, sum nor none")
+    _need(not _wants_grad(reference), "reference: requires a gradient, and is held; detach it")
+    grad = _wants_grad(losses)
+    rest = beta, margin, kind, smoothing, average
+    if grad:
+        values, kept = _Preference.apply(losses, reference, target, offsets, ignore_index, rest)
+    else:
+        values, _, _, kept = _preference_forward(losses, reference, target, offsets, *rest, ignore_index)
+    if reduction == "none":
+        return values
+    kept = kept if reduction == "mean" else None
+    return _Total.apply(values, kept, 0) if grad else _total(values, kept, 0)[0]
 
 
 # ---- rows of a table for ids -----------------------------------------------------------------

@@ -5,6 +5,7 @@
 #include "cleartext.h"
 #include "embedding.h"
 #include "norm.h"
+#include "preference.h"
 #include "products.h"
 #include "skinny.h"
 #include "teacher.h"
@@ -502,6 +503,32 @@ EmbedArgs embed_args(const EmbeddingArgs* a) {
 }
 size_t embedding_space(const EmbeddingArgs* a) { return embedding_grad_workspace(a->tokens, a->width, a->vocab, a->type); }
 
+// ---- preference ----
+constexpr long MAX_LINE = 1L << 40;
+void check_pairs(const PreferenceArgs* a) {
+  require(a, "no arguments");
+  require(a->pairs >= 0 && a->pairs < MAX_ROWS, "Preference: bad number of pairs");
+  require(a->length >= 0 && a->length <= MAX_LINE, "Preference: bad length");
+  require(a->kind == PAIR_LOGISTIC || a->kind == PAIR_HINGE, "Preference: unknown kind");
+  require(a->beta - a->beta == 0.0f && a->margin - a->margin == 0.0f, "Preference: beta and margin are not finite");
+  require(a->smoothing >= 0.0f && a->smoothing <= (a->kind == PAIR_LOGISTIC ? 1.0f : 0.0f), "Preference: bad smoothing");
+}
+// A line of tokens, or a matrix of them.
+void check_tokens(const PreferenceArgs* a, const void* p, long ld, const char* what) {
+  const bool any = a->length && (a->offsets || a->pairs);
+  require(p || !any, what);
+  require(a->offsets || a->pairs == 0 || ld >= a->length, what);
+}
+PairArgs pair_args(const PreferenceArgs* a) {
+  PairArgs p{};
+  p.target = a->target; p.ldtarget = a->ldtarget;
+  p.offsets = a->offsets;
+  p.slope = a->slope;
+  p.pairs = a->pairs; p.length = a->length;
+  p.ignore = a->ignore;
+  return p;
+}
+
 template <class F> long sized(F&& f) {
   try { return (long)f(); } catch (const std::exception& e) { return report_error(e.what()); }
 }
@@ -654,6 +681,42 @@ int LossTotal(const LossTotalArgs* a, void* stream) {
     require(a->total && a->factor, "LossTotal: total and factor");
     check_space(a->workspace, a->workspaceBytes, loss_total_bytes(a->rows));
     loss_total(a->loss, a->target, a->ignore, a->rows, a->workspace, a->total, a->factor, (hipStream_t)stream);
+  });
+}
+
+long PreferenceWorkspace(const PreferenceArgs* a) {
+  return sized([&] { check_pairs(a); return preference_workspace(a->pairs, a->length, a->offsets); });
+}
+int Preference(const PreferenceArgs* a, void* stream) {
+  return clr::guarded([&] {
+    check_pairs(a);
+    check_tokens(a, a->loss, a->ldloss, "Preference: loss");
+    if (a->reference) check_tokens(a, a->reference, a->ldreference, "Preference: reference");
+    if (a->target) check_tokens(a, a->target, a->ldtarget, "Preference: target");
+    require((a->value && a->ratio && a->slope && a->kept) || !a->pairs, "Preference: value, ratio, slope and kept");
+    check_space(a->workspace, a->workspaceBytes, preference_workspace(a->pairs, a->length, a->offsets));
+    if (!a->pairs) return;
+    PairArgs p = pair_args(a);
+    p.loss = a->loss; p.ldloss = a->ldloss;
+    p.reference = a->reference; p.ldreference = a->ldreference;
+    p.value = a->value; p.ratio = a->ratio; p.kept = a->kept;
+    p.workspace = a->workspace;
+    p.kind = a->kind; p.average = a->average;
+    p.beta = a->beta; p.margin = a->margin; p.smoothing = a->smoothing;
+    preference_launch(p, (hipStream_t)stream);
+  });
+}
+int PreferenceGrad(const PreferenceArgs* a, void* stream) {
+  return clr::guarded([&] {
+    check_pairs(a);
+    check_tokens(a, a->dloss, a->lddloss, "PreferenceGrad: dloss");
+    if (a->target) check_tokens(a, a->target, a->ldtarget, "PreferenceGrad: target");
+    require((a->slope && a->dvalue) || !a->pairs, "PreferenceGrad: slope and dvalue");
+    if (!a->length || (!a->pairs && !a->offsets)) return;
+    PairArgs p = pair_args(a);
+    p.dvalue = a->dvalue;
+    p.dloss = a->dloss; p.lddloss = a->lddloss;
+    preference_grad_launch(p, (hipStream_t)stream);
   });
 }
 

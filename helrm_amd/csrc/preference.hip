@@ -1,0 +1,188 @@
+// preference.hip -- a loss of pairs of sequences, of which the first is
+// preferred, from their tokens' losses and those of a reference model.
+//
+//   r[s] = sum over the tokens of s that count of (reference - loss), or its mean
+//   m = beta (r[0] - r[1]) - margin
+//   logistic: (1 - e) log(1 + exp(-m)) + e log(1 + exp(m)),  hinge: max(0, 1 - m)
+//   d/d loss[t] = -+ beta d/dm (/ the number of tokens that count)
+//
+// Sums are of 64 bits: long sequences differ by little of their sums.  A token is
+// read once in each direction.
+#include <algorithm>
+#include "plan.h"
+#include "preference.h"
+
+namespace {
+
+struct Sum { double sum; long count; };
+constexpr int WAVE = 64, MOST = 1024;
+constexpr int MOST_SPLITS = 64;
+
+__device__ __forceinline__ Sum wave_sum(Sum s) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) {
+    s.sum += __shfl_xor(s.sum, o);
+    s.count += __shfl_xor(s.count, o);
+  }
+  return s;
+}
+
+// Where a sequence's tokens are: elements of a line, or from a row's first one.
+struct Tokens { long from, to; };
+__device__ __forceinline__ Tokens tokens_of(const PairArgs& a, long sequence) {
+  if (!a.offsets) return {0, a.length};
+  // (whatever the offsets say, within the line)
+  const long from = min(max((long)a.offsets[sequence], 0L), a.length);
+  return {from, min(max((long)a.offsets[sequence + 1], from), a.length)};
+}
+__device__ __forceinline__ Tokens share_of(Tokens t, int split, int splits) {
+  const long n = t.to - t.from;
+  return {t.from + n / splits * split + min((long)split, n % splits), t.from + n / splits * (split + 1) + min((long)split + 1, n % splits)};
+}
+
+// What `threads` threads have of a sequence's share.
+__device__ __forceinline__ Sum sum_of(const PairArgs& a, long sequence, int split, int thread, int threads) {
+  const Tokens t = share_of(tokens_of(a, sequence), split, a.splits);
+  const long row = a.offsets ? 0 : sequence;
+  const float* loss = a.loss + row * a.ldloss;
+  const float* reference = a.reference ? a.reference + row * a.ldreference : nullptr;
+  const long long* target = a.target ? a.target + row * a.ldtarget : nullptr;
+  Sum s{0.0, 0};
+#pragma unroll 4
+  for (long i = t.from + thread; i < t.to; i += threads) {
+    const bool counts = !target || target[i] != a.ignore;
+    const double d = (reference ? (double)reference[i] : 0.0) - (double)loss[i];
+    s.sum += counts ? d : 0.0;
+    s.count += counts;
+  }
+  return s;
+}
+
+// softplus(m) = log(1 + exp m)
+__device__ __forceinline__ double softplus(double m) { return fmax(m, 0.0) + log1p(exp(-fabs(m))); }
+__device__ __forceinline__ double sigmoid(double m) { return 1.0 / (1.0 + exp(-m)); }
+
+__device__ __forceinline__ void finish(const PairArgs& a, long pair, Sum first, Sum second) {
+  const bool any = first.count + second.count > 0;
+  const double each[2] = {a.average ? 1.0 / (double)max(first.count, 1L) : 1.0, a.average ? 1.0 / (double)max(second.count, 1L) : 1.0};
+  double r[2] = {first.sum * each[0], second.sum * each[1]};
+  if (a.offsets) {   // sequences that leave the line, or run backwards
+    const long long o[3] = {a.offsets[2 * pair], a.offsets[2 * pair + 1], a.offsets[2 * pair + 2]};
+    if (o[0] < 0 || o[1] < o[0] || o[2] < o[1] || o[2] > a.length) r[0] = r[1] = NAN;
+  }
+  const double m = a.beta * (r[0] - r[1]) - a.margin;
+  double value, slope;
+  if (a.kind == PAIR_HINGE) {
+    value = m < 1.0 ? 1.0 - m : m >= 1.0 ? 0.0 : NAN;
+    slope = m < 1.0 ? -1.0 : m >= 1.0 ? 0.0 : NAN;
+  } else {
+    const double e = a.smoothing;
+    value = softplus(-m) * (1.0 - e);
+    slope = -sigmoid(-m) * (1.0 - e);
+    if (e > 0.0) {
+      value += softplus(m) * e;
+      slope += sigmoid(m) * e;
+    }
+  }
+  const bool none = !any && r[0] == 0.0;
+  a.kept[pair] = none ? 0 : 1;
+  a.value[pair] = none ? 0.0f : (float)value;
+  a.ratio[2 * pair] = (float)r[0];
+  a.ratio[2 * pair + 1] = (float)r[1];
+  a.slope[2 * pair] = (float)(-slope * a.beta * each[0]);
+  a.slope[2 * pair + 1] = (float)(slope * a.beta * each[1]);
+}
+
+// A wave a pair.
+__global__ __launch_bounds__(256) void wave_kernel(const PairArgs a, long base) {
+  const long pair = (base + blockIdx.x) * (256 / WAVE) + threadIdx.x / WAVE;
+  if (pair >= a.pairs) return;
+  const int lane = threadIdx.x % WAVE;
+  Sum s[2];
+  for (int k = 0; k < 2; k++) s[k] = wave_sum(sum_of(a, 2 * pair + k, 0, lane, WAVE));
+  if (lane == 0) finish(a, pair, s[0], s[1]);
+}
+
+// A workgroup a pair, or a share of one.
+__global__ __launch_bounds__(MOST) void pair_kernel(const PairArgs a, long base) {
+  __shared__ Sum lds[2][MOST / WAVE];
+  const long block = base + blockIdx.x, pair = block / a.splits;
+  const int split = (int)(block - pair * a.splits);
+  for (int k = 0; k < 2; k++) {
+    const Sum s = wave_sum(sum_of(a, 2 * pair + k, split, threadIdx.x, blockDim.x));
+    if (threadIdx.x % WAVE == 0) lds[k][threadIdx.x / WAVE] = s;
+  }
+  __syncthreads();
+  if (threadIdx.x) return;
+  Sum s[2] = {lds[0][0], lds[1][0]};
+  for (int w = 1; w < (int)blockDim.x / WAVE; w++)
+    for (int k = 0; k < 2; k++) {
+      s[k].sum += lds[k][w].sum;
+      s[k].count += lds[k][w].count;
+    }
+  if (a.splits == 1) return finish(a, pair, s[0], s[1]);
+  for (int k = 0; k < 2; k++) ((Sum*)a.workspace)[block * 2 + k] = s[k];
+}
+// The shares of a pair, a wave each.
+__global__ __launch_bounds__(256) void pair_join_kernel(const PairArgs a) {
+  const long pair = blockIdx.x * (256L / WAVE) + threadIdx.x / WAVE;
+  if (pair >= a.pairs) return;
+  const int lane = threadIdx.x % WAVE;
+  Sum s[2];
+  for (int k = 0; k < 2; k++) s[k] = wave_sum(lane < a.splits ? ((const Sum*)a.workspace)[(pair * a.splits + lane) * 2 + k] : Sum{0.0, 0});
+  if (lane == 0) finish(a, pair, s[0], s[1]);
+}
+
+// `threads` threads a share of a sequence; one sequence more are the tokens of a line before the first and behind the last.
+__global__ __launch_bounds__(256) void grad_kernel(const PairArgs a, int threads, long base) {
+  const long team = (base + blockIdx.x) * (256 / threads) + threadIdx.x / threads, sequence = team / a.splits;
+  const int split = (int)(team - sequence * a.splits), thread = threadIdx.x % threads;
+  const long all = 2 * a.pairs;
+  if (sequence >= all) {
+    if (!a.offsets || sequence > all) return;
+    const long first = min(max((long)a.offsets[0], 0L), a.length), last = min(max((long)a.offsets[all], 0L), a.length);
+    const Tokens t[2] = {share_of({0, first}, split, a.splits), share_of({last, a.length}, split, a.splits)};
+    for (int k = 0; k < 2; k++)
+      for (long i = t[k].from + thread; i < t[k].to; i += threads) a.dloss[i] = 0.0f;
+    return;
+  }
+  const Tokens t = share_of(tokens_of(a, sequence), split, a.splits);
+  const long row = a.offsets ? 0 : sequence;
+  const long long* target = a.target ? a.target + row * a.ldtarget : nullptr;
+  float* d = a.dloss + row * a.lddloss;
+  const float v = a.dvalue[sequence / 2] * a.slope[sequence];
+#pragma unroll 8
+  for (long i = t.from + thread; i < t.to; i += threads) d[i] = !target || target[i] != a.ignore ? v : 0.0f;
+}
+
+long mean_length(long pairs, long length, bool packed) { return packed ? clr::ceil_div(length, std::max(2 * pairs, 1L)) : length; }
+// Shares of a pair: where pairs are few and long, as many as give 256 workgroups, of 8,192 tokens at the least.
+int splits_of(long pairs, long length, bool packed) {
+  const long most = 2 * mean_length(pairs, length, packed) / 8192;
+  return (int)std::max(1L, std::min({clr::ceil_div(256, pairs), most, (long)MOST_SPLITS}));
+}
+
+}  // namespace
+
+size_t preference_workspace(long pairs, long length, bool packed) {
+  const int splits = pairs ? splits_of(pairs, length, packed) : 1;
+  return splits > 1 ? (size_t)pairs * splits * 2 * sizeof(Sum) : 0;
+}
+void preference_launch(PairArgs a, hipStream_t st) {
+  const long mean = mean_length(a.pairs, a.length, a.offsets);
+  a.splits = splits_of(a.pairs, a.length, a.offsets);
+  if (mean <= 64 && a.pairs >= 256) {
+    clr::in_launches(clr::ceil_div(a.pairs, 256 / WAVE), 256, [&](long base, unsigned n) { wave_kernel<<<n, 256, 0, st>>>(a, base); });
+    return;
+  }
+  const int threads = mean <= 1024 ? 256 : MOST;
+  clr::in_launches(a.pairs * a.splits, threads, [&](long base, unsigned n) { pair_kernel<<<n, threads, 0, st>>>(a, base); });
+  if (a.splits > 1) pair_join_kernel<<<clr::groups_of(clr::ceil_div(a.pairs, 256 / WAVE), 256), 256, 0, st>>>(a);
+}
+void preference_grad_launch(PairArgs a, hipStream_t st) {
+  const long mean = mean_length(a.pairs, a.length, a.offsets);
+  const int threads = mean <= 64 ? WAVE : 256;
+  a.splits = (int)std::max(1L, std::min(mean / 2048, 1L << 20));
+  const long teams = (2 * a.pairs + (a.offsets ? 1 : 0)) * a.splits;
+  clr::in_launches(clr::ceil_div(teams, 256 / threads), 256, [&](long base, unsigned n) { grad_kernel<<<n, 256, 0, st>>>(a, threads, base); });
+}

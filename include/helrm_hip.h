@@ -422,6 +422,37 @@ int Embedding(const EmbeddingArgs* args, void* stream);
 long EmbeddingGradWorkspace(const EmbeddingArgs* args);
 int EmbeddingGrad(const EmbeddingArgs* args, void* stream);
 
+/* A loss of pairs of sequences, the first of which is preferred, from their tokens'
+ * losses (negative log probabilities, as CrossEntropy gives them) and those of a
+ * reference model.  With r the sum of reference - loss over a sequence's tokens that
+ * count, or their mean (`average`), and m = beta (r[first] - r[second]) - margin,
+ * kind 0: (1 - smoothing) log(1 + exp(-m)) + smoothing log(1 + exp m), kind 1:
+ * max(0, 1 - m).  Tokens whose target is `ignore` count in nothing, whatever their
+ * losses are; a pair without tokens that count has value 0 and is not kept.
+ * Sequence s is row s of the matrices, or with `offsets` the tokens offsets[s] ..
+ * offsets[s + 1] of one line; offsets that descend or leave the line give NaN.
+ * Sums are of 64 bits.  PreferenceGrad writes the gradient of every token's loss,
+ * 0 of those that count in nothing. */
+typedef struct {
+  const float* loss; long ldloss;        /* [2 pairs][length]; with offsets [length] (no ld is read) */
+  const float* reference; long ldreference; /* as loss, or NULL: 0 */
+  const long long* target; long ldtarget; /* as loss, or NULL: every token counts */
+  const long long* offsets;              /* [2 pairs + 1], or NULL */
+  float* value;                          /* [pairs] */
+  float* ratio; float* slope;            /* [pairs][2]: r, and the derivative of value by each loss of the sequence that counts */
+  long long* kept;                       /* [pairs]: 1, or 0 */
+  const float* dvalue;                   /* [pairs]; PreferenceGrad, which reads slope, target and offsets too */
+  float* dloss; long lddloss;
+  void* workspace; size_t workspaceBytes; /* Preference only */
+  long pairs; long length;
+  long long ignore;
+  int kind; int average;
+  float beta; float margin; float smoothing; /* smoothing 0 to 1; 0 with kind 1 */
+} PreferenceArgs;
+long PreferenceWorkspace(const PreferenceArgs* args);
+int Preference(const PreferenceArgs* args, void* stream);
+int PreferenceGrad(const PreferenceArgs* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
