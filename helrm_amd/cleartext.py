@@ -544,25 +544,25 @@ def distillation(x, table, ids, logits, temperature=1.0, ignore_index=-100, redu
 _KINDS = {"logistic": 0, "hinge": 1}
 
 
-def _lines(t, shape, name, dtype, device, packed):
-    """Token values as the kernels take them, [2 pairs, length] or [length]."""
+def _lines(t, like, name, dtype, packed):
+    """(token values as the kernels take them, elements from one sequence's to the next's): of the shape and device of `like`."""
     if forward_ad._current_level >= 0:
         _no_tangent(t, name)
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name}: {list(t.shape)}, not {list(shape)}")
-    if t.dtype != dtype or t.device != device:
-        raise ValueError(f"{name}: {t.dtype} on {t.device}, not {dtype} on {device}")
-    if packed:
-        return t.contiguous()
-    rows, length = math.prod(shape[:-1]), shape[-1]
-    t = t.reshape(rows, length)
-    if (length > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < length):
+    if t.shape != like.shape:
+        raise ValueError(f"{name}: {list(t.shape)}, not {list(like.shape)}")
+    if t.dtype != dtype or t.device != like.device:
+        raise ValueError(f"{name}: {t.dtype} on {t.device}, not {dtype} on {like.device}")
+    length = t.shape[-1]
+    if packed or t.is_contiguous():
+        return t.contiguous(), length
+    t = t.flatten(0, -2)
+    if (length > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < length):
         t = t.contiguous()
-    return t
+    return t, t.stride(0) if t.shape[0] > 1 else length
 
 
 def _pairs(losses, target, offsets, ignore_index):
-    """(leading dimensions of a pair, number of pairs, length, target, offsets)."""
+    """(leading dimensions of a pair, number of pairs, length, target and its ld, offsets)."""
     _need(-(1 << 63) <= ignore_index < 1 << 63, "ignore_index: not an int64")
     if losses.dtype != torch.float32:
         raise ValueError(f"losses: {losses.dtype}, not {torch.float32}")
@@ -579,36 +579,38 @@ def _pairs(losses, target, offsets, ignore_index):
         raise ValueError("losses: not on the GPU")
     if offsets is not None:
         offsets = _vector(offsets, 2 * pairs + 1, "offsets", torch.int64, losses.device)
-    if target is not None:
-        target = _lines(target, losses.shape, "target", torch.int64, losses.device, offsets is not None)
-    return lead, pairs, losses.shape[-1], target, offsets
+    target, ld = (None, 0) if target is None else _lines(target, losses, "target", torch.int64, offsets is not None)
+    return lead, pairs, losses.shape[-1], target, ld, offsets
 
 
-def _line_ld(t, packed):
-    return 0 if t is None or packed else t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _values(t, name, device):
+    if forward_ad._current_level >= 0:
+        _no_tangent(t, name)
+    if t.dtype != torch.float32 or t.device != device:
+        raise ValueError(f"{name}: {t.dtype} on {t.device}, not {torch.float32} on {device}")
+    return t.contiguous()
 
 
 def _pointer(t):
     return None if t is None else t.data_ptr()
 
 
-def _preference_forward(losses, reference, target, offsets, beta, margin, kind, smoothing, average, ignore_index):
+def _preference_forward(losses, reference, target, offsets, beta, margin, kind, smoothing, average, ignore_index, keep=True):
     _need(kind in _KINDS, f"kind {kind!r}: neither logistic nor hinge")
     _need(math.isfinite(beta) and math.isfinite(margin), "beta and margin are not finite")
     _need(0.0 <= smoothing <= (1.0 if kind == "logistic" else 0.0), f"smoothing {smoothing}: not from 0 to 1, or not 0 with the hinge")
-    lead, pairs, length, target, offsets = _pairs(losses, target, offsets, ignore_index)
-    packed, shape, device = offsets is not None, losses.shape, losses.device
-    losses = _lines(losses, shape, "losses", torch.float32, device, packed)
-    if reference is not None:
-        reference = _lines(reference, shape, "reference", torch.float32, device, packed)
+    lead, pairs, length, target, ldtarget, offsets = _pairs(losses, target, offsets, ignore_index)
+    packed, device = offsets is not None, losses.device
+    held, ldreference = (None, 0) if reference is None else _lines(reference, losses, "reference", torch.float32, packed)
+    losses, ldloss = _lines(losses, losses, "losses", torch.float32, packed)
     values = torch.empty(lead, dtype=torch.float32, device=device)
-    ratios, slopes = (torch.empty((*lead, 2), dtype=torch.float32, device=device) for _ in "ab")
-    kept = torch.empty(pairs, dtype=torch.int64, device=device)
+    ratios = torch.empty((*lead, 2), dtype=torch.float32, device=device)
+    slopes = torch.empty_like(ratios)
+    kept = torch.empty(pairs, dtype=torch.int64, device=device) if keep else None
     _call("Preference", PreferenceArgs(
-        loss=losses.data_ptr(), ldloss=_line_ld(losses, packed), reference=_pointer(reference), ldreference=_line_ld(reference, packed),
-        target=_pointer(target), ldtarget=_line_ld(target, packed), offsets=_pointer(offsets), value=values.data_ptr(), ratio=ratios.data_ptr(),
-        slope=slopes.data_ptr(), kept=kept.data_ptr(), pairs=pairs, length=length, ignore=ignore_index, kind=_KINDS[kind], average=bool(average),
-        beta=beta, margin=margin, smoothing=smoothing), device)
+        loss=losses.data_ptr(), ldloss=ldloss, reference=_pointer(held), ldreference=ldreference, target=_pointer(target), ldtarget=ldtarget,
+        offsets=_pointer(offsets), value=values.data_ptr(), ratio=ratios.data_ptr(), slope=slopes.data_ptr(), kept=_pointer(kept), pairs=pairs,
+        length=length, ignore=ignore_index, kind=_KINDS[kind], average=bool(average), beta=beta, margin=margin, smoothing=smoothing), device)
     return values, ratios, slopes, kept
 
 
@@ -620,23 +622,22 @@ def preference_forward(losses, reference=None, target=None, offsets=None, beta=0
     sequence s the tokens from offsets[s] to offsets[s + 1].  Tokens whose target is `ignore_index` count in nothing.
     With m = beta * (ratio of the first - of the second) - margin: "logistic" (1 - smoothing) log(1 + exp -m) + smoothing log(1 +
     exp m), "hinge" max(0, 1 - m).  A pair without tokens that count has 0; offsets that descend or leave the tokens give NaN."""
-    return _preference_forward(losses, reference, target, offsets, beta, margin, kind, smoothing, average, ignore_index)[:3]
+    return _preference_forward(losses, reference, target, offsets, beta, margin, kind, smoothing, average, ignore_index, False)[:3]
 
 
 def preference_backward(grad, losses, slopes, target=None, offsets=None, ignore_index=-100):
     """The gradient of every token's loss, of losses' shape, for the gradient `grad` of the values; slopes as the forward call gave
     them.  Tokens that count in nothing have 0."""
-    lead, pairs, length, target, offsets = _pairs(losses, target, offsets, ignore_index)
-    packed, device = offsets is not None, losses.device
-    if tuple(grad.shape) != tuple(lead):
+    lead, pairs, length, target, ldtarget, offsets = _pairs(losses, target, offsets, ignore_index)
+    device = losses.device
+    if grad.shape != lead:
         raise ValueError(f"grad: {list(grad.shape)}, not {list(lead)}")
-    grad = _vector(grad.reshape(-1), pairs, "grad", torch.float32, device)
-    if tuple(slopes.shape) != (*lead, 2):
+    if slopes.shape != (*lead, 2):
         raise ValueError(f"slopes: {list(slopes.shape)}, not {[*lead, 2]}")
-    slopes = _vector(slopes.reshape(-1), 2 * pairs, "slopes", torch.float32, device)
+    grad, slopes = (_values(t, name, device) for t, name in ((grad, "grad"), (slopes, "slopes")))
     d = torch.empty(losses.shape, dtype=torch.float32, device=device)
     _call("PreferenceGrad", PreferenceArgs(
-        target=_pointer(target), ldtarget=_line_ld(target, packed), offsets=_pointer(offsets), slope=slopes.data_ptr(), dvalue=grad.data_ptr(),
+        target=_pointer(target), ldtarget=ldtarget, offsets=_pointer(offsets), slope=slopes.data_ptr(), dvalue=grad.data_ptr(),
         dloss=d.data_ptr(), lddloss=length, pairs=pairs, length=length, ignore=ignore_index), device)
     return d
 

@@ -693,7 +693,7 @@ int Preference(const PreferenceArgs* a, void* stream) {
     check_tokens(a, a->loss, a->ldloss, "Preference: loss");
     if (a->reference) check_tokens(a, a->reference, a->ldreference, "Preference: reference");
     if (a->target) check_tokens(a, a->target, a->ldtarget, "Preference: target");
-    require((a->value && a->ratio && a->slope && a->kept) || !a->pairs, "Preference: value, ratio, slope and kept");
+    require((a->value && a->ratio && a->slope) || !a->pairs, "Preference: value, ratio and slope");
     check_space(a->workspace, a->workspaceBytes, preference_workspace(a->pairs, a->length, a->offsets));
     if (!a->pairs) return;
     PairArgs p = pair_args(a);

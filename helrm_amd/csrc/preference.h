@@ -12,7 +12,7 @@ struct PairArgs {
   const long long* target; long ldtarget;     // may be null: every token counts
   const long long* offsets;
   float* value; float* ratio; float* slope;   // [pairs], [pairs][2], [pairs][2]
-  long long* kept;                            // [pairs]: whether a token of the pair counts
+  long long* kept;                            // [pairs]: whether a token of the pair counts; may be null
   const float* dvalue;                        // backward
   float* dloss; long lddloss;
   void* workspace;

@@ -17,6 +17,7 @@ namespace {
 struct Sum { double sum; long count; };
 constexpr int WAVE = 64, MOST = 1024;
 constexpr int MOST_SPLITS = 64;
+constexpr int EACH = 4;   // tokens a thread at once
 
 __device__ __forceinline__ Sum wave_sum(Sum s) {
 #pragma unroll
@@ -48,13 +49,25 @@ __device__ __forceinline__ Sum sum_of(const PairArgs& a, long sequence, int spli
   const float* reference = a.reference ? a.reference + row * a.ldreference : nullptr;
   const long long* target = a.target ? a.target + row * a.ldtarget : nullptr;
   Sum s{0.0, 0};
-#pragma unroll 4
-  for (long i = t.from + thread; i < t.to; i += threads) {
-    const bool counts = !target || target[i] != a.ignore;
-    const double d = (reference ? (double)reference[i] : 0.0) - (double)loss[i];
-    s.sum += counts ? d : 0.0;
+  auto add = [&](float l, float r, long long t) {
+    const bool counts = !target || t != a.ignore;
+    s.sum += counts ? (double)r - (double)l : 0.0;
     s.count += counts;
+  };
+  // four tokens at a time (loads of 16 bytes need no alignment)
+  const long whole = t.from + (t.to - t.from) / EACH * EACH;
+#pragma unroll 2
+  for (long i = t.from + thread * EACH; i < whole; i += threads * EACH) {
+    float l[EACH], r[EACH] = {};
+    long long k[EACH] = {};
+    __builtin_memcpy(l, loss + i, sizeof(l));
+    if (reference) __builtin_memcpy(r, reference + i, sizeof(r));
+    if (target) __builtin_memcpy(k, target + i, sizeof(k));
+#pragma unroll
+    for (int e = 0; e < EACH; e++) add(l[e], r[e], k[e]);
   }
+  const long i = whole + thread;
+  if (i < t.to) add(loss[i], reference ? reference[i] : 0.0f, target ? target[i] : 0);
   return s;
 }
 
@@ -85,7 +98,7 @@ __device__ __forceinline__ void finish(const PairArgs& a, long pair, Sum first, 
     }
   }
   const bool none = !any && r[0] == 0.0;
-  a.kept[pair] = none ? 0 : 1;
+  if (a.kept) a.kept[pair] = none ? 0 : 1;
   a.value[pair] = none ? 0.0f : (float)value;
   a.ratio[2 * pair] = (float)r[0];
   a.ratio[2 * pair + 1] = (float)r[1];
@@ -151,8 +164,18 @@ __global__ __launch_bounds__(256) void grad_kernel(const PairArgs a, int threads
   const long long* target = a.target ? a.target + row * a.ldtarget : nullptr;
   float* d = a.dloss + row * a.lddloss;
   const float v = a.dvalue[sequence / 2] * a.slope[sequence];
-#pragma unroll 8
-  for (long i = t.from + thread; i < t.to; i += threads) d[i] = !target || target[i] != a.ignore ? v : 0.0f;
+  const long whole = t.from + (t.to - t.from) / EACH * EACH;
+#pragma unroll 2
+  for (long i = t.from + thread * EACH; i < whole; i += threads * EACH) {
+    long long k[EACH];
+    float o[EACH];
+    if (target) __builtin_memcpy(k, target + i, sizeof(k));
+#pragma unroll
+    for (int e = 0; e < EACH; e++) o[e] = !target || k[e] != a.ignore ? v : 0.0f;
+    __builtin_memcpy(d + i, o, sizeof(o));
+  }
+  const long i = whole + thread;
+  if (i < t.to) d[i] = !target || target[i] != a.ignore ? v : 0.0f;
 }
 
 long mean_length(long pairs, long length, bool packed) { return packed ? clr::ceil_div(length, std::max(2 * pairs, 1L)) : length; }

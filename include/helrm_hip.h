@@ -440,7 +440,7 @@ typedef struct {
   const long long* offsets;              /* [2 pairs + 1], or NULL */
   float* value;                          /* [pairs] */
   float* ratio; float* slope;            /* [pairs][2]: r, and the derivative of value by each loss of the sequence that counts */
-  long long* kept;                       /* [pairs]: 1, or 0 */
+  long long* kept;                       /* [pairs]: 1, or 0; may be NULL */
   const float* dvalue;                   /* [pairs]; PreferenceGrad, which reads slope, target and offsets too */
   float* dloss; long lddloss;
   void* workspace; size_t workspaceBytes; /* Preference only */

@@ -47,8 +47,8 @@ def test_refusals_of_the_entry_points(lib):
         refused(lib, call, args(kind=1, smoothing=0.1), "smoothing")
         refused(lib, call, args(ldtarget=7), "target")
         refused(lib, call, args(slope=None), "slope")
-    for name in ("value", "ratio", "kept"):
-        refused(lib, "Preference", args(**{name: None}), "value, ratio, slope and kept")
+    for name in ("value", "ratio"):
+        refused(lib, "Preference", args(**{name: None}), "value, ratio and slope")
     refused(lib, "Preference", args(loss=None), ": loss")
     refused(lib, "Preference", args(loss=None, offsets=SOME), ": loss")
     refused(lib, "Preference", args(ldloss=7), ": loss")
