@@ -73,7 +73,7 @@ class LossTotalArgs(ctypes.Structure):
 class DistillationArgs(ctypes.Structure):
     _fields_ = [("x", ctypes.c_void_p), ("ldx", ctypes.c_long), ("table", ctypes.c_void_p), ("ldtable", ctypes.c_long),
                 ("ids", ctypes.c_void_p), ("logits", ctypes.c_void_p), ("loss", ctypes.c_void_p), ("lse", ctypes.c_void_p),
-                ("kept", ctypes.c_void_p), ("scores", ctypes.c_void_p), ("probs", ctypes.c_void_p),
+                ("kept", ctypes.c_void_p), ("scores", ctypes.c_void_p), ("probs", ctypes.c_void_p), ("cols", ctypes.c_void_p),
                 ("dloss", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("lddx", ctypes.c_long), ("dtable", ctypes.c_void_p),
                 ("workspace", ctypes.c_void_p), ("workspaceBytes", ctypes.c_size_t),
                 ("rows", ctypes.c_long), ("width", ctypes.c_int), ("vocab", ctypes.c_int), ("top", ctypes.c_int),

@@ -472,11 +472,11 @@ def distillation_forward(x, table, ids, logits, temperature=1.0, ignore_index=-1
     losses = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     lse = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
     kept = torch.empty(rows, dtype=torch.int64, device=x.device)
-    held = torch.empty((2, rows, top), dtype=torch.float32, device=x.device)
+    held = torch.empty((3, rows, top), dtype=torch.float32, device=x.device)     # scores, probabilities, and int32 ids
     _call("Distillation", DistillationArgs(
         x=x2.data_ptr(), ldx=_ld(x2), table=table.data_ptr(), ldtable=_ld(table), ids=ids2.data_ptr(), logits=logits.data_ptr(),
-        loss=losses.data_ptr(), lse=lse.data_ptr(), kept=kept.data_ptr(), scores=held.data_ptr(), probs=held.data_ptr() + 2 * held.numel(),
-        rows=rows, width=table.shape[1], vocab=table.shape[0], top=top, type=_TYPES[x.dtype], teacherType=_TYPES[logits.dtype],
+        loss=losses.data_ptr(), lse=lse.data_ptr(), kept=kept.data_ptr(), scores=held.data_ptr(), probs=held.data_ptr() + 4 * rows * top,
+        cols=held.data_ptr() + 8 * rows * top, rows=rows, width=table.shape[1], vocab=table.shape[0], top=top, type=_TYPES[x.dtype], teacherType=_TYPES[logits.dtype],
         ignore=ignore_index, temperature=temperature), x.device)
     return losses, lse, (kept, held)
 
@@ -492,13 +492,13 @@ def distillation_backward(grad, x, table, ids, lse, saved, temperature=1.0, igno
     lse = _vector(lse.reshape(-1), rows, "lse", torch.float32, x.device)
     kept, held = saved
     _need(tuple(kept.shape) == (rows,) and kept.dtype == torch.int64 and kept.device == x.device and kept.is_contiguous()
-          and tuple(held.shape) == (2, *ids.shape) and held.dtype == torch.float32 and held.device == x.device and held.is_contiguous(),
+          and tuple(held.shape) == (3, *ids.shape) and held.dtype == torch.float32 and held.device == x.device and held.is_contiguous(),
           "saved: not what the forward call returned")
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     dtable = torch.empty(table.shape, dtype=x.dtype, device=x.device)
     _call("DistillationGrad", DistillationArgs(
-        x=x2.data_ptr(), ldx=_ld(x2), table=table.data_ptr(), ldtable=_ld(table), ids=ids.data_ptr(), lse=lse.data_ptr(), kept=kept.data_ptr(),
-        scores=held.data_ptr(), probs=held.data_ptr() + 2 * held.numel(), dloss=grad.data_ptr(), dx=dx.data_ptr(), lddx=width,
+        x=x2.data_ptr(), ldx=_ld(x2), table=table.data_ptr(), ldtable=_ld(table), lse=lse.data_ptr(), kept=kept.data_ptr(),
+        scores=held.data_ptr(), probs=held.data_ptr() + 4 * ids.numel(), cols=held.data_ptr() + 8 * ids.numel(), dloss=grad.data_ptr(), dx=dx.data_ptr(), lddx=width,
         dtable=dtable.data_ptr(), rows=rows, width=width, vocab=table.shape[0], top=ids.shape[1], type=_TYPES[x.dtype],
         teacherType=_TYPES[x.dtype], ignore=ignore_index, temperature=temperature), x.device)
     return dx, dtable

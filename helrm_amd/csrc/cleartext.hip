@@ -404,17 +404,37 @@ void check_teach(const DistillationArgs* a) {
 void check_teach_tensors(const DistillationArgs* a) {
   check_matrix(a->x, a->ldx, a->rows, a->width, "Distillation: x");
   check_matrix(a->table, a->ldtable, a->vocab, a->width, "Distillation: table");
-  require(a->ids || !a->rows, "Distillation: ids");
   require(a->lse || !a->rows, "Distillation: lse");
-  require((a->kept && a->scores && a->probs) || !a->rows, "Distillation: kept, scores and probs");
+  require((a->kept && a->scores && a->probs && a->cols) || !a->rows, "Distillation: kept, scores, probs and cols");
+}
+
+// Whether the entries' scores are picked out of the product's tiles, or
+// computed from the table's rows.  Microseconds, measured: the rows at 3.4 TB/s
+// (a common one comes from the caches); two launches more, a row's order 0.005,
+// the end of a tile 1.6.  8,192 x 2,048 against 131,072 rows, 64 entries, bfloat16,
+// both directions: 14,350 picked, 14,890 computed; 1,999 x 416 against 50,021,
+// 17 entries, float32: 2,253 and 2,243.
+bool teach_picks(const DistillationArgs* a) {
+  const double tiles = (double)clr::ceil_div(a->rows, 256) * (double)clr::ceil_div(a->vocab, 256);
+  const double computed = (double)a->rows * a->top * a->width * dtype_size(a->type) / 3.4e6;
+  return computed > 5 + 0.005 * (double)a->rows + 1.6 * tiles / 256;
 }
 
 size_t teach_forward(const DistillationArgs* a, bool count, hipStream_t st) {
   Arena m{count ? nullptr : (char*)a->workspace};
   const long n = a->rows;
   const float rate = 1.0f / a->temperature;
-  TeachArgs e{a->x, a->ldx, a->table, a->ldtable, a->ids, a->logits, a->scores, a->probs, a->kept, n, a->width, a->vocab, a->top, a->type,
-              a->teacherType, a->ignore, a->temperature, 0};
+  TeachArgs e{};
+  e.x = a->x; e.ldx = a->ldx;
+  e.table = a->table; e.ldtable = a->ldtable;
+  e.ids = a->ids; e.logits = a->logits;
+  e.scores = a->scores; e.probs = a->probs; e.cols = a->cols;
+  e.kept = a->kept;
+  e.rows = n; e.width = a->width; e.vocab = a->vocab; e.top = a->top;
+  e.dtype = a->type; e.teacher_type = a->teacherType;
+  e.ignore = a->ignore;
+  e.temperature = a->temperature;
+  e.parts = n ? entry_parts(n, a->top) : 1;
   TeachFinish f{};
   f.scores = a->scores; f.probs = a->probs; f.kept = a->kept;
   f.loss = a->loss; f.lse = a->lse;
@@ -429,8 +449,8 @@ size_t teach_forward(const DistillationArgs* a, bool count, hipStream_t st) {
     p.rate = rate;
     f.parts = skinny_softmax_parts(a->vocab);
     f.part = p.part = m.take<float2>((size_t)n * f.parts);
+    p.entries = e;
     if (count) return m.used;
-    teach_entries(e, st);
     skinny_teach(p, st);
     teach_finish(f, st);
     return m.used;
@@ -441,12 +461,21 @@ size_t teach_forward(const DistillationArgs* a, bool count, hipStream_t st) {
   r.loss = a->loss; r.lse = a->lse;
   const Held x = hold(m, n, a->width, a->type);
   float2* part = m.take<float2>((size_t)n * plan.parts);
+  const bool picks = teach_picks(a);
+  if (picks) {
+    e.starts = m.take<uint16_t>((size_t)n * (plan.parts + 1));
+    e.tiles = plan.parts;
+    e.shift = plan.plan.big ? 8 : 7;
+    e.which = r.rows; e.count = r.count;
+  }
   Copies copy;
   copy.add(x, a->x, a->ldx, n, a->width, r.rows, r.count);
   const Held table = copy.held(m, a->table, a->ldtable, a->vocab, a->width, a->type);
   if (count) return m.used;
-  teach_entries(e, st);
+  if (picks) teach_kept(e, st);
+  else teach_entries(e, st);
   kept_rows(r, st);
+  if (picks) teach_order(e, st);
   lay_out(copy.j, copy.n, a->type, st);
   ProductArgs p{};
   p.dtype = a->type;
@@ -454,6 +483,8 @@ size_t teach_forward(const DistillationArgs* a, bool count, hipStream_t st) {
   add_pairs(p, x, table);
   p.count = r.count; p.part = part;
   p.rate = rate;
+  p.starts = e.starts; p.ldstarts = plan.parts + 1;
+  p.rows = r.rows; p.cols = a->cols; p.scores = a->scores; p.top = a->top;
   product_teach(p, plan, st);
   f.part = part; f.parts = plan.parts;
   f.rows = r.rows; f.count = r.count;
@@ -471,7 +502,7 @@ size_t teach_backward(const DistillationArgs* a, bool count, hipStream_t st) {
     t.dl = (uint16_t*)dl.p; t.ld = dl.ld; t.part = dl.part;
     t.rows = r.rows; t.tgt = r.tgt; t.count = r.count;
     t.lse = r.lse_kept; t.grad = r.grad_kept; t.scale = r.scale;
-    t.ids = a->ids; t.scores = a->scores; t.probs = a->probs;
+    t.cols = a->cols; t.scores = a->scores; t.probs = a->probs;
     t.n = a->rows; t.top = a->top; t.dtype = a->type;
     t.v0 = p.n0; t.len = p.N;
     teach_patch(t, st);
@@ -645,6 +676,7 @@ int Distillation(const DistillationArgs* a, void* stream) {
   return clr::guarded([&] {
     check_teach(a);
     check_teach_tensors(a);
+    require(a->ids || !a->rows, "Distillation: ids");
     require(a->logits || !a->rows, "Distillation: logits");
     require(a->loss || !a->rows, "Distillation: loss");
     if (!a->rows) return;

@@ -41,6 +41,10 @@ struct ProductArgs {
   const float* lse; const float* grad;  // of row i of the tiles
   const float* scale;        // the gradient's factor in a 16-bit type
   float rate;                // teach: of the logits, 1 / temperature
+  // (may be null) the columns of each row whose logits are wanted, in order: those of row m in tile n are number
+  // starts[m][n] .. starts[m][n + 1] of cols[rows[m]][top], whose logits go to scores
+  const uint16_t* starts; long ldstarts;
+  const int* rows; const int* cols; float* scores; int top;
 };
 
 // h = act(A B^T) * (A B2^T); rows of all three run along k

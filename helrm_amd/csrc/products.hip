@@ -54,7 +54,6 @@ struct Batch {
 constexpr unsigned OUTSIDE = 0x80000000u;  // an offset past every descriptor's bound
 
 enum Epi { EPI_STORE, EPI_GATE, EPI_GATE_GRAD, EPI_SOFTMAX, EPI_SOFTMAX_GRAD, EPI_TEACH, EPI_TEACH_GRAD };
-constexpr bool is_softmax(int epi) { return epi == EPI_SOFTMAX || epi == EPI_TEACH; }
 constexpr bool is_softmax_grad(int epi) { return epi == EPI_SOFTMAX_GRAD || epi == EPI_TEACH_GRAD; }
 
 __device__ __forceinline__ u16 bits(__bf16 v) { return __builtin_bit_cast(u16, v); }
@@ -205,6 +204,48 @@ __device__ __forceinline__ void tile_of(int id, int total, int nm, int nn, int& 
   n = in / rows;
 }
 
+// A wave's accumulators, 64 rows of 64 float32 columns of them, into its own
+// part of LDS: 16 bytes c of row r at c ^ (r & 15).
+template <int FM> __device__ __forceinline__ void stage(const f32x4 (&acc)[FM][4], int part, float* own) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      const int r = i * 16 + (lane & 15), at = j * 4 + (lane >> 4);
+      *(f32x4*)(own + r * 64 + ((at ^ (r & 15)) * 4)) = acc[part * 4 + i][j];
+    }
+}
+
+// The logits that are wanted of a wave's rows and columns, a lane a row.
+// span: of row r of the tile, the first and last + 1 of them, and where the row's are.
+struct Span { unsigned which; int row; };
+template <int FM> struct Wanted { long at[FM / 4]; unsigned left[FM / 4]; int column[FM / 4]; };
+template <int FM> __device__ __forceinline__ Wanted<FM> wanted(const ProductArgs& p, int r0, const Span* spans) {
+  Wanted<FM> w;
+#pragma unroll
+  for (int part = 0; part < FM / 4; part++) {
+    const Span s = spans[r0 + part * 64 + (threadIdx.x & 63)];
+    w.left[part] = (s.which >> 16) - (s.which & 0xffff);
+    w.at[part] = (long)s.row * p.top + (s.which & 0xffff);
+    w.column[part] = w.left[part] ? p.cols[w.at[part]] : 0;
+  }
+  return w;
+}
+template <int FM> __device__ __forceinline__ void pick(const ProductArgs& p, const f32x4 (&acc)[FM][4], long column, Wanted<FM>& w, float* own) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int part = 0; part < FM / 4; part++) {
+    stage(acc, part, own);
+    while (w.left[part]) {
+      const long c = w.column[part] - column;
+      if (c >= 0 && c < 64) p.scores[w.at[part]] = own[lane * 64 + (((int)c / 4 ^ (lane & 15)) * 4) + (int)c % 4] * p.rate;
+      w.at[part]++;
+      if (--w.left[part]) w.column[part] = p.cols[w.at[part]];
+    }
+  }
+}
+
 // A row's maximum and sum over the tile's columns: over the lane's, over the
 // four lanes that share the row, over the waves beside one another.  acc[i][j][e]
 // is (m, n) = (mw + 16 i + lane % 16, n_wave + 16 j + 4 (lane / 16) + e).
@@ -319,8 +360,8 @@ template <int EPI> __device__ __host__ __forceinline__ long sum_cols(const Produ
 template <int EPI> __device__ __host__ __forceinline__ long sum_ld(const ProductArgs& p) { return sum_cols<EPI>(p) * (EPI == EPI_GATE ? 2 : 1); }
 
 // A wave's accumulators go through its own part of LDS, 64 rows of 64 float32
-// columns at a time (16 bytes c of row r at c ^ (r & 15)), so that what is
-// stored are whole lines of a row and the code of it is there once.  A place is
+// columns at a time, so that what is stored are whole lines of a row and the
+// code of it is there once.  A place is
 // a 32-bit offset from the wave's first element: of up to 128 rows, which are
 // under 2^24 elements apart in a caller's result, 2^21 in an intermediate, 2^22
 // in split sums; all the rows of a loss's dl are under 2^27 elements, or 2^10
@@ -340,13 +381,7 @@ __device__ __forceinline__ void emit(const ProductArgs& p, const f32x4 (&acc)[FM
   static_assert(FN == 4 && FM % 4 == 0, "64 x 64 a time");
 #pragma unroll
   for (int part = 0; part < FM / 4; part++) {
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int r = i * 16 + (lane & 15), at = j * 4 + (lane >> 4);
-        *(f32x4*)(own + r * 64 + ((at ^ (r & 15)) * 4)) = acc[part * 4 + i][j];
-      }
+    stage(acc, part, own);
     const long first = (sums ? (long)split * p.M * ld : 0) + mw * ld + n_wave;
     // columns that there are from the lane's first one on, and columns with the zeros that fill an intermediate's row up
     const int left = (int)min((long)p.N - n_wave, 64L) - col * 4;
@@ -443,6 +478,17 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Batch batch)
   if (m0 >= M) return;
   // a row along k is filled up with zeros to a multiple of 8
   const int KA = A_K ? (K + 7) & ~7 : K, KB = B_K ? (K + 7) & ~7 : K;
+
+  __shared__ Span spans[EPI == EPI_TEACH ? BM : 1];
+  if constexpr (EPI == EPI_TEACH)
+    if (p.starts && threadIdx.x < BM) {   // (read after the last barrier)
+      Span s{0, 0};
+      if (m0 + threadIdx.x < M) {
+        const uint16_t* at = p.starts + (m0 + threadIdx.x) * p.ldstarts + tile_n;
+        s = {at[0] | (unsigned)at[1] << 16, p.rows[m0 + threadIdx.x]};
+      }
+      spans[threadIdx.x] = s;
+    }
 
   constexpr int LA = Loader<A_K, BM, W>::N, LB = Loader<B_K, BN, W>::N;
   static_assert(LA == 4 && LB == 4, "the steps below");
@@ -577,12 +623,18 @@ __global__ __launch_bounds__(WM* WN * 64) void product_kernel(const Batch batch)
   }
   if (PARTS && corrections >= to - from) settle();
   arrive<0>();   // no load may still write LDS when it is used again, or given away
-  if constexpr (is_softmax(EPI)) {
-    softmax_piece<EPI == EPI_TEACH, FM, FN, WM, WN>(p, acc, M, m0, n0, wave_m, wave_n, tile_n, (float2*)a0);
+  const int q = BM == 256 ? wave >> 1 : wave;   // 16 KiB of LDS a wave
+  float* mine = (float*)((q == 0 ? a0 : q == 1 ? b0 : q == 2 ? a1 : b1) + (BM == 256 ? (wave & 1) * 8192 : 0));
+  if constexpr (EPI == EPI_SOFTMAX) {
+    softmax_piece<false, FM, FN, WM, WN>(p, acc, M, m0, n0, wave_m, wave_n, tile_n, (float2*)a0);
+  } else if constexpr (EPI == EPI_TEACH) {
+    __shared__ float2 pieces[BM * WN];   // (the rest is for the logits)
+    Wanted<FM> w;
+    if (p.starts) w = wanted<FM>(p, wave_m * FM * 16, spans);   // (the first ones arrive meanwhile)
+    softmax_piece<true, FM, FN, WM, WN>(p, acc, M, m0, n0, wave_m, wave_n, tile_n, pieces);
+    if (p.starts) pick<FM>(p, acc, p.n0 + n0 + wave_n * FN * 16, w, mine);
   } else {
-    const int q = BM == 256 ? wave >> 1 : wave;   // 16 KiB a wave
-    u16* mine = (q == 0 ? a0 : q == 1 ? b0 : q == 2 ? a1 : b1) + (BM == 256 ? (wave & 1) * 8192 : 0);
-    emit<T, EPI, FM, FN>(p, acc, M, m0 + wave_m * FM * 16, n0 + wave_n * FN * (EPI == EPI_GATE ? 8 : 16), split, (float*)mine);
+    emit<T, EPI, FM, FN>(p, acc, M, m0 + wave_m * FM * 16, n0 + wave_n * FN * (EPI == EPI_GATE ? 8 : 16), split, mine);
   }
 }
 
@@ -882,6 +934,7 @@ template <int EPI> static void softmax_launches(const ProductArgs& p, const clr:
     for (int k = 0; k < q.pairs; k++) q.b[k] += v0 * q.ldb;
     q.parts = plan.parts;
     q.part += v0 / plan.plan.tile();
+    if (q.starts) q.starts += v0 / plan.plan.tile();
     launch<true, true, EPI>({q}, plan.plan, st);
   }
 }

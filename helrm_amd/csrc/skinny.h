@@ -1,6 +1,7 @@
 // skinny.h -- launches of skinny.hip.
 #pragma once
 #include "cleartext.h"
+#include "teacher.h"
 
 inline long skinny_rows(int dtype) { return dtype == DT_F32 ? 64 : 16; }   // the most rows of X
 
@@ -15,6 +16,7 @@ struct SkinnyArgs {
   const long long* target; float* picked; float2* part;   // softmax: [T], [T], [T][parts]
   int parts, groups; bool alone;     // (of the launch)
   float rate;                        // teach: of the products
+  TeachArgs entries; int entry_groups;   // teach: of the rows of X; the workgroups that have them, rows * parts of the first ones
 };
 // out = act(X W^T) * (X W2^T)
 void skinny_gate(SkinnyArgs p, hipStream_t st);
@@ -23,5 +25,5 @@ void skinny_store(SkinnyArgs p, hipStream_t st);
 // loss and lse of every row of X against the rows of W
 int skinny_softmax_parts(int N);
 void skinny_softmax(SkinnyArgs p, long long ignore, float* loss, float* lse, hipStream_t st);
-// the pieces of the softmax of rate X W^T, p.part, of every row of X
+// the pieces of the softmax of rate X W^T, p.part, of every row of X, and teach_entries of p.entries beside it
 void skinny_teach(SkinnyArgs p, hipStream_t st);

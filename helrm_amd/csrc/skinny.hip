@@ -18,6 +18,7 @@
 // (a copy: 4.95); the gate and up projections of one row of 1,024 to 4,096, 17
 // MB, 6.5 us; the down projection, 8 MB, 10.7 us: its 1,024 results are 64
 // workgroups, on a quarter of the CUs.
+#include "entries.h"
 #include "skinny.h"
 #include "tiles.h"
 
@@ -109,10 +110,17 @@ template <class T, bool ALIGNED, int NB> constexpr int most_waves() { return siz
 template <class T, class X, bool ALIGNED, int NB, int EPI>
 __global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_kernel(const SkinnyArgs p) {
   constexpr int MATS = EPI == SKINNY_GATE ? 2 : 1, TURNS = !ALIGNED || sizeof(T) == 4 ? 2 : 4;
-  extern __shared__ float lds[];   // [waves][MATS * NB][64][4]
+  extern __shared__ __align__(16) float lds[];   // [waves][MATS * NB][64][4]
+  if constexpr (EPI == SKINNY_TEACH)
+    if ((int)blockIdx.x < p.entry_groups) {   // (beside the others, which the memory holds up)
+      if (p.entries.teacher_type == DT_F32) row_entries<T, float>(p.entries, blockIdx.x, (char*)lds);
+      else row_entries<T, T>(p.entries, blockIdx.x, (char*)lds);
+      return;
+    }
+  const int block = EPI == SKINNY_TEACH ? blockIdx.x - p.entry_groups : blockIdx.x;
   const int lane = threadIdx.x & 63, own = threadIdx.x >> 6;
   const int wave = p.alone ? 0 : own, waves = p.alone ? 1 : blockDim.x >> 6;   // of those that share k
-  const long team = p.alone ? (long)blockIdx.x * (blockDim.x >> 6) + own : blockIdx.x;
+  const long team = p.alone ? (long)block * (blockDim.x >> 6) + own : block;
   const int t = lane & 15, quad = lane >> 4;
   float2 run[NB];   // softmax: the team's piece of row t (of wave b)
 #pragma unroll
@@ -276,8 +284,8 @@ template <int EPI> void launch(SkinnyArgs p, hipStream_t st) {
     auto go = [&](auto nb) {
       constexpr int NB = decltype(nb)::value;
       const int waves = p.alone ? 4 : waves_of(p.N, p.K, p.dtype, aligned ? most_waves<T, true, NB>() : most_waves<T, false, NB>());
-      const unsigned grid = clr::groups_of(p.alone ? clr::ceil_div(teams, 4) : teams, waves * 64);
-      const size_t lds = (size_t)waves * (EPI == SKINNY_GATE ? 2 : 1) * NB * 1024;
+      const unsigned grid = clr::groups_of((p.alone ? clr::ceil_div(teams, 4) : teams) + p.entry_groups, waves * 64);
+      const size_t lds = std::max((size_t)waves * (EPI == SKINNY_GATE ? 2 : 1) * NB * 1024, EPI == SKINNY_TEACH ? entries_bytes(p.entries.top) : 0);
       if (aligned) skinny_kernel<T, X, true, NB, EPI><<<grid, waves * 64, lds, st>>>(p);
       else skinny_kernel<T, X, false, NB, EPI><<<grid, waves * 64, lds, st>>>(p);
     };
@@ -305,5 +313,6 @@ void skinny_softmax(SkinnyArgs p, long long ignore, float* loss, float* lse, hip
 void skinny_teach(SkinnyArgs p, hipStream_t st) {
   p.groups = softmax_groups(p.N);
   p.parts = skinny_softmax_parts(p.N);
+  p.entry_groups = p.T * p.entries.parts;
   launch<SKINNY_TEACH>(p, st);
 }

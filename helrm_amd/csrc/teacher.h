@@ -1,28 +1,38 @@
 // teacher.h -- launches of teacher.hip: what a distillation does beside the
 // products of products.hip and skinny.hip.
 #pragma once
+#include <algorithm>
 #include "cleartext.h"
 
 constexpr int MOST_TOP = 1024;   // a teacher's logits of a row
 
 // Of each row, its entries (ids other than `ignore`, logits above -inf):
-// scores[j] = <x, table[ids[j]]> / temperature, probs[j] the softmax of logits
-// / temperature, of an id that is there again with the first one; -1 of
-// what is no entry, or again.  kept: 0 of a row without entries, 2 of one with an
-// id outside [0, vocab) (NaN in both), else 1.
+// cols[j] the table's row, probs[j] the softmax of logits / temperature, of an id
+// that is there again with the first one, scores[j] = <x, table[cols[j]]> /
+// temperature.  Places that are no entry have -1 in cols and probs; NaN in
+// probs of an id outside [0, vocab).
 struct TeachArgs {
   const void* x; long ldx;
   const void* table; long ldtable;
   const long long* ids; const void* logits;   // [rows][top]
-  float* scores; float* probs;
-  long long* kept;                            // [rows]
+  float* scores; float* probs; int* cols;     // [rows][top]
+  long long* kept;                            // [rows]: 0 of a row without entries, 2 of one with an id outside, else 1
   long rows; int width, vocab, top, dtype, teacher_type;
   long long ignore;
   float temperature;
-  int parts;                                  // (of the launch)
+  int parts;                                  // workgroups a row, of a launch that computes scores (entry_parts)
+  // teach_order: rows that count, and where its entries of each tile of 2^shift columns begin
+  const int* which; const int* count;
+  uint16_t* starts; int tiles, shift;         // [rows][tiles + 1]
 };
 constexpr int TEACH_NONE = 0, TEACH_FINE = 1, TEACH_OUTSIDE = 2;
-void teach_entries(TeachArgs a, hipStream_t st);
+// 512 workgroups, if there are as many times the 16 entries that the smallest one takes at once
+inline int entry_parts(long rows, int top) { return (int)std::max(1L, std::min((511 + rows) / rows, (top + 15L) / 16)); }
+inline size_t entries_bytes(int top) { return (size_t)((top + 3) & ~3) * 8 + 16 * 4; }   // of LDS
+void teach_entries(const TeachArgs& a, hipStream_t st);
+// The same in two steps, in the order of cols, for scores that a product picks out: kept; the rest but scores.
+void teach_kept(const TeachArgs& a, hipStream_t st);
+void teach_order(const TeachArgs& a, hipStream_t st);
 
 // The pieces of each row's softmax joined: lse, and loss = temperature^2 times
 // the divergence of the teacher's distribution from the softmax.
@@ -42,7 +52,7 @@ struct TeachPatch {
   uint16_t* dl; long ld, part;
   const int* rows; const int* tgt; const int* count;   // of the rows that count
   const float* lse; const float* grad; const float* scale;
-  const long long* ids; const float* scores; const float* probs;
+  const int* cols; const float* scores; const float* probs;
   long n; int top, dtype;
   long v0; int len;
 };

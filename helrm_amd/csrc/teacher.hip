@@ -4,128 +4,102 @@
 //   loss = T^2 sum_j p[j] (log p[j] - (s[j] - lse)),  dl[v] = T (exp(<x, table[v]> / T - lse) - p of v) dloss
 //
 // The softmax over the table and the products with dl are those of the cross
-// entropy (products.hip, skinny.hip).  Here the entries' scores are computed from
-// the table's rows, which are few of them and mostly common ones; a tile of the
-// product would have to find them among its columns.  The scores are kept for the
-// gradient, whose places of the entries are written again from them: the
+// entropy (products.hip, skinny.hip).  The entries' scores come out of the
+// product's tiles, which are told which of their columns each row wants; or,
+// where a row has few of them, from the table's rows themselves.  They are kept for
+// the gradient, whose places of the entries are written again from them: the
 // difference of two probabilities is taken in float32 and rounded once.
 #include <algorithm>
+#include "entries.h"
 #include "teacher.h"
 #include "tiles.h"
 
 namespace {
 
 constexpr int BLOCK = 256;
-constexpr int AT_ONCE = 4;   // entries of a wave
 
-// V elements from p[k] on, 0 past the end.
-template <class T, int V> __device__ __forceinline__ void load_part(const T* p, int k, int width, float (&v)[V]) {
-  T t[V] = {};
-  if (k + V <= width) __builtin_memcpy(t, p + k, sizeof(t));   // (global loads of 16 bytes need no alignment)
-  else
-#pragma unroll
-    for (int e = 0; e < V; e++) if (k + e < width) t[e] = p[k + e];
-#pragma unroll
-  for (int e = 0; e < V; e++) v[e] = (float)t[e];
-}
-
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
-}
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
-}
-
-// A workgroup has a row, or where there are few rows a share of its entries,
-// and the first of them the teacher's probabilities.  L: the type of its logits.
 template <class T, class L>
 __global__ __launch_bounds__(BLOCK) void entries_kernel(const TeachArgs a, long base) {
-  constexpr int V = 16 / sizeof(T), WAVES = BLOCK / 64;
-  __shared__ long long ids[MOST_TOP];   // a.ignore of what is no entry
-  __shared__ float probs[MOST_TOP];
-  __shared__ float sums[WAVES];
-  const long block = base + blockIdx.x, row = block / a.parts;
-  const int part = (int)(block - row * a.parts), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const long first = row * a.top;
-  float top = -INFINITY;
-  int any = 0;
-  for (int j = threadIdx.x; j < a.top; j += BLOCK) {
-    const float t = (float)((const L*)a.logits)[first + j];
-    const long long id = t == -INFINITY ? a.ignore : a.ids[first + j];
-    ids[j] = id;
-    probs[j] = t;
-    if (id == a.ignore) continue;
-    any |= id < 0 || id >= a.vocab ? 3 : 1;
-    top = fmaxf(top, t);
+  extern __shared__ __align__(16) char lds[];
+  row_entries<T, L>(a, base + blockIdx.x, lds);
+}
+
+// A wave a row.
+template <class L>
+__global__ __launch_bounds__(BLOCK) void kept_kernel(const TeachArgs a, long base) {
+  const long row = (base + blockIdx.x) * (BLOCK / 64) + (threadIdx.x >> 6);
+  if (row >= a.rows) return;
+  bool found = false, outside = false;
+  for (int j = threadIdx.x & 63; j < a.top; j += 64) {
+    float t;
+    const int id = entry_of<L>(a, row * a.top + j, t);
+    found |= id != NOTHING;
+    outside |= id == OUTSIDE;
   }
-  const int found = __syncthreads_or(any);
-  const bool outside = __syncthreads_or(any & 2);
-  if (part == 0) {
-    top = wave_max(top);
-    if (lane == 0) sums[wave] = top;
-    __syncthreads();
+  const bool any = __ballot(found), out = __ballot(outside);
+  if ((threadIdx.x & 63) == 0) a.kept[row] = !any ? TEACH_NONE : out ? TEACH_OUTSIDE : TEACH_FINE;
+}
+
+// A workgroup a row that counts: its entries in the order of the table's rows.  WAVES: 1 where there are few of them.
+constexpr int order_most(int waves) { return waves == 1 ? 256 : MOST_TOP; }
+template <class L, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void order_kernel(const TeachArgs a, long base) {
+  extern __shared__ __align__(16) char lds[];
+  const Entries e(lds, a.top);
+  int* leads = (int*)e.behind();     // the table's row of an entry that is the first of its id, else -1
+  int* tiles = leads + e.padded;     // of the entries, in order
+  const long i = base + blockIdx.x;
+  if (i >= *a.count) return;
+  const long row = a.which[i], first = row * a.top;
+  int any;
+  const float top = read_entries<L>(a, row, e, any);
+  __syncthreads();
+  const float sum = weigh(a, top, e);
+  __syncthreads();
+  constexpr int MINE = order_most(WAVES) / 64 / WAVES;
+  float probs[MINE];
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) top = fmaxf(top, sums[w]);
-    __syncthreads();
-    float sum = 0;
-    for (int j = threadIdx.x; j < a.top; j += BLOCK) {
-      // (the difference first: of lowest values alone it is 0, whatever the temperature)
-      const float e = ids[j] == a.ignore ? 0.0f : expf((probs[j] - top) / a.temperature);
-      probs[j] = e;
-      sum += e;
-    }
-    sum = wave_sum(sum);
-    if (lane == 0) sums[wave] = sum;
-    __syncthreads();
-    sum = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) sum += sums[w];
-    for (int j = threadIdx.x; j < a.top; j += BLOCK) {
-      const long long id = ids[j];
-      float p = 0;
-      bool again = false;
-      for (int k = 0; k < a.top; k++) {
-        if (ids[k] != id) continue;
-        again |= k < j;
-        p += probs[k];
-      }
-      a.probs[first + j] = id == a.ignore || again ? -1.0f : id < 0 || id >= a.vocab ? NAN : p / sum;
-    }
-    if (threadIdx.x == 0) a.kept[row] = !found ? TEACH_NONE : outside ? TEACH_OUTSIDE : TEACH_FINE;
+  for (int n = 0; n < MINE; n++) {
+    const int j = threadIdx.x + n * WAVES * 64;
+    if (j >= e.padded) break;
+    bool l;
+    const float p = together(e, j, l);
+    const int id = e.ids[j];
+    leads[j] = id >= 0 && l ? id : -1;
+    probs[n] = id == OUTSIDE ? NAN : id == NOTHING || !l ? -1.0f : p / sum;
   }
-  const T* x = (const T*)a.x + row * a.ldx;
-  for (int j0 = (part * WAVES + wave) * AT_ONCE; j0 < a.top; j0 += a.parts * WAVES * AT_ONCE) {
-    long long id[AT_ONCE];
-    bool in[AT_ONCE];
-    float sum[AT_ONCE] = {};
-    bool some = false;
+  __syncthreads();
+  int entries = 0;   // all of them
 #pragma unroll
-    for (int e = 0; e < AT_ONCE; e++) {
-      id[e] = j0 + e < a.top ? ids[j0 + e] : a.ignore;
-      in[e] = id[e] != a.ignore && id[e] >= 0 && id[e] < a.vocab;
-      some |= in[e];
-    }
-    if (some)
-      for (int k = lane * V; k < a.width; k += 64 * V) {
-        float u[V], w[AT_ONCE][V];
-        load_part<T, V>(x, k, a.width, u);
+  for (int n = 0; n < MINE; n++) {
+    const int j = threadIdx.x + n * WAVES * 64;
+    if (j >= e.padded) break;
+    const int id = leads[j];
+    int below = 0, others = 0;   // entries of rows before; places that are none before
+    entries = 0;
+    for (int k = 0; k < e.padded; k += 4) {
+      const int4 at = *(const int4*)(leads + k);
+      const int q[4] = {at.x, at.y, at.z, at.w};
 #pragma unroll
-        for (int e = 0; e < AT_ONCE; e++) load_part<T, V>((const T*)a.table + (in[e] ? id[e] : 0) * a.ldtable, k, a.width, w[e]);
-#pragma unroll
-        for (int e = 0; e < AT_ONCE; e++)
-#pragma unroll
-          for (int i = 0; i < V; i++) sum[e] = __builtin_fmaf(u[i], w[e][i], sum[e]);
+      for (int m = 0; m < 4; m++) {
+        entries += q[m] >= 0;
+        below += q[m] >= 0 && q[m] < id;
+        others += q[m] < 0 && k + m < j;
       }
-#pragma unroll
-    for (int e = 0; e < AT_ONCE; e++) sum[e] = wave_sum(sum[e]);
-    if (lane == 0)
-#pragma unroll
-      for (int e = 0; e < AT_ONCE; e++)
-        if (j0 + e < a.top) a.scores[first + j0 + e] = in[e] ? sum[e] / a.temperature : id[e] == a.ignore ? 0.0f : NAN;
+    }
+    const int at = id >= 0 ? below : entries + others;
+    if (j < e.top) {
+      a.probs[first + at] = probs[n];
+      a.cols[first + at] = id;
+    }
+    if (id >= 0) tiles[at] = id >> a.shift;
+  }
+  entries = __builtin_amdgcn_readfirstlane(entries);
+  __syncthreads();
+  uint16_t* starts = a.starts + i * (a.tiles + 1L);
+  for (int k = threadIdx.x >> 6; k <= entries; k += WAVES) {   // tiles whose first entry is number k
+    const int from = k ? tiles[k - 1] + 1 : 0, to = k < entries ? tiles[k] : a.tiles;
+    for (int t = from + (int)(threadIdx.x & 63); t <= to; t += 64) starts[t] = (uint16_t)k;
   }
 }
 
@@ -178,9 +152,9 @@ __global__ __launch_bounds__(BLOCK) void patch_kernel(const TeachPatch a, int la
   const long first = a.rows[i] * (long)a.top;
   const float grad = a.tgt[i] < 0 ? NAN : a.grad[i] * (a.scale ? *a.scale : 1.0f), lse = a.lse[i];
   for (int j = threadIdx.x % lanes; j < a.top; j += lanes) {
-    const long col = a.ids[first + j] - a.v0;
+    const long col = a.cols[first + j] - a.v0;
+    if (a.cols[first + j] < 0 || col < 0 || col >= a.len) continue;
     const float p = a.probs[first + j];
-    if (p < 0.0f || col < 0 || col >= a.len) continue;
     const float v = (__expf(a.scores[first + j] - lse) - p) * grad;
     uint16_t* o = a.dl + i * a.ld + col;
     if constexpr (sizeof(T) == 4) {
@@ -198,14 +172,28 @@ __global__ __launch_bounds__(BLOCK) void patch_kernel(const TeachPatch a, int la
 
 }  // namespace
 
-void teach_entries(TeachArgs a, hipStream_t st) {
-  // 512 workgroups, if there are as many times the entries that one takes at once
-  a.parts = (int)std::max<long>(1, std::min<long>(clr::ceil_div(512, a.rows), clr::ceil_div(a.top, AT_ONCE * (BLOCK / 64))));
+void teach_entries(const TeachArgs& a, hipStream_t st) {
   clr::with_type(a.dtype, [&](auto t) {
     using T = decltype(t);
     clr::in_launches(a.rows * a.parts, BLOCK, [&](long base, unsigned n) {
-      if (a.teacher_type == DT_F32) entries_kernel<T, float><<<n, BLOCK, 0, st>>>(a, base);
-      else entries_kernel<T, T><<<n, BLOCK, 0, st>>>(a, base);
+      if (a.teacher_type == DT_F32) entries_kernel<T, float><<<n, BLOCK, entries_bytes(a.top), st>>>(a, base);
+      else entries_kernel<T, T><<<n, BLOCK, entries_bytes(a.top), st>>>(a, base);
+    });
+  });
+}
+// f(L{}): of the type of the teacher's logits
+template <class F> static void with_teacher(const TeachArgs& a, F&& f) { clr::with_type(a.teacher_type, f); }
+void teach_kept(const TeachArgs& a, hipStream_t st) {
+  with_teacher(a, [&](auto l) {
+    clr::in_launches(clr::ceil_div(a.rows, BLOCK / 64), BLOCK, [&](long base, unsigned n) { kept_kernel<decltype(l)><<<n, BLOCK, 0, st>>>(a, base); });
+  });
+}
+void teach_order(const TeachArgs& a, hipStream_t st) {
+  const size_t bytes = entries_bytes(a.top) + (size_t)((a.top + 3) & ~3) * 8;
+  with_teacher(a, [&](auto l) {
+    clr::in_launches(a.rows, BLOCK, [&](long base, unsigned n) {
+      if (a.top <= order_most(1)) order_kernel<decltype(l), 1><<<n, 64, bytes, st>>>(a, base);
+      else order_kernel<decltype(l), 4><<<n, BLOCK, bytes, st>>>(a, base);
     });
   });
 }

@@ -377,15 +377,15 @@ int LossTotal(const LossTotalArgs* args, void* stream);
  * the teacher's divergence from the model, without keeping the model's logits.  A
  * row without entries has loss, lse and gradients 0, and nothing it holds reaches
  * another row's; an entry whose id is outside [0, vocab) gives a loss and
- * gradients of NaN.  kept, scores and probs are what the gradient and a mean over
+ * gradients of NaN.  kept, scores, probs and cols are what the gradient and a mean over
  * the rows with a teacher need (kept is 0 for the others).  dtable is contiguous. */
 typedef struct {
   const void* x; long ldx;               /* [rows][width] */
   const void* table; long ldtable;       /* [vocab][width] */
-  const long long* ids; const void* logits; /* [rows][top]; Distillation reads logits, of teacherType */
+  const long long* ids; const void* logits; /* [rows][top], logits of teacherType; Distillation */
   float* loss; float* lse;               /* [rows]; DistillationGrad reads lse */
-  long long* kept;                       /* [rows]; written by Distillation, as the next two */
-  float* scores; float* probs;           /* [rows][top]: z, and p or -1 */
+  long long* kept;                       /* [rows]; written by Distillation, as the next three */
+  float* scores; float* probs; int* cols; /* [rows][top]: z, p and the table's row, in some order; -1 where there is no entry */
   const float* dloss;                    /* [rows] */
   void* dx; long lddx;                   /* [rows][width] */
   void* dtable;                          /* [vocab][width] */

@@ -19,7 +19,7 @@ def lib():
 
 
 def args(**kw):
-    a = DistillationArgs(x=SOME, ldx=8, table=SOME, ldtable=8, ids=SOME, logits=SOME, loss=SOME, lse=SOME, kept=SOME, scores=SOME, probs=SOME,
+    a = DistillationArgs(x=SOME, ldx=8, table=SOME, ldtable=8, ids=SOME, logits=SOME, loss=SOME, lse=SOME, kept=SOME, scores=SOME, probs=SOME, cols=SOME,
                          dloss=SOME, dx=SOME, lddx=8, dtable=SOME, rows=4, width=8, vocab=16, top=3, ignore=-100, temperature=1.0)
     for k, v in kw.items():
         setattr(a, k, v)
@@ -50,9 +50,9 @@ def test_refusals_of_the_entry_points(lib, call):
     refused(lib, call, args(ldx=7), ": x")
     refused(lib, call, args(x=None), ": x")
     refused(lib, call, args(ldtable=7), "table")
-    for name in ("ids", "lse", "kept", "scores", "probs"):
+    for name in ("lse", "kept", "scores", "probs", "cols"):
         refused(lib, call, args(**{name: None}), name)
-    for name in ("logits", "loss") if call == "Distillation" else ("dx", "dtable", "dloss"):
+    for name in ("ids", "logits", "loss") if call == "Distillation" else ("dx", "dtable", "dloss"):
         refused(lib, call, args(**{name: None}), name)
     size = getattr(lib, call + "Workspace")
     need = size(ctypes.byref(args()))

@@ -117,6 +117,41 @@ def test_large_tiles(ct, dtype, rows, width, vocab, top):  # noqa: F811
     teach_check(ct, *tensors(seeded(rows), rows, width, vocab, top, dtype, none=0.1, ragged=True), 0.75)
 
 
+# so many entries of such width that their scores are picked out of the product's tiles, small and large ones
+PICKED = [(300, 600, 700, 200), (520, 1040, 3000, 64), (260, 300, 2000, 400), (40, 1000, 1500, 1024), (2040, 520, 8100, 40), (129, 2000, 129, 129)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width,vocab,top", PICKED)
+def test_scores_out_of_the_tiles(ct, dtype, rows, width, vocab, top):  # noqa: F811
+    gen = seeded(rows + top)
+    x, table, ids, logits, grad = tensors(gen, rows, width, vocab, top, dtype, none=0.1, ragged=True)
+    ids[1, :3] = torch.tensor([0, vocab - 1, vocab // 2])
+    teach_check(ct, x, table, ids, logits, grad, 1.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width,vocab,top", PICKED[:3])
+def test_scores_out_of_the_tiles_of_odd_entries(ct, dtype, rows, width, vocab, top):  # noqa: F811
+    gen = seeded(rows)
+    x, table, ids, logits, grad = tensors(gen, rows, width, vocab, top, dtype, none=0.1, ragged=True)
+    full = torch.randint(vocab, (top,), generator=gen).to(DEV)
+    ids[3], ids[4], ids[5], ids[6] = full, full[0], full.sort().values, full.sort(descending=True).values     # ids again and again
+    ids[7, ::2] = IGNORE
+    logits[8] = torch.finfo(dtype).min
+    logits[9, 1:] = -float("inf")
+    logits[10] = -float("inf")
+    teach_check(ct, x, table, ids, logits, grad, 0.7)
+    ids[20, 3], ids[21, 0], ids[22], logits[23, 1] = vocab, -1, 1 << 40, float("nan")
+    ids[23, 1] = 5
+    losses, lse, saved = ct.distillation_forward(x, table, ids, logits, 1.0)
+    dx, dtable = ct.distillation_backward(grad, x, table, ids, lse, saved, 1.0)
+    bad = torch.zeros(rows, dtype=torch.bool)
+    bad[20:24] = True
+    assert torch.equal(torch.isnan(losses).cpu(), bad) and torch.equal(torch.isnan(dx).any(1).cpu(), bad) and torch.isfinite(lse).all()
+    assert torch.isnan(dtable).all()
+
+
 def test_two_pieces_of_16_bits(ct):  # noqa: F811
     x, table, ids, logits, grad = tensors(seeded(8), 2100, 24, 64100, 4, torch.bfloat16)
     ids[:4, 0] = torch.tensor([63487, 63488, 64099, 0])     # beside the cut, and at the ends
@@ -289,6 +324,7 @@ def test_streams_and_graphs(ct):  # noqa: F811
     side = torch.cuda.Stream()
     cases = [tensors(seeded(k), rows, 40, vocab, 7, dtype, none=0.1, ragged=True)
              for k, (rows, vocab, dtype) in enumerate(((3, 300, torch.float32), (50, 700, torch.bfloat16), (300, 900, torch.float16)))]
+    cases.append(tensors(seeded(9), 300, 600, 700, 200, torch.bfloat16, none=0.1))
     torch.cuda.synchronize()
 
     def all_of():
