@@ -113,7 +113,12 @@ Held hold(Arena& m, long rows, long width, int type, bool exact = false) {
 // 1,024 against 65,536 172 and 162.  The parts are of the operator's type, with
 // its range: float16 hidden values and their gradients are infinite beyond 65504
 // and lose bits below 2^-14 (a loss in float16 is scaled; dl is by itself).
-bool few_rows(long rows, int type) { return type != DT_F32 && rows <= 64; }
+// A teacher's few largest probabilities are most of dl, one or two values a row:
+// its rows count as few up to 256 (94 x 172 against 43,339, bfloat16: dtable off
+// by 0.0025 in one part and 0.0017 in two, 159 and 167 us; 256 x 1,024 against
+// 65,536 240 and 302 us).
+constexpr long FEW = 64, FEW_TAUGHT = 256;
+bool few_rows(long rows, int type, long most = FEW) { return type != DT_F32 && rows <= most; }
 // Matrices that are copied first, all in one launch: where alignment, an odd
 // width or float32 does not let the tiles be loaded from a matrix itself.  A
 // pass over it; a product of more than a few rows reads it many times.
@@ -324,22 +329,21 @@ size_t ce_forward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
 // there are 1,024 of them.
 constexpr long PIECE_BYTES = 256L << 20;
 static_assert(PIECE_BYTES < 1L << 31 && 256 * 1024 * 2 < 1L << 31, "the rows of a tile of dl are within 31-bit offsets, whatever their number and width");
-int piece_rows(long rows, int vocab, int type) {
-  const long most = PIECE_BYTES / (std::max<long>(rows, 1) * (type == DT_F32 ? 6 : few_rows(rows, type) ? 4 : 2));
+int piece_rows(long rows, int vocab, int type, bool few) {
+  const long most = PIECE_BYTES / (std::max<long>(rows, 1) * (type == DT_F32 ? 6 : few ? 4 : 2));
   return (int)std::min<long>(up8(vocab), std::max<long>(1024, most / 1024 * 1024));
 }
 
 // The gradients of a loss against a table, dx = dl table and dtable = dl^T x, from `logits_grad`, which leaves dl for
 // some of the table's rows.  The arguments' targets and gradients, of which `r` says which.
-template <class Args, class F> size_t table_backward(const Args* a, RowsArgs r, bool count, hipStream_t st, F&& logits_grad) {
+template <class Args, class F> size_t table_backward(const Args* a, RowsArgs r, bool few, bool count, hipStream_t st, F&& logits_grad) {
   Arena m{count ? nullptr : (char*)a->workspace};
   const long n = a->rows, D = a->width;
-  const int piece = piece_rows(a->rows, a->vocab, a->type);
+  const int piece = piece_rows(a->rows, a->vocab, a->type, few);
   r.rows = m.take<int>(n); r.tgt = m.take<int>(n); r.place = m.take<int>(n); r.count = m.take<int>(1);
   float* scale = m.take<float>(1);
   if (a->type == DT_F16) r.scale = scale;
   r.lse = a->lse; r.lse_kept = m.take<float>(n); r.grad_kept = m.take<float>(n);
-  const bool few = few_rows(n, a->type);
   const Held x = hold(m, n, a->width, a->type), dl = hold(m, n, piece, a->type, few);
   // two parts are twice as many rows for dx, in a tile that has room for them (the table is read once); scatter_rows adds them
   const long stacked = few ? 2 * n : n;
@@ -384,7 +388,7 @@ template <class Args, class F> size_t table_backward(const Args* a, RowsArgs r, 
 }
 
 size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
-  return table_backward(a, RowsArgs{a->target, a->dloss, a->rows, a->ignore, a->vocab}, count, st,
+  return table_backward(a, RowsArgs{a->target, a->dloss, a->rows, a->ignore, a->vocab}, few_rows(a->rows, a->type), count, st,
                         [&](const ProductArgs& p, const RowsArgs&, const Held&) { product_softmax_grad(p, st); });
 }
 
@@ -495,7 +499,7 @@ size_t teach_forward(const DistillationArgs* a, bool count, hipStream_t st) {
 size_t teach_backward(const DistillationArgs* a, bool count, hipStream_t st) {
   RowsArgs r{a->kept, a->dloss, a->rows, TEACH_NONE, TEACH_OUTSIDE};
   r.factor = a->temperature;
-  return table_backward(a, r, count, st, [&](ProductArgs p, const RowsArgs& r, const Held& dl) {
+  return table_backward(a, r, few_rows(a->rows, a->type, FEW_TAUGHT), count, st, [&](ProductArgs p, const RowsArgs& r, const Held& dl) {
     p.rate = 1.0f / a->temperature;
     product_teach_grad(p, st);
     TeachPatch t{};

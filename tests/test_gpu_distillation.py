@@ -159,7 +159,8 @@ def test_two_pieces_of_16_bits(ct):  # noqa: F811
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("rows,width,vocab", [(1, 72, 264), (3, 264, 1000), (17, 64, 4096), (40, 100, 301), (64, 520, 1300)])
+@pytest.mark.parametrize("rows,width,vocab", [(1, 72, 264), (3, 264, 1000), (17, 64, 4096), (40, 100, 301), (64, 520, 1300), (94, 172, 3000),
+                                              (130, 64, 4100), (256, 264, 700)])
 def test_few_rows_round_once(ct, dtype, rows, width, vocab):  # noqa: F811
     teach_check(ct, *tensors(seeded(rows + vocab), rows, width, vocab, 16, dtype), 1.0, once=True)
 
