@@ -336,7 +336,7 @@ int piece_rows(long rows, int vocab, int type, bool few) {
 
 // The gradients of a loss against a table, dx = dl table and dtable = dl^T x, from `logits_grad`, which leaves dl for
 // some of the table's rows.  The arguments' targets and gradients, of which `r` says which.
-template <class Args, class F> size_t table_backward(const Args* a, RowsArgs r, bool few, bool count, hipStream_t st, F&& logits_grad) {
+template <class Args, class F> size_t table_backward(const Args* a, RowsArgs r, bool few, int most, bool count, hipStream_t st, F&& logits_grad) {
   Arena m{count ? nullptr : (char*)a->workspace};
   const long n = a->rows, D = a->width;
   const int piece = piece_rows(a->rows, a->vocab, a->type, few);
@@ -349,7 +349,7 @@ template <class Args, class F> size_t table_backward(const Args* a, RowsArgs r, 
   const long stacked = few ? 2 * n : n;
   float* acc = m.take<float>((size_t)stacked * D);
   const int parts = a->type == DT_F32 ? 6 : 1, sums = parts * (few ? 2 : 1), last = a->vocab % piece ? a->vocab % piece : piece;
-  float* partial = scratch(m, {product_scratch({{stacked, D}}, piece, parts), product_scratch({{stacked, D}}, last, parts),
+  float* partial = scratch(m, {product_scratch({{stacked, D}}, piece, parts, false, most), product_scratch({{stacked, D}}, last, parts, false, most),
                                product_scratch({{piece, D}}, n, sums), product_scratch({{last, D}}, n, sums)});
   Copies copy;
   copy.add(x, a->x, a->ldx, n, a->width, r.rows, r.count);
@@ -372,6 +372,7 @@ template <class Args, class F> size_t table_backward(const Args* a, RowsArgs r, 
     q.M = (int)stacked; q.N = a->width; q.K = len;
     add_pairs(q, {dl.p, dl.ld, dl.part, few ? 1 : dl.parts}, rows);
     q.partial = partial;
+    q.most = most;
     q.c = acc; q.ldc = D; q.add = v0 > 0;
     product_nn(q, st);
     ProductArgs w{};
@@ -388,7 +389,7 @@ template <class Args, class F> size_t table_backward(const Args* a, RowsArgs r, 
 }
 
 size_t ce_backward(const CrossEntropyArgs* a, bool count, hipStream_t st) {
-  return table_backward(a, RowsArgs{a->target, a->dloss, a->rows, a->ignore, a->vocab}, few_rows(a->rows, a->type), count, st,
+  return table_backward(a, RowsArgs{a->target, a->dloss, a->rows, a->ignore, a->vocab}, few_rows(a->rows, a->type), clr::SPLITS, count, st,
                         [&](const ProductArgs& p, const RowsArgs&, const Held&) { product_softmax_grad(p, st); });
 }
 
@@ -499,7 +500,7 @@ size_t teach_forward(const DistillationArgs* a, bool count, hipStream_t st) {
 size_t teach_backward(const DistillationArgs* a, bool count, hipStream_t st) {
   RowsArgs r{a->kept, a->dloss, a->rows, TEACH_NONE, TEACH_OUTSIDE};
   r.factor = a->temperature;
-  return table_backward(a, r, few_rows(a->rows, a->type, FEW_TAUGHT), count, st, [&](ProductArgs p, const RowsArgs& r, const Held& dl) {
+  return table_backward(a, r, few_rows(a->rows, a->type, FEW_TAUGHT), clr::MANY_SPLITS, count, st, [&](ProductArgs p, const RowsArgs& r, const Held& dl) {
     p.rate = 1.0f / a->temperature;
     product_teach_grad(p, st);
     TeachPatch t{};

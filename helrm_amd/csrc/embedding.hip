@@ -20,6 +20,7 @@
 // us, and 24 + 6 + 5 of short launches.
 #include <algorithm>
 #include "embedding.h"
+#include "places.h"
 
 namespace {
 
@@ -54,21 +55,6 @@ bool streams(long rows, int width, int dtype) { return rows * width * dtype_size
 
 // First element of a row's pack: the last one begins earlier, where the width is not a multiple, and holds some elements again.
 template <int V> __device__ __forceinline__ int pack_at(int pack, int width) { return min(pack * V, width - V); }
-
-// Places of a [rows][packs] grid by their number: item `first` + j, j < 2^30.
-struct Places {
-  long row; int in, packs; float rate;
-  __device__ __forceinline__ Places(long first, int packs_) : row(first / packs_), in((int)(first - row * packs_)), packs(packs_), rate(1.0f / packs_) {}
-  __device__ __forceinline__ void of(int j, long& r, int& pack) const {
-    const int i = in + j;
-    int q = (int)(i * rate);   // within one of i / packs: it is under 1,025 unless packs is 1
-    int left = i - q * packs;
-    if (left < 0) { q--; left += packs; }
-    if (left >= packs) { q++; left -= packs; }
-    r = row + q;
-    pack = left;
-  }
-};
 
 constexpr int TURNS = 4;   // packs a thread
 
@@ -480,6 +466,80 @@ template <class F> void with_items(int n, F&& f) {
   else if (n <= 4) f(std::integral_constant<int, 4>{});
   else f(std::integral_constant<int, 8>{});
 }
+// ---- few ids ----
+// One launch: a workgroup an id (and column block), which adds the rows of all
+// that are equal if it is the first of them, and others that clear rows of the
+// table that no id names.  A workgroup compares all ids, and one id's rows are
+// added by one: 64 ids x 408 against 960 float32 FEWFIG
+constexpr int FEW = 256;
+struct FewArgs {
+  EmbedArgs e;
+  int packs, blocks, chunk;   // packs of a row; column blocks of BLOCK of them; rows that a workgroup clears
+};
+constexpr int MOST_CHUNK = 4096;
+template <class T, int V>
+__global__ __launch_bounds__(BLOCK) void few_kernel(const FewArgs a, long base) {
+  __shared__ int ids[FEW], list[FEW];
+  __shared__ unsigned named[MOST_CHUNK / 32];
+  __shared__ int sums[BLOCK / 64];
+  const int n = (int)a.e.tokens, mine = threadIdx.x;
+  const long long id = mine < n ? a.e.ids[mine] : a.e.ignore;
+  const bool in = mine < n && inside(a.e, id);
+  const long block = base + blockIdx.x;
+  if (block >= (long)n * a.blocks) {
+    const long first = (block - (long)n * a.blocks) * a.chunk;
+    const int rows = (int)min((long)a.chunk, a.e.vocab - first);
+    for (int k = threadIdx.x; k < MOST_CHUNK / 32; k += BLOCK) named[k] = 0;
+    __syncthreads();
+    if (in && id >= first && id < first + rows) atomicOr(&named[(id - first) >> 5], 1u << ((id - first) & 31));
+    __syncthreads();
+    const Places places(0, a.packs);
+    const int items = rows * a.packs;   // (under 2^20, or a single row)
+    for (int j = threadIdx.x; j < items; j += BLOCK) {
+      long r;
+      int pack;
+      if (rows == 1) { r = 0; pack = j; }
+      else places.of(j, r, pack);
+      if (named[r >> 5] >> (r & 31) & 1) continue;
+      const float zero[V] = {};
+      store_pack<false, T, V>((T*)a.e.dtable + (first + r) * a.e.width + pack_at<V>(pack, a.e.width), zero);
+    }
+    return;
+  }
+  const int token = (int)(block / a.blocks);
+  ids[mine] = in ? (int)id : -1;
+  __syncthreads();
+  const int key = ids[token];
+  const bool same = key >= 0 && ids[mine] == key;
+  if (__syncthreads_or((same && mine < token) || key < 0)) return;
+  // the equal ones, in order
+  const unsigned long long mask = __ballot(same);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane == 0) sums[wave] = __popcll(mask);
+  __syncthreads();
+  int before = __popcll(mask & ((1ull << lane) - 1)), all = 0;
+#pragma unroll
+  for (int w = 0; w < BLOCK / 64; w++) {
+    before += w < wave ? sums[w] : 0;
+    all += sums[w];
+  }
+  if (same) list[before] = mine;
+  __syncthreads();
+  const int pack = (int)(block - (long)token * a.blocks) * BLOCK + threadIdx.x;
+  if (pack >= a.packs) return;
+  const int at = pack_at<V>(pack, a.e.width);
+  float sum[V] = {};
+#pragma unroll 8
+  for (int k = 0; k < all; k++) {
+    const Pack<T, V> t = load_pack<T, V>((const T*)a.e.y + list[k] * a.e.ldy + at);
+#pragma unroll
+    for (int e = 0; e < V; e++) sum[e] += (float)t.v[e];
+  }
+#pragma unroll
+  for (int e = 0; e < V; e++) sum[e] *= a.e.scale;
+  store_pack<false, T, V>((T*)a.e.dtable + (long)key * a.e.width + at, sum);
+}
+
 // f(T{}, V): packs of 16 bytes, or single elements of rows that have no 16 bytes
 template <class F> void with_packs(int dtype, int width, F&& f) {
   clr::with_type(dtype, [&](auto t) {
@@ -544,9 +604,21 @@ void embedding_launch(const EmbedArgs& a, hipStream_t st) {
   });
 }
 
-size_t embedding_grad_workspace(long tokens, int width, int vocab, int dtype) { return space_of(nullptr, tokens, width, vocab, dtype).bytes; }
+size_t embedding_grad_workspace(long tokens, int width, int vocab, int dtype) { return tokens <= FEW ? 0 : space_of(nullptr, tokens, width, vocab, dtype).bytes; }
+
+static void few_launch(const EmbedArgs& e, hipStream_t st) {
+  FewArgs a{e};
+  a.packs = packs_of(e.width, e.dtype);
+  a.blocks = (int)clr::ceil_div(a.packs, BLOCK);
+  a.chunk = std::max(1, std::min(MOST_CHUNK, 4096 / a.packs));   // 64 KiB of packs
+  const long groups = e.tokens * a.blocks + clr::ceil_div(e.vocab, a.chunk);
+  with_packs(e.dtype, e.width, [&](auto t, auto v) {
+    clr::in_launches(groups, BLOCK, [&](long base, unsigned n) { few_kernel<decltype(t), decltype(v)::value><<<n, BLOCK, 0, st>>>(a, base); });
+  });
+}
 
 void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
+  if (a.tokens <= FEW) return few_launch(a, st);
   const Space space = space_of((char*)a.workspace, a.tokens, a.width, a.vocab, a.dtype);
   SortArgs s{};
   s.ids = a.ids;
@@ -595,7 +667,6 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
       with_items(items, [&](auto n) { scatter_kernel<decltype(n)::value><<<groups, SORT, 0, st>>>(s, c); });
     }
   }
-  if (!a.tokens) return;
   const int packs = packs_of(a.width, a.dtype);
   SumArgs m{};
   m.keys = space.keys[out];

@@ -24,6 +24,7 @@ struct ProductArgs {
   const int* count;          // on the device, may be null: the rows present, in the place of M
   bool count_k;              // in the place of K
   float* partial;            // product_scratch bytes (but softmax)
+  int most = clr::SPLITS;    // splits of k
   int splits;                // (of the launch)
   // store
   void* c; long ldc; int ctype; bool add;  // add: c (float32) += the product
@@ -53,7 +54,7 @@ void product_gate(const ProductArgs& p, hipStream_t st);
 void product_gate_grad(const ProductArgs& p, hipStream_t st);
 // Bytes that a product (softmax but) of these shapes needs at `partial`, or products in one launch together.
 using clr::Shape;
-size_t product_scratch(std::initializer_list<Shape> shapes, long K, int pairs, bool gate = false);
+size_t product_scratch(std::initializer_list<Shape> shapes, long K, int pairs, bool gate = false, int most = clr::SPLITS);
 void product_nt(const ProductArgs& p, hipStream_t st);  // A B^T
 void product_nn(const ProductArgs& p, hipStream_t st);  // A B
 void product_tn(const ProductArgs& p, hipStream_t st);  // A^T B

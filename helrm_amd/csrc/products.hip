@@ -37,6 +37,7 @@
 // TFLOP/s, with random values the clock falls to 1.57 GHz and the matrix units
 // are busy 64 % of the time.  The gate and its gradient are bound by memory at
 // the end of a tile, when a CU does nothing else.
+#include "places.h"
 #include "products.h"
 #include "tiles.h"
 
@@ -650,7 +651,7 @@ __global__ __launch_bounds__(256) void join_kernel(const Batch batch) {
   const long m = i / cols, n = (i - m * cols) * 4;
   if (m >= (p.count && !p.count_k ? *p.count : p.M)) return;
   float v[4] = {0, 0, 0, 0}, u[4] = {0, 0, 0, 0};
-#pragma unroll 4
+#pragma unroll 8
   for (int s = 0; s < p.splits; s++) {
     const float* at = p.partial + ((long)s * p.M + m) * sum_ld<EPI>(p) + n;
     float t[4];
@@ -714,55 +715,59 @@ template <bool A_K, bool B_K, int EPI> void launch(std::initializer_list<Product
 }
 template <bool A_K, bool B_K, int EPI> void launch(const ProductArgs& p, hipStream_t st) {
   constexpr bool may_split = EPI == EPI_STORE || EPI == EPI_GATE || EPI == EPI_GATE_GRAD;
-  launch<A_K, B_K, EPI>({p}, plan_of({{p.M, p.N}}, steps_of(p.K, p.pairs), EPI == EPI_GATE, may_split), st);
+  launch<A_K, B_K, EPI>({p}, plan_of({{p.M, p.N}}, steps_of(p.K, p.pairs), EPI == EPI_GATE, may_split ? p.most : 1), st);
 }
 
 // Up to 8 matrices into the layout that the tiles are loaded from, one launch:
 // rows[i] (or i) of `from` to row i of `to`, filled up with zeros to ldto;
-// float32 as three parts.  Bound by memory: 50,021 x 416 float32, 208 MB read
-// and written, 45 us = 4.7 TB/s.
+// float32 as three parts.  Eight elements a thread and turn, whatever the rows'
+// lengths and alignment.  Bound by memory: 50,021 x 416 float32, 208 MB read
+// and written, 35 us = 5.9 TB/s; 130,880 x 66 float16, 36 MB, 10 us.
 struct LayOuts { LayOut j[8]; long first[8]; int count; };
+constexpr int LAY_BLOCK = 256, LAY_TURNS = 2;
+long lay_blocks(const LayOut& j) { return clr::ceil_div(j.n * (j.ldto / 8), LAY_BLOCK * LAY_TURNS); }
 template <class T>
-__global__ __launch_bounds__(256) void lay_out_kernel(const LayOuts all, long base) {
+__global__ __launch_bounds__(LAY_BLOCK) void lay_out_kernel(const LayOuts all, long base) {
   const long id = base + blockIdx.x;
   int which = 0;
   while (which + 1 < all.count && id >= all.first[which + 1]) which++;
   const LayOut& j = all.j[which];
-  const long i = id - all.first[which];
-  if (j.count && i >= *j.count) return;
-  const T* f = (const T*)j.from + (j.rows ? (long)j.rows[i] : i) * j.ld;
-  u16* to = (u16*)j.to + i * j.ldto;
-  constexpr int V = 16 / sizeof(T);
-  if (((uintptr_t)f & 15) == 0 && j.width % V == 0) {
-    for (int k = threadIdx.x * V; k < j.ldto; k += 256 * V) {
-      T v[V];
-      if (k < j.width) __builtin_memcpy(v, __builtin_assume_aligned(f + k, 16), 16);
-      else for (int e = 0; e < V; e++) v[e] = (T)0.0f;
-      if constexpr (sizeof(T) == 4) {
-        float q[3][4];
+  const long first = (id - all.first[which]) * (LAY_BLOCK * LAY_TURNS), n = j.count ? *j.count : j.n, items = n * (j.ldto / 8);
+  if (first >= items) return;
+  const Places places(first, (int)(j.ldto / 8));
+  const int last = (int)min(items - first, (long)LAY_BLOCK * LAY_TURNS) - 1;   // (the last workgroup's threads do that one again)
+  long row[LAY_TURNS];
+  int k[LAY_TURNS];
+  T v[LAY_TURNS][8];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          __bf16 s[3];
-          split3(v[e], s);
-#pragma unroll
-          for (int t = 0; t < 3; t++) q[t][e] = (float)s[t];
-        }
-#pragma unroll
-        for (int t = 0; t < 3; t++) *(uint2*)(to + t * j.part + k) = pack4<__bf16>(q[t]);
-      } else {
-        __builtin_memcpy(__builtin_assume_aligned(to + k, 16), v, 16);
-      }
-    }
-    return;
+  for (int u = 0; u < LAY_TURNS; u++) {
+    places.of(min(u * LAY_BLOCK + (int)threadIdx.x, last), row[u], k[u]);
+    k[u] *= 8;
   }
-  for (int k = threadIdx.x; k < j.ldto; k += 256) {
-    const T v = k < j.width ? f[k] : (T)0.0f;
+#pragma unroll
+  for (int u = 0; u < LAY_TURNS; u++) {
+    const T* f = (const T*)j.from + (j.rows ? (long)j.rows[row[u]] : row[u]) * j.ld + k[u];
+    if (k[u] + 8 <= j.width) __builtin_memcpy(v[u], f, sizeof(v[u]));   // (global loads of 16 bytes need no alignment)
+    else
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[u][e] = k[u] + e < j.width ? f[e] : (T)0.0f;
+  }
+#pragma unroll
+  for (int u = 0; u < LAY_TURNS; u++) {
+    u16* to = (u16*)j.to + row[u] * j.ldto + k[u];
     if constexpr (sizeof(T) == 4) {
-      __bf16 s[3];
-      split3(v, s);
-      for (int t = 0; t < 3; t++) to[t * j.part + k] = bits(s[t]);
+      __bf16 q[3][8];
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        __bf16 s[3];
+        split3(v[u][e], s);
+#pragma unroll
+        for (int t = 0; t < 3; t++) q[t][e] = s[t];
+      }
+#pragma unroll
+      for (int t = 0; t < 3; t++) __builtin_memcpy(__builtin_assume_aligned(to + t * j.part, 16), q[t], 16);
     } else {
-      to[k] = bits(v);
+      __builtin_memcpy(__builtin_assume_aligned(to, 16), v[u], 16);
     }
   }
 }
@@ -907,8 +912,8 @@ __global__ void zero_kernel(uint16_t* p, size_t n) {
 
 }  // namespace
 
-size_t product_scratch(std::initializer_list<Shape> shapes, long K, int pairs, bool gate) {
-  const Plan plan = plan_of(shapes, steps_of(K, pairs), gate, true);
+size_t product_scratch(std::initializer_list<Shape> shapes, long K, int pairs, bool gate, int most) {
+  const Plan plan = plan_of(shapes, steps_of(K, pairs), gate, most);
   size_t n = 0;
   if (plan.splits > 1)
     for (const Shape& s : shapes) n += (size_t)plan.splits * s.M * ((s.N + 7) & ~7L) * (gate ? 2 : 1);
@@ -920,7 +925,7 @@ void product_nt(const ProductArgs& p, hipStream_t st) { launch<true, true, EPI_S
 void product_nn(const ProductArgs& p, hipStream_t st) { launch<true, false, EPI_STORE>(p, st); }
 void product_tn(const ProductArgs& p, hipStream_t st) { launch<false, false, EPI_STORE>(p, st); }
 void product_tn(ProductArgs a, ProductArgs b, ProductArgs c, hipStream_t st) {
-  const Plan plan = plan_of({{a.M, a.N}, {b.M, b.N}, {c.M, c.N}}, steps_of(a.K, a.pairs), false, true);
+  const Plan plan = plan_of({{a.M, a.N}, {b.M, b.N}, {c.M, c.N}}, steps_of(a.K, a.pairs), false, a.most);
   auto sums = [&](const ProductArgs& p) { return (size_t)plan.splits * p.M * ((p.N + 7) & ~7L); };
   b.partial = a.partial + (plan.splits > 1 ? sums(a) : 0);
   c.partial = b.partial + (plan.splits > 1 ? sums(b) : 0);
@@ -950,10 +955,10 @@ void lay_out(const LayOut* jobs, int n, int dtype, hipStream_t st) {
     if (jobs[i].n > 0) {
       all.first[all.count] = blocks;
       all.j[all.count++] = jobs[i];
-      blocks += jobs[i].n;
+      blocks += lay_blocks(jobs[i]);
     }
   clr::with_type(dtype, [&](auto t) {
-    clr::in_launches(blocks, 256, [&](long base, unsigned n) { lay_out_kernel<decltype(t)><<<n, 256, 0, st>>>(all, base); });
+    clr::in_launches(blocks, LAY_BLOCK, [&](long base, unsigned n) { lay_out_kernel<decltype(t)><<<n, LAY_BLOCK, 0, st>>>(all, base); });
   });
 }
 void kept_rows(const RowsArgs& a, hipStream_t st) { kept_rows_kernel<<<1, ROWS_BLOCK, 0, st>>>(a); }

@@ -48,13 +48,14 @@ def test_refusals_of_the_entry_points(lib):
     refused(lib, "EmbeddingGrad", args(dy=None), "dy")
     refused(lib, "EmbeddingGrad", args(lddy=7), "dy")
     refused(lib, "EmbeddingGrad", args(dtable=None), "dtable")
-    need = lib.EmbeddingGradWorkspace(ctypes.byref(args()))
+    assert lib.EmbeddingGradWorkspace(ctypes.byref(args())) == 0           # (few ids take none)
+    need = lib.EmbeddingGradWorkspace(ctypes.byref(args(tokens=1000)))
     assert need > 0 and lib.EmbeddingGradWorkspace(ctypes.byref(args(type=3))) == -1
-    assert lib.EmbeddingGradWorkspace(ctypes.byref(args(ids=None, dy=None, dtable=None))) == need
+    assert lib.EmbeddingGradWorkspace(ctypes.byref(args(tokens=1000, ids=None, dy=None, dtable=None))) == need
     assert lib.EmbeddingGradWorkspace(ctypes.byref(args(tokens=100000))) > need
     assert lib.EmbeddingGradWorkspace(ctypes.byref(args(tokens=100000, width=800))) > lib.EmbeddingGradWorkspace(ctypes.byref(args(tokens=100000)))
-    refused(lib, "EmbeddingGrad", args(workspace=SOME, workspaceBytes=need - 1), "workspace too small")
-    refused(lib, "EmbeddingGrad", args(workspace=SOME + 8, workspaceBytes=need), "aligned")
+    refused(lib, "EmbeddingGrad", args(tokens=1000, workspace=SOME, workspaceBytes=need - 1), "workspace too small")
+    refused(lib, "EmbeddingGrad", args(tokens=1000, workspace=SOME + 8, workspaceBytes=need), "aligned")
 
 
 def test_refusals_of_the_tensors():

@@ -53,7 +53,8 @@ def embed_check(ct, ids, table, grad, scale, ignore=IGNORE):  # noqa: F811
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("tokens,width,vocab", [(0, 8, 5), (1, 1, 1), (1, 512, 300), (3, 7, 2), (15, 8, 40), (16, 9, 3), (17, 16, 100), (65, 33, 64),
+@pytest.mark.parametrize("tokens,width,vocab", [(0, 8, 5), (1, 1, 1), (1, 512, 300), (3, 7, 2), (15, 8, 40), (16, 9, 3), (17, 16, 100), (65, 33, 64), (255, 2056, 30),
+                                                (256, 12, 5000), (257, 12, 5000), (256, 20000, 3),
                                                 (200, 416, 1000), (1000, 1001, 50), (1024, 3, 511), (1025, 64, 512), (700, 2048, 9000), (37, 4097, 20),
                                                 (5000, 24, 4000), (8191, 5, 3), (8192, 16, 70000), (8193, 16, 300), (12289, 40, 260000),
                                                 (20000, 4, 1), (30011, 130, 5000)])
@@ -72,21 +73,22 @@ def test_runs_that_end_anywhere(ct, width):  # noqa: F811
     gen = seeded(width)
     lengths = [1, 15, 16, 17, 31, 32, 33, 47, 63, 64, 65, 127, 128, 129, 1, 1, 200, 1000, 3, 2500, 5]
     ids = torch.cat([torch.full((n,), 3 * k) for k, n in enumerate(lengths)])
-    for ids in (ids, ids[torch.randperm(len(ids), generator=gen)], torch.cat([ids, ids, ids])):
+    for ids in (ids, ids[torch.randperm(len(ids), generator=gen)], torch.cat([ids, ids, ids]), ids[torch.randperm(len(ids), generator=gen)][:250]):
         embed_check(ct, ids.to(DEV), normal(gen, 70, width), normal(gen, len(ids), width), 1.0)
 
 
-def test_equal_ids_are_added_in_their_order(ct):  # noqa: F811
+@pytest.mark.parametrize("more", [0, 500])
+def test_equal_ids_are_added_in_their_order(ct, more):  # noqa: F811
     # 2^24 + 1 + 1 + ... in float32 stays 2^24, 1 + 1 + ... + 2^24 does not: each id's rows are in order within a piece
-    ids = torch.tensor([4, 2] * 8, device=DEV)
-    grad = torch.ones(16, 8, device=DEV)
+    ids = torch.tensor([4, 2] * 8 + [5] * more, device=DEV)
+    grad = torch.ones(16 + more, 8, device=DEV)
     grad[0], grad[15] = 2.0 ** 24, 2.0 ** 24
     d = ct.embedding_backward(grad, ids, 6)
     assert (d[4] == 2.0 ** 24).all() and (d[2] == 2.0 ** 24 + 8).all()      # (7 + 2^24, to the even neighbour)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("tokens", [50, 9000])
+@pytest.mark.parametrize("tokens", [50, 700, 9000])
 def test_ids_without_a_row(ct, dtype, tokens):  # noqa: F811
     gen = seeded(tokens)
     table = normal(gen, 33, 40, dtype=dtype)
@@ -212,7 +214,7 @@ def test_streams_and_graphs(ct):  # noqa: F811
     gen = seeded(6)
     side = torch.cuda.Stream()
     cases = []
-    for tokens, width, vocab in ((100, 24, 40), (10000, 24, 300), (3000, 520, 9000)):
+    for tokens, width, vocab in ((100, 24, 40), (500, 24, 40), (10000, 24, 300), (3000, 520, 9000)):
         ids = heavy(gen, tokens, vocab).to(DEV)
         cases.append((ids, normal(gen, vocab, width), normal(gen, tokens, width)))
     torch.cuda.synchronize()
@@ -255,6 +257,7 @@ def test_refusals(ct):  # noqa: F811
             call()
     from helrm_amd.backend import EmbeddingArgs
     ct.embedding(ids, table)
+    many, rows = ids.repeat(100), grad.repeat(100, 1)
     with pytest.raises(HipError, match="workspace too small"):
-        ct._call("EmbeddingGrad", EmbeddingArgs(ids=ids.data_ptr(), dy=grad.data_ptr(), lddy=8, dtable=table.data_ptr(), workspace=256, workspaceBytes=8,
-                                                tokens=3, width=8, vocab=5, ignore=IGNORE, scale=1.0), table.device)
+        ct._call("EmbeddingGrad", EmbeddingArgs(ids=many.data_ptr(), dy=rows.data_ptr(), lddy=8, dtable=table.data_ptr(), workspace=256, workspaceBytes=8,
+                                                tokens=300, width=8, vocab=5, ignore=IGNORE, scale=1.0), table.device)
