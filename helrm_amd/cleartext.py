@@ -85,8 +85,9 @@ def _call(name, args, device):
         need = size(ref)
         if need < 0:
             _refused()
-        space = torch.empty(need, dtype=torch.uint8, device=device)
-        args.workspace, args.workspaceBytes = space.data_ptr(), need
+        if need:
+            space = torch.empty(need, dtype=torch.uint8, device=device)
+            args.workspace, args.workspaceBytes = space.data_ptr(), need
     if call(ref, _raw_stream(index)):
         _refused()
 

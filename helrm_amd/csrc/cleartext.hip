@@ -415,14 +415,16 @@ void check_teach_tensors(const DistillationArgs* a) {
 
 // Whether the entries' scores are picked out of the product's tiles, or
 // computed from the table's rows.  Microseconds, measured: the rows at 3.4 TB/s
-// (a common one comes from the caches); two launches more, a row's order 0.005,
-// the end of a tile 1.6.  8,192 x 2,048 against 131,072 rows, 64 entries, bfloat16,
-// both directions: 14,350 picked, 14,890 computed; 1,999 x 416 against 50,021,
-// 17 entries, float32: 2,253 and 2,243.
+// (a common one comes from the caches); two launches more and the order of the
+// entries, each compared with each, the end of a tile 1.6, a row's entries of a
+// tile one after another 0.4.  8,192 x 2,048 against 131,072 rows, 64 entries,
+// bfloat16, both directions: 14,290 picked, 14,885 computed; 192 x 560 against
+// 448, 104 entries, the forward kernels: 74 and 38.
 bool teach_picks(const DistillationArgs* a) {
-  const double tiles = (double)clr::ceil_div(a->rows, 256) * (double)clr::ceil_div(a->vocab, 256);
-  const double computed = (double)a->rows * a->top * a->width * dtype_size(a->type) / 3.4e6;
-  return computed > 5 + 0.005 * (double)a->rows + 1.6 * tiles / 256;
+  const double rows = (double)a->rows, top = a->top, across = (double)clr::ceil_div(a->vocab, 256);
+  const double computed = rows * top * a->width * dtype_size(a->type) / 3.4e6 + 5e-7 * rows * top * top;
+  const double picked = 12 + (3.4e-4 + 1e-6 * rows) * top * top + 1.6 * (double)clr::ceil_div(a->rows, 256) * across / 256 + 0.4 * top / across;
+  return computed > picked;
 }
 
 size_t teach_forward(const DistillationArgs* a, bool count, hipStream_t st) {

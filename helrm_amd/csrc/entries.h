@@ -111,7 +111,7 @@ __device__ __forceinline__ float together(const Entries& e, int j, bool& first) 
 }
 
 // A workgroup has a row's entries, or where there are few rows a share of them,
-// and the first of them the teacher's probabilities.  lds: entries_bytes.
+// the teacher's probabilities among them.  lds: entries_bytes.
 template <class T, class L> __device__ __forceinline__ void row_entries(const TeachArgs& a, long block, char* lds) {
   constexpr int V = 16 / sizeof(T);
   const Entries e(lds, a.top);
@@ -122,18 +122,16 @@ template <class T, class L> __device__ __forceinline__ void row_entries(const Te
   const float top = read_entries<L>(a, row, e, any);
   const int found = __syncthreads_or(any);
   const bool outside = __syncthreads_or(any & 2);
-  if (part == 0) {
-    const float sum = weigh(a, top, e);
-    __syncthreads();
-    for (int j = threadIdx.x; j < a.top; j += blockDim.x) {
-      bool leads;
-      const float p = together(e, j, leads);
-      const int id = e.ids[j];
-      a.probs[first + j] = id == OUTSIDE ? NAN : id == NOTHING || !leads ? -1.0f : p / sum;
-      a.cols[first + j] = id >= 0 && leads ? id : -1;
-    }
-    if (threadIdx.x == 0) a.kept[row] = !found ? TEACH_NONE : outside ? TEACH_OUTSIDE : TEACH_FINE;
+  const float sum = weigh(a, top, e);
+  __syncthreads();
+  for (int j = part * blockDim.x + threadIdx.x; j < a.top; j += a.parts * blockDim.x) {
+    bool leads;
+    const float p = together(e, j, leads);
+    const int id = e.ids[j];
+    a.probs[first + j] = id == OUTSIDE ? NAN : id == NOTHING || !leads ? -1.0f : p / sum;
+    a.cols[first + j] = id >= 0 && leads ? id : -1;
   }
+  if (part == 0 && threadIdx.x == 0) a.kept[row] = !found ? TEACH_NONE : outside ? TEACH_OUTSIDE : TEACH_FINE;
   const T* x = (const T*)a.x + row * a.ldx;
   for (int j0 = (part * waves + wave) * AT_ONCE; j0 < a.top; j0 += a.parts * waves * AT_ONCE) {
     int id[AT_ONCE];

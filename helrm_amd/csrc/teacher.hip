@@ -41,7 +41,7 @@ __global__ __launch_bounds__(BLOCK) void kept_kernel(const TeachArgs a, long bas
 }
 
 // A workgroup a row that counts: its entries in the order of the table's rows.  WAVES: 1 where there are few of them.
-constexpr int order_most(int waves) { return waves == 1 ? 256 : MOST_TOP; }
+constexpr int order_most(int waves) { return waves == 1 ? 64 : MOST_TOP; }
 template <class L, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void order_kernel(const TeachArgs a, long base) {
   extern __shared__ __align__(16) char lds[];
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(WAVES * 64) void order_kernel(const TeachArgs a, lo
     probs[n] = id == OUTSIDE ? NAN : id == NOTHING || !l ? -1.0f : p / sum;
   }
   __syncthreads();
-  int entries = 0;   // all of them
+  int entries = 0;   // all of them, of a thread that has a place
 #pragma unroll
   for (int n = 0; n < MINE; n++) {
     const int j = threadIdx.x + n * WAVES * 64;
@@ -94,11 +94,12 @@ __global__ __launch_bounds__(WAVES * 64) void order_kernel(const TeachArgs a, lo
     }
     if (id >= 0) tiles[at] = id >> a.shift;
   }
-  entries = __builtin_amdgcn_readfirstlane(entries);
+  __shared__ int all;   // (waves whose threads have no place have not counted)
+  if (threadIdx.x == 0) all = entries;
   __syncthreads();
   uint16_t* starts = a.starts + i * (a.tiles + 1L);
-  for (int k = threadIdx.x >> 6; k <= entries; k += WAVES) {   // tiles whose first entry is number k
-    const int from = k ? tiles[k - 1] + 1 : 0, to = k < entries ? tiles[k] : a.tiles;
+  for (int k = threadIdx.x >> 6; k <= all; k += WAVES) {   // tiles whose first entry is number k
+    const int from = k ? tiles[k - 1] + 1 : 0, to = k < all ? tiles[k] : a.tiles;
     for (int t = from + (int)(threadIdx.x & 63); t <= to; t += 64) starts[t] = (uint16_t)k;
   }
 }
