@@ -8,8 +8,8 @@ against the same table:
 
     z = block(layer_norm(table[item]));  p(next) = softmax(<z, table>)
 
-Training takes `helrm_amd.cleartext`: layer_norm, gated_mlp and cross_entropy
-on the GPU.  The trained model is then evaluated on an encrypted one-hot
+Training takes `helrm_amd.cleartext`: embedding, layer_norm, gated_mlp and
+cross_entropy on the GPU.  The trained model is then evaluated on an encrypted one-hot
 selector with what the backend has: the normalisation folds into the table
 (the norm of a looked-up row is a look-up in the table of normalised rows), so
 the encrypted path is a lookup, two Linears, the activation, a product of
@@ -62,7 +62,7 @@ def train(steps=400, batch=1024, seed=0, log=print):
         item = torch.randint(ITEMS, (batch,), generator=gen, device="cuda")
         target = successor[item]
         target = torch.where(torch.rand(batch, generator=gen, device="cuda") < 0.1, torch.full_like(target, -100), target)
-        loss = score(model, block(model, model["table"][item]), target)
+        loss = score(model, block(model, ct.embedding(item, model["table"])), target)
         opt.zero_grad()
         loss.backward()
         opt.step()

@@ -295,10 +295,16 @@ def test_autograd_and_reductions(ct, rows):  # noqa: F811
         with torch.no_grad():
             assert torch.equal(ct.distillation(a, b, ids, logits, 2.0, reduction=reduction), total.detach())
     assert ct.distillation(x[:0], table, ids[:0], logits[:0]).item() == 0
+    b.grad = None
+    ct.distillation(x[:0], b, ids[:0], logits[:0], reduction="sum").backward()
+    assert b.grad.shape == table.shape and not b.grad.any()
     nothing = ct.distillation(a, b, torch.full_like(ids, IGNORE), logits)
     a.grad = None
     nothing.backward()
     assert nothing.item() == 0 and not a.grad.any()
+    (g,) = torch.autograd.grad(ct.distillation(a, b, ids, logits).square(), a, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
     # one of the two without a gradient
     a.grad = None
     ct.distillation(a, table, ids, logits, 2.0, reduction="sum").backward()

@@ -222,6 +222,9 @@ def test_autograd_and_reductions(ct):  # noqa: F811
     line, offsets = losses.view(-1).clone().requires_grad_(), torch.arange(0, 19 * 70, 70, device=DEV)
     ct.preference(line, reference.view(-1), target.view(-1), offsets, smoothing=0.1, reduction="sum").backward()
     assert torch.equal(line.grad.view(9, 2, 70), leaf.grad)
+    (g,) = torch.autograd.grad(ct.preference(leaf, reference, target).square(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
     with torch.no_grad():
         assert not ct.preference(leaf, reference, target).requires_grad
     assert ct.preference(losses[:0], reference[:0]).item() == 0
