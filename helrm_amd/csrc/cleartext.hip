@@ -456,9 +456,8 @@ size_t teach_forward(const DistillationArgs* a, bool count, hipStream_t st) {
     p.rate = rate;
     f.parts = skinny_softmax_parts(a->vocab);
     f.part = p.part = m.take<float2>((size_t)n * f.parts);
-    p.entries = e;
     if (count) return m.used;
-    skinny_teach(p, st);
+    skinny_teach(p, e, st);
     teach_finish(f, st);
     return m.used;
   }

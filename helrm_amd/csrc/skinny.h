@@ -16,7 +16,6 @@ struct SkinnyArgs {
   const long long* target; float* picked; float2* part;   // softmax: [T], [T], [T][parts]
   int parts, groups; bool alone;     // (of the launch)
   float rate;                        // teach: of the products
-  TeachArgs entries; int entry_groups;   // teach: of the rows of X; the workgroups that have them, rows * parts of the first ones
 };
 // out = act(X W^T) * (X W2^T)
 void skinny_gate(SkinnyArgs p, hipStream_t st);
@@ -25,5 +24,5 @@ void skinny_store(SkinnyArgs p, hipStream_t st);
 // loss and lse of every row of X against the rows of W
 int skinny_softmax_parts(int N);
 void skinny_softmax(SkinnyArgs p, long long ignore, float* loss, float* lse, hipStream_t st);
-// the pieces of the softmax of rate X W^T, p.part, of every row of X, and teach_entries of p.entries beside it
-void skinny_teach(SkinnyArgs p, hipStream_t st);
+// the pieces of the softmax of rate X W^T, p.part, of every row of X, and teach_entries of those rows beside it
+void skinny_teach(SkinnyArgs p, const TeachArgs& entries, hipStream_t st);

@@ -105,19 +105,24 @@ template <class T> __device__ __forceinline__ void dot8(const Eight<T>& w, const
 // saves the exchange of sums.  Lane l of a wave holds, of a
 // group, row l % 16 and the k 16 (l / 16) + 0..15 of 64; its sums are row t = l % 16
 // of X and the columns 4 (l / 16) + 0..3.
+// What a launch does beside its product.
+struct Nothing {};
+template <int EPI> using Beside = std::conditional_t<EPI == SKINNY_TEACH, TeachArgs, Nothing>;
 template <class T, bool ALIGNED, int NB> constexpr int most_waves() { return sizeof(T) == 2 && ALIGNED && NB == 1 ? 16 : 8; }
 // X: the type of x, T or float.
 template <class T, class X, bool ALIGNED, int NB, int EPI>
-__global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_kernel(const SkinnyArgs p) {
+__global__ __launch_bounds__((most_waves<T, ALIGNED, NB>()) * 64) void skinny_kernel(const SkinnyArgs p, const Beside<EPI> beside) {
   constexpr int MATS = EPI == SKINNY_GATE ? 2 : 1, TURNS = !ALIGNED || sizeof(T) == 4 ? 2 : 4;
   extern __shared__ __align__(16) float lds[];   // [waves][MATS * NB][64][4]
-  if constexpr (EPI == SKINNY_TEACH)
-    if ((int)blockIdx.x < p.entry_groups) {   // (beside the others, which the memory holds up)
-      if (p.entries.teacher_type == DT_F32) row_entries<T, float>(p.entries, blockIdx.x, (char*)lds);
-      else row_entries<T, T>(p.entries, blockIdx.x, (char*)lds);
+  int block = blockIdx.x;
+  if constexpr (EPI == SKINNY_TEACH) {
+    block -= p.T * beside.parts;
+    if (block < 0) {   // the first workgroups (the memory holds up the others meanwhile)
+      if (beside.teacher_type == DT_F32) row_entries<T, float>(beside, blockIdx.x, (char*)lds);
+      else row_entries<T, T>(beside, blockIdx.x, (char*)lds);
       return;
     }
-  const int block = EPI == SKINNY_TEACH ? blockIdx.x - p.entry_groups : blockIdx.x;
+  }
   const int lane = threadIdx.x & 63, own = threadIdx.x >> 6;
   const int wave = p.alone ? 0 : own, waves = p.alone ? 1 : blockDim.x >> 6;   // of those that share k
   const long team = p.alone ? (long)block * (blockDim.x >> 6) + own : block;
@@ -271,7 +276,7 @@ int waves_of(int N, int K, int type, int most) {
   return w;
 }
 
-template <int EPI> void launch(SkinnyArgs p, hipStream_t st) {
+template <int EPI> void launch(SkinnyArgs p, hipStream_t st, const Beside<EPI>& beside = {}) {
   if (p.T <= 0 || p.N <= 0) return;
   const long teams = clr::ceil_div(p.N, 16L * p.groups);
   p.alone = teams >= 2048;
@@ -284,10 +289,15 @@ template <int EPI> void launch(SkinnyArgs p, hipStream_t st) {
     auto go = [&](auto nb) {
       constexpr int NB = decltype(nb)::value;
       const int waves = p.alone ? 4 : waves_of(p.N, p.K, p.dtype, aligned ? most_waves<T, true, NB>() : most_waves<T, false, NB>());
-      const unsigned grid = clr::groups_of((p.alone ? clr::ceil_div(teams, 4) : teams) + p.entry_groups, waves * 64);
-      const size_t lds = std::max((size_t)waves * (EPI == SKINNY_GATE ? 2 : 1) * NB * 1024, EPI == SKINNY_TEACH ? entries_bytes(p.entries.top) : 0);
-      if (aligned) skinny_kernel<T, X, true, NB, EPI><<<grid, waves * 64, lds, st>>>(p);
-      else skinny_kernel<T, X, false, NB, EPI><<<grid, waves * 64, lds, st>>>(p);
+      long groups = p.alone ? clr::ceil_div(teams, 4) : teams;
+      size_t lds = (size_t)waves * (EPI == SKINNY_GATE ? 2 : 1) * NB * 1024;
+      if constexpr (EPI == SKINNY_TEACH) {
+        groups += (long)p.T * beside.parts;
+        lds = std::max(lds, entries_bytes(beside.top));
+      }
+      const unsigned grid = clr::groups_of(groups, waves * 64);
+      if (aligned) skinny_kernel<T, X, true, NB, EPI><<<grid, waves * 64, lds, st>>>(p, beside);
+      else skinny_kernel<T, X, false, NB, EPI><<<grid, waves * 64, lds, st>>>(p, beside);
     };
     if (p.T <= 16) go(std::integral_constant<int, 1>{});
     if constexpr (sizeof(T) == 4) {
@@ -310,9 +320,8 @@ void skinny_softmax(SkinnyArgs p, long long ignore, float* loss, float* lse, hip
   launch<SKINNY_SOFTMAX>(p, st);
   skinny_finish_kernel<<<(unsigned)p.T, FINISH, 0, st>>>(p.part, p.parts, p.picked, p.target, ignore, p.N, loss, lse);
 }
-void skinny_teach(SkinnyArgs p, hipStream_t st) {
+void skinny_teach(SkinnyArgs p, const TeachArgs& entries, hipStream_t st) {
   p.groups = softmax_groups(p.N);
   p.parts = skinny_softmax_parts(p.N);
-  p.entry_groups = p.T * p.entries.parts;
-  launch<SKINNY_TEACH>(p, st);
+  launch<SKINNY_TEACH>(p, st, entries);
 }
