@@ -107,17 +107,18 @@ __device__ __forceinline__ unsigned key_of(const SortArgs& a, int i) {
   return inside(a, id) ? (unsigned)id : (unsigned)a.vocab;
 }
 
-// Item j of a lane is number wave * 64 ITEMS + 64 j + lane of the tile; the
+// Item j < per of a lane is number (wave * per + j) * 64 + lane of the tile; the
 // first n of them are there.  rank[j]: how many items of the wave with the same
 // digit are before it; counts[wave][digit]: how many the wave has.
 template <int ITEMS>
-__device__ __forceinline__ void rank_items(const unsigned (&key)[ITEMS], int n, int shift, int bits, int (&rank)[ITEMS], int (*counts)[MOST_DIGITS]) {
+__device__ __forceinline__ void rank_items(const unsigned (&key)[ITEMS], int per, int n, int shift, int bits, int (&rank)[ITEMS], int (*counts)[MOST_DIGITS]) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int k = lane; k < 1 << bits; k += 64) counts[wave][k] = 0;
   asm volatile("" ::: "memory");
 #pragma unroll
   for (int j = 0; j < ITEMS; j++) {
-    const bool there = (wave * ITEMS + j) * 64 + lane < n;
+    if (j >= per) break;
+    const bool there = (wave * per + j) * 64 + lane < n;
     const unsigned digit = key[j] >> shift & ((1u << bits) - 1);
     const unsigned long long all = __ballot(there);
     unsigned low = (unsigned)all, high = (unsigned)(all >> 32);   // lanes with the same digit
@@ -139,21 +140,26 @@ __device__ __forceinline__ void rank_items(const unsigned (&key)[ITEMS], int n, 
     __builtin_amdgcn_wave_barrier();
   }
 }
-// counts[wave][digit] becomes what the waves before have; the result, of thread `digit`, what all have.
-__device__ __forceinline__ int over_waves(int digits, int (*counts)[MOST_DIGITS]) {
-  int sum = 0;
-  if ((int)threadIdx.x < digits) {
-    int c[WAVES];
+// What the waves have of a digit, of thread `digit`.
+struct Column {
+  int count[WAVES];
+  __device__ __forceinline__ int read(int digits, const int (*counts)[MOST_DIGITS]) {
+    int sum = 0;
+    if ((int)threadIdx.x < digits)
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) c[w] = counts[w][threadIdx.x];
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) {
-      counts[w][threadIdx.x] = sum;
-      sum += c[w];
-    }
+      for (int w = 0; w < WAVES; w++) sum += count[w] = counts[w][threadIdx.x];
+    return sum;
   }
-  return sum;
-}
+  // counts[wave][digit] becomes where the wave's first one goes, where those of the digit begin at `first`
+  __device__ __forceinline__ void place(int digits, int first, int (*counts)[MOST_DIGITS]) const {
+    if ((int)threadIdx.x < digits)
+#pragma unroll
+      for (int w = 0; w < WAVES; w++) {
+        counts[w][threadIdx.x] = first;
+        first += count[w];
+      }
+  }
+};
 // The sum of v over the threads before this one.  Two barriers.
 __device__ __forceinline__ int before_me(int v, int* lds) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -210,31 +216,32 @@ __device__ __forceinline__ void clear_share(const Clear& c, int group) {
 // The whole sort of up to SORT * ITEMS ids.
 template <int ITEMS>
 __global__ __launch_bounds__(SORT) void sort_one_kernel(const SortArgs a, const Clear c) {
-  __shared__ int counts[WAVES][MOST_DIGITS], start[MOST_DIGITS], sums[WAVES];
+  __shared__ int counts[WAVES][MOST_DIGITS], sums[WAVES];
   __shared__ unsigned keys[SORT * ITEMS], ats[SORT * ITEMS];
   if (blockIdx.x) return clear_share(c, blockIdx.x - 1);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = (a.n + SORT - 1) / SORT;   // (as many for every wave)
   unsigned key[ITEMS], at[ITEMS];
   int rank[ITEMS];
 #pragma unroll
   for (int j = 0; j < ITEMS; j++) {
-    const int i = (wave * ITEMS + j) * 64 + lane;
-    key[j] = i < a.n ? key_of(a, i) : 0;
+    const int i = (wave * per + j) * 64 + lane;
+    key[j] = j < per && i < a.n ? key_of(a, i) : 0;
     at[j] = i;
   }
   for (int pass = 0; pass < a.passes; pass++) {
     const int shift = pass * a.bits;
-    rank_items<ITEMS>(key, a.n, shift, a.bits, rank, counts);
+    rank_items<ITEMS>(key, per, a.n, shift, a.bits, rank, counts);
     __syncthreads();
-    const int base = before_me(over_waves(1 << a.bits, counts), sums);
-    if ((int)threadIdx.x < 1 << a.bits) start[threadIdx.x] = base;
+    Column column;
+    const int all = column.read(1 << a.bits, counts);
+    column.place(1 << a.bits, before_me(all, sums), counts);
     __syncthreads();
     const bool last = pass == a.passes - 1;
 #pragma unroll
     for (int j = 0; j < ITEMS; j++)
-      if ((wave * ITEMS + j) * 64 + lane < a.n) {
+      if (j < per && (wave * per + j) * 64 + lane < a.n) {
         const unsigned digit = key[j] >> shift & ((1u << a.bits) - 1);
-        const int to = start[digit] + counts[wave][digit] + rank[j];
+        const int to = counts[wave][digit] + rank[j];
         (last ? a.to : keys)[to] = key[j];
         (last ? a.to_at : ats)[to] = at[j];
       }
@@ -242,9 +249,9 @@ __global__ __launch_bounds__(SORT) void sort_one_kernel(const SortArgs a, const 
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < ITEMS; j++) {
-      const int i = (wave * ITEMS + j) * 64 + lane;
-      key[j] = i < a.n ? keys[i] : 0;
-      at[j] = i < a.n ? ats[i] : 0;
+      const int i = (wave * per + j) * 64 + lane;
+      key[j] = j < per && i < a.n ? keys[i] : 0;
+      at[j] = j < per && i < a.n ? ats[i] : 0;
     }
     // (the next pass writes them after three barriers)
   }
@@ -293,7 +300,7 @@ __global__ __launch_bounds__(SORT) void scan_kernel(const SortArgs a) {
 // ... and every item to its place.
 template <int ITEMS>
 __global__ __launch_bounds__(SORT) void scatter_kernel(const SortArgs a, const Clear c) {
-  __shared__ int counts[WAVES][MOST_DIGITS], start[MOST_DIGITS], sums[WAVES], others[2][MOST_DIGITS];
+  __shared__ int counts[WAVES][MOST_DIGITS], sums[WAVES], others[2][MOST_DIGITS];
   if ((int)blockIdx.x >= a.tiles) return clear_share(c, blockIdx.x - a.tiles);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, digits = 1 << a.bits, tile = blockIdx.x, first = tile * SORT * ITEMS;
   unsigned key[ITEMS], at[ITEMS];
@@ -327,17 +334,18 @@ __global__ __launch_bounds__(SORT) void scatter_kernel(const SortArgs a, const C
     others[0][digit] = before;
     others[1][digit] = all;
   }
-  rank_items<ITEMS>(key, n, a.shift, a.bits, rank, counts);
+  rank_items<ITEMS>(key, ITEMS, n, a.shift, a.bits, rank, counts);
   __syncthreads();
-  over_waves(digits, counts);
+  Column column;
+  column.read(digits, counts);
   const int base = before_me(half ? 0 : all + others[1][digit], sums);
-  if (!half) start[digit] = base + before + others[0][digit];
+  column.place(digits, half ? 0 : base + before + others[0][digit], counts);
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < ITEMS; j++)
     if ((wave * ITEMS + j) * 64 + lane < n) {
       const unsigned d = key[j] >> a.shift & (digits - 1);
-      const int to = start[d] + counts[wave][d] + rank[j];
+      const int to = counts[wave][d] + rank[j];
       a.to[to] = key[j];
       a.to_at[to] = at[j];
     }
