@@ -6,7 +6,7 @@
 // that equal ids keep their order), the sorted ids are cut into pieces of equal
 // length, and each piece adds the rows of its runs of equal ids in registers.  A
 // run inside a piece is a row of the gradient; what a run has in each of several
-// pieces is added in order by a second launch.  So a common id is as parallel
+// pieces is added in a fixed order by a second launch.  So a common id is as parallel
 // as any, and a result is the same on every run.  Sums are float32, scaled and
 // rounded once.  Rows that no id names are cleared by workgroups beside the
 // sort's, which so costs nothing where the table is large.
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(SORT) void sort_one_kernel(const SortArgs a, const 
 
 // One pass over many tiles: how often each digit is in a tile, ...
 template <int ITEMS>
-__global__ __launch_bounds__(SORT) void count_kernel(const SortArgs a, const Clear c) {
+__global__ __launch_bounds__(SORT) void sort_count_kernel(const SortArgs a, const Clear c) {
   __shared__ int counts[MOST_DIGITS];
   if ((int)blockIdx.x >= a.tiles) return clear_share(c, blockIdx.x - a.tiles);
   const int digits = 1 << a.bits, first = blockIdx.x * SORT * ITEMS;
@@ -275,7 +275,7 @@ __global__ __launch_bounds__(SORT) void count_kernel(const SortArgs a, const Cle
 }
 // ... (of many tiles) in the tiles before, and in all, in a row behind the last; 64 digits a workgroup, ...
 constexpr int FEW_TILES = 128;   // the most that every workgroup adds up by itself
-__global__ __launch_bounds__(SORT) void scan_kernel(const SortArgs a) {
+__global__ __launch_bounds__(SORT) void sort_scan_kernel(const SortArgs a) {
   __shared__ int sums[WAVES][64];
   const int digits = 1 << a.bits, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, digit = blockIdx.x * 64 + lane;
   const int from = (int)((long)a.tiles * wave / WAVES), to = (int)((long)a.tiles * (wave + 1) / WAVES);
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(SORT) void scan_kernel(const SortArgs a) {
 }
 // ... and every item to its place.
 template <int ITEMS>
-__global__ __launch_bounds__(SORT) void scatter_kernel(const SortArgs a, const Clear c) {
+__global__ __launch_bounds__(SORT) void sort_scatter_kernel(const SortArgs a, const Clear c) {
   __shared__ int counts[WAVES][MOST_DIGITS], sums[WAVES], others[2][MOST_DIGITS];
   if ((int)blockIdx.x >= a.tiles) return clear_share(c, blockIdx.x - a.tiles);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, digits = 1 << a.bits, tile = blockIdx.x, first = tile * SORT * ITEMS;
@@ -367,7 +367,7 @@ struct SumArgs {
 
 // WAVE: a team is a wave.
 template <class T, int V, bool WAVE>
-__global__ __launch_bounds__(BLOCK) void sum_kernel(const SumArgs a, long base) {
+__global__ __launch_bounds__(BLOCK) void run_sum_kernel(const SumArgs a, long base) {
   constexpr int AHEAD = 8;
   const int lane = WAVE ? threadIdx.x & 63 : threadIdx.x & (a.lanes - 1);
   unsigned team = (unsigned)(((base + blockIdx.x) * BLOCK + threadIdx.x) / (WAVE ? 64 : a.lanes));
@@ -426,7 +426,7 @@ __global__ __launch_bounds__(BLOCK) void sum_kernel(const SumArgs a, long base) 
 // most pieces have none, a common id's has thousands of sums behind it.
 constexpr int JOIN = 1024;   // the most threads
 template <class T, int V>
-__global__ __launch_bounds__(JOIN) void join_kernel(const SumArgs a, long base) {
+__global__ __launch_bounds__(JOIN) void run_join_kernel(const SumArgs a, long base) {
   extern __shared__ float lds[];   // [threads][V]
   const int piece = (int)(base + blockIdx.x), from = piece * a.piece, to = from + a.piece;
   if (to >= a.n) return;
@@ -474,6 +474,7 @@ template <class F> void with_items(int n, F&& f) {
   else if (n <= 4) f(std::integral_constant<int, 4>{});
   else f(std::integral_constant<int, 8>{});
 }
+
 // ---- few ids ----
 // One launch: a workgroup an id (and column block), which adds the rows of all
 // that are equal if it is the first of them, and others that clear rows of the
@@ -670,10 +671,10 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
       s.to = space.keys[out];
       s.to_at = space.ats[out];
       unsigned groups = s.tiles + clearing(3 * pass, 1, 3 * s.passes);
-      with_items(items, [&](auto n) { count_kernel<decltype(n)::value><<<groups, SORT, 0, st>>>(s, c); });
-      if (s.tiles > FEW_TILES) scan_kernel<<<(unsigned)clr::ceil_div(1 << s.bits, 64), SORT, 0, st>>>(s);
+      with_items(items, [&](auto n) { sort_count_kernel<decltype(n)::value><<<groups, SORT, 0, st>>>(s, c); });
+      if (s.tiles > FEW_TILES) sort_scan_kernel<<<(unsigned)clr::ceil_div(1 << s.bits, 64), SORT, 0, st>>>(s);
       groups = s.tiles + clearing(3 * pass + 1, 2, 3 * s.passes);
-      with_items(items, [&](auto n) { scatter_kernel<decltype(n)::value><<<groups, SORT, 0, st>>>(s, c); });
+      with_items(items, [&](auto n) { sort_scatter_kernel<decltype(n)::value><<<groups, SORT, 0, st>>>(s, c); });
     }
   }
   const int packs = packs_of(a.width, a.dtype);
@@ -696,10 +697,10 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
     constexpr int V = decltype(v)::value;
     const long teams = (long)m.pieces * m.blocks;
     clr::in_launches(clr::ceil_div(teams * m.lanes, BLOCK), BLOCK, [&](long base, unsigned n) {
-      if (m.lanes == 64) sum_kernel<T, V, true><<<n, BLOCK, 0, st>>>(m, base);
-      else sum_kernel<T, V, false><<<n, BLOCK, 0, st>>>(m, base);
+      if (m.lanes == 64) run_sum_kernel<T, V, true><<<n, BLOCK, 0, st>>>(m, base);
+      else run_sum_kernel<T, V, false><<<n, BLOCK, 0, st>>>(m, base);
     });
     if (m.pieces > 1)
-      clr::in_launches(m.pieces, threads, [&](long base, unsigned n) { join_kernel<T, V><<<n, threads, threads * V * sizeof(float), st>>>(m, base); });
+      clr::in_launches(m.pieces, threads, [&](long base, unsigned n) { run_join_kernel<T, V><<<n, threads, threads * V * sizeof(float), st>>>(m, base); });
   });
 }
