@@ -4,18 +4,19 @@ The encrypted path (`orion_host`) evaluates a model that was trained: its
 table, its Linears, its degree-3 activations.  These are the operators of
 that training and of scoring beside it, on the same card:
 
+    embedding       y[i] = scale * table[ids[i]]
     layer_norm      y = (x - mean) / sqrt(var + eps) * weight + bias
     gated_mlp       y = (act(x gate^T) * (x up^T)) down^T
     cross_entropy   log sum_v exp <x, table[v]> - <x, table[target]>
     distillation    the divergence of a teacher's top logits from the softmax of <x, table[v]>
-    preference      log(1 + exp -m) of the difference m of two sequences' log ratios to a reference
-    embedding       y[i] = scale * table[ids[i]]
+    preference      log(1 + exp -m), m the difference of two sequences' log ratios to a reference
 
 Each has a `_forward` and a `_backward` call, which a training loop of one's
 own makes, and a form for torch's autograd.  The matrices' last dimension is
 the vector; leading dimensions are rows.  Types: float32, bfloat16, float16,
-one for all of an operator's tensors (a norm's weight and bias may be float32
-beside any); sums and softmax statistics are float32.  Tensors of the same rows
+one for all of an operator's tensors (a norm's weight and bias and a teacher's
+logits may be float32 beside any; tokens' losses are float32); sums and softmax
+statistics are float32.  Tensors of the same rows
 have the same leading dimensions, or the rows in one.
 
 Work goes to torch's current stream of the tensors' device and nothing waits
