@@ -362,6 +362,7 @@ struct SumArgs {
   int piece, pieces;           // length and number
   int lanes, blocks;           // of a team, which adds `lanes` packs of the rows of a piece; teams beside one another
   int across;                  // lanes of a team that joins
+  int group;                   // pieces whose shares of one run are added beforehand, where there are so many pieces
   float scale;
 };
 
@@ -422,9 +423,62 @@ __global__ __launch_bounds__(BLOCK) void run_sum_kernel(const SumArgs a, long ba
   else done();
 }
 
-// The runs that go on over pieces, a workgroup for the piece that one begins in:
-// most pieces have none, a common id's has thousands of sums behind it.
+// Sums of `items` partial sums, number i of them item(i), a column of packs a
+// lane, by the teams of a workgroup; put(at, sum) of each pack.
+template <int V, class I, class F> __device__ __forceinline__ void add_partials(const SumArgs& a, int items, float* lds, I&& item, F&& put) {
+  const int lane = threadIdx.x & (a.across - 1), team = threadIdx.x / a.across, teams = blockDim.x / a.across;
+  for (int first = 0; first < a.packs; first += a.across) {
+    const int pack = first + lane, at = pack_at<V>(pack, a.width);
+    float sum[V] = {};
+    if (pack < a.packs)
+#pragma unroll 8
+      for (int i = team; i < items; i += teams) {
+        float v[V];
+        __builtin_memcpy(v, a.partial + item(i) * a.width + at, sizeof(v));
+#pragma unroll
+        for (int e = 0; e < V; e++) sum[e] += v[e];
+      }
+    if (first) __syncthreads();
+#pragma unroll
+    for (int e = 0; e < V; e++) lds[threadIdx.x * V + e] = sum[e];
+    __syncthreads();
+    if (team || pack >= a.packs) continue;
+    for (int t = 1; t < min(teams, items); t++)
+#pragma unroll
+      for (int e = 0; e < V; e++) sum[e] += lds[(t * a.across + lane) * V + e];
+    put(at, sum);
+  }
+}
+// How many of the pieces from, from + step, ... before `end` begin with `key`: those in front, as long as they do.
+__device__ __forceinline__ int beginning_with(const SumArgs& a, unsigned key, int from, int step, int end) {
+  int count = 0;
+  for (long q = from; q < end; q += (long)step * blockDim.x) {
+    const long mine = q + (long)step * threadIdx.x;
+    const int n = __syncthreads_count(mine < end && a.keys[mine * a.piece] == key);
+    count += n;
+    if (n < (int)blockDim.x) break;
+  }
+  return count;
+}
+// A run that goes on over groups of pieces: what it has in several pieces of one
+// is added up, a workgroup a group, into the second place of the first of
+// them, which no other run can need: that piece is the run's from end to end.
 constexpr int JOIN = 1024;   // the most threads
+template <int V>
+__global__ __launch_bounds__(JOIN) void run_group_kernel(const SumArgs a, long base) {
+  extern __shared__ float lds[];   // [threads][V]
+  const int piece = (int)(base + blockIdx.x) * a.group, from = piece * a.piece;
+  if (!from) return;
+  const unsigned key = a.keys[from];
+  if (key >= (unsigned)a.vocab || a.keys[from - 1] != key) return;
+  const int items = beginning_with(a, key, piece, 1, min(piece + a.group, a.pieces));
+  if (items == 1) return;
+  add_partials<V>(a, items, lds, [&](int i) { return ((long)piece + i) * 2; }, [&](int at, const float(&sum)[V]) {
+    __builtin_memcpy(a.partial + ((long)piece * 2 + 1) * a.width + at, sum, sizeof(sum));
+  });
+}
+// The runs that go on over pieces, a workgroup for the piece that one begins in:
+// most pieces have none.
 template <class T, int V>
 __global__ __launch_bounds__(JOIN) void run_join_kernel(const SumArgs a, long base) {
   extern __shared__ float lds[];   // [threads][V]
@@ -432,40 +486,20 @@ __global__ __launch_bounds__(JOIN) void run_join_kernel(const SumArgs a, long ba
   if (to >= a.n) return;
   const unsigned key = a.keys[to];
   if (key >= (unsigned)a.vocab || a.keys[to - 1] != key || (from > 0 && a.keys[from - 1] == key)) return;
-  // pieces that begin with the run: those behind this one, as long as there are any
-  int more = 0;
-  for (int q = piece + 1;; q += blockDim.x) {
-    const int mine = q + threadIdx.x;
-    const int n = __syncthreads_count(mine < a.pieces && a.keys[(long)mine * a.piece] == key);
-    more += n;
-    if (n < (int)blockDim.x) break;
-  }
-  const int lane = threadIdx.x & (a.across - 1), team = threadIdx.x / a.across, teams = blockDim.x / a.across;
-  for (int first = 0; first < a.packs; first += a.across) {
-    const int pack = first + lane, at = pack_at<V>(pack, a.width);
-    float sum[V] = {};
-    if (pack < a.packs)
-#pragma unroll 8
-      for (int i = team; i <= more; i += teams) {
-        float v[V];
-        __builtin_memcpy(v, a.partial + (((long)piece + i) * 2 + (i == 0)) * a.width + at, sizeof(v));
+  // the pieces that it goes on in: the rest of the group, then groups
+  const int next = (int)min((piece / a.group + 1L) * a.group, (long)a.pieces);
+  const int own = beginning_with(a, key, piece + 1, 1, next), groups = piece + 1 + own == next ? beginning_with(a, key, next, a.group, a.pieces) : 0;
+  add_partials<V>(a, 1 + own + groups, lds,
+                  [&](int i) {
+                    if (i <= own) return ((long)piece + i) * 2 + (i == 0);
+                    const long first = next + (i - own - 1L) * a.group;   // of a group
+                    return first * 2 + (first + 1 < a.pieces && a.keys[(first + 1) * a.piece] == key);
+                  },
+                  [&](int at, float(&sum)[V]) {
 #pragma unroll
-        for (int e = 0; e < V; e++) sum[e] += v[e];
-      }
-    if (teams > 1) {
-      if (first) __syncthreads();
-#pragma unroll
-      for (int e = 0; e < V; e++) lds[threadIdx.x * V + e] = sum[e];
-      __syncthreads();
-    }
-    if (team || pack >= a.packs) continue;
-    for (int t = 1; t < min(teams, more + 1); t++)
-#pragma unroll
-      for (int e = 0; e < V; e++) sum[e] += lds[(t * a.across + lane) * V + e];
-#pragma unroll
-    for (int e = 0; e < V; e++) sum[e] *= a.scale;
-    store_pack<false, T, V>((T*)a.dtable + (long)key * a.width + at, sum);
-  }
+                    for (int e = 0; e < V; e++) sum[e] *= a.scale;
+                    store_pack<false, T, V>((T*)a.dtable + (long)key * a.width + at, sum);
+                  });
 }
 
 template <class F> void with_items(int n, F&& f) {
@@ -563,6 +597,10 @@ int packs_of(int width, int dtype) {
   return width >= v ? (int)clr::ceil_div(width, v) : width;
 }
 
+// Pieces from which on a launch adds up groups of them before each run is joined
+// by a workgroup: 4 us more where runs are short (53,248 x 16, 3,328 pieces: 39 us,
+// 44 with it); 2^20 equal ids x 512, 16,384 pieces, 347 us with it and 1,711 without.
+constexpr int MANY_PIECES = 4096;
 // The pieces of the workspace, or only their bytes.
 struct Space {
   unsigned *keys[2], *ats[2];
@@ -691,6 +729,7 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
   m.blocks = (int)clr::ceil_div(packs, m.lanes);
   m.piece = piece_of(a.tokens, m.blocks, m.lanes);
   m.pieces = (int)clr::ceil_div(a.tokens, m.piece);
+  m.group = m.pieces > MANY_PIECES ? 32 : m.pieces;
   m.scale = a.scale;
   with_packs(a.dtype, a.width, [&](auto t, auto v) {
     using T = decltype(t);
@@ -700,6 +739,9 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
       if (m.lanes == 64) run_sum_kernel<T, V, true><<<n, BLOCK, 0, st>>>(m, base);
       else run_sum_kernel<T, V, false><<<n, BLOCK, 0, st>>>(m, base);
     });
+    if (m.group < m.pieces)
+      clr::in_launches(clr::ceil_div(m.pieces, m.group), threads,
+                       [&](long base, unsigned n) { run_group_kernel<V><<<n, threads, threads * V * sizeof(float), st>>>(m, base); });
     if (m.pieces > 1)
       clr::in_launches(m.pieces, threads, [&](long base, unsigned n) { run_join_kernel<T, V><<<n, threads, threads * V * sizeof(float), st>>>(m, base); });
   });

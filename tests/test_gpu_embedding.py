@@ -77,6 +77,33 @@ def test_runs_that_end_anywhere(ct, width):  # noqa: F811
         embed_check(ct, ids.to(DEV), normal(gen, 70, width), normal(gen, len(ids), width), 1.0)
 
 
+@pytest.mark.parametrize("width", [3, 24, 600])
+def test_runs_over_groups_of_pieces(ct, width):  # noqa: F811
+    # so many ids that pieces' sums are added in groups of 32 before: runs of about one, two and many groups, that begin and end anywhere
+    gen = seeded(width)
+    lengths = [1, 15, 500, 511, 512, 513, 1023, 1024, 1025, 3, 2000, 16, 16, 4096, 40, 9000, 30000, 1, 700, 700, 700, 20]
+    ids = torch.cat([torch.full((n,), 2 * k) for k, n in enumerate(lengths)])
+    ids = torch.cat([ids, 2 * len(lengths) + torch.arange(max(0, 66000 - len(ids))) // 3])
+    for ids in (ids, ids[torch.randperm(len(ids), generator=gen)]):
+        embed_check(ct, ids.to(DEV), normal(gen, int(ids.max()) + 2, width), normal(gen, len(ids), width), 1.0)
+
+
+def test_a_run_over_groups_of_rows_wider_than_a_workgroup(ct):  # noqa: F811
+    # the last pack of a row overlaps one of another turn's
+    width = 1024 * 8 + 3
+    n = 4200 * 64 + 5
+    ids = torch.full((n,), 1)
+    ids[::1000] = 0
+    grad = torch.randn(n, width, generator=torch.Generator(DEV).manual_seed(1), device=DEV).bfloat16()
+    d = ct.embedding_backward(grad, ids.to(DEV), 3)
+    for v in (0, 1):
+        rows = grad[(ids == v).to(DEV)]
+        want, size = (sum(part.double().sum(0) for part in t.split(4096)) for t in (rows, rows.abs()))
+        # a term is in at most 64 additions of its piece, 32 of its group and 132 of the groups
+        assert ((d[v].double() - want).abs() <= size * 230 * F32 + want.abs() * ref.U[torch.bfloat16]).all()
+    assert not d[2].any()
+
+
 @pytest.mark.parametrize("more", [0, 500])
 def test_equal_ids_are_added_in_their_order(ct, more):  # noqa: F811
     # 2^24 + 1 + 1 + ... in float32 stays 2^24, 1 + 1 + ... + 2^24 does not: each id's rows are in order within a piece
