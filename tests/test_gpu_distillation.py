@@ -152,6 +152,28 @@ def test_scores_out_of_the_tiles_of_odd_entries(ct, dtype, rows, width, vocab, t
     assert torch.isnan(dtable).all()
 
 
+def test_scores_out_of_the_tiles_of_several_launches(ct):  # noqa: F811
+    # 4,096 x 1,025 tiles go in two launches, cut at column 131,328; all vectors but a few are 0
+    rows, vocab, width, top = 1 << 20, (1 << 18) + 200, 1024, 64
+    gen = torch.Generator(DEV).manual_seed(3)
+    table = (torch.randn(vocab, width, generator=gen, device=DEV) * 0.03).bfloat16()
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device=DEV)
+    some = torch.cat([torch.arange(40), torch.arange(rows // 2 - 20, rows // 2 + 20), torch.arange(rows - 40, rows)]).to(DEV)
+    x[some] = torch.randn(len(some), width, generator=gen, device=DEV).bfloat16()
+    ids = torch.randint(vocab // top, (rows, top), generator=gen, device=DEV) * top + torch.arange(top, device=DEV)     # different in a row
+    ids[some, :4] = torch.tensor([131327, 131328, vocab - 1, 131584], device=DEV)
+    logits = torch.randn(rows, top, generator=gen, device=DEV)
+    losses, lse, _ = ct.distillation_forward(x, table, ids, logits)
+    p = torch.softmax(logits.double(), 1)
+    ref.check(lse[40:1000], torch.full((960,), float(vocab), dtype=torch.float64).log(), torch.ones(960), 1e-5, "lse")
+    want = (p * (p.log() + torch.tensor(float(vocab), dtype=torch.float64).log().item())).sum(1)
+    z = x[some].double() @ table.double().T
+    norm = torch.logsumexp(z, 1)
+    want[some] = (p[some] * (p[some].log() - z.gather(1, ids[some]) + norm[:, None])).sum(1)
+    ref.check(lse[some], norm.cpu(), torch.ones(len(some)), 1e-4, "lse")
+    ref.check(losses, want.cpu(), torch.ones(rows), 2e-4, "losses")
+
+
 def test_two_pieces_of_16_bits(ct):  # noqa: F811
     x, table, ids, logits, grad = tensors(seeded(8), 2100, 24, 64100, 4, torch.bfloat16)
     ids[:4, 0] = torch.tensor([63487, 63488, 64099, 0])     # beside the cut, and at the ends
