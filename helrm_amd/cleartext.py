@@ -444,8 +444,11 @@ def _teach_tensors(x, table, ids, temperature, ignore_index):
     _sized(table.shape[0], "table: rows")
     _sized(table.shape[1], "table: the last dimension")
     _need(-(1 << 63) <= ignore_index < 1 << 63, "ignore_index: not an int64")
-    _need(2.0 ** -60 <= temperature <= 2.0 ** 60, f"temperature {temperature}: not positive, or out of range")
-    _need(ids.dim() >= 1 and 1 <= ids.shape[-1] <= 1024, f"ids: {list(ids.shape)}, not [..., top] with top from 1 to 1024")
+    # (messages are made where they are needed: a shape's is a microsecond of a small call)
+    if not 2.0 ** -60 <= temperature <= 2.0 ** 60:
+        raise ValueError(f"temperature {temperature}: not positive, or out of range")
+    if not (ids.dim() >= 1 and 1 <= ids.shape[-1] <= 1024):
+        raise ValueError(f"ids: {list(ids.shape)}, not [..., top] with top from 1 to 1024")
     _same_order(ids.shape[:-1], x.shape[:-1], "ids")
     x2 = _rows(x, table.shape[1], "x")
     if ids.dtype != torch.int64 or ids.device != x.device:
@@ -569,12 +572,15 @@ def _pairs(losses, target, offsets, ignore_index):
     if losses.dtype != torch.float32:
         raise ValueError(f"losses: {losses.dtype}, not {torch.float32}")
     if offsets is None:
-        _need(losses.dim() >= 2 and losses.shape[-2] == 2, f"losses: {list(losses.shape)}, not [..., 2, length]")
+        if losses.dim() < 2 or losses.shape[-2] != 2:
+            raise ValueError(f"losses: {list(losses.shape)}, not [..., 2, length]")
         lead = losses.shape[:-2]
         pairs = math.prod(lead)
     else:
-        _need(losses.dim() == 1, f"losses: {list(losses.shape)}, not [tokens] beside offsets")
-        _need(offsets.dim() == 1 and offsets.shape[0] % 2 == 1, f"offsets: {list(offsets.shape)}, not [2 * pairs + 1]")
+        if losses.dim() != 1:
+            raise ValueError(f"losses: {list(losses.shape)}, not [tokens] beside offsets")
+        if offsets.dim() != 1 or offsets.shape[0] % 2 != 1:
+            raise ValueError(f"offsets: {list(offsets.shape)}, not [2 * pairs + 1]")
         pairs = offsets.shape[0] // 2
         lead = (pairs,)
     if not losses.is_cuda:
@@ -598,9 +604,11 @@ def _pointer(t):
 
 
 def _preference_forward(losses, reference, target, offsets, beta, margin, kind, smoothing, average, ignore_index, keep=True):
-    _need(kind in _KINDS, f"kind {kind!r}: neither logistic nor hinge")
+    if kind not in _KINDS:
+        raise ValueError(f"kind {kind!r}: neither logistic nor hinge")
     _need(math.isfinite(beta) and math.isfinite(margin), "beta and margin are not finite")
-    _need(0.0 <= smoothing <= (1.0 if kind == "logistic" else 0.0), f"smoothing {smoothing}: not from 0 to 1, or not 0 with the hinge")
+    if not 0.0 <= smoothing <= (1.0 if kind == "logistic" else 0.0):
+        raise ValueError(f"smoothing {smoothing}: not from 0 to 1, or not 0 with the hinge")
     lead, pairs, length, target, ldtarget, offsets = _pairs(losses, target, offsets, ignore_index)
     packed, device = offsets is not None, losses.device
     held, ldreference = (None, 0) if reference is None else _lines(reference, losses, "reference", torch.float32, packed)
@@ -686,7 +694,7 @@ def _embedding_ids(ids, vocab, ignore_index, device):
     _need(-(1 << 63) <= ignore_index < 1 << 63, "ignore_index: not an int64")
     if ids.dtype != torch.int64 or ids.device != device:
         raise ValueError(f"ids: {ids.dtype} on {ids.device}, not {torch.int64} on {device}")
-    return ids.reshape(-1).contiguous()
+    return ids.contiguous() if ids.dim() == 1 else ids.reshape(-1).contiguous()
 
 
 def embedding_forward(ids, table, scale=1.0, ignore_index=-100):
