@@ -8,9 +8,9 @@
 //
 // Sums are of 64 bits: long sequences differ by little of their sums.  A token is
 // read once in each direction.  Bound by memory where there are many (512 pairs of
-// 2 x 8,192, 134 MB read, 24 us = 5.7 TB/s; backward 100 MB, 15 us, from the
+// 2 x 8,192, 134 MB read, 23 us = 5.8 TB/s; backward 100 MB, 16 us, from the
 // caches; four tokens a load, a token a load 34 and 16), by launches otherwise
-// (128 pairs of 1,700 tokens: 7 + 4 us, and 26 with the host's time).
+// (128 pairs of 1,700 tokens: 6 + 3 us, and 25 with the host's time).
 #include <algorithm>
 #include "plan.h"
 #include "preference.h"
@@ -22,9 +22,9 @@ constexpr int WAVE = 64, MOST = 1024;
 constexpr int MOST_SPLITS = 64;
 constexpr int EACH = 4;   // tokens a thread at once
 
-__device__ __forceinline__ Sum wave_sum(Sum s) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) {
+// Over `lanes` lanes beside one another, a power of two.
+__device__ __forceinline__ Sum wave_sum(Sum s, int lanes = WAVE) {
+  for (int o = lanes / 2; o; o >>= 1) {
     s.sum += __shfl_xor(s.sum, o);
     s.count += __shfl_xor(s.count, o);
   }
@@ -109,13 +109,13 @@ __device__ __forceinline__ void finish(const PairArgs& a, long pair, Sum first, 
   a.slope[2 * pair + 1] = (float)(slope * a.beta * each[1]);
 }
 
-// A wave a pair.
-__global__ __launch_bounds__(256) void pair_wave_kernel(const PairArgs a, long base) {
-  const long pair = (base + blockIdx.x) * (256 / WAVE) + threadIdx.x / WAVE;
+// `lanes` lanes of a wave a pair.
+__global__ __launch_bounds__(256) void pair_lanes_kernel(const PairArgs a, int lanes, long base) {
+  const long pair = (base + blockIdx.x) * (256 / lanes) + threadIdx.x / lanes;
   if (pair >= a.pairs) return;
-  const int lane = threadIdx.x % WAVE;
+  const int lane = threadIdx.x % lanes;
   Sum s[2];
-  for (int k = 0; k < 2; k++) s[k] = wave_sum(sum_of(a, 2 * pair + k, 0, lane, WAVE));
+  for (int k = 0; k < 2; k++) s[k] = wave_sum(sum_of(a, 2 * pair + k, 0, lane, lanes), lanes);
   if (lane == 0) finish(a, pair, s[0], s[1]);
 }
 
@@ -182,7 +182,14 @@ __global__ __launch_bounds__(256) void pair_grad_kernel(const PairArgs a, int th
 }
 
 long mean_length(long pairs, long length, bool packed) { return packed ? clr::ceil_div(length, std::max(2 * pairs, 1L)) : length; }
-// Shares of a pair: where pairs are few and long, as many as give 256 workgroups, of 8,192 tokens at the least.
+// Threads of a sequence, which take four tokens each at once; in a line, where
+// one may be much longer than the mean, more for the shortest.  50,000 pairs of
+// 2 x 16 tokens, forward and backward: 7 + 5 us with 4 lanes, 18 + 10 with 16, 51 + 28
+// with 64.  Of long sequences, forward: 512 pairs of 2 x 8,192 tokens 22.8 us
+// with 256 threads, 23.3 with 1,024; 300 of 3,000 9.5 and 11.3; 8 of 100,000 15.1 and 11.6.
+int lanes_of(long mean, bool packed) { return mean <= 16 && !packed ? 4 : mean <= 64 ? 16 : mean <= 256 ? WAVE : 256; }
+// Shares of a pair: where pairs are few and long, as many as give 256 workgroups,
+// of 8,192 tokens at the least (8 pairs of 2 x 100,000 tokens 12 us, 32 with one share; backward 5 and 25).
 int splits_of(long pairs, long length, bool packed) {
   const long most = 2 * mean_length(pairs, length, packed) / 8192;
   return (int)std::max(1L, std::min({clr::ceil_div(256, pairs), most, (long)MOST_SPLITS}));
@@ -197,17 +204,18 @@ size_t preference_workspace(long pairs, long length, bool packed) {
 void preference_launch(PairArgs a, hipStream_t st) {
   const long mean = mean_length(a.pairs, a.length, a.offsets);
   a.splits = splits_of(a.pairs, a.length, a.offsets);
-  if (mean <= 64 && a.pairs >= 256) {
-    clr::in_launches(clr::ceil_div(a.pairs, 256 / WAVE), 256, [&](long base, unsigned n) { pair_wave_kernel<<<n, 256, 0, st>>>(a, base); });
+  const int lanes = lanes_of(mean, a.offsets);
+  if (lanes <= WAVE && a.pairs >= 256) {
+    clr::in_launches(clr::ceil_div(a.pairs, 256 / lanes), 256, [&](long base, unsigned n) { pair_lanes_kernel<<<n, 256, 0, st>>>(a, lanes, base); });
     return;
   }
-  const int threads = mean <= 1024 ? 256 : MOST;
+  const int threads = a.pairs >= 256 || mean <= 2048 ? 256 : MOST;
   clr::in_launches(a.pairs * a.splits, threads, [&](long base, unsigned n) { pair_kernel<<<n, threads, 0, st>>>(a, base); });
   if (a.splits > 1) pair_join_kernel<<<clr::groups_of(clr::ceil_div(a.pairs, 256 / WAVE), 256), 256, 0, st>>>(a);
 }
 void preference_grad_launch(PairArgs a, hipStream_t st) {
   const long mean = mean_length(a.pairs, a.length, a.offsets);
-  const int threads = mean <= 64 ? WAVE : 256;
+  const int threads = lanes_of(mean, a.offsets);
   a.splits = (int)std::max(1L, std::min(mean / 2048, 1L << 20));
   const long teams = (2 * a.pairs + (a.offsets ? 1 : 0)) * a.splits;
   clr::in_launches(clr::ceil_div(teams, 256 / threads), 256, [&](long base, unsigned n) { pair_grad_kernel<<<n, 256, 0, st>>>(a, threads, base); });

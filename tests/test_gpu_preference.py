@@ -92,7 +92,7 @@ FORMS = [dict(), dict(kind="hinge"), dict(smoothing=0.1, margin=0.5), dict(avera
          dict(smoothing=1.0), dict(beta=0.0), dict(beta=-0.3)]
 
 
-@pytest.mark.parametrize("pairs,length", [(0, 5), (1, 0), (3, 1), (1, 200), (7, 65), (5, 1025), (300, 3), (257, 64), (300, 65), (2, 4097), (1, 40001),
+@pytest.mark.parametrize("pairs,length", [(0, 5), (1, 0), (3, 1), (1, 200), (7, 65), (5, 1025), (300, 3), (257, 16), (257, 17), (257, 64), (300, 65), (256, 256), (256, 257), (2, 4097), (1, 40001),
                                           (3, 16385), (40, 9000)])
 def test_preference(ct, pairs, length):  # noqa: F811
     gen = seeded(pairs + length)
@@ -101,7 +101,7 @@ def test_preference(ct, pairs, length):  # noqa: F811
         pref_check(ct, losses, reference if k % 3 else None, target if k % 2 else None, **form)
 
 
-@pytest.mark.parametrize("pairs,mean", [(0, 4), (1, 300), (5, 1), (7, 90), (300, 5), (300, 40), (100, 1200), (2, 30000), (33, 3000)])
+@pytest.mark.parametrize("pairs,mean", [(0, 4), (1, 300), (5, 1), (7, 90), (300, 5), (300, 40), (300, 200), (100, 1200), (2, 30000), (33, 3000)])
 def test_sequences_in_a_line(ct, pairs, mean):  # noqa: F811
     gen = seeded(pairs + mean)
     lengths = (torch.rand(2 * pairs, generator=gen) ** 3 * 4 * mean).long()       # many short, a few long; some without tokens
