@@ -90,8 +90,10 @@ __global__ __launch_bounds__(BLOCK) void embed_kernel(const EmbedArgs a, int pac
 // Keys are ids, `vocab` of an id that has no row (sorted last); values are the ids' places.
 
 constexpr int SORT = 1024, WAVES = SORT / 64, MOST_BITS = 9, MOST_DIGITS = 1 << MOST_BITS;
-constexpr long ONE = SORT * 8;   // the most ids that one workgroup sorts alone
-// Ids a thread of a workgroup's share otherwise: as few as leave 32 tiles, whose counts every workgroup adds up.
+// The most ids that one workgroup sorts alone (16,384 of them: 38 us, and 33 in four launches of many workgroups).
+constexpr long ONE = SORT * 8;
+// Ids a thread of a workgroup's share otherwise: as few as leave 32 tiles, whose
+// counts every workgroup adds up (16,384 ids, a scatter: 9 us with one, 14 with four).
 int items_of(long tokens) { return tokens <= 32 * SORT ? 1 : tokens <= 64 * SORT ? 2 : 4; }
 
 struct SortArgs {
@@ -369,7 +371,7 @@ struct SumArgs {
 // WAVE: a team is a wave.
 template <class T, int V, bool WAVE>
 __global__ __launch_bounds__(BLOCK) void run_sum_kernel(const SumArgs a, long base) {
-  constexpr int AHEAD = 8;
+  constexpr int AHEAD = 8;   // rows on their way (131,072 x 2,048: 260 us; 269 with 4, 399 with 16, for which there are too few registers)
   const int lane = WAVE ? threadIdx.x & 63 : threadIdx.x & (a.lanes - 1);
   unsigned team = (unsigned)(((base + blockIdx.x) * BLOCK + threadIdx.x) / (WAVE ? 64 : a.lanes));
   if (WAVE) team = __builtin_amdgcn_readfirstlane(team);
@@ -608,7 +610,10 @@ struct Space {
   float* partial;
   size_t bytes = 0;
 };
-// Ids of a piece: as many as leave 2,048 waves, of 16 to 64.
+// Ids of a piece: as many as leave 2,048 waves, of 16 to 64.  A longer piece has
+// fewer sums that are joined, a shorter one keeps more waves at work: 16,384 x
+// 1,024, both directions, 66 us with 2,048 or 1,024 waves, 75 with 512; 131,072 x
+// 2,048 423 us with pieces of 64, 426 of 128, 454 of 256.
 int piece_of(long tokens, int blocks, int lanes) {
   const long waves = tokens * blocks * lanes / 64;
   return waves >= 64 * 2048 ? 64 : waves >= 32 * 2048 ? 32 : 16;
@@ -725,7 +730,7 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
   m.n = (int)a.tokens; m.vocab = a.vocab; m.width = a.width; m.packs = packs;
   m.lanes = lanes_of(packs, 64);
   m.across = lanes_of(packs, JOIN);
-  const int threads = std::min(std::max(4 * m.across, 256), JOIN);
+  const int threads = std::min(std::max(4 * m.across, 256), JOIN);   // (1,024 for rows of 4 packs: 17 us, 5 with 256)
   m.blocks = (int)clr::ceil_div(packs, m.lanes);
   m.piece = piece_of(a.tokens, m.blocks, m.lanes);
   m.pieces = (int)clr::ceil_div(a.tokens, m.piece);
