@@ -11,13 +11,13 @@
 // rounded once.  Rows that no id names are cleared by workgroups beside the
 // sort's, which so costs nothing where the table is large.
 //
-// Bound by memory where rows are long (a copy here: 4.95 TB/s), by launches
-// where they are few.  131,072 ids x 2,048 against 131,072 rows bfloat16: rows
-// 120-186 us (537 MB written, the common ids' rows come from the caches),
-// gradient 245: 94 for 537 MB cleared beside the sort, 132 for the sums (537
-// MB read, 155 written), 20 for the runs over several pieces.  16,384 x 1,024
-// against 65,536 rows: rows 8-10 us, gradient 33 + 13 + 9.  53,248 x 16 float32: 3
-// us, and 24 + 6 + 5 of short launches.
+// Bound by memory where rows are long (a copy here: 5.0 TB/s), by launches where
+// they are few.  131,072 ids x 2,048 against 131,072 rows bfloat16: rows 120-186
+// us (537 MB written, the common ids' rows come from the caches), gradient
+// 245: 94 for 537 MB cleared beside the sort, 132 for the sums (537 MB read, 155
+// written), 20 for the runs over several pieces.  16,384 x 1,024 against 65,536
+// rows: rows 8-10 us, gradient SORTFIG.  53,248 x 16 float32: 3 us, and 24 + 6 + 5
+// of short launches.
 #include <algorithm>
 #include "embedding.h"
 #include "places.h"
@@ -90,11 +90,15 @@ __global__ __launch_bounds__(BLOCK) void embed_kernel(const EmbedArgs a, int pac
 // Keys are ids, `vocab` of an id that has no row (sorted last); values are the ids' places.
 
 constexpr int SORT = 1024, WAVES = SORT / 64, MOST_BITS = 9, MOST_DIGITS = 1 << MOST_BITS;
-// The most ids that one workgroup sorts alone (16,384 of them: 38 us, and 33 in four launches of many workgroups).
-constexpr long ONE = SORT * 8;
-// Ids a thread of a workgroup's share otherwise: as few as leave 32 tiles, whose
+// The most ids that one workgroup sorts alone, and the most whose tiles of SORT
+// are sorted each by itself and merged.  Gradient against 65,536 rows, alone and
+// merged: 5,120 x 64 25.1 and 23.5 us, 5,120 x 1,024 31.3 and 32.3, 6,144 x 64
+// 27.2 and 23.5; merged and by tiles' counts: 16,384 x 1,024 43.5 and 49.8,
+// 32,768 x 1,024 56.9 and 59.1 (more ids do not fit into LDS).
+constexpr long ONE = SORT * 5, MERGED = SORT * 32;
+// Ids a thread of a workgroup's share of more: as few as leave 32 tiles, whose
 // counts every workgroup adds up (16,384 ids, a scatter: 9 us with one, 14 with four).
-int items_of(long tokens) { return tokens <= 32 * SORT ? 1 : tokens <= 64 * SORT ? 2 : 4; }
+int items_of(long tokens) { return tokens <= 64 * SORT ? 2 : 4; }
 
 struct SortArgs {
   const long long* ids;                     // of the first pass
@@ -215,24 +219,25 @@ __device__ __forceinline__ void clear_share(const Clear& c, int group) {
   else clear_places<2>(c, group);
 }
 
-// The whole sort of up to SORT * ITEMS ids.
+// The whole sort of up to SORT * ITEMS ids, or of each of several tiles of so many by itself.
 template <int ITEMS>
-__global__ __launch_bounds__(SORT) void sort_one_kernel(const SortArgs a, const Clear c) {
+__global__ __launch_bounds__(SORT) void sort_tile_kernel(const SortArgs a, const Clear c) {
   __shared__ int counts[WAVES][MOST_DIGITS], sums[WAVES];
   __shared__ unsigned keys[SORT * ITEMS], ats[SORT * ITEMS];
-  if (blockIdx.x) return clear_share(c, blockIdx.x - 1);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = (a.n + SORT - 1) / SORT;   // (as many for every wave)
+  if ((int)blockIdx.x >= a.tiles) return clear_share(c, blockIdx.x - a.tiles);
+  const int first = blockIdx.x * SORT * ITEMS, n = min(SORT * ITEMS, a.n - first);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = (n + SORT - 1) / SORT;   // (as many for every wave)
   unsigned key[ITEMS], at[ITEMS];
   int rank[ITEMS];
 #pragma unroll
   for (int j = 0; j < ITEMS; j++) {
     const int i = (wave * per + j) * 64 + lane;
-    key[j] = j < per && i < a.n ? key_of(a, i) : 0;
-    at[j] = i;
+    key[j] = j < per && i < n ? key_of(a, first + i) : 0;
+    at[j] = first + i;
   }
   for (int pass = 0; pass < a.passes; pass++) {
     const int shift = pass * a.bits;
-    rank_items<ITEMS>(key, per, a.n, shift, a.bits, rank, counts);
+    rank_items<ITEMS>(key, per, n, shift, a.bits, rank, counts);
     __syncthreads();
     Column column;
     const int all = column.read(1 << a.bits, counts);
@@ -241,22 +246,66 @@ __global__ __launch_bounds__(SORT) void sort_one_kernel(const SortArgs a, const 
     const bool last = pass == a.passes - 1;
 #pragma unroll
     for (int j = 0; j < ITEMS; j++)
-      if (j < per && (wave * per + j) * 64 + lane < a.n) {
+      if (j < per && (wave * per + j) * 64 + lane < n) {
         const unsigned digit = key[j] >> shift & ((1u << a.bits) - 1);
         const int to = counts[wave][digit] + rank[j];
-        (last ? a.to : keys)[to] = key[j];
-        (last ? a.to_at : ats)[to] = at[j];
+        (last ? a.to + first : keys)[to] = key[j];
+        (last ? a.to_at + first : ats)[to] = at[j];
       }
     if (last) break;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < ITEMS; j++) {
       const int i = (wave * per + j) * 64 + lane;
-      key[j] = j < per && i < a.n ? keys[i] : 0;
-      at[j] = j < per && i < a.n ? ats[i] : 0;
+      key[j] = j < per && i < n ? keys[i] : 0;
+      at[j] = j < per && i < n ? ats[i] : 0;
     }
     // (the next pass writes them after three barriers)
   }
+}
+
+// Up to TILES sorted tiles of SORT ids into one: an id goes behind the smaller
+// ones of every tile, found by bisection in LDS, and the equal ones of the tiles
+// before.  Four threads an id, which share the tiles out.
+template <int TILES>
+__global__ __launch_bounds__(SORT) void sort_merge_kernel(const SortArgs a, const Clear c) {
+  __shared__ __align__(16) unsigned keys[TILES * SORT];
+  constexpr int EACH = SORT / 4, MINE = TILES / 4;
+  const int groups = (a.n + EACH - 1) / EACH;
+  if ((int)blockIdx.x >= groups) return clear_share(c, blockIdx.x - groups);
+#pragma unroll
+  for (int u = 0; u < MINE; u++) {
+    const int i = (u * SORT + threadIdx.x) * 4;
+    uint4 v = make_uint4(~0u, ~0u, ~0u, ~0u);   // behind every key
+    if (i + 4 <= a.n) v = *(const uint4*)(a.from + i);
+    else {
+      if (i < a.n) v.x = a.from[i];
+      if (i + 1 < a.n) v.y = a.from[i + 1];
+      if (i + 2 < a.n) v.z = a.from[i + 2];
+    }
+    *(uint4*)(keys + i) = v;
+  }
+  __syncthreads();
+  const int e = blockIdx.x * EACH + threadIdx.x / 4, part = threadIdx.x & 3, own = e / SORT;
+  const unsigned key = keys[e];
+  int at[MINE] = {}, to = 0;
+#pragma unroll
+  for (int step = SORT / 2; step; step /= 2)
+#pragma unroll
+    for (int u = 0; u < MINE; u++) {
+      const int tile = u * 4 + part;
+      at[u] += keys[tile * SORT + at[u] + step - 1] < key + (tile < own) ? step : 0;
+    }
+#pragma unroll
+  for (int u = 0; u < MINE; u++) {
+    const int tile = u * 4 + part;
+    to += tile == own ? e % SORT : at[u] + (keys[tile * SORT + at[u]] < key + (tile < own));
+  }
+  to += __shfl_xor(to, 1);
+  to += __shfl_xor(to, 2);
+  if (part || e >= a.n) return;
+  a.to[to] = key;
+  a.to_at[to] = a.from_at[e];
 }
 
 // One pass over many tiles: how often each digit is in a tile, ...
@@ -682,10 +731,10 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
   while (a.vocab >> bits) bits++;
   s.passes = (int)clr::ceil_div(bits, MOST_BITS);
   s.bits = (int)clr::ceil_div(bits, s.passes);
-  const bool one = a.tokens <= ONE;
+  const bool one = a.tokens <= ONE, merged = !one && a.tokens <= MERGED;
   const int items = items_of(a.tokens);
-  if (!one) s.tiles = (int)clr::ceil_div(a.tokens, SORT * items);
-  // the table's places, shared out by how long the launches take: a scatter twice as long as a count
+  s.tiles = one ? 1 : (int)clr::ceil_div(a.tokens, merged ? SORT : SORT * items);
+  // the table's places, shared out by how long the launches take: a scatter twice as long as a count, 6 to 4 of tiles and their merging
   Clear c{};
   c.table = (char*)a.dtable;
   c.row = (long)a.width * dtype_size(a.dtype);
@@ -702,8 +751,21 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
   if (one) {
     s.to = space.keys[0];
     s.to_at = space.ats[0];
-    const unsigned groups = 1 + clearing(0, 1, 1);
-    with_items((int)clr::ceil_div(a.tokens, SORT), [&](auto n) { sort_one_kernel<decltype(n)::value><<<groups, SORT, 0, st>>>(s, c); });
+    const unsigned groups = s.tiles + clearing(0, 1, 1);
+    with_items((int)clr::ceil_div(a.tokens, SORT), [&](auto n) { sort_tile_kernel<decltype(n)::value><<<groups, SORT, 0, st>>>(s, c); });
+  } else if (merged) {
+    s.to = space.keys[0];
+    s.to_at = space.ats[0];
+    unsigned groups = s.tiles + clearing(0, 6, 10);
+    sort_tile_kernel<1><<<groups, SORT, 0, st>>>(s, c);
+    out = 1;
+    s.from = s.to;
+    s.from_at = s.to_at;
+    s.to = space.keys[1];
+    s.to_at = space.ats[1];
+    groups = (unsigned)clr::ceil_div(a.tokens, SORT / 4) + clearing(6, 4, 10);
+    if (s.tiles <= 16) sort_merge_kernel<16><<<groups, SORT, 0, st>>>(s, c);
+    else sort_merge_kernel<32><<<groups, SORT, 0, st>>>(s, c);
   } else {
     s.counts = space.counts;
     for (int pass = 0; pass < s.passes; pass++) {
@@ -714,10 +776,12 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
       s.to = space.keys[out];
       s.to_at = space.ats[out];
       unsigned groups = s.tiles + clearing(3 * pass, 1, 3 * s.passes);
-      with_items(items, [&](auto n) { sort_count_kernel<decltype(n)::value><<<groups, SORT, 0, st>>>(s, c); });
+      if (items == 2) sort_count_kernel<2><<<groups, SORT, 0, st>>>(s, c);
+      else sort_count_kernel<4><<<groups, SORT, 0, st>>>(s, c);
       if (s.tiles > FEW_TILES) sort_scan_kernel<<<(unsigned)clr::ceil_div(1 << s.bits, 64), SORT, 0, st>>>(s);
       groups = s.tiles + clearing(3 * pass + 1, 2, 3 * s.passes);
-      with_items(items, [&](auto n) { sort_scatter_kernel<decltype(n)::value><<<groups, SORT, 0, st>>>(s, c); });
+      if (items == 2) sort_scatter_kernel<2><<<groups, SORT, 0, st>>>(s, c);
+      else sort_scatter_kernel<4><<<groups, SORT, 0, st>>>(s, c);
     }
   }
   const int packs = packs_of(a.width, a.dtype);
