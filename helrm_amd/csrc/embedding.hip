@@ -16,8 +16,9 @@
 // us (537 MB written, the common ids' rows come from the caches), gradient
 // 245: 94 for 537 MB cleared beside the sort, 132 for the sums (537 MB read, 155
 // written), 20 for the runs over several pieces.  16,384 x 1,024 against 65,536
-// rows: rows 8-10 us, gradient SORTFIG.  53,248 x 16 float32: 3 us, and 24 + 6 + 5
-// of short launches.
+// rows: rows 8-10 us, gradient 44: 13 + 10 for the sort with 134 MB cleared beside
+// it, 12 and 9 for the sums.  53,248 x 16 float32: 3 us, and 24 + 6 + 5 of short
+// launches.
 #include <algorithm>
 #include "embedding.h"
 #include "places.h"
@@ -685,7 +686,7 @@ Space space_of(char* base, long tokens, int width, int vocab, int dtype) {
     s.keys[i] = i && one ? s.keys[0] : (unsigned*)take(tokens * 4);
     s.ats[i] = i && one ? s.ats[0] : (unsigned*)take(tokens * 4);
   }
-  s.counts = one ? nullptr : (int*)take((clr::ceil_div(tokens, SORT * items_of(tokens)) + 1) * MOST_DIGITS * 4);
+  s.counts = tokens <= MERGED ? nullptr : (int*)take((clr::ceil_div(tokens, SORT * items_of(tokens)) + 1) * MOST_DIGITS * 4);
   s.partial = (float*)take(clr::ceil_div(tokens, piece_of(tokens, blocks, lanes)) * 2 * width * sizeof(float));
   return s;
 }

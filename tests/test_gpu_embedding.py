@@ -58,7 +58,8 @@ def embed_check(ct, ids, table, grad, scale, ignore=IGNORE):  # noqa: F811
                                                 (200, 416, 1000), (1000, 1001, 50), (1024, 3, 511), (1025, 64, 512), (700, 2048, 9000), (37, 4097, 20),
                                                 (5000, 24, 4000), (5120, 24, 400), (5121, 24, 400), (8191, 5, 3), (8192, 16, 70000), (8193, 16, 300), (12289, 40, 260000), (16384, 24, 9000), (16385, 24, 9000),
                                                 (20000, 4, 1), (30011, 130, 5000), (32768, 12, 70000), (32769, 12, 70000),
-                                                (70001, 8, 600)])
+                                                (70001, 8, 600), (33000, 8, 65534),
+                                                (33000, 8, 65535), (65536, 5, 300), (65535, 8, 65534), (65537, 5, 300)])
 def test_embedding(ct, dtype, tokens, width, vocab):  # noqa: F811
     gen = seeded(tokens + 7 * width + vocab)
     table, grad = normal(gen, vocab, width, dtype=dtype), normal(gen, tokens, width, dtype=dtype)
