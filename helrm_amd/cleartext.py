@@ -631,13 +631,14 @@ def preference_forward(losses, reference=None, target=None, offsets=None, beta=0
     value by each of those losses.  losses [..., 2, length] are the tokens' (float32, as cross_entropy gives them); or [tokens],
     sequence s the tokens from offsets[s] to offsets[s + 1].  Tokens whose target is `ignore_index` count in nothing.
     With m = beta * (ratio of the first - of the second) - margin: "logistic" (1 - smoothing) log(1 + exp -m) + smoothing log(1 +
-    exp m), "hinge" max(0, 1 - m).  A pair without tokens that count has 0; offsets that descend or leave the tokens give NaN."""
+    exp m), "hinge" max(0, 1 - m).  A pair without tokens that count has 0, one whose offsets descend or leave the tokens NaN."""
     return _preference_forward(losses, reference, target, offsets, beta, margin, kind, smoothing, average, ignore_index, False)[:3]
 
 
 def preference_backward(grad, losses, slopes, target=None, offsets=None, ignore_index=-100):
     """The gradient of every token's loss, of losses' shape, for the gradient `grad` of the values; slopes as the forward call gave
-    them.  Tokens that count in nothing have 0."""
+    them.  Tokens that count in nothing have 0.  Of offsets that descend somewhere, a token has the gradient of one of the sequences
+    that hold it, NaN or 0, the same on every run."""
     lead, pairs, length, target, ldtarget, offsets = _pairs(losses, target, offsets, ignore_index)
     device = losses.device
     if grad.shape != lead:

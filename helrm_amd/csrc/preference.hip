@@ -149,23 +149,14 @@ __global__ __launch_bounds__(256) void pair_join_kernel(const PairArgs a) {
   if (lane == 0) finish(a, pair, s[0], s[1]);
 }
 
-// `threads` threads a share of a sequence; one sequence more are the tokens of a line before the first and behind the last.
+// The gradient in rows, `threads` threads a share of a sequence.
 __global__ __launch_bounds__(256) void pair_grad_kernel(const PairArgs a, int threads, long base) {
   const long team = (base + blockIdx.x) * (256 / threads) + threadIdx.x / threads, sequence = team / a.splits;
   const int split = (int)(team - sequence * a.splits), thread = threadIdx.x % threads;
-  const long all = 2 * a.pairs;
-  if (sequence >= all) {
-    if (!a.offsets || sequence > all) return;
-    const long first = min(max((long)a.offsets[0], 0L), a.length), last = min(max((long)a.offsets[all], 0L), a.length);
-    const Tokens t[2] = {share_of({0, first}, split, a.splits), share_of({last, a.length}, split, a.splits)};
-    for (int k = 0; k < 2; k++)
-      for (long i = t[k].from + thread; i < t[k].to; i += threads) a.dloss[i] = 0.0f;
-    return;
-  }
-  const Tokens t = share_of(tokens_of(a, sequence), split, a.splits);
-  const long row = a.offsets ? 0 : sequence;
-  const long long* target = a.target ? a.target + row * a.ldtarget : nullptr;
-  float* d = a.dloss + row * a.lddloss;
+  if (sequence >= 2 * a.pairs) return;
+  const Tokens t = share_of({0, a.length}, split, a.splits);
+  const long long* target = a.target ? a.target + sequence * a.ldtarget : nullptr;
+  float* d = a.dloss + sequence * a.lddloss;
   const float v = a.dvalue[sequence / 2] * a.slope[sequence];
   const long whole = t.from + (t.to - t.from) / EACH * EACH;
 #pragma unroll 2
@@ -179,6 +170,102 @@ __global__ __launch_bounds__(256) void pair_grad_kernel(const PairArgs a, int th
   }
   const long i = whole + thread;
   if (i < t.to) d[i] = !target || target[i] != a.ignore ? v : 0.0f;
+}
+
+// The gradient in a line.  A workgroup has tokens beside one another, EACH of a
+// thread, marks where sequences begin among them and takes the running maximum of
+// the marks, so that a token is written once whatever the offsets say (a sequence
+// that wrote its own tokens would meet others' where offsets descend), and a long
+// sequence is as parallel as short ones.  Bound by the four loads that wait for
+// one another: 128 pairs of 2 x 1,500 tokens on average 4.1 us (3.5 a sequence by
+// itself), 300 of 2 x 40 with one of 10,000 among them 3.4 (32).
+constexpr int MARKED = 1024;
+template <int EACH> __global__ __launch_bounds__(256) void line_grad_kernel(const PairArgs a, long base) {
+  constexpr int LINE = 256 * EACH;
+  __shared__ __align__(16) unsigned marks[LINE];
+  __shared__ unsigned tops[256 / WAVE];
+  const long all = 2 * a.pairs, first = (base + blockIdx.x) * LINE, last = min(first + LINE, a.length) - 1;
+  const int at = threadIdx.x * EACH;
+  const long i = first + at;
+  const bool whole = i + EACH <= a.length;
+  long long k[EACH] = {};
+  if (a.target) {
+    if (whole) __builtin_memcpy(k, a.target + i, sizeof(k));
+    else
+      for (int e = 0; e < EACH; e++) if (i + e < a.length) k[e] = a.target[i + e];
+  }
+#pragma unroll
+  for (int e = 0; e < EACH; e += 4) *(uint4*)(marks + at + e) = make_uint4(0, 0, 0, 0);
+  // How many offsets are at most the first token's place, and the last one's: from ..
+  // to of them, narrowed with as many probes at a time as there are threads until
+  // few are between.  (Of offsets that descend, some number.)
+  long from[2] = {0, 0}, to[2] = {all + 1, all + 1};
+  while (to[1] - from[0] > MARKED && (from[0] < to[0] || from[1] < to[1])) {   // (the same of all threads)
+    bool below[2];
+    long step[2];
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+      step[w] = (to[w] - from[w] + 255) / 256;
+      const long probe = from[w] + (threadIdx.x + 1) * step[w] - 1;
+      below[w] = from[w] < to[w] && probe < to[w] && a.offsets[probe] <= (w ? last : first);
+    }
+#pragma unroll
+    for (int w = 0; w < 2; w++) {
+      const int count = __syncthreads_count(below[w]);
+      if (from[w] == to[w]) continue;
+      from[w] = min(from[w] + count * step[w], to[w]);
+      to[w] = min(from[w] + step[w] - 1, to[w]);
+    }
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (long j = from[0] + threadIdx.x; j < to[1]; j += 256) {
+    const long o = a.offsets[j];
+    if (o <= last) atomicMax(&marks[o <= first ? 0 : o - first], (unsigned)(j - from[0]) + 1);   // (any number may be an offset)
+  }
+  __syncthreads();
+  unsigned m[EACH];
+  __builtin_memcpy(m, __builtin_assume_aligned(marks + at, 16), sizeof(m));
+#pragma unroll
+  for (int e = 1; e < EACH; e++) m[e] = max(m[e], m[e - 1]);
+  const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+  unsigned top = m[EACH - 1];
+#pragma unroll
+  for (int o = 1; o < WAVE; o *= 2) {
+    const unsigned t = __shfl_up(top, o);
+    if (lane >= o) top = max(top, t);
+  }
+  if (lane == WAVE - 1) tops[wave] = top;
+  __syncthreads();
+  top = __shfl_up(top, 1);
+  if (lane == 0) top = 0;
+  for (int w = 0; w < wave; w++) top = max(top, tops[w]);
+#pragma unroll
+  for (int e = 0; e < EACH; e++) m[e] = max(m[e], top);
+  // of token t, behind m offsets
+  auto value = [&](long t, unsigned m) {
+    const long s = from[0] + m;   // in sequence s - 1
+    const long begin = s > 0 ? a.offsets[s - 1] : 0, end = s <= all ? a.offsets[s] : a.length;
+    const float v = s > 0 && s <= all ? a.dvalue[(s - 1) / 2] * a.slope[s - 1] : 0.0f;
+    return t < begin || t >= end ? NAN : v;   // (not in it: offsets that descend)
+  };
+  if (i > last) return;
+  float o[EACH];
+  if (m[0] == m[EACH - 1] && whole) {
+    const long s = from[0] + m[0];
+    const long end = s <= all ? a.offsets[s] : a.length;
+    const float v = value(i, m[0]);
+#pragma unroll
+    for (int e = 0; e < EACH; e++) o[e] = i + e < end ? v : NAN;
+  } else {
+#pragma unroll
+    for (int e = 0; e < EACH; e++) o[e] = value(i + e, m[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < EACH; e++) if (a.target && k[e] == a.ignore) o[e] = 0.0f;
+  if (whole) __builtin_memcpy(a.dloss + i, o, sizeof(o));
+  else
+    for (int e = 0; e < EACH; e++) if (i + e < a.length) a.dloss[i + e] = o[e];
 }
 
 long mean_length(long pairs, long length, bool packed) { return packed ? clr::ceil_div(length, std::max(2 * pairs, 1L)) : length; }
@@ -214,9 +301,17 @@ void preference_launch(PairArgs a, hipStream_t st) {
   if (a.splits > 1) pair_join_kernel<<<clr::groups_of(clr::ceil_div(a.pairs, 256 / WAVE), 256), 256, 0, st>>>(a);
 }
 void preference_grad_launch(PairArgs a, hipStream_t st) {
-  const long mean = mean_length(a.pairs, a.length, a.offsets);
-  const int threads = lanes_of(mean, a.offsets);
-  a.splits = (int)std::max(1L, std::min(mean / 2048, 1L << 20));
-  const long teams = (2 * a.pairs + (a.offsets ? 1 : 0)) * a.splits;
-  clr::in_launches(clr::ceil_div(teams, 256 / threads), 256, [&](long base, unsigned n) { pair_grad_kernel<<<n, 256, 0, st>>>(a, threads, base); });
+  if (a.offsets) {
+    // (512 pairs of 2 x 8,192 tokens on average 23.1 us with 4 a thread, 21.4 with 8; 128 of 2 x 1,500 4.1 and 4.8)
+    auto go = [&](auto each) {
+      constexpr int N = decltype(each)::value;
+      clr::in_launches(clr::ceil_div(a.length, 256 * N), 256, [&](long base, unsigned n) { line_grad_kernel<N><<<n, 256, 0, st>>>(a, base); });
+    };
+    if (a.length < 1L << 20) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 8>{});
+    return;
+  }
+  const int threads = lanes_of(a.length, false);
+  a.splits = (int)std::max(1L, std::min(a.length / 2048, 1L << 20));
+  clr::in_launches(clr::ceil_div(2 * a.pairs * a.splits, 256 / threads), 256, [&](long base, unsigned n) { pair_grad_kernel<<<n, 256, 0, st>>>(a, threads, base); });
 }

@@ -430,7 +430,9 @@ int EmbeddingGrad(const EmbeddingArgs* args, void* stream);
  * max(0, 1 - m).  Tokens whose target is `ignore` count in nothing, whatever their
  * losses are; a pair without tokens that count has value 0 and is not kept.
  * Sequence s is row s of the matrices, or with `offsets` the tokens offsets[s] ..
- * offsets[s + 1] of one line; offsets that descend or leave the line give NaN.
+ * offsets[s + 1] of one line.  A pair whose offsets descend or leave the line has
+ * NaN; where they descend anywhere, a token's gradient is that of one of the
+ * sequences that hold it, NaN or 0, the same on every run.
  * Sums are of 64 bits.  PreferenceGrad writes the gradient of every token's loss,
  * 0 of those that count in nothing. */
 typedef struct {

@@ -321,3 +321,44 @@ def test_refusals(ct):  # noqa: F811
                           (lambda: ct.preference_backward(values, losses, slopes.double(), target), "slopes")):
         with pytest.raises(ValueError, match=message):
             call()
+
+
+def test_offsets_that_descend_write_each_token_once(ct):  # noqa: F811
+    # [0, 10, 20, 5, 8, 9, 12]: the first and the third pair are ascending by themselves and share tokens
+    gen = seeded(11)
+    cases = [([0, 10, 20, 5, 8, 9, 12], 24), ([0, -(1 << 63), (1 << 63) - 1, 9, 3, 1 << 32, 40], 33)]
+    for pairs, length in ((3, 40), (200, 3000), (3000, 50000)):
+        o = torch.randint(0, length + 1, (2 * pairs + 1,), generator=gen)
+        cases += [(o.tolist(), length), (o.sort().values.roll(pairs).tolist(), length)]
+    for o, length in cases:
+        losses, offsets = torch.rand(length, generator=gen).to(DEV), torch.tensor(o, device=DEV)
+        values, ratios, slopes = ct.preference_forward(losses, offsets=offsets)
+        o = torch.tensor(o)
+        descends = o[1:] < o[:-1]
+        assert torch.equal(values.isnan().cpu(), descends.view(-1, 2).any(1)) and values.isnan().any()
+        grad = torch.ones_like(values)
+        slopes = torch.arange(1.0, 2 * len(values) + 1, device=DEV).view(-1, 2)   # finite ones: which sequence's it is can be read off
+        d = ct.preference_backward(grad, losses, slopes, offsets=offsets)
+        for _ in range(20):
+            assert torch.equal(ct.preference_backward(grad, losses, slopes, offsets=offsets).nan_to_num(-1.0), d.nan_to_num(-1.0))
+        d, t = d.cpu(), torch.arange(length)
+        s = (d.nan_to_num(1.0).long() - 1).clamp(min=0)
+        holds = (d > 0) & (o[s] <= t) & (t < o[s + 1])
+        assert (holds | d.isnan() | ((d == 0) & ((t < o[0]) | (t >= o[-1])))).all()
+
+
+@pytest.mark.parametrize("pairs,long", [(1, 30000), (40, 70000), (300, 10000), (70000, 4001)])
+def test_a_long_sequence_among_short_ones(ct, pairs, long):  # noqa: F811
+    gen = seeded(pairs)
+    lengths = torch.randint(0, 9, (2 * pairs,), generator=gen)
+    lengths[torch.randint(2 * pairs, (pairs // 3,), generator=gen)] = 0
+    lengths[pairs] = long                                       # many sequences without tokens stand beside one another too
+    lengths[pairs + 1:pairs + 1 + pairs // 2] = 0
+    lead, tail = 2500, 1031
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), lengths.cumsum(0)]) + lead
+    n = int(offsets[-1]) + tail
+    losses, reference, target = (t.reshape(-1)[:n].contiguous() for t in batch(gen, 1, n))
+    for form in (dict(), dict(average=True, beta=2.0)):
+        *_, d = pref_check(ct, losses, reference, target, offsets.to(DEV), **form)
+        assert not d[:lead].any() and not d[n - tail:].any()
+    pref_check(ct, losses[:n - 3], None, None, offsets.to(DEV))
