@@ -92,8 +92,8 @@ __device__ __forceinline__ void finish(const PairArgs& a, long pair, Sum first, 
     value = m < 1.0 ? 1.0 - m : m >= 1.0 ? 0.0 : NAN;
     slope = m < 1.0 ? -1.0 : m >= 1.0 ? 0.0 : NAN;
   } else {
-    const double e = a.smoothing;
-    value = softplus(-m) * (1.0 - e);
+    const double e = a.smoothing;   // (0 and 1: one of the two alone, or its infinity would be 0 * inf)
+    value = e < 1.0 ? softplus(-m) * (1.0 - e) : 0.0;
     slope = -sigmoid(-m) * (1.0 - e);
     if (e > 0.0) {
       value += softplus(m) * e;

@@ -362,3 +362,13 @@ def test_a_long_sequence_among_short_ones(ct, pairs, long):  # noqa: F811
         *_, d = pref_check(ct, losses, reference, target, offsets.to(DEV), **form)
         assert not d[:lead].any() and not d[n - tail:].any()
     pref_check(ct, losses[:n - 3], None, None, offsets.to(DEV))
+
+
+def test_infinities_where_one_side_counts_nothing(ct):  # noqa: F811
+    # a smoothing of 1 leaves log(1 + exp m) alone, of 0 log(1 + exp -m): the other one's infinity is no 0 * inf
+    losses = torch.ones(2, 2, 3, device=DEV)
+    losses[0, 0, 1] = losses[1, 1, 1] = float("inf")           # m is -inf, inf
+    for smoothing, values, slopes in ((0.0, [float("inf"), 0.0], [[0.5, -0.5], [0.0, 0.0]]), (1.0, [0.0, float("inf")], [[0.0, 0.0], [-0.5, 0.5]]),
+                                      (0.5, [float("inf")] * 2, [[0.25, -0.25], [-0.25, 0.25]])):
+        v, _, s = ct.preference_forward(losses, beta=0.5, smoothing=smoothing)
+        assert v.tolist() == values and s.tolist() == slopes
