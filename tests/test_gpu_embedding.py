@@ -290,3 +290,65 @@ def test_refusals(ct):  # noqa: F811
     with pytest.raises(HipError, match="workspace too small"):
         ct._call("EmbeddingGrad", EmbeddingArgs(ids=many.data_ptr(), dy=rows.data_ptr(), lddy=8, dtable=table.data_ptr(), workspace=256, workspaceBytes=8,
                                                 tokens=300, width=8, vocab=5, ignore=IGNORE, scale=1.0), table.device)
+
+
+@pytest.mark.parametrize("vocab", [(1 << 18) + 1, (1 << 27) + 1, (1 << 31) - 1])
+@pytest.mark.parametrize("tokens", [257, 1025, 5120, 5121, 20000, 40000, 600001])
+def test_keys_of_many_digits(ct, tokens, vocab):  # noqa: F811
+    # two to four passes of digits (and one more key for ids without a row), in one workgroup, of tiles that are merged, and by digits' counts
+    gen = seeded(tokens)
+    ids = torch.randint(vocab, (tokens,), generator=gen)
+    ids[::5] = ids[1::5][:1] ^ (1 << torch.arange(len(ids[::5])) % 31)        # that differ by a single bit
+    ids[::7] = ids[:len(ids[::7])]                                             # some twice, some oftener
+    ids[3::11], ids[4::11] = vocab - 1 - torch.arange(len(ids[3::11])) % 3, torch.arange(len(ids[4::11])) % 3
+    ids[5::11] = vocab                                                         # outside, and ignored below
+    ids[6::11] = IGNORE
+    ids = torch.where(ids > vocab, ids - vocab, ids)
+    inside = (ids >= 0) & (ids < vocab)
+    grad = (torch.arange(tokens) % 3 - 1.0).to(torch.bfloat16).view(tokens, 1)  # sums of whole numbers are exact in float32, and rounded once
+    d = ct.embedding_backward(grad.to(DEV), ids.to(DEV), vocab)
+    rows, of = ids[inside].unique(return_inverse=True)
+    sums = torch.zeros(len(rows), dtype=torch.float64).index_add_(0, of, grad[inside, 0].double())
+    assert torch.equal(d[rows.to(DEV), 0].cpu(), sums.to(torch.bfloat16))
+    assert sum(int(d[k:k + (1 << 28)].count_nonzero()) for k in range(0, vocab, 1 << 28)) == int(sums.count_nonzero())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens", [40000, 530000])
+def test_ids_without_a_row_among_many(ct, dtype, tokens):  # noqa: F811
+    # sorted by digits' counts, which every workgroup adds up, or a launch before
+    test_ids_without_a_row(ct, dtype, tokens)
+
+
+def test_streams_and_graphs_of_many_ids(ct):  # noqa: F811
+    gen = seeded(7)
+    side = torch.cuda.Stream()
+    cases = []
+    # digits' counts; groups of pieces; a launch that adds up counts; tiles that are merged
+    for tokens, width, vocab in ((40000, 24, 300), (70000, 8, 300000), (530001, 4, 9000), (32768, 40, 700)):
+        cases.append((heavy(gen, tokens, vocab).to(DEV), normal(gen, vocab, width), normal(gen, tokens, width)))
+    torch.cuda.synchronize()
+
+    def all_of():
+        return [t for ids, table, grad in cases for t in (ct.embedding_forward(ids, table, 2.0), ct.embedding_backward(grad, ids, len(table), 2.0))]
+
+    first = all_of()
+    with torch.cuda.stream(side):
+        second = all_of()
+    side.synchronize()
+    for a, b in zip(first, second, strict=True):
+        assert torch.equal(a, b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = all_of()
+    for turn in range(3):
+        for ids, table, grad in cases:
+            ids.copy_(heavy(gen, len(ids), len(table)))
+            ids[turn::13] = (IGNORE, len(table), -1)[turn]
+            grad.mul_(-1.5)
+        for t in held:
+            t.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, all_of(), strict=True):
+            assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
