@@ -113,10 +113,12 @@ Held hold(Arena& m, long rows, long width, int type, bool exact = false) {
 // 1,024 against 65,536 172 and 162.  The parts are of the operator's type, with
 // its range: float16 hidden values and their gradients are infinite beyond 65504
 // and lose bits below 2^-14 (a loss in float16 is scaled; dl is by itself).
-// A teacher's few largest probabilities are most of dl, one or two values a row:
-// its rows count as few up to 256 (94 x 172 against 43,339, bfloat16: dtable off
-// by 0.0025 in one part and 0.0017 in two, 159 and 167 us; 256 x 1,024 against
-// 65,536 240 and 302 us).
+// A teacher's few largest probabilities are most of dl, one or two values a row,
+// of any number of rows: its rounding to one part is a rounding of what a table's row
+// gets.  Two parts are kept up to 256 rows, a bound of cost alone.  Backward pass in
+// bfloat16, one part and two (dx and dtable off by 0.0023-0.0024 and 0.0017): 94 x 172
+// against 43,339 81 and 92 us, 256 x 1,024 against 65,536 197 and 275; 1,024 rows
+// 469 and 723, 4,096 1,560 and 2,510.  A caller who needs the exact one has float32.
 constexpr long FEW = 64, FEW_TAUGHT = 256;
 bool few_rows(long rows, int type, long most = FEW) { return type != DT_F32 && rows <= most; }
 // Matrices that are copied first, all in one launch: where alignment, an odd

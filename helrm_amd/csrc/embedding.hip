@@ -7,17 +7,20 @@
 // length, and each piece adds the rows of its runs of equal ids in registers.  A
 // run inside a piece is a row of the gradient; what a run has in each of several
 // pieces is added in a fixed order by a second launch.  So a common id is as parallel
-// as any, and a result is the same on every run.  Sums are float32, scaled and
-// rounded once.  Rows that no id names are cleared by workgroups beside the
-// sort's, which so costs nothing where the table is large.
+// as any, and the same call gives the same result on every run (the length of the
+// pieces goes by the row's width and type too: a column beside others of another
+// width may differ in its last bit).  Sums are float32, scaled and rounded once.
+// The whole table is cleared by workgroups beside the sort's, which hide it
+// where it is small and are hidden by it where it is large; rows that an id names
+// are so written twice.  (Up to 256 ids, only the rows that no id names are cleared.)
 //
 // Bound by memory where rows are long (a copy here: 5.0 TB/s), by launches where
 // they are few.  131,072 ids x 2,048 against 131,072 rows bfloat16: rows 120-186
 // us (537 MB written, the common ids' rows come from the caches), gradient
-// 245: 94 for 537 MB cleared beside the sort, 132 for the sums (537 MB read, 155
-// written), 20 for the runs over several pieces.  16,384 x 1,024 against 65,536
-// rows: rows 8-10 us, gradient 44: 13 + 10 for the sort with 134 MB cleared beside
-// it, 12 and 9 for the sums.  53,248 x 16 float32: 3 us, and 24 + 6 + 5 of short
+// 244: 90 for 537 MB cleared beside the sort, 132 for the sums (537 MB read, 155
+// written), 22 for the runs over several pieces.  16,384 x 1,024 against 65,536
+// rows: rows 11 us, gradient 44: 13 + 10 for the sort with 134 MB cleared beside
+// it, 13 and 10 for the sums.  53,248 x 16 float32: 3 us, and 24 + 7 + 6 of short
 // launches.
 #include <algorithm>
 #include "embedding.h"
@@ -50,8 +53,9 @@ template <bool STREAM, class T, int V> __device__ __forceinline__ void store_pac
   else __builtin_nontemporal_store(__builtin_bit_cast(Wide, t), (Wide*)p);
 }
 // Results larger than the last-level cache go past it, so that it keeps the
-// common ids' rows: 131,072 x 2,048 bfloat16, both directions, 446 us, 480 with
-// ordinary stores; of 16,384 x 1,024, whose reader finds them in the cache, 66 and 63.
+// common ids' rows: 131,072 x 2,048 bfloat16, both directions, 424 us, 433 with
+// ordinary stores, 2^20 x 512 498 and 610.  Smaller ones stay for their reader, which costs
+// 40,000 x 1,024, 82 MB, 4 us here (91, 87 past the cache).
 bool streams(long rows, int width, int dtype) { return (double)rows * width * dtype_size(dtype) > 256L << 20; }
 
 // First element of a row's pack: the last one begins earlier, where the width is not a multiple, and holds some elements again.
@@ -97,8 +101,10 @@ constexpr int SORT = 1024, WAVES = SORT / 64, MOST_BITS = 9, MOST_DIGITS = 1 << 
 // 27.2 and 23.5; merged and by tiles' counts: 16,384 x 1,024 43.5 and 49.8,
 // 32,768 x 1,024 56.9 and 59.1 (more ids do not fit into LDS).
 constexpr long ONE = SORT * 5, MERGED = SORT * 32;
-// Ids a thread of a workgroup's share of more: as few as leave 32 tiles, whose
-// counts every workgroup adds up (16,384 ids, a scatter: 9 us with one, 14 with four).
+// Ids a thread of a workgroup's share of more: fewer are done sooner, but every
+// workgroup adds up the counts of all (up to FEW_TILES) tiles.  Gradient against
+// 65,536 rows x 64 with two and four: 40,000 ids 36.5 and 43.6 us, 65,536 40.7 and
+// 45.8, 131,072 53 and 57, 2^20 123 and 119.
 int items_of(long tokens) { return tokens <= 64 * SORT ? 2 : 4; }
 
 struct SortArgs {
@@ -421,7 +427,7 @@ struct SumArgs {
 // WAVE: a team is a wave.
 template <class T, int V, bool WAVE>
 __global__ __launch_bounds__(BLOCK) void run_sum_kernel(const SumArgs a, long base) {
-  constexpr int AHEAD = 8;   // rows on their way (131,072 x 2,048: 260 us; 269 with 4, 399 with 16, for which there are too few registers)
+  constexpr int AHEAD = 8;   // rows on their way (the gradient of 131,072 x 2,048: 257 us; 268 with 4, 391 with 16, for which there are too few registers)
   const int lane = WAVE ? threadIdx.x & 63 : threadIdx.x & (a.lanes - 1);
   unsigned team = (unsigned)(((base + blockIdx.x) * BLOCK + threadIdx.x) / (WAVE ? 64 : a.lanes));
   if (WAVE) team = __builtin_amdgcn_readfirstlane(team);
@@ -566,7 +572,7 @@ template <class F> void with_items(int n, F&& f) {
 // that are equal if it is the first of them, and others that clear rows of the
 // table that no id names.  A workgroup compares all ids, and one id's rows are
 // added by one: more ids are sorted.  64 ids x 408 against 960 rows float32, both
-// directions, 27 us in four launches, 21 in two (the host's time).
+// directions, 24 us in four launches, 18 in two (the host's time).
 constexpr int FEW = 256;
 struct FewArgs {
   EmbedArgs e;
@@ -650,8 +656,8 @@ int packs_of(int width, int dtype) {
 }
 
 // Pieces from which on a launch adds up groups of them before each run is joined
-// by a workgroup: 4 us more where runs are short (53,248 x 16, 3,328 pieces: 39 us,
-// 44 with it); 2^20 equal ids x 512, 16,384 pieces, 347 us with it and 1,711 without.
+// by a workgroup: 5 us more where runs are short (53,248 x 16, 3,328 pieces, gradient
+// 35 us, 41 with it; 2^20 x 64 113 and 120); 2^20 equal ids x 512, 16,384 pieces, 337 us with it and 1,773 without.
 constexpr int MANY_PIECES = 4096;
 // The pieces of the workspace, or only their bytes.
 struct Space {
@@ -661,9 +667,9 @@ struct Space {
   size_t bytes = 0;
 };
 // Ids of a piece: as many as leave 2,048 waves, of 16 to 64.  A longer piece has
-// fewer sums that are joined, a shorter one keeps more waves at work: 16,384 x
-// 1,024, both directions, 66 us with 2,048 or 1,024 waves, 75 with 512; 131,072 x
-// 2,048 423 us with pieces of 64, 426 of 128, 454 of 256.
+// fewer sums that are joined, a shorter one keeps more waves at work: gradient of
+// 16,384 x 1,024 44 us with 2,048 or 1,024 waves, 50 with 512; of 131,072 x 2,048
+// 257 us with pieces of 64, 261 of 128, 270 of 256.
 int piece_of(long tokens, int blocks, int lanes) {
   const long waves = tokens * blocks * lanes / 64;
   return waves >= 64 * 2048 ? 64 : waves >= 32 * 2048 ? 32 : 16;
@@ -795,7 +801,7 @@ void embedding_grad_launch(const EmbedArgs& a, hipStream_t st) {
   m.n = (int)a.tokens; m.vocab = a.vocab; m.width = a.width; m.packs = packs;
   m.lanes = lanes_of(packs, 64);
   m.across = lanes_of(packs, JOIN);
-  const int threads = std::min(std::max(4 * m.across, 256), JOIN);   // (1,024 for rows of 4 packs: 17 us, 5 with 256)
+  const int threads = std::min(std::max(4 * m.across, 256), JOIN);   // (the gradient of 53,248 x 16, rows of 4 packs: 50 us with 1,024, 37 with 256)
   m.blocks = (int)clr::ceil_div(packs, m.lanes);
   m.piece = piece_of(a.tokens, m.blocks, m.lanes);
   m.pieces = (int)clr::ceil_div(a.tokens, m.piece);

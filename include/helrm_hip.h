@@ -378,7 +378,10 @@ int LossTotal(const LossTotalArgs* args, void* stream);
  * row without entries has loss, lse and gradients 0, and nothing it holds reaches
  * another row's; an entry whose id is outside [0, vocab) gives a loss and
  * gradients of NaN.  kept, scores, probs and cols are what the gradient and a mean over
- * the rows with a teacher need (kept is 0 for the others).  dtable is contiguous. */
+ * the rows with a teacher need (kept is 0 for the others).  dtable is contiguous.
+ * In 16-bit types the gradient of the logits is a factor of two products and rounded
+ * to the type from 257 rows on, as the cross entropy's from 65 on: gradients have
+ * that rounding and their own. */
 typedef struct {
   const void* x; long ldx;               /* [rows][width] */
   const void* table; long ldtable;       /* [vocab][width] */
@@ -402,7 +405,8 @@ int DistillationGrad(const DistillationArgs* args, void* stream);
 
 /* y[i] = scale table[ids[i]]: rows of a table, and the table's gradient
  * dtable[v] = scale * the sum of dy[i] over ids[i] = v, 0 for rows that no id
- * names.  Sums are float32, rounded once, in an order that only the ids decide.
+ * names.  Sums are float32, rounded once, in an order that the ids, the width and
+ * the type decide: the same call gives the same result on every run.
  * An id that is `ignore` gives a row of zeros and takes nothing back, whatever
  * its row of dy holds; another one outside [0, vocab) gives a row of NaN and
  * takes nothing back. */
