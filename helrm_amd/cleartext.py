@@ -368,7 +368,8 @@ def cross_entropy_forward(x, table, target, ignore_index=-100):
 
 def cross_entropy_backward(grad, x, table, target, lse, ignore_index=-100):
     """(dx, dtable) for the gradient `grad` of the losses (float32); lse as the forward call gave it.  The logits are
-    computed again, a piece of the table at a time."""
+    computed again, a piece of the table at a time.  Their gradient is a factor of two products: in 16-bit types of more than 64
+    rows it is rounded to the type, and dx and dtable have that rounding and their own."""
     x2, table, target = _loss_tensors(x, table, target, ignore_index)
     rows, width = x2.shape
     _same_order(grad.shape, x.shape[:-1], "grad")
@@ -488,7 +489,8 @@ def distillation_forward(x, table, ids, logits, temperature=1.0, ignore_index=-1
 
 def distillation_backward(grad, x, table, ids, lse, saved, temperature=1.0, ignore_index=-100):
     """(dx, dtable) for the gradient `grad` of the losses (float32); lse and saved as the forward call gave them.  The logits are
-    computed again, a piece of the table at a time."""
+    computed again, a piece of the table at a time.  Their gradient is a factor of two products: in 16-bit types of more than 256
+    rows it is rounded to the type, and dx and dtable have that rounding and their own."""
     x2, table, ids = _teach_tensors(x, table, ids, temperature, ignore_index)
     rows, width = x2.shape
     _same_order(grad.shape, x.shape[:-1], "grad")

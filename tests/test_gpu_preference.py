@@ -372,3 +372,22 @@ def test_infinities_where_one_side_counts_nothing(ct):  # noqa: F811
                                       (0.5, [float("inf")] * 2, [[0.25, -0.25], [-0.25, 0.25]])):
         v, _, s = ct.preference_forward(losses, beta=0.5, smoothing=smoothing)
         assert v.tolist() == values and s.tolist() == slopes
+
+
+@pytest.mark.parametrize("tail", [0, 1, 7, 2048])
+@pytest.mark.parametrize("pairs", [3, 600, 40000, 600000])
+def test_gradients_of_a_long_line(ct, pairs, tail):  # noqa: F811
+    # eight tokens a thread; a token's gradient is one product of the pair's and its sequence's, or 0
+    gen = seeded(pairs + tail)
+    lengths = torch.randint((1 << 19) // pairs, (1 << 21) // pairs + 2, (2 * pairs,), generator=gen)
+    lengths[torch.randint(2 * pairs, (pairs // 2,), generator=gen)] = 0
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), lengths.cumsum(0)]) + 11
+    n = int(offsets[-1]) + tail
+    assert n >= 1 << 20
+    line, target = torch.zeros(n, device=DEV), torch.where(torch.rand(n, generator=gen) < 0.8, 5, IGNORE).to(DEV)
+    grad, slopes = torch.randn(pairs, generator=gen).to(DEV), torch.randn(pairs, 2, generator=gen).to(DEV)
+    d = ct.preference_backward(grad, line, slopes, target, offsets.to(DEV))
+    want = torch.zeros(n, device=DEV)
+    want[11:n - tail] = (grad[:, None] * slopes).view(-1).repeat_interleave(lengths.to(DEV))
+    assert torch.equal(d, torch.where(target != IGNORE, want, 0.0))
+    assert torch.equal(ct.preference_backward(grad, line, slopes, offsets=offsets.to(DEV)), want)
